@@ -127,6 +127,11 @@ _SIGS = {
     "ckq_rmsnorm_q8_k_fused_dev": (_i, [_vp, _vp, _vp, _i, _i, _i, _c.c_float, _vp]),
     "ckq_swiglu_q8_k_dev": (_i, [_vp, _vp, _vp, _i, _i, _c.c_long, _vp]),
     "ckq_gemm_nt_f32act_dev": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i, _i, _c.c_long, _vp]),
+    "ckq_quantize_i8_dev": (_i, [_i, _vp, _l, _vp, _l, _vp, _i, _i, _vp]),
+    "ckq_dequantize_i8_dev": (_i, [_vp, _l, _vp, _i, _vp, _l, _i, _i, _vp]),
+    "ckq_rmsnorm_i8_dev": (_i, [_i, _vp, _l, _vp, _vp, _l, _vp, _c.c_float, _vp, _l, _vp, _i, _i, _vp]),
+    "ckq_swiglu_i8_dev": (_i, [_i, _vp, _vp, _l, _vp, _l, _vp, _i, _i, _vp]),
+    "ckq_gemm_nt_i8_dev": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _i, _vp, _l, _i, _i, _i, _vp]),
     "ckq_matmul_sequence_dev": (_i, [_vp, _i, _i, _vp]),
     "ckq_subblock_dots_dev": (_i, [_i, _vp, _vp, _vp, _i, _i, _vp]),
     "ckq_subblock_dots_tokens_dev": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _vp]),

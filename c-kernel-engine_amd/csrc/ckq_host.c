@@ -119,6 +119,7 @@ const char *ckq_error_string(int code)
     case CKQ_EINVAL: return "invalid argument (NULL pointer or non-positive dimension)";
     case CKQ_ESHAPE: return "K is not a multiple of the quantization block size";
     case CKQ_EFORMAT: return "unknown weight format";
+    case CKQ_EROWS: return "int8 rows: pointers and pitches of a matmul's operands have to be multiples of 16 bytes, pitches at most 4 MiB, K at most 131071; floats have to be aligned to their size";
     case CKQ_ENODUMP: return "the integer dumps of the exactness tests are built into libckernel_quant_hip_dump.so, not into this library";
     case CKQ_ESCRATCH: return "the call is of a size that ckq_gemm_nt_noalloc_dev counts with more scratch than it holds (4 MiB); use ckq_gemm_nt_dev or fewer tokens per call";
     default: return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown error";
@@ -1463,6 +1464,33 @@ int ckq_gemm_nt_f32act_dev(int fmt, const float *A, const void *B, const float *
                 : fmt == CKQ_FMT_Q8_0 ? CKQ_KERNEL_Q80_F32 : -1;
     if (k < 0) return CKQ_EFORMAT;
     return ckq_launch_gemv(k, C, B, A, bias, N, K, M, ldc, 0, N, NULL, stream);
+}
+
+int ckq_quantize_i8_dev(ckq_ck_dtype type, const void *x, long ldx, int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
+{
+    return ckq_launch_quantize_i8((int)type, x, ldx, q, ldq, scale, rows, k, stream);
+}
+
+int ckq_dequantize_i8_dev(const int8_t *q, long ldq, const float *scale, ckq_ck_dtype type, void *y, long ldy, int rows, int k, void *stream)
+{
+    return ckq_launch_dequantize_i8(q, ldq, scale, (int)type, y, ldy, rows, k, stream);
+}
+
+int ckq_rmsnorm_i8_dev(ckq_ck_dtype type, const void *x, long ldx, const void *residual, void *sum, long ldr, const float *gamma, float eps,
+                       int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
+{
+    return ckq_launch_rmsnorm_i8((int)type, x, ldx, residual, sum, ldr, gamma, eps, q, ldq, scale, rows, k, stream);
+}
+
+int ckq_swiglu_i8_dev(ckq_ck_dtype type, const void *gate, const void *up, long ld, int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
+{
+    return ckq_launch_swiglu_i8((int)type, gate, up, ld, q, ldq, scale, rows, k, stream);
+}
+
+int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,
+                       ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream)
+{
+    return ckq_launch_gemm_i8(A, lda, sa, B, ldb, sb, bias, (int)type, C, ldc, M, N, K, stream);
 }
 
 static int ranges_overlap(const void *a, size_t na, const void *b, size_t nb) { return ckq_ranges_overlap(a, na, b, nb); }

@@ -1,0 +1,327 @@
+/*
+ * ckq_int8_rows.hip - rows in 8 bits with one scale each: the activations (and, when a model is loaded, the
+ * weights) of the int8 matmul of ckq_gemm_int8.hip, and the rows read back.
+ *
+ *   v       = x                                        quantize
+ *           = h * r * gamma,  h = T(x + residual),  r = 1 / sqrt(sum h^2 / k + eps)    rmsnorm
+ *           = gate / (1 + exp(-gate)) * up             swiglu
+ *   a       = max(max_i |v_i|, 2^-100)                 (a row of zeros divides by nothing)
+ *   q_i     = rne(v_i * (127 / a)),  scale = a / 127
+ *
+ * All of it in fp32.  The norm's factor r is the same for a whole row, so the largest |h * gamma| is looked for in
+ * the pass that sums the squares, and r comes into the two factors of the row afterwards: one reduction across the
+ * waves where the order of the formula would need two.  A row with an infinity or a NaN in v has that as its scale
+ * and zeros as its quants, so that whatever is computed from it is not a number either; the maximum is taken over
+ * bit patterns, where NaN > inf > everything else, and no order of lanes or waves can lose one.
+ */
+#include "ckq_device.hpp"
+#include "ckq_launch.h"
+
+enum { ROWS_QUANTIZE, ROWS_RMSNORM, ROWS_SWIGLU };
+
+template <int T> struct RowType;
+template <> struct RowType<CKQ_T_F32>  { typedef float type; };
+template <> struct RowType<CKQ_T_BF16> { typedef __bf16 type; };
+template <> struct RowType<CKQ_T_F16>  { typedef _Float16 type; };
+
+/* Eight consecutive elements; rows start anywhere an element can (the loads and stores take that as they are). */
+template <class E> struct __attribute__((packed, aligned(sizeof(E)))) row8 { E v[8]; };
+struct __attribute__((packed, aligned(1))) row8q { u32 v[2]; };
+
+template <class E>
+__device__ __forceinline__ void load8(float (&f)[8], const E *p, int left)
+{
+    if (left >= 8) {
+        const row8<E> r = *reinterpret_cast<const row8<E> *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)r.v[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < left ? (float)p[i] : 0.0f;
+    }
+}
+template <class E>
+__device__ __forceinline__ void store8(E *p, const float (&f)[8], int left)
+{
+    if (left >= 8) {
+        row8<E> r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r.v[i] = (E)f[i];
+        *reinterpret_cast<row8<E> *>(p) = r;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) p[i] = (E)f[i];
+    }
+}
+
+struct RowsArgs {
+    const void  *x;          /* rows; gate */
+    const void  *y;          /* rmsnorm: residual or null; swiglu: up */
+    void        *h;          /* rmsnorm: x + residual, where there is one */
+    const float *gamma;
+    int8_t      *q;
+    float       *scale;
+    long         ldx, ldy, ldh, ldq;
+    float        eps;
+    int          rows, k;
+};
+
+/* The values of vector `v` (eight elements) of a row, rmsnorm's without its factor r; `ss` collects the squares. */
+template <int OP, class E, bool AGAIN>
+__device__ __forceinline__ void row_values(float (&f)[8], const RowsArgs &a, const E *x, const E *y, E *h, int v, float &ss)
+{
+    const int left = a.k - 8 * v;
+    if (OP == ROWS_RMSNORM && AGAIN && y) {
+        load8(f, (const E *)h + 8 * v, left);          /* this thread wrote them; x + residual may be gone by now */
+    } else {
+        load8(f, x + 8 * v, left);
+        if (OP == ROWS_SWIGLU || (OP == ROWS_RMSNORM && y)) {
+            float g[8];
+            load8(g, y + 8 * v, left);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (OP == ROWS_SWIGLU) {
+                    /* v_exp_f32 and v_rcp_f32, an ulp each: what they are off is 2^-22 of a value that is about to
+                     * be rounded to one part in 254 of the row's largest */
+                    const float e = __builtin_amdgcn_exp2f(f[i] * -1.44269504f);
+                    f[i] = f[i] * __builtin_amdgcn_rcpf(1.0f + e) * g[i];
+                } else
+                    f[i] = (float)(E)(f[i] + g[i]);    /* the norm is of the stream as it is stored */
+            }
+            if (OP == ROWS_RMSNORM) store8(h + 8 * v, f, left);
+        }
+    }
+    if (OP == ROWS_RMSNORM) {
+        float g[8];
+        load8(g, a.gamma + 8 * v, left);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            ss = __builtin_fmaf(f[i], f[i], ss);
+            f[i] *= g[i];
+        }
+    }
+}
+
+__device__ __forceinline__ u32 top_bits(const float (&f)[8], u32 top)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __builtin_bit_cast(u32, f[i]) & 0x7fffffffu);
+    return top;
+}
+
+__device__ __forceinline__ u32 wave_top(u32 v)
+{
+    v = max(v, (u32)dpp_get<0xB1>((int)v));
+    v = max(v, (u32)dpp_get<0x4E>((int)v));
+    v = max(v, (u32)dpp_get<0x141>((int)v));
+    v = max(v, (u32)dpp_get<0x140>((int)v));
+    v = max(v, (u32)dpp_get<0x142, 0xA>((int)v));
+    v = max(v, (u32)dpp_get<0x143, 0xC>((int)v));
+    return (u32)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ float wave_sum(float v)
+{
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, group_sum<64>(v)), 63));
+}
+
+/* NV > 0: `wpr` waves have a row, each thread at most NV vectors of it, held in registers between the two passes (k <= 512 wpr NV);
+ * NV = 0: rows of any length, read again for the second pass. */
+template <int OP, class E, int NV>
+__global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
+{
+    __shared__ float red_ss[16];
+    __shared__ u32   red_top[16];
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), nw = blockDim.x >> 6;
+    const int row = __builtin_amdgcn_readfirstlane(wpr == 1 ? (int)blockIdx.x * nw + wave : (int)blockIdx.x);
+    const bool live = row < a.rows;                          /* wpr == 1: waves behind the last row have nothing to do */
+    if (wpr == 1 && !live) return;
+    const E *x = (const E *)a.x + (size_t)row * a.ldx;
+    const E *y = a.y ? (const E *)a.y + (size_t)row * a.ldy : nullptr;
+    E *h = a.h ? (E *)a.h + (size_t)row * a.ldh : nullptr;
+    const int nvec = (a.k >> 3) + ((a.k & 7) != 0), first = wpr == 1 ? lane : (int)threadIdx.x, step = 64 * wpr;
+
+    float f[NV > 0 ? NV : 1][8], ss = 0.0f;
+    u32 top = 0;
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = first + i * step;
+            if (v < nvec) {
+                row_values<OP, E, false>(f[i], a, x, y, h, v, ss);
+                top = top_bits(f[i], top);
+            }
+        }
+    } else
+        for (int v = first; v < nvec; v += step) {
+            row_values<OP, E, false>(f[0], a, x, y, h, v, ss);
+            top = top_bits(f[0], top);
+        }
+
+    top = wave_top(top);
+    if (OP == ROWS_RMSNORM) ss = wave_sum(ss);
+    if (wpr > 1) {
+        if (lane == 0) {
+            red_top[wave] = top;
+            if (OP == ROWS_RMSNORM) red_ss[wave] = ss;
+        }
+        __syncthreads();
+        top = 0;
+        ss = 0.0f;
+        for (int w = 0; w < nw; ++w) {                       /* in the same order for every wave */
+            top = max(top, red_top[w]);
+            if (OP == ROWS_RMSNORM) ss += red_ss[w];
+        }
+    }
+
+    const float ftop = __builtin_bit_cast(float, top);
+    const float r = OP == ROWS_RMSNORM ? 1.0f / sqrtf(ss / (float)a.k + a.eps) : 1.0f;
+    /* an infinity or a NaN in the row; the squares' sum beyond fp32 (r = 0); a row of zeros and no eps (r infinite) */
+    const bool finite = ftop * r < __builtin_inff() && r > 0.0f;
+    const float amax = fmaxf(ftop * r, 0x1p-100f);
+    const float inv = 127.0f / amax * r;
+    if (first == 0) a.scale[row] = finite ? amax / 127.0f : top >= 0x7f800000u ? ftop : r > 0.0f ? ftop * r : __builtin_nanf("");
+
+    int8_t *q = a.q + (size_t)row * a.ldq;
+    auto put = [&](const float (&e)[8], int v) {
+        u32 p[2] = {0u, 0u};
+        if (finite) q8_round(e, inv, p);
+        const int left = a.k - 8 * v;
+        if (left >= 8) {
+            row8q o;
+            o.v[0] = p[0];
+            o.v[1] = p[1];
+            *reinterpret_cast<row8q *>(q + 8 * v) = o;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < left) q[8 * v + i] = (int8_t)sbyte(p[i >> 2], i & 3);
+        }
+    };
+    if (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int v = first + i * step;
+            if (v < nvec) put(f[i], v);
+        }
+    } else
+        for (int v = first; v < nvec; v += step) {
+            row_values<OP, E, true>(f[0], a, x, y, h, v, ss);
+            put(f[0], v);
+        }
+}
+
+template <int OP, class E>
+static int launch_rows(RowsArgs a, hipStream_t s)
+{
+    const int nvec = a.k / 8 + (a.k % 8 != 0);
+    const int wpr = nvec <= 64 ? 1 : nvec <= 256 ? 4 : 16, per = (nvec - 1) / (64 * wpr) + 1;
+    const dim3 block(wpr == 1 ? 256u : 64u * (unsigned)wpr);
+    /* a launch has fewer than 2^32 threads */
+    for (;;) {
+        const int left = a.rows, now = min(left, 1 << 21);
+        a.rows = now;
+        const dim3 grid((unsigned)(wpr == 1 ? (now + 3) / 4 : now));
+        if (per <= 1)      hipLaunchKernelGGL((rows_i8_kernel<OP, E, 1>), grid, block, 0, s, a, wpr);
+        else if (per <= 2) hipLaunchKernelGGL((rows_i8_kernel<OP, E, 2>), grid, block, 0, s, a, wpr);
+        else               hipLaunchKernelGGL((rows_i8_kernel<OP, E, 0>), grid, block, 0, s, a, wpr);
+        const int rc = (int)hipGetLastError();
+        if (rc || left == now) return rc;
+        a.x = (const E *)a.x + (size_t)now * a.ldx;
+        if (a.y) a.y = (const E *)a.y + (size_t)now * a.ldy;
+        if (a.h) a.h = (E *)a.h + (size_t)now * a.ldh;
+        a.q += (size_t)now * a.ldq;
+        a.scale += now;
+        a.rows = left - now;
+    }
+}
+
+template <int OP>
+static int launch_rows(int type, const RowsArgs &a, void *stream)
+{
+    switch (type) {
+    case CKQ_T_F32:  return launch_rows<OP, float>(a, (hipStream_t)stream);
+    case CKQ_T_BF16: return launch_rows<OP, __bf16>(a, (hipStream_t)stream);
+    case CKQ_T_F16:  return launch_rows<OP, _Float16>(a, (hipStream_t)stream);
+    default:         return CKQ_EFORMAT;
+    }
+}
+
+static int row_size(int type) { return type == CKQ_T_F32 ? 4 : type == CKQ_T_BF16 || type == CKQ_T_F16 ? 2 : 0; }
+
+extern "C" int ckq_launch_quantize_i8(int type, const void *x, long ldx, int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
+{
+    if (!x || !q || !scale || rows <= 0 || k <= 0 || ldx < k || ldq < k) return CKQ_EINVAL;
+    if (!row_size(type)) return CKQ_EFORMAT;
+    if ((uintptr_t)x % row_size(type) || (uintptr_t)scale % 4) return CKQ_EROWS;
+    const RowsArgs a = {x, nullptr, nullptr, nullptr, q, scale, ldx, 0, 0, ldq, 0.0f, rows, k};
+    return launch_rows<ROWS_QUANTIZE>(type, a, stream);
+}
+
+extern "C" int ckq_launch_rmsnorm_i8(int type, const void *x, long ldx, const void *residual, void *sum, long ldr, const float *gamma, float eps,
+                                     int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
+{
+    if (!x || !gamma || !q || !scale || rows <= 0 || k <= 0 || ldx < k || ldq < k) return CKQ_EINVAL;
+    if (!residual != !sum || (residual && ldr < k) || !(eps >= 0.0f)) return CKQ_EINVAL;
+    if (!row_size(type)) return CKQ_EFORMAT;
+    if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum) % row_size(type) || ((uintptr_t)scale | (uintptr_t)gamma) % 4) return CKQ_EROWS;
+    const RowsArgs a = {x, residual, sum, gamma, q, scale, ldx, ldr, ldr, ldq, eps, rows, k};
+    return launch_rows<ROWS_RMSNORM>(type, a, stream);
+}
+
+extern "C" int ckq_launch_swiglu_i8(int type, const void *gate, const void *up, long ld, int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
+{
+    if (!gate || !up || !q || !scale || rows <= 0 || k <= 0 || ld < k || ldq < k) return CKQ_EINVAL;
+    if (!row_size(type)) return CKQ_EFORMAT;
+    if (((uintptr_t)gate | (uintptr_t)up) % row_size(type) || (uintptr_t)scale % 4) return CKQ_EROWS;
+    const RowsArgs a = {gate, up, nullptr, nullptr, q, scale, ld, ld, 0, ldq, 0.0f, rows, k};
+    return launch_rows<ROWS_SWIGLU>(type, a, stream);
+}
+
+/* y = T(scale * q), eight elements a thread.  Bound by memory: 1 byte read and the type's written. */
+template <class E>
+__global__ void __launch_bounds__(256) dequantize_i8_kernel(const int8_t *__restrict__ q, long ldq, const float *__restrict__ scale,
+                                                            E *__restrict__ y, long ldy, u32 rows, int k, u32 nvec)
+{
+    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (t >= (size_t)rows * nvec) return;
+    const u32 row = (u32)(t / nvec), v = (u32)(t - (size_t)row * nvec);
+    const int8_t *p = q + (size_t)row * ldq + 8 * (size_t)v;
+    const int left = k - 8 * (int)v;
+    const float s = scale[row];
+    float f[8];
+    if (left >= 8) {
+        const row8q r = *reinterpret_cast<const row8q *>(p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = s * (float)sbyte(r.v[i >> 2], i & 3);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < left ? s * (float)p[i] : 0.0f;
+    }
+    store8(y + (size_t)row * ldy + 8 * (size_t)v, f, left);
+}
+
+extern "C" int ckq_launch_dequantize_i8(const int8_t *q, long ldq, const float *scale, int type, void *y, long ldy, int rows, int k, void *stream)
+{
+    if (!q || !scale || !y || rows <= 0 || k <= 0 || ldq < k || ldy < k) return CKQ_EINVAL;
+    if (!row_size(type)) return CKQ_EFORMAT;
+    if ((uintptr_t)y % row_size(type) || (uintptr_t)scale % 4) return CKQ_EROWS;
+    const u32 nvec = (u32)(k / 8 + (k % 8 != 0));
+    const hipStream_t s = (hipStream_t)stream;
+    /* a launch has fewer than 2^32 threads */
+    const int most = (int)min((size_t)rows, max((size_t)1, ((size_t)1 << 31) / nvec));
+    for (int row = 0; row < rows;) {
+        const int n = min(rows - row, most);
+        const int8_t *qr = q + (size_t)row * ldq;
+        const dim3 grid((unsigned)(((size_t)n * nvec + 255) / 256)), block(256);
+        switch (type) {
+        case CKQ_T_F32:  hipLaunchKernelGGL(dequantize_i8_kernel<float>, grid, block, 0, s, qr, ldq, scale + row, (float *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec); break;
+        case CKQ_T_BF16: hipLaunchKernelGGL(dequantize_i8_kernel<__bf16>, grid, block, 0, s, qr, ldq, scale + row, (__bf16 *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec); break;
+        default:         hipLaunchKernelGGL(dequantize_i8_kernel<_Float16>, grid, block, 0, s, qr, ldq, scale + row, (_Float16 *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec); break;
+        }
+        const int rc = (int)hipGetLastError();
+        if (rc) return rc;
+        row += n;
+    }
+    return 0;
+}

@@ -20,6 +20,7 @@ extern "C" {
 #define CKQ_EFORMAT (-3)  /* unknown format tag */
 #define CKQ_ESCRATCH (-4) /* the call is counted with more scratch than the entry point that allocates nothing holds */
 #define CKQ_ENOGROUP (-7) /* internal: a grouped GEMM launch was declined; the caller launches the matrices one by one */
+#define CKQ_EROWS (-8)    /* rows of int8, or the floats beside them, that are not as the kernels take them (ckernel_quant_hip.h) */
 #define CKQ_ENODUMP (-6)  /* the integer dumps are compiled into libckernel_quant_hip_dump.so only */
 /* 1 in the test library (same sources, same templates, plus the DUMP instantiations that also
  * store the integers behind every output); 0 in the product library, which stays smaller for it. */
@@ -150,6 +151,21 @@ int ckq_launch_gemv_noalloc(int fmt, float *y, const void *W, const void *X, con
  * tiles per launch): chunk c of `per` tokens out of `total` covers
  * [*first, *first + *count).  Exported for the index test. */
 void ckq_grid_chunk(long total, long per, long c, long *first, long *count);
+
+/* Rows in 8 bits with one scale each (ckq_int8_rows.hip, ckq_gemm_int8.hip); `type` is one of CKQ_T_*, the values that the
+ * reference's CKDataType has for them.  See ckernel_quant_hip.h for what they compute and take. */
+#define CKQ_T_F32  0
+#define CKQ_T_BF16 1
+#define CKQ_T_F16  2
+#define CKQ_I8_K_MAX 131071              /* 128 * 128 * k < 2^31 */
+#define CKQ_I8_PITCH_MAX (1l << 22)      /* a tile's rows lie within 32-bit offsets */
+int ckq_launch_quantize_i8(int type, const void *x, long ldx, int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
+int ckq_launch_dequantize_i8(const int8_t *q, long ldq, const float *scale, int type, void *y, long ldy, int rows, int k, void *stream);
+int ckq_launch_rmsnorm_i8(int type, const void *x, long ldx, const void *residual, void *sum, long ldr, const float *gamma, float eps,
+                          int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
+int ckq_launch_swiglu_i8(int type, const void *gate, const void *up, long ld, int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
+int ckq_launch_gemm_i8(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,
+                       int type, void *C, long ldc, int M, int N, int K, void *stream);
 
 /* Plain device copy kernel (calibration of the memory counters / roofline). */
 int ckq_launch_copy(void *dst, const void *src, size_t bytes, void *stream);

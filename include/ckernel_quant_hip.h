@@ -284,6 +284,34 @@ int ckq_swiglu_q8_k_dev(const float *gate, const float *up, void *y, int rows, i
 int ckq_gemm_nt_f32act_dev(int fmt, const float *A, const void *B, const float *bias, float *C,
                            int M, int N, int K, long ldc, void *stream);
 
+/* Rows of int8 with one scale each: the value of q[row][i] is scale[row] * q[row][i].  The other common 8-bit form of a
+ * model's projections: weights with a scale a channel (N rows), activations with a scale a token (M rows).  No counterpart in
+ * the reference.  `type` of the floats is CKQ_CK_DTYPE_FP32, _BF16 or _FP16, anything else is CKQ_EFORMAT (-3); rows of
+ * floats lie ld elements apart, rows of int8 ld bytes, at least their length (else CKQ_EINVAL, -1).  Floats are aligned to their own
+ * size, else CKQ_EROWS (-8).  Nothing is allocated, no scratch is shared between calls, and every call may be captured.
+ *
+ * ckq_quantize_i8_dev: a = max(largest |x| of the row, 2^-100), q = RNE(x * (127 / a)), scale = a / 127, in fp32.  A row with a
+ * NaN or an infinity gets that as its scale (NaN if there is one) and zeros as its quants.  Bytes of q behind a row's k-th stay
+ * as they are.
+ * ckq_dequantize_i8_dev: y = scale * q, rounded to the type.
+ * ckq_rmsnorm_i8_dev: sum = x + residual, rounded to the type (`residual` and `sum` both NULL: there is none, and the norm is of
+ * x); then sum * (1 / sqrt(mean of sum^2 + eps)) * gamma in 8 bits as above.  residual and sum have one pitch, ldr; sum may be
+ * residual itself, or x (with ldr = ldx).  Squares are summed in fp32: a row whose sum of squares, or whose sum * gamma, exceeds fp32
+ * gets a scale that is not finite, and zeros as its quants, as do zeros without an eps.
+ * ckq_swiglu_i8_dev: gate / (1 + exp(-gate)) * up in 8 bits as above; gate and up have one pitch, ld, so that both may be halves
+ * of one row (the output of a projection that holds the rows of both).
+ * ckq_gemm_nt_i8_dev: C[m*ldc + n] = sa[m] * sb[n] * (sum over k of A[m][k] * B[n][k]) (+ bias[n]), the sum exact in int32, the
+ * rest in fp32, rounded once to the type of C.  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are,
+ * multiples of 16 bytes, pitches at most 4 MiB, K at most 131071 (else CKQ_EROWS).  K may be odd: of the 16 bytes that hold a
+ * row's last, those behind it may be read and are not used. */
+int ckq_quantize_i8_dev(ckq_ck_dtype type, const void *x, long ldx, int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
+int ckq_dequantize_i8_dev(const int8_t *q, long ldq, const float *scale, ckq_ck_dtype type, void *y, long ldy, int rows, int k, void *stream);
+int ckq_rmsnorm_i8_dev(ckq_ck_dtype type, const void *x, long ldx, const void *residual, void *sum, long ldr, const float *gamma, float eps,
+                       int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
+int ckq_swiglu_i8_dev(ckq_ck_dtype type, const void *gate, const void *up, long ld, int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
+int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,
+                       ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream);
+
 /* A list of steps enqueued back-to-back, the whole list `repeat` times: the
  * per-token chain of a decoder layer (norm -> Q8_K -> Q/K/V ... -> down) is one
  * such list.  A matmul entry (fmt = a ckq_format weight tag) computes

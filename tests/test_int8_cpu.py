@@ -1,0 +1,96 @@
+"""CPU checks of the int8 entry points: what they refuse, before anything touches a device, and with which code.  No
+kernel is launched here."""
+import ctypes
+import importlib
+import os
+
+import pytest
+
+ckq = importlib.import_module("c-kernel-engine_amd")
+EINVAL, EFORMAT, EROWS = -1, -3, -8
+F32, BF16, F16 = 0, 1, 2
+
+
+@pytest.fixture(scope="module")
+def L():
+    if not os.path.exists(ckq.lib_path()):
+        ckq.build()
+    return ckq.lib()
+
+
+P = ctypes.c_void_p(4096)
+
+
+def odd(n):
+    return ctypes.c_void_p(4096 + n)
+
+
+def test_quantize_and_dequantize_refusals(L):
+    def quantize(t=BF16, x=P, ldx=64, q=P, ldq=64, scale=P, rows=2, k=64):
+        return L.ckq_quantize_i8_dev(t, x, ldx, q, ldq, scale, rows, k, None)
+
+    def dequantize(q=P, ldq=64, scale=P, t=BF16, y=P, ldy=64, rows=2, k=64):
+        return L.ckq_dequantize_i8_dev(q, ldq, scale, t, y, ldy, rows, k, None)
+
+    for bad in ({"x": None}, {"q": None}, {"scale": None}, {"rows": 0}, {"rows": -1}, {"k": 0}, {"k": -5}, {"ldx": 63}, {"ldq": 63}):
+        assert quantize(**bad) == EINVAL, bad
+    for bad in ({"q": None}, {"y": None}, {"scale": None}, {"rows": 0}, {"k": 0}, {"ldq": 63}, {"ldy": 63}):
+        assert dequantize(**bad) == EINVAL, bad
+    for t in (-1, 3, 7, 9, 13):
+        assert quantize(t=t) == EFORMAT and dequantize(t=t) == EFORMAT
+    assert quantize(x=odd(1)) == EROWS and quantize(scale=odd(2)) == EROWS
+    assert quantize(t=F32, x=odd(2)) == EROWS
+    assert dequantize(y=odd(1)) == EROWS and dequantize(t=F32, y=odd(2)) == EROWS and dequantize(scale=odd(3)) == EROWS
+
+
+def test_rmsnorm_refusals(L):
+    def norm(t=F16, x=P, ldx=64, residual=P, out=P, ldr=64, gamma=P, eps=1e-5, q=P, ldq=64, scale=P, rows=2, k=64):
+        return L.ckq_rmsnorm_i8_dev(t, x, ldx, residual, out, ldr, gamma, ctypes.c_float(eps), q, ldq, scale, rows, k, None)
+
+    for bad in ({"x": None}, {"gamma": None}, {"q": None}, {"scale": None}, {"residual": None}, {"out": None}, {"rows": 0}, {"k": 0},
+                {"ldx": 63}, {"ldr": 63}, {"ldq": 63}, {"eps": -1e-5}, {"eps": float("nan")}):
+        assert norm(**bad) == EINVAL, bad
+    assert norm(t=5) == EFORMAT
+    for bad in ({"x": odd(1)}, {"residual": odd(1)}, {"out": odd(1)}, {"gamma": odd(2)}, {"scale": odd(2)}, {"t": F32, "residual": odd(2)}):
+        assert norm(**bad) == EROWS, bad
+
+
+def test_swiglu_refusals(L):
+    def swiglu(t=BF16, gate=P, up=P, ld=128, q=P, ldq=64, scale=P, rows=2, k=64):
+        return L.ckq_swiglu_i8_dev(t, gate, up, ld, q, ldq, scale, rows, k, None)
+
+    for bad in ({"gate": None}, {"up": None}, {"q": None}, {"scale": None}, {"rows": 0}, {"k": 0}, {"ld": 63}, {"ldq": 63}):
+        assert swiglu(**bad) == EINVAL, bad
+    assert swiglu(t=4) == EFORMAT
+    for bad in ({"gate": odd(1)}, {"up": odd(1)}, {"scale": odd(1)}, {"t": F32, "up": odd(2)}):
+        assert swiglu(**bad) == EROWS, bad
+
+
+def test_matmul_refusals(L):
+    def gemm(a=P, lda=64, sa=P, b=P, ldb=64, sb=P, bias=P, t=BF16, c=P, ldc=32, M=2, N=32, K=50):
+        return L.ckq_gemm_nt_i8_dev(a, lda, sa, b, ldb, sb, bias, t, c, ldc, M, N, K, None)
+
+    for bad in ({"a": None}, {"sa": None}, {"b": None}, {"sb": None}, {"c": None}, {"M": 0}, {"N": 0}, {"K": 0}, {"M": -1}, {"K": 65},
+                {"lda": 48}, {"ldb": 48}, {"ldc": 31}):
+        assert gemm(**bad) == EINVAL, bad
+    assert gemm(t=3) == EFORMAT and gemm(t=-1) == EFORMAT
+    long = {"lda": 131072, "ldb": 131072}
+    for bad in ({"a": odd(8)}, {"b": odd(4)}, {"lda": 72}, {"ldb": 50}, {"lda": (1 << 22) + 16}, {"ldb": 1 << 30}, {"K": 131072, **long},
+                {"c": odd(1)}, {"t": F32, "c": odd(2)}, {"sa": odd(2)}, {"sb": odd(1)}, {"bias": odd(3)}):
+        assert gemm(**bad) == EROWS, bad
+    assert b"16 bytes" in L.ckq_error_string(EROWS)
+
+
+def test_front_ends_refuse_what_a_pointer_cannot_tell():
+    import torch
+    par, err = ckq.parity, ckq.CkqError
+    x = torch.zeros(3, 32)
+    with pytest.raises(err, match="not on the current device"):
+        par.dev_quantize_i8(x)
+    with pytest.raises(err, match="shape"):
+        par.dev_quantize_i8(x[0])
+    with pytest.raises(err):
+        par.dev_rmsnorm_i8(x, torch.ones(32))
+    with pytest.raises(err):
+        par.dev_gemm_nt_i8(torch.zeros(2, 32, dtype=torch.uint8), x[0], x, x[0])
+    assert par.empty_i8(3, 33, device="cpu").shape == (3, 33) and par.empty_i8(3, 33, device="cpu").stride() == (48, 1)
