@@ -6,6 +6,7 @@
  * The sum is exact in int32 for k <= 131071 (128 * 128 * k < 2^31), so no order of it, and no split, changes a bit.
  */
 #include "ckq_gemm_common.hpp"
+#include <atomic>
 
 template <int T> struct I8Out;
 template <> struct I8Out<CKQ_T_F32>  { typedef float type; };
@@ -22,56 +23,605 @@ struct I8Args {
 
 __device__ __forceinline__ float i8_scaled(int sum, float sa, float sb) { return (sa * (float)sum) * sb; }
 
-/* A wave has 16 tokens x 16 rows; every lane fetches its own operands, 16 bytes of one row (v_mfma_i32_16x16x64_i8: lane l holds
- * bytes 16 (l / 16) .. of row l % 16 of both operands; result: rows 4 (l / 16) + r of the first, row l % 16 of the second). */
-template <class E>
-__global__ void __launch_bounds__(256) gemm_i8_simple_kernel(I8Args a)
+/* ---- tiles through LDS ---------------------------------------------------------------------------------------------- */
+
+/* Which tile the t-th of a launch is: tiles are dealt to the XCDs in equal runs (gemm_deal), and in the order of a run eight token
+ * tiles lie beside each other for every tile of rows, so that the tiles an XCD works on at a time share both operands in its L2. */
+__device__ __forceinline__ bool i8_which_tile(int t, int ntt, int nnt, int &tt, int &nt)
 {
+    if (t < 0) return false;
+    const int band = t / (8 * nnt), in = t - band * 8 * nnt, wide = min(8, ntt - 8 * band);
+    nt = in / wide;
+    tt = 8 * band + in - nt * wide;
+    return true;
+}
+
+typedef float ckq_v4f __attribute__((ext_vector_type(4)));
+template <class E> struct __attribute__((packed, aligned(sizeof(E)))) i8_out8 { E v[8]; };
+
+/* Results leave non-temporally: they are not read again by the launch that writes them, and what stays in the L2s is written back
+ * when it ends, with nothing beside it (2048 x 8192 x 4096 in bf16, 64.9 -> 60.7 us, of which the results' 33 MB 7 at the rate of a copy). */
+typedef u32 i8_u4 __attribute__((ext_vector_type(4)));
+typedef i8_u4 __attribute__((aligned(2))) i8_u4_at_2;        /* one store of 16 bytes, wherever it falls */
+template <class E> __device__ __forceinline__ void i8_put(E *out, const i8_out8<E> &o)
+{
+    struct { i8_u4 v[sizeof(o) / 16]; } w = __builtin_bit_cast(decltype(w), o);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(o) / 16); ++i) __builtin_nontemporal_store(w.v[i], reinterpret_cast<i8_u4_at_2 *>(out) + i);
+}
+
+/* A wave: the sums of 32 tokens (from t0) x ROWS rows (from n) at `sums`, `pitch` bytes a token, scaled and stored, eight rows a lane;
+ * sa, sb, bias: the scales of those tokens and of those rows, and their bias, in LDS too. */
+template <class E, int ROWS>
+__device__ __forceinline__ void i8_store_rows(const I8Args &a, const uint8_t *sums, int pitch, const float *sa, const float *sb, const float *bias, int t0, int n, int lane)
+{
+    constexpr int PER = ROWS / 8;                             /* lanes of a token */
+#pragma unroll
+    for (int e0 = 0; e0 < 32 * PER; e0 += 64) {
+        const int e = e0 + lane, row = e / PER, c = 8 * (e % PER), t = t0 + row, n8 = n + c, left = a.N - n8;
+        const ckq_v4i *s = reinterpret_cast<const ckq_v4i *>(sums + row * pitch + 4 * c);
+        const ckq_v4f *fb = reinterpret_cast<const ckq_v4f *>(sb + c), *fc = reinterpret_cast<const ckq_v4f *>(bias + c);
+        float v[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) v[r] = i8_scaled(s[r >> 2][r & 3], sa[row], fb[r >> 2][r & 3]);
+        if (a.bias) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r) v[r] += fc[r >> 2][r & 3];
+        }
+        i8_out8<E> o;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) o.v[r] = (E)v[r];
+        if (t >= a.M || left <= 0) continue;
+        E *out = (E *)a.C + (size_t)t * a.ldc + n8;
+        if (left >= 8) i8_put(out, o);
+        else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < left) out[r] = o.v[r];
+        }
+    }
+}
+/* WT x WN waves, each 32 TT tokens x 32 TN rows, S stages in LDS; SP, FM: see `multiply`. */
+template <int WT_, int WN_, int TT_, int TN_, int S_, int SP_, int FM_> struct I8Tile {
+    static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, S = S_, SP = SP_, FM = FM_;
+    static constexpr int NW = WT * WN, BT = 32 * TT * WT, BN = 32 * TN * WN, KS = 128, STAGE = (BT + BN) * KS;
+    static constexpr int NCA = BT / 8 / NW, NCB = BN / 8 / NW;           /* copies of a wave a step: eight rows each */
+    static constexpr int PITCH = 32 * TN * 4 + 16;                       /* of a token's sums in LDS */
+    static constexpr int SCALES = S * STAGE > NW * 32 * PITCH ? S * STAGE : NW * 32 * PITCH, LDS = SCALES + 4 * (BT + 2 * BN);
+    static_assert(NW % 2 == 0 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole copies");
+    static_assert(BT % 64 == 0 && BN % 64 == 0, "whole copies of the scales");
+};
+
+template <class E, class T>
+__device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t *lds)
+{
+    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, S = T::S, SP = T::SP, FM = T::FM, NW = T::NW, BT = T::BT, BN = T::BN, KS = T::KS, STAGE = T::STAGE, NCA = T::NCA;
+    constexpr int NC = T::NCA + T::NCB, NM = TT * TN, NF = TT + TN, PITCH = T::PITCH;
     const int lane = threadIdx.x & 63, wave = wave_in_block();
-    const int ntn = (a.N + 15) / 16, ntm = (a.M + 15) / 16;
-    const long tile = (long)blockIdx.x * 4 + wave;
-    if (tile >= (long)ntn * ntm) return;
-    const int n0 = 16 * (int)(tile % ntn), m0 = 16 * (int)(tile / ntn);
-    const int r = lane & 15, c = 16 * (lane >> 4);
-    const int8_t *pa = a.A + (size_t)min(m0 + r, a.M - 1) * a.lda, *pb = a.B + (size_t)min(n0 + r, a.N - 1) * a.ldb;
-    ckq_v4i acc = {0, 0, 0, 0};
-    for (int k = 0; k < a.K; k += 64) {
-        ckq_v4i va = {0, 0, 0, 0}, vb = {0, 0, 0, 0};
-        const int left = a.K - (k + c);
-        if (left > 0) {
-            va = *reinterpret_cast<const ckq_v4i *>(pa + k + c);
-            vb = *reinterpret_cast<const ckq_v4i *>(pb + k + c);
-            /* bytes behind the row's last are not zero: take them out of one operand */
+    const ckq_v4i rsa = gemm_buffer((const uint8_t *)a.A + (size_t)m0 * a.lda), rsb = gemm_buffer((const uint8_t *)a.B + (size_t)n0 * a.ldb);
+    const u32 base = lds_address(lds);
+    const int niter = (a.K + KS - 1) / KS, last = niter - 1, tail = a.K - last * KS;      /* bytes of the last step, 1 .. 128 */
+
+    /* a copy takes eight rows of 128 bytes; the chunk of 16 that a lane fetches is the one that belongs in its place, c ^ (row / 2 % 8):
+     * sixteen rows' chunks c, which a phase of a read of 16 bytes a lane takes, then lie on all 64 banks once (c ^ (row % 8): twice, 8.3 cycles a read and not 4.2) */
+    u32 ofs[NC];
+    const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int row = 8 * (wave + NW * (i < NCA ? i : i - NCA)) + (lane >> 3);
+        ofs[i] = i < NCA ? (u32)min(row, a.M - 1 - m0) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb;
+        ofs[i] += 16u * (u32)chunk;
+    }
+    auto copy = [&](int i, int it, int buf) {
+        /* chunks behind the row's last are read from its start; the tokens' are zeroed (clear_tail) */
+        const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
+        const u32 dst = base + (u32)(buf * STAGE + 1024 * (wave + NW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * KS));
+        lds_copy16(i < NCA ? rsa : rsb, dst, o, it * KS);
+    };
+    auto clear_tail = [&](int buf) {
+        for (int e = threadIdx.x; e < BT * 8; e += 64 * NW) {
+            const int row = e >> 3, left = tail - 16 * ((e & 7) ^ ((row >> 1) & 7));
+            if (left >= 16) continue;
+            ckq_v4i *p = reinterpret_cast<ckq_v4i *>(lds + buf * STAGE + 16 * e);
+            ckq_v4i v = *p;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int n = left - 4 * i;
-                va[i] = n >= 4 ? va[i] : n <= 0 ? 0 : va[i] & (int)((1u << (8 * n)) - 1u);
+                v[i] = n >= 4 ? v[i] : n <= 0 ? 0 : v[i] & (int)((1u << (8 * n)) - 1u);
             }
+            *p = v;
         }
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(vb, va, acc, 0, 0, 0);
-    }
-    const int m = m0 + r;
-    if (m >= a.M) return;
-    const float sa = a.sa[m];
-    E *out = (E *)a.C + (size_t)m * a.ldc;
+    };
+
+    /* where a lane's operands are: row lane % 32 of a group of 32, bytes 16 (lane / 32) of the 32 of a multiplication */
+    const int wt = wave / WN, wn = wave % WN, half = lane >> 5;
+    u32 ra[4], rb[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int n = n0 + 4 * (lane >> 4) + i;
-        if (n < a.N) {
-            float v = i8_scaled(acc[i], sa, a.sb[n]);
+    for (int kk = 0; kk < 4; ++kk) {
+        const u32 pos = 16u * (u32)((2 * kk + half) ^ ((lane >> 1) & 7));
+        ra[kk] = (u32)(32 * TT * wt + (lane & 31)) * KS + pos;
+        rb[kk] = (u32)(BT + 32 * TN * wn + (lane & 31)) * KS + pos;
+    }
+    ckq_v16i acc[TT][TN];
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = ckq_v16i{};
+    ckq_v4i fa[2][TT], fb[2][TN];
+    auto fetch = [&](int to, int buf, int kk, int f) {         /* operand f of 32 bytes of K, in the order of their use: a row group, all tokens, the other rows */
+        const uint8_t *p = lds + buf * STAGE;
+        if (f == 0)       fb[to][0] = *reinterpret_cast<const ckq_v4i *>(p + rb[kk]);
+        else if (f <= TT) fa[to][f - 1] = *reinterpret_cast<const ckq_v4i *>(p + ra[kk] + 32 * KS * (f - 1));
+        else              fb[to][f - TT] = *reinterpret_cast<const ckq_v4i *>(p + rb[kk] + 32 * KS * (f - TT));
+    };
+    /* The multiplications of 32 bytes of K; among the first FM of them the reads of the next 32 bytes' operands, and over the
+     * first SP quarters of a step the copies of a later one: a copy holds its wave until the address unit has taken it, 16
+     * cycles, and a burst of all waves' copies leaves the matrix cores idle for their sum; the last of them has to arrive in
+     * what is left of the step where there are two stages. */
+    auto multiply = [&](int from, int quarter, int it, int buf, int fbuf, int fkk) {
+        const bool more = it < niter;
+#pragma unroll
+        for (int m = 0; m < NM; ++m) {
+            const int j = m / TT, i = m % TT;
+            acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[from][j], fa[from][i], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int f = 0; f < NF; ++f)
+                if (f * FM / NF == m && fbuf >= 0) fetch(from ^ 1, fbuf, fkk, f);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (c * NM * SP / NC == quarter * NM + m && more) copy(c, it, buf);
+            __builtin_amdgcn_sched_barrier(0);                 /* or the compiler moves the reads to where they are used, and waits for each */
+        }
+    };
+
+    /* the scales and the bias, BT, BN and BN floats, behind the stages: fetched first, used last */
+    float *scales = reinterpret_cast<float *>(lds + T::SCALES);
+    for (int i = wave; i < (BT + 2 * BN) / 64; i += NW) {
+        const bool tok = i < BT / 64, ch = i < (BT + BN) / 64;
+        const float *p = tok ? a.sa : ch ? a.sb : a.bias;
+        if (!p) continue;
+        const int e = 64 * i + lane - (tok ? 0 : ch ? BT : BT + BN);
+        lds_copy4(gemm_buffer((const uint8_t *)(p + (tok ? m0 : n0))), base + (u32)T::SCALES + 256u * (u32)i, 4u * (u32)min(e, tok ? a.M - 1 - m0 : a.N - 1 - n0), 0);
+    }
+
+    /* Step `it` has stage it % S.  A step's last operands are read before its last quarter is multiplied; the barrier is there, so
+     * that no wave waits with nothing to multiply, and from there on the stage takes the copies of step it + S. */
+#pragma unroll
+    for (int st = 0; st < S - 1; ++st)
+        if (st < niter) {
+#pragma unroll
+            for (int c = 0; c < NC; ++c) copy(c, st, st);
+        }
+    if (S > 2 && niter > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * NC) : "memory");
+    else                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (last == 0 && tail < KS) {
+        clear_tail(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    }
+    if (S - 1 < niter) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (c * SP / NC == 0) copy(c, S - 1, S - 1);
+    }
+#pragma unroll
+    for (int f = 0; f < NF; ++f) fetch(0, 0, 0, f);
+    int buf = 0;
+    for (int it = 0; it < niter; ++it) {
+        const int next = buf + 1 == S ? 0 : buf + 1, prev = buf == 0 ? S - 1 : buf - 1;
+#pragma unroll
+        for (int kk = 0; kk < 3; ++kk) multiply(kk & 1, kk + 1, it + S - 1, prev, buf, kk + 1);
+        if (S > 2 && it + S - 1 < niter) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * NC) : "memory");
+        else                             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (it + 1 == last && tail < KS) {
+            clear_tail(next);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+        }
+        multiply(1, 0, it + S, buf, it < last ? next : -1, 0);
+        buf = next;
+    }
+
+    /* sums, 32 tokens at a time through LDS, so that a lane has eight rows' results of one token side by side and a token's leave in
+     * whole lines: every wave has its own piece, behind everything that is still read from the last step's stage */
+    __syncthreads();
+    uint8_t *mine = lds + wave * 32 * PITCH;
+    const int nw = n0 + 32 * TN * wn;
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+        const int t0 = m0 + 32 * (TT * wt + i);
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<ckq_v4i *>(mine + (lane & 31) * PITCH + 4 * (32 * j + 8 * g + 4 * half)) =
+                    ckq_v4i{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        i8_store_rows<E, 32 * TN>(a, mine, PITCH, scales + t0 - m0, scales + BT + nw - n0, scales + BT + T::BN + nw - n0, t0, nw, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+template <class E, class T>
+__global__ void __launch_bounds__(64 * T::NW) gemm_i8_tile_kernel(I8Args a, int ntt, int nnt)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
+    int tt, nt;
+    if (i8_which_tile(gemm_deal(blockIdx.x, ntt * nnt), ntt, nnt, tt, nt)) i8_tile<E, T>(a, tt * T::BT, nt * T::BN, lds);
+}
+
+/* The first nnt1 columns of tiles of T1, `blocks1` blocks of them, and the rows that they leave in tiles of T2. */
+template <class E, class T1, class T2>
+__global__ void __launch_bounds__(64 * T1::NW) gemm_i8_two_tiles_kernel(I8Args a, int ntt1, int nnt1, int blocks1, int ntt2, int nnt2)
+{
+    static_assert(T1::NW == T2::NW, "one size of block");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T1::LDS > T2::LDS ? T1::LDS : T2::LDS];
+    int tt, nt;
+    if ((int)blockIdx.x < blocks1) {
+        if (i8_which_tile(gemm_deal(blockIdx.x, ntt1 * nnt1), ntt1, nnt1, tt, nt)) i8_tile<E, T1>(a, tt * T1::BT, nt * T1::BN, lds);
+    } else if (i8_which_tile(gemm_deal(blockIdx.x - blocks1, ntt2 * nnt2), ntt2, nnt2, tt, nt))
+        i8_tile<E, T2>(a, tt * T2::BT, nnt1 * T1::BN + nt * T2::BN, lds);
+}
+
+template <class E, class T>
+static int launch_i8_tiles(const I8Args &a, hipStream_t s)
+{
+    const int ntt = (a.M + T::BT - 1) / T::BT, nnt = (a.N + T::BN - 1) / T::BN;
+    if ((long)ntt * nnt > 0x3fffff) return CKQ_EINVAL;       /* results beyond any memory */
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<E, T>), dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::NW), 0, s, a, ntt, nnt);
+    return (int)hipGetLastError();
+}
+template <class E, class T1, class T2>
+static int launch_i8_two_tiles(const I8Args &a, int nnt1, hipStream_t s)
+{
+    const int ntt1 = (a.M + T1::BT - 1) / T1::BT, ntt2 = (a.M + T2::BT - 1) / T2::BT, nnt2 = (a.N - nnt1 * T1::BN + T2::BN - 1) / T2::BN;
+    const int blocks1 = gemm_blocks(ntt1, nnt1);
+    hipLaunchKernelGGL((gemm_i8_two_tiles_kernel<E, T1, T2>), dim3((unsigned)(blocks1 + gemm_blocks(ntt2, nnt2))), dim3(64u * T1::NW), 0, s,
+                       a, ntt1, nnt1, blocks1, ntt2, nnt2);
+    return (int)hipGetLastError();
+}
+
+/* ---- K split among the waves of a block ------------------------------------------------------------------------------ */
+
+/* 16 TG tokens x 16 RN rows a block of NW waves; every wave has all of the tile and each NW-th step of 128 bytes of K, through S stages of
+ * its own, so that nothing is waited for but its own copies until the waves' sums meet at the end. */
+template <int NW_, int RN_, int TG_, int S_> struct I8Split {
+    static constexpr int NW = NW_, RN = RN_, TG = TG_, S = S_, KS = 128;
+    static constexpr int BT = 16 * TG, BN = 16 * RN, STAGE = (BT + BN) * KS, PITCH = BN * 4 + 16;
+    static constexpr int LDS = NW * (S * STAGE > BT * PITCH ? S * STAGE : BT * PITCH);
+    static_assert(LDS <= 160 * 1024, "one block fits");
+};
+
+template <class E, class T>
+__global__ void __launch_bounds__(64 * T::NW) gemm_i8_split_kernel(I8Args a, int ntt, int nnt)
+{
+    constexpr int NW = T::NW, RN = T::RN, TG = T::TG, S = T::S, KS = T::KS, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = 2 * (RN + TG), PITCH = T::PITCH;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
+    const int lane = threadIdx.x & 63, wave = wave_in_block();
+    int tt, nt;
+    {
+        const int t = gemm_deal(blockIdx.x, ntt * nnt);
+        if (t < 0) return;
+        nt = t / ntt;                                         /* token tiles side by side: they share the rows */
+        tt = t - nt * ntt;
+    }
+    const int m0 = tt * BT, n0 = nt * BN;
+
+    /* what this thread stores in the end: eight rows of a token; their scales are here by then */
+    constexpr int PER = BN / 8, JOBS = BT * PER, TRIPS = (JOBS + 64 * NW - 1) / (64 * NW);
+    const ckq_v4i rsa = gemm_buffer((const uint8_t *)a.A + (size_t)m0 * a.lda), rsb = gemm_buffer((const uint8_t *)a.B + (size_t)n0 * a.ldb);
+    const u32 mine = (u32)(wave * S * STAGE);
+    const int niter = (a.K + KS - 1) / KS, last = niter - 1, tail = a.K - last * KS, steps = wave < niter ? (niter - 1 - wave) / NW + 1 : 0;
+
+    u32 ofs[NC];
+    const int half8 = lane >> 3;                              /* row of a copy's eight */
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int row = 8 * (i < 2 * TG ? i : i - 2 * TG) + half8, chunk = (lane & 7) ^ ((row >> 1) & 7);
+        ofs[i] = (i < 2 * TG ? (u32)min(row, a.M - 1 - m0) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
+    }
+    auto copy = [&](int j, int slot) {
+        const int it = wave + NW * j;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int row = 8 * (i < 2 * TG ? i : i - 2 * TG) + half8, chunk = (lane & 7) ^ ((row >> 1) & 7);
+            const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
+            lds_copy16(i < 2 * TG ? rsa : rsb, lds_address(lds) + mine + (u32)(slot * STAGE + 1024 * i), o, it * KS);
+        }
+    };
+    ckq_v4i acc[TG][RN];
+#pragma unroll
+    for (int i = 0; i < TG; ++i)
+#pragma unroll
+        for (int j = 0; j < RN; ++j) acc[i][j] = ckq_v4i{0, 0, 0, 0};
+
+#pragma unroll
+    for (int j = 0; j < S - 1; ++j)
+        if (j < steps) copy(j, j);
+    int slot = 0;
+    for (int j = 0; j < steps; ++j) {
+        if (j + S - 1 < steps) {
+            copy(j + S - 1, slot == 0 ? S - 1 : slot - 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * NC) : "memory");
+        } else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint8_t *p = lds + mine + slot * STAGE;
+        const bool cut = wave + NW * j == last && tail < KS;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int c = 4 * kk + (lane >> 4);
+            const u32 at = (u32)((lane & 15) * KS + 16 * (c ^ ((lane >> 1) & 7)));
+            ckq_v4i fa[TG], fb[RN];
+#pragma unroll
+            for (int i = 0; i < TG; ++i) fa[i] = *reinterpret_cast<const ckq_v4i *>(p + at + 16 * KS * i);
+#pragma unroll
+            for (int i = 0; i < RN; ++i) fb[i] = *reinterpret_cast<const ckq_v4i *>(p + at + (BT + 16 * i) * KS);
+            if (cut) {                                        /* bytes behind the row's last are anything: not the tokens' */
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int n = tail - 16 * c - 4 * w;
+                    const int keep = n >= 4 ? -1 : n <= 0 ? 0 : (int)((1u << (8 * n)) - 1u);
+#pragma unroll
+                    for (int i = 0; i < TG; ++i) fa[i][w] &= keep;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < TG; ++i)
+#pragma unroll
+                for (int n = 0; n < RN; ++n) acc[i][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[n], fa[i], acc[i][n], 0, 0, 0);
+        }
+        asm volatile("" ::: "memory");                        /* the next copies into this slot come after its reads, which the multiplications have waited for */
+        slot = slot + 1 == S ? 0 : slot + 1;
+    }
+
+    /* the waves' sums meet in LDS; eight rows of a token a thread */
+    __syncthreads();
+    uint8_t *red = lds + wave * BT * PITCH;
+#pragma unroll
+    for (int i = 0; i < TG; ++i)
+#pragma unroll
+        for (int n = 0; n < RN; ++n)
+            *reinterpret_cast<ckq_v4i *>(red + (16 * i + (lane & 15)) * PITCH + 4 * (16 * n + 4 * (lane >> 4))) = acc[i][n];
+    __syncthreads();
+#pragma unroll
+    for (int trip = 0; trip < TRIPS; ++trip) {
+        const int e = trip * 64 * NW + threadIdx.x, row = e / PER, c = 8 * (e % PER), t = m0 + row, n8 = n0 + c, left = a.N - n8;
+        if (e >= JOBS || t >= a.M || left <= 0) continue;
+        ckq_v4i s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const ckq_v4i *s = reinterpret_cast<const ckq_v4i *>(lds + w * BT * PITCH + row * PITCH + 4 * c);
+            s0 += s[0];
+            s1 += s[1];
+        }
+        const float sa = a.sa[t];
+        i8_out8<E> o;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int n = n8 + min(r, left - 1);
+            float v = i8_scaled(r < 4 ? s0[r] : s1[r - 4], sa, a.sb[n]);
             if (a.bias) v += a.bias[n];
-            out[n] = (E)v;
+            o.v[r] = (E)v;
+        }
+        E *out = (E *)a.C + (size_t)t * a.ldc + n8;
+        if (left >= 8) i8_put(out, o);
+        else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (r < left) out[r] = o.v[r];
         }
     }
+}
+
+template <class E, class T>
+static int launch_i8_split(const I8Args &a, hipStream_t s)
+{
+    const int ntt = (a.M + T::BT - 1) / T::BT, nnt = (a.N + T::BN - 1) / T::BN;
+    if ((long)ntt * nnt > 0x3fffff) return CKQ_EINVAL;       /* results beyond any memory */
+    hipLaunchKernelGGL((gemm_i8_split_kernel<E, T>), dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::NW), 0, s, a, ntt, nnt);
+    return (int)hipGetLastError();
+}
+
+/* ---- few tokens: rows streamed ----------------------------------------------------------------------------------------- */
+
+/* MT tokens; a wave has R rows and every KS-th piece of KU KB of K; 4 waves a block. */
+template <class E, int MT, int R, int KU, int KS>
+__global__ void __launch_bounds__(256) gemv_i8_kernel(I8Args a)
+{
+    constexpr int G = 4 / KS;
+    __shared__ int red[KS > 1 ? 4 * R * MT : 1];
+    const int lane = threadIdx.x & 63, wave = wave_in_block();
+    const int part = wave % KS, n0 = ((int)blockIdx.x * G + wave / KS) * R;
+    if (KS == 1 && n0 >= a.N) return;
+    const uint8_t *pb[R], *pa[MT];
+#pragma unroll
+    for (int r = 0; r < R; ++r) pb[r] = (const uint8_t *)a.B + (size_t)min(n0 + r, a.N - 1) * a.ldb;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) pa[t] = (const uint8_t *)a.A + (size_t)min(t, a.M - 1) * a.lda;
+    int acc[R][MT];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[r][t] = 0;
+    for (int k0 = part * KU * 1024; k0 < a.K; k0 += KS * KU * 1024) {
+        ckq_v4i w[R][KU], x[MT][KU];
+        u32 at[KU];
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            at[u] = (u32)k0 + 1024u * u + 16u * (u32)lane;
+            if ((int)at[u] >= a.K) at[u] = 0;                /* counted out below */
+        }
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) w[r][u] = __builtin_nontemporal_load(reinterpret_cast<const ckq_v4i *>(pb[r] + at[u]));
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) x[t][u] = *reinterpret_cast<const ckq_v4i *>(pa[t] + at[u]);
+        if (k0 + KU * 1024 > a.K) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int n = a.K - (k0 + 1024 * u + 16 * lane + 4 * i), keep = n >= 4 ? -1 : n <= 0 ? 0 : (int)((1u << (8 * n)) - 1u);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) x[t][u][i] &= keep;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[r][t] = dot4(w[r][u][i], x[t][u][i], acc[r][t]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[r][t] = __builtin_amdgcn_readlane(group_sum<64>(acc[r][t]), 63);
+    if (KS > 1) {
+        if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) red[(wave * R + r) * MT + t] = acc[r][t];
+        }
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int w = 1; w < KS; ++w) acc[r][t] += red[((wave + w) * R + r) * MT + t];
+    }
+    /* lane r + R t has row r of token t */
+    int sum = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) sum = lane == r + R * t ? acc[r][t] : sum;
+    const int r = lane % R, t = lane / R, n = n0 + r;
+    if (lane < R * MT && t < a.M && n < a.N) {
+        float v = i8_scaled(sum, a.sa[t], a.sb[n]);
+        if (a.bias) v += a.bias[n];
+        ((E *)a.C)[(size_t)t * a.ldc + n] = (E)v;
+    }
+}
+
+template <class E, int MT, int R, int KU, int KS>
+static int launch_i8_stream(const I8Args &a, hipStream_t s)
+{
+    constexpr int per = 4 / KS * R;
+    hipLaunchKernelGGL((gemv_i8_kernel<E, MT, R, KU, KS>), dim3((unsigned)((a.N + per - 1) / per)), dim3(256), 0, s, a);
+    return (int)hipGetLastError();
+}
+
+/* ---- which kernel ------------------------------------------------------------------------------------------------------ */
+
+typedef I8Tile<2, 4, 4, 2, 2, 2, 3> T256x256;
+typedef I8Tile<4, 2, 2, 2, 3, 4, 2> T256x128;
+typedef I8Tile<4, 2, 1, 3, 3, 4, 2> T128x192;
+typedef I8Tile<2, 2, 2, 2, 2, 2, 2> T128x128;        /* two blocks a CU */
+typedef I8Tile<4, 2, 1, 2, 4, 4, 2> T128x128_8;
+typedef I8Tile<2, 4, 1, 1, 5, 4, 1> T64x128;
+typedef I8Split<4, 2, 4, 2> S64x32;
+typedef I8Split<4, 3, 2, 2> S32x48;                   /* two blocks a CU */
+typedef I8Split<4, 2, 2, 2> S32x32;                   /* two */
+typedef I8Split<8, 1, 1, 2> S16x16;                   /* two */
+typedef I8Split<4, 2, 1, 2> S16x32;                   /* three */
+
+enum { I8_256x256, I8_256x128, I8_128x192, I8_128x128, I8_128x128_8, I8_64x128, I8_S64x32, I8_S32x48, I8_S32x32, I8_S16x16, I8_S16x32, I8_TILINGS,
+       I8_TWO = I8_TILINGS, I8_STREAM };
+
+/* What a launch takes, in us: t0, and for every round of blocks t_tile and, for each of its steps of K, s0 + s1 * (the part of
+ * the round's places that have a block: CUs that share the L2s and the power are slower).  Fitted to some hundred sizes of 5 to 2048
+ * tokens (64 to 32000 rows, K 64 to 11008) as measured on one box: each within 5 to 11 % (rms); the kernel so chosen is 2 %
+ * slower than the best of all on average, 1.27 times at worst. */
+struct I8Cost { int bt, bn, places, split; float t0, t_tile, s0, s1; };
+static const I8Cost i8_costs[I8_TILINGS] = {
+    {256, 256, 256, 1, 2.00f, 5.94f, 1.063f, 0.497f},
+    {256, 128, 256, 1, 2.00f, 4.11f, 0.601f, 0.271f},
+    {128, 192, 256, 1, 2.00f, 3.47f, 0.524f, 0.232f},
+    {128, 128, 512, 1, 2.00f, 3.59f, 0.473f, 0.606f},
+    {128, 128, 256, 1, 2.00f, 2.65f, 0.441f, 0.143f},
+    {64, 128, 256, 1, 2.00f, 1.86f, 0.330f, 0.084f},
+    {64, 32, 256, 4, 2.00f, 1.62f, 0.359f, 0.191f},
+    {32, 48, 512, 4, 2.07f, 1.45f, 0.280f, 0.601f},
+    {32, 32, 512, 4, 2.14f, 1.31f, 0.207f, 0.459f},
+    {16, 16, 512, 8, 2.25f, 1.22f, 0.217f, 0.385f},
+    {16, 32, 768, 4, 2.23f, 1.14f, 0.214f, 0.508f},
+};
+
+static float i8_rounds(const I8Cost &c, long tiles, int K)
+{
+    const int steps = ((K + 127) / 128 + c.split - 1) / c.split;
+    const long full = tiles / c.places, rest = tiles % c.places;
+    float t = (float)full * (c.t_tile + (float)steps * (c.s0 + c.s1));
+    if (rest) t += c.t_tile + (float)steps * (c.s0 + c.s1 * (float)rest / (float)c.places);
+    return t;
+}
+static long i8_tiles(const I8Cost &c, int M, int N) { return (long)((M + c.bt - 1) / c.bt) * ((N + c.bn - 1) / c.bn); }
+
+/* Columns of 256 x 256 tiles that make whole rounds of the 256 CUs: what they leave goes in tiles of 128 x 192, a shorter last round
+ * (2048 x 11008 x 4096: 344 tiles of 256 x 256 in two rounds 102 us; 256 of them and 240 small ones 85). */
+static int i8_whole_columns(int M, int N)
+{
+    const int ntt = (M + 255) / 256, nnt = (N + 255) / 256;
+    return (int)((long)ntt * nnt / 256 * 256 / ntt);
+}
+
+static std::atomic<int> g_i8_kernel{-1};
+extern "C" void ckq_launch_set_i8_kernel(int kernel) { g_i8_kernel.store(kernel < 0 || kernel > I8_STREAM ? -1 : kernel); }
+
+/* Up to four tokens rows are streamed (gemv_i8_kernel): 11008 x 4096 at one token 7.4 us, at four 9.6; the split tiles 9.5 at any number up to 16. */
+extern "C" int ckq_launch_i8_kernel(int M, int N, int K)
+{
+    const int forced = g_i8_kernel.load();
+    if (forced >= 0 && (forced != I8_STREAM || M <= 4) && (forced != I8_TWO || i8_whole_columns(M, N) > 0)) return forced;
+    if (M <= 4) return I8_STREAM;
+    int best = 0;
+    float t = 1e30f;
+    for (int i = 0; i < I8_TILINGS; ++i) {
+        const float ti = i8_costs[i].t0 + i8_rounds(i8_costs[i], i8_tiles(i8_costs[i], M, N), K);
+        if (ti < t) { t = ti; best = i; }
+    }
+    const int cols = i8_whole_columns(M, N);
+    if (cols > 0 && 256 * cols < N) {
+        const I8Cost &a = i8_costs[I8_256x256], &b = i8_costs[I8_128x192];
+        if (a.t0 + i8_rounds(a, (long)((M + 255) / 256) * cols, K) + i8_rounds(b, i8_tiles(b, M, N - 256 * cols), K) < t) best = I8_TWO;
+    }
+    return best;
 }
 
 template <class E>
 static int launch_gemm_i8(const I8Args &a, hipStream_t s)
 {
-    const size_t blocks = ((size_t)((a.M + 15) / 16) * (size_t)((a.N + 15) / 16) + 3) / 4;
-    if (blocks > 0x7fffffff) return CKQ_EROWS;
-    hipLaunchKernelGGL(gemm_i8_simple_kernel<E>, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    return (int)hipGetLastError();
+    switch (ckq_launch_i8_kernel(a.M, a.N, a.K)) {
+    case I8_256x256:   return launch_i8_tiles<E, T256x256>(a, s);
+    case I8_256x128:   return launch_i8_tiles<E, T256x128>(a, s);
+    case I8_128x192:   return launch_i8_tiles<E, T128x192>(a, s);
+    case I8_128x128:   return launch_i8_tiles<E, T128x128>(a, s);
+    case I8_128x128_8: return launch_i8_tiles<E, T128x128_8>(a, s);
+    case I8_64x128:    return launch_i8_tiles<E, T64x128>(a, s);
+    case I8_S64x32:    return launch_i8_split<E, S64x32>(a, s);
+    case I8_S32x48:    return launch_i8_split<E, S32x48>(a, s);
+    case I8_S32x32:    return launch_i8_split<E, S32x32>(a, s);
+    case I8_S16x16:    return launch_i8_split<E, S16x16>(a, s);
+    case I8_S16x32:    return launch_i8_split<E, S16x32>(a, s);
+    case I8_TWO:       return launch_i8_two_tiles<E, T256x256, T128x192>(a, i8_whole_columns(a.M, a.N), s);
+    }
+    /* Rows of up to 1 KB are one trip of a wave: four rows a wave, no exchange.  Longer ones are shared by two or four waves of a
+     * block, so that a launch of few rows has all its bytes in flight at once: one token, 4096 x 11008 7.6 us (a wave for four rows 11.4);
+     * but 151936 x 896 20.0 and not 27.7. */
+    if (a.M == 1) return a.K <= 1024 ? launch_i8_stream<E, 1, 4, 1, 1>(a, s) : a.K <= 2048 ? launch_i8_stream<E, 1, 4, 2, 1>(a, s) : launch_i8_stream<E, 1, 4, 2, 2>(a, s);
+    if (a.M == 2) return a.K <= 1024 ? launch_i8_stream<E, 2, 4, 1, 1>(a, s) : launch_i8_stream<E, 2, 4, 1, 4>(a, s);
+    return a.K <= 1024 ? launch_i8_stream<E, 4, 4, 1, 1>(a, s) : launch_i8_stream<E, 4, 4, 1, 4>(a, s);
 }
 
 extern "C" int ckq_launch_gemm_i8(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,
@@ -82,10 +632,15 @@ extern "C" int ckq_launch_gemm_i8(const int8_t *A, long lda, const float *sa, co
     if (!size) return CKQ_EFORMAT;
     if (((uintptr_t)A | (uintptr_t)B) % 16 || lda % 16 || ldb % 16 || lda > CKQ_I8_PITCH_MAX || ldb > CKQ_I8_PITCH_MAX || K > CKQ_I8_K_MAX) return CKQ_EROWS;
     if ((uintptr_t)C % size || ((uintptr_t)sa | (uintptr_t)sb | (uintptr_t)bias) % 4) return CKQ_EROWS;
-    const I8Args a = {A, B, sa, sb, bias, C, lda, ldb, ldc, M, N, K};
-    switch (type) {
-    case CKQ_T_F32:  return launch_gemm_i8<float>(a, (hipStream_t)stream);
-    case CKQ_T_BF16: return launch_gemm_i8<__bf16>(a, (hipStream_t)stream);
-    default:         return launch_gemm_i8<_Float16>(a, (hipStream_t)stream);
-    }
+    /* a launch has fewer than 2^32 threads */
+    constexpr int MOST = 1 << 22;
+    for (int m = 0; m < M; m += min(MOST, M - m))
+        for (int n = 0; n < N; n += min(MOST, N - n)) {
+            const I8Args a = {A + (size_t)m * lda, B + (size_t)n * ldb, sa + m, sb + n, bias ? bias + n : nullptr,
+                              (char *)C + ((size_t)m * ldc + n) * size, lda, ldb, ldc, min(MOST, M - m), min(MOST, N - n), K};
+            const hipStream_t s = (hipStream_t)stream;
+            const int rc = type == CKQ_T_F32 ? launch_gemm_i8<float>(a, s) : type == CKQ_T_BF16 ? launch_gemm_i8<__bf16>(a, s) : launch_gemm_i8<_Float16>(a, s);
+            if (rc) return rc;
+        }
+    return 0;
 }

@@ -308,8 +308,58 @@ def test_matmul_tail_of_k(M):
         matmul_case(M, 37, K, "f32", bias=False, seed=K)
 
 
+# the kernels that a call may be sent to (ckq_launch_i8_kernel), by the tokens and the rows of their tiles
+KERNELS = [(256, 256), (256, 128), (128, 192), (128, 128), (128, 128), (64, 128), (64, 32), (32, 48), (32, 32), (16, 16), (16, 32)]
+TWO, STREAM = 11, 12
+
+
+@pytest.fixture
+def kernel():
+    yield ckq.lib().ckq_launch_set_i8_kernel
+    ckq.lib().ckq_launch_set_i8_kernel(-1)
+
+
+@pytest.mark.parametrize("which", range(len(KERNELS)))
+def test_matmul_every_kernel(kernel, which):
+    bt, bn = KERNELS[which]
+    kernel(which)
+    L = ckq.lib()
+    assert L.ckq_launch_i8_kernel(5, 5, 5) == which
+    for i, (M, N, K) in enumerate([(1, 1, 1), (bt, bn, 128), (bt + 1, bn + 1, 129), (2 * bt - 1, 3 * bn - 5, 300), (3, 9 * bn + 7, 1100), (9 * bt + 3, 5, 700),
+                                   (bt - 1, bn - 1, 127), (2 * bt + 5, 2 * bn + 8, 2048), (17 * bt + 9, 3 * bn, 256)]):
+        matmul_case(M, N, K, list(TYPES)[i % 3], bias=i % 2 == 0, seed=i, pitch_a=i % 3, pitch_b=i % 2, pitch_c=i % 4)
+
+
+@pytest.mark.parametrize("which", range(len(KERNELS)))
+def test_matmul_every_kernel_tail_of_k(kernel, which):
+    kernel(which)
+    for K in list(range(1, 18)) + [31, 33, 47, 63, 64, 65, 111, 112, 113, 127, 128, 129, 143, 145, 255, 256, 257, 383, 384, 385, 400, 511, 512, 513, 640, 641, 895, 1023, 1025, 1151]:
+        matmul_case(5, 37, K, "f32", bias=False, seed=K)
+
+
+@pytest.mark.parametrize("M,N,K", [(4000, 4300, 130), (2048, 8193, 128), (8100, 2100, 200)])
+def test_matmul_two_sizes_of_tiles(kernel, M, N, K):
+    kernel(TWO)
+    assert ckq.lib().ckq_launch_i8_kernel(M, N, K) == TWO
+    matmul_case(M, N, K, "bf16", bias=True)
+
+
+@pytest.mark.parametrize("K", [1, 15, 16, 17, 100, 1008, 1023, 1024, 1025, 1040, 2047, 2048, 2049, 4095, 4097, 6000, 8191, 8193, 11008])
+def test_matmul_rows_streamed(kernel, K):
+    for M in (1, 2, 3, 4):
+        assert ckq.lib().ckq_launch_i8_kernel(M, 100, K) == STREAM
+        for i, N in enumerate((1, 3, 4, 5, 16, 18, 61)):
+            matmul_case(M, N, K, list(TYPES)[i % 3], bias=i % 2 == 0, seed=K + N, pitch_b=i % 2, pitch_c=i % 3)
+
+
 @pytest.mark.parametrize("M", [1, 2, 6, 16, 33, 130, 260])
-def test_matmul_sums_are_exact_to_the_longest_row(M):
+def test_matmul_sums_are_exact_to_the_longest_row(kernel, M):
+    for which in [-1] + list(range(len(KERNELS))) * (M == 6):
+        kernel(which)
+        longest_row(M)
+
+
+def longest_row(M):
     K, N = 131071, 19
     a = torch.full((M, K + 1), -128, dtype=torch.int8, device="cuda")[:, :K]
     b = torch.full((N, K + 1), -128, dtype=torch.int8, device="cuda")[:, :K]
