@@ -203,38 +203,65 @@ def dev_gemm_nt_f32act(fmt, A_t, B_t, bias_t, M, N, K, out=None):
 
 
 # ---- rows of int8 with one scale each ---------------------------------------------
+# A decode step makes these calls one by one, each for a kernel of a few microseconds, so their checks are kept
+# to one look at a tensor's shape, strides, type and device each.
+
+_TYPES = None
+
+
+def _i8_types():
+    """CKDataType value of an element type."""
+    global _TYPES
+    if _TYPES is None:
+        import torch
+        _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    return _TYPES
+
 
 def _i8_type(t):
-    """The CKDataType value of a tensor's or a result's element type."""
-    import torch
-    v = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}.get(t)
+    v = _i8_types().get(t)
     if v is None:
         raise CkqError("rows of %s: float32, bfloat16 or float16 are taken" % t)
     return v
 
 
-def _i8_rows(t, what, rows=None, k=None, dtype=None):
-    """Checks a 2-d tensor of rows on the current device, elements of a row side by side; returns its pitch in elements.  A
-    single row (or none) has any stride in torch: it counts as one that is as long as the row."""
+def _i8_where():
+    """The current device and its current stream (what torch.cuda.current_device and current_stream say, a tenth of their cost);
+    without a device, a number that no tensor's device has."""
     import torch
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (k is not None and t.shape[1] != k):
-        raise CkqError("%s has the shape %s, not %s x %s" % (what, tuple(t.shape), "rows" if rows is None else rows, "k" if k is None else k))
+    if not torch.cuda.is_initialized():
+        if not torch.cuda.is_available():
+            return -2, None
+        torch.cuda.init()
+    dev = torch._C._cuda_getDevice()
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _i8_rows(t, what, dev, shape=None, dtype=None):
+    """Checks a 2-d tensor of rows on device `dev`, elements of a row side by side; returns rows, their length and their pitch in
+    elements.  A single row has any stride in torch: its pitch counts as its length."""
+    s = t.shape
+    if len(s) != 2 or (shape is not None and s != shape):
+        raise CkqError("%s has the shape %s, not %s" % (what, tuple(s), "rows x k" if shape is None else tuple(shape)))
     if dtype is not None and t.dtype != dtype:
         raise CkqError("%s is %s, not %s" % (what, t.dtype, dtype))
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != dev:
         raise CkqError("%s is on %s, not on the current device" % (what, t.device))
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    rows, k = s
+    pitch, step = t.stride()
+    if step != 1 and k > 1:
         raise CkqError("%s: the elements of a row have to lie side by side" % what)
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    return rows, k, pitch if rows > 1 else k
 
 
-def _i8_floats(t, what, n):
-    """A contiguous vector of n floats on the current device."""
+def _i8_floats(t, what, dev, n):
+    """A contiguous vector of n floats on device `dev`: its address."""
     import torch
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise CkqError("%s has to be %d contiguous float32" % (what, n))
-    if not t.is_cuda or t.device.index != torch.cuda.current_device():
+    if t.get_device() != dev:
         raise CkqError("%s is on %s, not on the current device" % (what, t.device))
+    return t.data_ptr()
 
 
 def empty_i8(rows, k, device="cuda"):
@@ -243,69 +270,66 @@ def empty_i8(rows, k, device="cuda"):
     return torch.empty(rows, -(-k // 16) * 16, dtype=torch.int8, device=device)[:, :k]
 
 
-def _i8_out(out, rows, k, device):
+def _i8_out(out, rows, k, x, dev):
     import torch
-    q, scale = out if out is not None else (empty_i8(rows, k, device), torch.empty(rows, dtype=torch.float32, device=device))
-    ldq = _i8_rows(q, "q", rows, k, torch.int8)
-    _i8_floats(scale, "scale", rows)
-    return q, scale, ldq
+    q, scale = out if out is not None else (empty_i8(rows, k, x.device), torch.empty(rows, dtype=torch.float32, device=x.device))
+    ldq = _i8_rows(q, "q", dev, (rows, k), torch.int8)[2]
+    return q, scale, ldq, _i8_floats(scale, "scale", dev, rows)
 
 
 def dev_quantize_i8(x, out=None):
     """Rows of x [rows, k] in 8 bits: (q int8 [rows, k], scale float32 [rows])."""
-    ldx = _i8_rows(x, "x")
-    rows, k = x.shape
-    q, scale, ldq = _i8_out(out, rows, k, x.device)
-    check(lib().ckq_quantize_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr(), rows, k, _stream()),
-          "ckq_quantize_i8_dev")
+    dev, stream = _i8_where()
+    rows, k, ldx = _i8_rows(x, "x", dev)
+    q, scale, ldq, sp = _i8_out(out, rows, k, x, dev)
+    check(lib().ckq_quantize_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, q.data_ptr(), ldq, sp, rows, k, stream), "ckq_quantize_i8_dev")
     return q, scale
 
 
 def dev_dequantize_i8(q, scale, dtype=None, out=None):
     """scale * q as rows of dtype (float32), or into `out`."""
     import torch
-    ldq = _i8_rows(q, "q", dtype=torch.int8)
-    rows, k = q.shape
-    _i8_floats(scale, "scale", rows)
+    dev, stream = _i8_where()
+    rows, k, ldq = _i8_rows(q, "q", dev, None, torch.int8)
+    sp = _i8_floats(scale, "scale", dev, rows)
     y = out if out is not None else torch.empty(rows, k, dtype=dtype or torch.float32, device=q.device)
-    ldy = _i8_rows(y, "out", rows, k, dtype)
-    check(lib().ckq_dequantize_i8_dev(q.data_ptr(), ldq, scale.data_ptr(), _i8_type(y.dtype), y.data_ptr(), ldy, rows, k, _stream()),
-          "ckq_dequantize_i8_dev")
+    ldy = _i8_rows(y, "out", dev, (rows, k), dtype)[2]
+    check(lib().ckq_dequantize_i8_dev(q.data_ptr(), ldq, sp, _i8_type(y.dtype), y.data_ptr(), ldy, rows, k, stream), "ckq_dequantize_i8_dev")
     return y
 
 
 def dev_rmsnorm_i8(x, gamma, eps=1e-6, residual=None, residual_out=None, out=None):
     """RMSNorm(x (+ residual)) * gamma in 8 bits: (q, scale), or (q, scale, x + residual) with a residual; residual_out
     may be the residual itself, or x."""
-    import torch
-    ldx = _i8_rows(x, "x")
-    rows, k = x.shape
-    _i8_floats(gamma, "gamma", k)
-    q, scale, ldq = _i8_out(out, rows, k, x.device)
-    ldr, rp, sp = 0, None, None
+    dev, stream = _i8_where()
+    rows, k, ldx = _i8_rows(x, "x", dev)
+    gp = _i8_floats(gamma, "gamma", dev, k)
+    q, scale, ldq, sp = _i8_out(out, rows, k, x, dev)
+    ldr, rp, op = 0, None, None
     if residual is not None:
+        ldr = _i8_rows(residual, "residual", dev, (rows, k), x.dtype)[2]
         if residual_out is None:
+            import torch
             residual_out = torch.empty_strided(residual.shape, residual.stride(), dtype=x.dtype, device=x.device)
-        ldr = _i8_rows(residual, "residual", rows, k, x.dtype)
-        if _i8_rows(residual_out, "residual_out", rows, k, x.dtype) != ldr:
+        if _i8_rows(residual_out, "residual_out", dev, (rows, k), x.dtype)[2] != ldr:
             raise CkqError("residual and residual_out need one pitch")
-        rp, sp = residual.data_ptr(), residual_out.data_ptr()
+        rp, op = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise CkqError("residual_out without a residual")
-    check(lib().ckq_rmsnorm_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, rp, sp, ldr, gamma.data_ptr(), eps, q.data_ptr(), ldq,
-                                   scale.data_ptr(), rows, k, _stream()), "ckq_rmsnorm_i8_dev")
+    check(lib().ckq_rmsnorm_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, rp, op, ldr, gp, eps, q.data_ptr(), ldq, sp, rows, k, stream),
+          "ckq_rmsnorm_i8_dev")
     return (q, scale) if residual is None else (q, scale, residual_out)
 
 
 def dev_swiglu_i8(gate, up, out=None):
     """SiLU(gate) * up in 8 bits: (q, scale); gate and up have one pitch (halves of one tensor, say)."""
-    ld = _i8_rows(gate, "gate")
-    rows, k = gate.shape
-    if _i8_rows(up, "up", rows, k, gate.dtype) != ld:
+    dev, stream = _i8_where()
+    rows, k, ld = _i8_rows(gate, "gate", dev)
+    if _i8_rows(up, "up", dev, (rows, k), gate.dtype)[2] != ld:
         raise CkqError("gate and up need one pitch")
-    q, scale, ldq = _i8_out(out, rows, k, gate.device)
-    check(lib().ckq_swiglu_i8_dev(_i8_type(gate.dtype), gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), rows, k,
-                                  _stream()), "ckq_swiglu_i8_dev")
+    q, scale, ldq, sp = _i8_out(out, rows, k, gate, dev)
+    check(lib().ckq_swiglu_i8_dev(_i8_type(gate.dtype), gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, sp, rows, k, stream),
+          "ckq_swiglu_i8_dev")
     return q, scale
 
 
@@ -313,22 +337,20 @@ def dev_gemm_nt_i8(a, sa, b, sb, bias=None, dtype=None, out=None):
     """C [M, N] = sa[m] * sb[n] * (a b^T) (+ bias[n]): int8 rows a [M, K] (tokens), b [N, K] (channels); C of dtype (float32),
     or into `out`."""
     import torch
-    lda = _i8_rows(a, "a", dtype=torch.int8)
-    M, K = a.shape
-    ldb = _i8_rows(b, "b", k=K, dtype=torch.int8)
-    N = b.shape[0]
+    dev, stream = _i8_where()
+    M, K, lda = _i8_rows(a, "a", dev, None, torch.int8)
+    N, Kb, ldb = _i8_rows(b, "b", dev, None, torch.int8)
+    if Kb != K:
+        raise CkqError("a and b have rows of %d and %d" % (K, Kb))
     if M == 1:
         lda = -(-K // 16) * 16
     if N == 1:
         ldb = -(-K // 16) * 16
-    _i8_floats(sa, "sa", M)
-    _i8_floats(sb, "sb", N)
-    if bias is not None:
-        _i8_floats(bias, "bias", N)
+    sap, sbp = _i8_floats(sa, "sa", dev, M), _i8_floats(sb, "sb", dev, N)
+    bp = None if bias is None else _i8_floats(bias, "bias", dev, N)
     c = out if out is not None else torch.empty(M, N, dtype=dtype or torch.float32, device=b.device)
-    ldc = _i8_rows(c, "out", M, N, dtype)
-    check(lib().ckq_gemm_nt_i8_dev(a.data_ptr(), lda, sa.data_ptr(), b.data_ptr(), ldb, sb.data_ptr(),
-                                   None if bias is None else bias.data_ptr(), _i8_type(c.dtype), c.data_ptr(), ldc, M, N, K, _stream()),
+    ldc = _i8_rows(c, "out", dev, (M, N), dtype)[2]
+    check(lib().ckq_gemm_nt_i8_dev(a.data_ptr(), lda, sap, b.data_ptr(), ldb, sbp, bp, _i8_type(c.dtype), c.data_ptr(), ldc, M, N, K, stream),
           "ckq_gemm_nt_i8_dev")
     return c
 
