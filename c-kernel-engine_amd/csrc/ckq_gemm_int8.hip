@@ -192,8 +192,9 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
 #pragma unroll
             for (int c = 0; c < NC; ++c) copy(c, st, st);
         }
-    if (S > 2 && niter > 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * NC) : "memory");
-    else                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    /* the first step is here once no more than the S - 2 behind it are in flight, where there are as many */
+    if (S > 2 && niter >= S - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * NC) : "memory");
+    else                         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     if (last == 0 && tail < KS) {
         clear_tail(0);
