@@ -211,11 +211,23 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
         }
 }
 
+/* Waves of a row: as few as leave a thread three vectors (24 elements), so that loads, reduction and stores of several rows share
+ * a CU; where every row has a CU to itself, as many as leave it one.  us with 2 | 4 | 8 | 16 waves a row: norm of 2048 x 4096 in bf16 13.2 |
+ * 11.9 | 13.2 | 15.4, SwiGLU of 2048 x 11008 31.0 | 21.3 | 20.4 | 20.9, quantizer of 11008 x 4096 in fp32 34.1 | 32.1 | 31.8 | 38.0 and of
+ * 11008 x 896 9.3 | 10.2 | 14.9 | 29.3 (one wave 8.7); SwiGLU of 93 x 4863 in fp32 5.1 | 4.3 | 4.2 | 3.7.  Bound by memory beyond a few hundred
+ * rows: 4.9 to 7 TB/s of what is read and written (a copy has 4.8 beyond the caches), and by the latency of one trip below. */
+static int rows_waves(int nvec, int rows)
+{
+    int wpr = 1;
+    while (wpr < 16 && nvec > 64 * wpr * (rows <= 256 ? 1 : 3)) wpr *= 2;
+    return wpr;
+}
+
 template <int OP, class E>
 static int launch_rows(RowsArgs a, hipStream_t s)
 {
     const int nvec = a.k / 8 + (a.k % 8 != 0);
-    const int wpr = nvec <= 64 ? 1 : nvec <= 256 ? 4 : 16, per = (nvec - 1) / (64 * wpr) + 1;
+    const int wpr = rows_waves(nvec, a.rows), per = (nvec - 1) / (64 * wpr) + 1;
     const dim3 block(wpr == 1 ? 256u : 64u * (unsigned)wpr);
     /* a launch has fewer than 2^32 threads */
     for (;;) {
@@ -224,6 +236,7 @@ static int launch_rows(RowsArgs a, hipStream_t s)
         const dim3 grid((unsigned)(wpr == 1 ? (now + 3) / 4 : now));
         if (per <= 1)      hipLaunchKernelGGL((rows_i8_kernel<OP, E, 1>), grid, block, 0, s, a, wpr);
         else if (per <= 2) hipLaunchKernelGGL((rows_i8_kernel<OP, E, 2>), grid, block, 0, s, a, wpr);
+        else if (per <= 4) hipLaunchKernelGGL((rows_i8_kernel<OP, E, 4>), grid, block, 0, s, a, wpr);
         else               hipLaunchKernelGGL((rows_i8_kernel<OP, E, 0>), grid, block, 0, s, a, wpr);
         const int rc = (int)hipGetLastError();
         if (rc || left == now) return rc;
@@ -278,27 +291,30 @@ extern "C" int ckq_launch_swiglu_i8(int type, const void *gate, const void *up, 
     return launch_rows<ROWS_SWIGLU>(type, a, stream);
 }
 
-/* y = T(scale * q), eight elements a thread.  Bound by memory: 1 byte read and the type's written. */
+/* y = T(scale * q), sixteen elements a thread, so that a load is as wide as it can be (eight: 2048 x 4096 to bf16 6.9 us, 5.5 now; 11008 x 4096
+ * 25.0 and 22.2).  Bound by memory: 1 byte read and the type's written, 4.6 to 6.1 TB/s. */
+struct __attribute__((packed, aligned(1))) row16q { u32 v[4]; };
 template <class E>
 __global__ void __launch_bounds__(256) dequantize_i8_kernel(const int8_t *__restrict__ q, long ldq, const float *__restrict__ scale,
                                                             E *__restrict__ y, long ldy, u32 rows, int k, u32 nvec)
 {
-    const size_t t = (size_t)blockIdx.x * 256 + threadIdx.x;
-    if (t >= (size_t)rows * nvec) return;
-    const u32 row = (u32)(t / nvec), v = (u32)(t - (size_t)row * nvec);
-    const int8_t *p = q + (size_t)row * ldq + 8 * (size_t)v;
-    const int left = k - 8 * (int)v;
+    const u32 t = blockIdx.x * 256 + threadIdx.x, row = t / nvec, v = t - row * nvec;      /* fewer than 2^32 threads */
+    if (row >= rows) return;
+    const int8_t *p = q + (size_t)row * ldq + 16 * (size_t)v;
+    E *o = y + (size_t)row * ldy + 16 * (size_t)v;
+    const int left = k - 16 * (int)v;
     const float s = scale[row];
-    float f[8];
-    if (left >= 8) {
-        const row8q r = *reinterpret_cast<const row8q *>(p);
+    float f[2][8];
+    if (left >= 16) {
+        const row16q r = *reinterpret_cast<const row16q *>(p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = s * (float)sbyte(r.v[i >> 2], i & 3);
+        for (int i = 0; i < 16; ++i) f[i >> 3][i & 7] = s * (float)sbyte(r.v[i >> 2], i & 3);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < left ? s * (float)p[i] : 0.0f;
+        for (int i = 0; i < 16; ++i) f[i >> 3][i & 7] = i < left ? s * (float)p[i] : 0.0f;
     }
-    store8(y + (size_t)row * ldy + 8 * (size_t)v, f, left);
+    store8(o, f[0], left);
+    if (left > 8) store8(o + 8, f[1], left - 8);
 }
 
 extern "C" int ckq_launch_dequantize_i8(const int8_t *q, long ldq, const float *scale, int type, void *y, long ldy, int rows, int k, void *stream)
@@ -306,7 +322,7 @@ extern "C" int ckq_launch_dequantize_i8(const int8_t *q, long ldq, const float *
     if (!q || !scale || !y || rows <= 0 || k <= 0 || ldq < k || ldy < k) return CKQ_EINVAL;
     if (!row_size(type)) return CKQ_EFORMAT;
     if ((uintptr_t)y % row_size(type) || (uintptr_t)scale % 4) return CKQ_EROWS;
-    const u32 nvec = (u32)(k / 8 + (k % 8 != 0));
+    const u32 nvec = (u32)(k / 16 + (k % 16 != 0));
     const hipStream_t s = (hipStream_t)stream;
     /* a launch has fewer than 2^32 threads */
     const int most = (int)min((size_t)rows, max((size_t)1, ((size_t)1 << 31) / nvec));

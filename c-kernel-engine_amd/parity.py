@@ -206,20 +206,20 @@ def dev_gemm_nt_f32act(fmt, A_t, B_t, bias_t, M, N, K, out=None):
 # A decode step makes these calls one by one, each for a kernel of a few microseconds, so their checks are kept
 # to one look at a tensor's shape, strides, type and device each.
 
-_TYPES = None
+_torch, _I8_TYPES = None, {}
 
 
-def _i8_types():
-    """CKDataType value of an element type."""
-    global _TYPES
-    if _TYPES is None:
-        import torch
-        _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    return _TYPES
+def _i8_torch():
+    """torch, once: an import statement in each call costs it 0.3 us a time."""
+    global _torch
+    import torch
+    _I8_TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})   # CKDataType values
+    _torch = torch
+    return torch
 
 
 def _i8_type(t):
-    v = _i8_types().get(t)
+    v = _I8_TYPES.get(t)
     if v is None:
         raise CkqError("rows of %s: float32, bfloat16 or float16 are taken" % t)
     return v
@@ -228,7 +228,7 @@ def _i8_type(t):
 def _i8_where():
     """The current device and its current stream (what torch.cuda.current_device and current_stream say, a tenth of their cost);
     without a device, a number that no tensor's device has."""
-    import torch
+    torch = _torch or _i8_torch()
     if not torch.cuda.is_initialized():
         if not torch.cuda.is_available():
             return -2, None
@@ -256,8 +256,7 @@ def _i8_rows(t, what, dev, shape=None, dtype=None):
 
 def _i8_floats(t, what, dev, n):
     """A contiguous vector of n floats on device `dev`: its address."""
-    import torch
-    if t.dtype != torch.float32 or t.shape != (n,) or not t.is_contiguous():
+    if t.dtype is not _torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise CkqError("%s has to be %d contiguous float32" % (what, n))
     if t.get_device() != dev:
         raise CkqError("%s is on %s, not on the current device" % (what, t.device))
@@ -266,14 +265,13 @@ def _i8_floats(t, what, dev, n):
 
 def empty_i8(rows, k, device="cuda"):
     """int8 [rows, k] whose rows begin at multiples of 16 bytes, as dev_gemm_nt_i8 takes them."""
-    import torch
+    torch = _torch or _i8_torch()
     return torch.empty(rows, -(-k // 16) * 16, dtype=torch.int8, device=device)[:, :k]
 
 
 def _i8_out(out, rows, k, x, dev):
-    import torch
-    q, scale = out if out is not None else (empty_i8(rows, k, x.device), torch.empty(rows, dtype=torch.float32, device=x.device))
-    ldq = _i8_rows(q, "q", dev, (rows, k), torch.int8)[2]
+    q, scale = out if out is not None else (empty_i8(rows, k, x.device), _torch.empty(rows, dtype=_torch.float32, device=x.device))
+    ldq = _i8_rows(q, "q", dev, (rows, k), _torch.int8)[2]
     return q, scale, ldq, _i8_floats(scale, "scale", dev, rows)
 
 
@@ -288,11 +286,10 @@ def dev_quantize_i8(x, out=None):
 
 def dev_dequantize_i8(q, scale, dtype=None, out=None):
     """scale * q as rows of dtype (float32), or into `out`."""
-    import torch
     dev, stream = _i8_where()
-    rows, k, ldq = _i8_rows(q, "q", dev, None, torch.int8)
+    rows, k, ldq = _i8_rows(q, "q", dev, None, _torch.int8)
     sp = _i8_floats(scale, "scale", dev, rows)
-    y = out if out is not None else torch.empty(rows, k, dtype=dtype or torch.float32, device=q.device)
+    y = out if out is not None else _torch.empty(rows, k, dtype=dtype or _torch.float32, device=q.device)
     ldy = _i8_rows(y, "out", dev, (rows, k), dtype)[2]
     check(lib().ckq_dequantize_i8_dev(q.data_ptr(), ldq, sp, _i8_type(y.dtype), y.data_ptr(), ldy, rows, k, stream), "ckq_dequantize_i8_dev")
     return y
@@ -309,8 +306,7 @@ def dev_rmsnorm_i8(x, gamma, eps=1e-6, residual=None, residual_out=None, out=Non
     if residual is not None:
         ldr = _i8_rows(residual, "residual", dev, (rows, k), x.dtype)[2]
         if residual_out is None:
-            import torch
-            residual_out = torch.empty_strided(residual.shape, residual.stride(), dtype=x.dtype, device=x.device)
+            residual_out = _torch.empty_strided(residual.shape, residual.stride(), dtype=x.dtype, device=x.device)
         if _i8_rows(residual_out, "residual_out", dev, (rows, k), x.dtype)[2] != ldr:
             raise CkqError("residual and residual_out need one pitch")
         rp, op = residual.data_ptr(), residual_out.data_ptr()
@@ -336,10 +332,9 @@ def dev_swiglu_i8(gate, up, out=None):
 def dev_gemm_nt_i8(a, sa, b, sb, bias=None, dtype=None, out=None):
     """C [M, N] = sa[m] * sb[n] * (a b^T) (+ bias[n]): int8 rows a [M, K] (tokens), b [N, K] (channels); C of dtype (float32),
     or into `out`."""
-    import torch
     dev, stream = _i8_where()
-    M, K, lda = _i8_rows(a, "a", dev, None, torch.int8)
-    N, Kb, ldb = _i8_rows(b, "b", dev, None, torch.int8)
+    M, K, lda = _i8_rows(a, "a", dev, None, _torch.int8)
+    N, Kb, ldb = _i8_rows(b, "b", dev, None, _torch.int8)
     if Kb != K:
         raise CkqError("a and b have rows of %d and %d" % (K, Kb))
     if M == 1:
@@ -348,7 +343,7 @@ def dev_gemm_nt_i8(a, sa, b, sb, bias=None, dtype=None, out=None):
         ldb = -(-K // 16) * 16
     sap, sbp = _i8_floats(sa, "sa", dev, M), _i8_floats(sb, "sb", dev, N)
     bp = None if bias is None else _i8_floats(bias, "bias", dev, N)
-    c = out if out is not None else torch.empty(M, N, dtype=dtype or torch.float32, device=b.device)
+    c = out if out is not None else _torch.empty(M, N, dtype=dtype or _torch.float32, device=b.device)
     ldc = _i8_rows(c, "out", dev, (M, N), dtype)[2]
     check(lib().ckq_gemm_nt_i8_dev(a.data_ptr(), lda, sap, b.data_ptr(), ldb, sbp, bp, _i8_type(c.dtype), c.data_ptr(), ldc, M, N, K, stream),
           "ckq_gemm_nt_i8_dev")
