@@ -310,8 +310,21 @@ __global__ void __launch_bounds__(64 * T::NW) gemm_i8_split_kernel(I8Args a, int
     }
     const int m0 = tt * BT, n0 = nt * BN;
 
-    /* what this thread stores in the end: eight rows of a token; their scales are here by then */
-    constexpr int PER = BN / 8, JOBS = BT * PER, TRIPS = (JOBS + 64 * NW - 1) / (64 * NW);
+    /* what this thread stores in the end, eight rows of a token: their scales and bias are fetched before anything else, or the block would
+     * end with a trip to memory */
+    constexpr int PER = BN / 8, JOBS = BT * PER;
+    static_assert(JOBS <= 64 * NW, "a job a thread");
+    const int row = (int)threadIdx.x / PER, col = 8 * ((int)threadIdx.x % PER), t = m0 + row, n8 = n0 + col, left = a.N - n8;
+    const bool job = (int)threadIdx.x < JOBS && t < a.M && left > 0;
+    float sa = 0.0f, sb[8], bias[8];
+    if (job) {
+        sa = a.sa[t];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            sb[r] = a.sb[n8 + min(r, left - 1)];
+            bias[r] = a.bias ? a.bias[n8 + min(r, left - 1)] : 0.0f;
+        }
+    }
     const ckq_v4i rsa = gemm_buffer((const uint8_t *)a.A + (size_t)m0 * a.lda), rsb = gemm_buffer((const uint8_t *)a.B + (size_t)n0 * a.ldb);
     const u32 mine = (u32)(wave * S * STAGE);
     const int niter = (a.K + KS - 1) / KS, last = niter - 1, tail = a.K - last * KS, steps = wave < niter ? (niter - 1 - wave) / NW + 1 : 0;
@@ -320,14 +333,14 @@ __global__ void __launch_bounds__(64 * T::NW) gemm_i8_split_kernel(I8Args a, int
     const int half8 = lane >> 3;                              /* row of a copy's eight */
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int row = 8 * (i < 2 * TG ? i : i - 2 * TG) + half8, chunk = (lane & 7) ^ ((row >> 1) & 7);
-        ofs[i] = (i < 2 * TG ? (u32)min(row, a.M - 1 - m0) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
+        const int cr = 8 * (i < 2 * TG ? i : i - 2 * TG) + half8, chunk = (lane & 7) ^ ((cr >> 1) & 7);
+        ofs[i] = (i < 2 * TG ? (u32)min(cr, a.M - 1 - m0) * (u32)a.lda : (u32)min(cr, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
     }
     auto copy = [&](int j, int slot) {
         const int it = wave + NW * j;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const int row = 8 * (i < 2 * TG ? i : i - 2 * TG) + half8, chunk = (lane & 7) ^ ((row >> 1) & 7);
+            const int cr = 8 * (i < 2 * TG ? i : i - 2 * TG) + half8, chunk = (lane & 7) ^ ((cr >> 1) & 7);
             const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
             lds_copy16(i < 2 * TG ? rsa : rsb, lds_address(lds) + mine + (u32)(slot * STAGE + 1024 * i), o, it * KS);
         }
@@ -386,33 +399,26 @@ __global__ void __launch_bounds__(64 * T::NW) gemm_i8_split_kernel(I8Args a, int
         for (int n = 0; n < RN; ++n)
             *reinterpret_cast<ckq_v4i *>(red + (16 * i + (lane & 15)) * PITCH + 4 * (16 * n + 4 * (lane >> 4))) = acc[i][n];
     __syncthreads();
+    if (!job) return;
+    ckq_v4i s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
-    for (int trip = 0; trip < TRIPS; ++trip) {
-        const int e = trip * 64 * NW + threadIdx.x, row = e / PER, c = 8 * (e % PER), t = m0 + row, n8 = n0 + c, left = a.N - n8;
-        if (e >= JOBS || t >= a.M || left <= 0) continue;
-        ckq_v4i s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
+    for (int w = 0; w < NW; ++w) {
+        const ckq_v4i *s = reinterpret_cast<const ckq_v4i *>(lds + w * BT * PITCH + row * PITCH + 4 * col);
+        s0 += s[0];
+        s1 += s[1];
+    }
+    i8_out8<E> o;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const ckq_v4i *s = reinterpret_cast<const ckq_v4i *>(lds + w * BT * PITCH + row * PITCH + 4 * c);
-            s0 += s[0];
-            s1 += s[1];
-        }
-        const float sa = a.sa[t];
-        i8_out8<E> o;
+    for (int r = 0; r < 8; ++r) {
+        const float v = i8_scaled(r < 4 ? s0[r] : s1[r - 4], sa, sb[r]);
+        o.v[r] = (E)(a.bias ? v + bias[r] : v);
+    }
+    E *out = (E *)a.C + (size_t)t * a.ldc + n8;
+    if (left >= 8) i8_put(out, o);
+    else {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int n = n8 + min(r, left - 1);
-            float v = i8_scaled(r < 4 ? s0[r] : s1[r - 4], sa, a.sb[n]);
-            if (a.bias) v += a.bias[n];
-            o.v[r] = (E)v;
-        }
-        E *out = (E *)a.C + (size_t)t * a.ldc + n8;
-        if (left >= 8) i8_put(out, o);
-        else {
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (r < left) out[r] = o.v[r];
-        }
+        for (int r = 0; r < 8; ++r)
+            if (r < left) out[r] = o.v[r];
     }
 }
 
@@ -441,6 +447,10 @@ __global__ void __launch_bounds__(256) gemv_i8_kernel(I8Args a)
     for (int r = 0; r < R; ++r) pb[r] = (const uint8_t *)a.B + (size_t)min(n0 + r, a.N - 1) * a.ldb;
 #pragma unroll
     for (int t = 0; t < MT; ++t) pa[t] = (const uint8_t *)a.A + (size_t)min(t, a.M - 1) * a.lda;
+    /* lane r + R t has row r of token t in the end; its scales and bias come first, or the wave would end with a trip to memory */
+    const int n = n0 + lane % R, tok = lane / R;
+    const bool job = lane < R * MT && tok < a.M && n < a.N;
+    const float sa = a.sa[job ? tok : 0], sb = a.sb[job ? n : 0], bias = a.bias ? a.bias[job ? n : 0] : 0.0f;
     int acc[R][MT];
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -501,18 +511,14 @@ __global__ void __launch_bounds__(256) gemv_i8_kernel(I8Args a)
 #pragma unroll
                 for (int w = 1; w < KS; ++w) acc[r][t] += red[((wave + w) * R + r) * MT + t];
     }
-    /* lane r + R t has row r of token t */
     int sum = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int t = 0; t < MT; ++t) sum = lane == r + R * t ? acc[r][t] : sum;
-    const int r = lane % R, t = lane / R, n = n0 + r;
-    if (lane < R * MT && t < a.M && n < a.N) {
-        float v = i8_scaled(sum, a.sa[t], a.sb[n]);
-        if (a.bias) v += a.bias[n];
-        ((E *)a.C)[(size_t)t * a.ldc + n] = (E)v;
-    }
+    if (!job) return;
+    const float v = i8_scaled(sum, sa, sb);
+    ((E *)a.C)[(size_t)tok * a.ldc + n] = (E)(a.bias ? v + bias : v);
 }
 
 template <class E, int MT, int R, int KU, int KS>
@@ -528,8 +534,7 @@ static int launch_i8_stream(const I8Args &a, hipStream_t s)
 typedef I8Tile<2, 4, 4, 2, 2, 2, 3> T256x256;
 typedef I8Tile<4, 2, 2, 2, 3, 4, 2> T256x128;
 typedef I8Tile<4, 2, 1, 3, 3, 4, 2> T128x192;
-typedef I8Tile<2, 2, 2, 2, 2, 2, 2> T128x128;        /* two blocks a CU */
-typedef I8Tile<4, 2, 1, 2, 4, 4, 2> T128x128_8;
+typedef I8Tile<4, 2, 1, 2, 4, 4, 2> T128x128;
 typedef I8Tile<2, 4, 1, 1, 5, 4, 1> T64x128;
 typedef I8Split<4, 2, 4, 2> S64x32;
 typedef I8Split<4, 3, 2, 2> S32x48;                   /* two blocks a CU */
@@ -537,34 +542,34 @@ typedef I8Split<4, 2, 2, 2> S32x32;                   /* two */
 typedef I8Split<8, 1, 1, 2> S16x16;                   /* two */
 typedef I8Split<4, 2, 1, 2> S16x32;                   /* three */
 
-enum { I8_256x256, I8_256x128, I8_128x192, I8_128x128, I8_128x128_8, I8_64x128, I8_S64x32, I8_S32x48, I8_S32x32, I8_S16x16, I8_S16x32, I8_TILINGS,
+enum { I8_256x256, I8_256x128, I8_128x192, I8_128x128, I8_64x128, I8_S64x32, I8_S32x48, I8_S32x32, I8_S16x16, I8_S16x32, I8_TILINGS,
        I8_TWO = I8_TILINGS, I8_STREAM };
 
-/* What a launch takes, in us: t0, and for every round of blocks t_tile and, for each of its steps of K, s0 + s1 * (the part of
- * the round's places that have a block: CUs that share the L2s and the power are slower).  Fitted to some hundred sizes of 5 to 2048
- * tokens (64 to 32000 rows, K 64 to 11008) as measured on one box: each within 5 to 11 % (rms); the kernel so chosen is 2 %
- * slower than the best of all on average, 1.27 times at worst. */
-struct I8Cost { int bt, bn, places, split; float t0, t_tile, s0, s1; };
+/* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all
+ * places have a block; a last round of fewer steps faster, for the most part by how many blocks share a CU, a fifth by how many there
+ * are in all (L2, power).  Fitted to 239 sizes of 5 to 2048 tokens (64 to 32000 rows, K 64 to 11008; operands from the 256 MB cache, as three
+ * sets in turn leave them), each kernel within 4 to 9 % (rms); the kernel so chosen is 0.9 % slower than the best of all on average, 1.20
+ * times at worst.  Without one of them: 1.1 to 2.6 % on average, 1.2 to 1.5 times at worst. */
+struct I8Cost { int bt, bn, places, split; float t0, t_tile, step; };
 static const I8Cost i8_costs[I8_TILINGS] = {
-    {256, 256, 256, 1, 2.00f, 5.94f, 1.063f, 0.497f},
-    {256, 128, 256, 1, 2.00f, 4.11f, 0.601f, 0.271f},
-    {128, 192, 256, 1, 2.00f, 3.47f, 0.524f, 0.232f},
-    {128, 128, 512, 1, 2.00f, 3.59f, 0.473f, 0.606f},
-    {128, 128, 256, 1, 2.00f, 2.65f, 0.441f, 0.143f},
-    {64, 128, 256, 1, 2.00f, 1.86f, 0.330f, 0.084f},
-    {64, 32, 256, 4, 2.00f, 1.62f, 0.359f, 0.191f},
-    {32, 48, 512, 4, 2.07f, 1.45f, 0.280f, 0.601f},
-    {32, 32, 512, 4, 2.14f, 1.31f, 0.207f, 0.459f},
-    {16, 16, 512, 8, 2.25f, 1.22f, 0.217f, 0.385f},
-    {16, 32, 768, 4, 2.23f, 1.14f, 0.214f, 0.508f},
+    {256, 256, 256, 1, 1.50f, 7.74f, 1.452f},
+    {256, 128, 256, 1, 1.50f, 4.90f, 0.850f},
+    {128, 192, 256, 1, 1.50f, 4.08f, 0.740f},
+    {128, 128, 256, 1, 1.50f, 3.16f, 0.587f},
+    {64, 128, 256, 1, 1.50f, 2.32f, 0.441f},
+    {64, 32, 256, 4, 1.77f, 1.62f, 0.546f},
+    {32, 48, 512, 4, 2.27f, 1.06f, 0.941f},
+    {32, 32, 512, 4, 2.44f, 0.90f, 0.708f},
+    {16, 16, 512, 8, 2.44f, 1.05f, 0.552f},
+    {16, 32, 768, 4, 2.82f, 0.60f, 0.810f},
 };
 
 static float i8_rounds(const I8Cost &c, long tiles, int K)
 {
-    const int steps = ((K + 127) / 128 + c.split - 1) / c.split;
+    const int steps = ((K + 127) / 128 + c.split - 1) / c.split, share = c.places / 256;      /* blocks that share a CU */
     const long full = tiles / c.places, rest = tiles % c.places;
-    float t = (float)full * (c.t_tile + (float)steps * (c.s0 + c.s1));
-    if (rest) t += c.t_tile + (float)steps * (c.s0 + c.s1 * (float)rest / (float)c.places);
+    float t = (float)full * (c.t_tile + (float)steps * c.step);
+    if (rest) t += c.t_tile + (float)steps * c.step * (0.2f * (float)rest / (float)c.places + 0.8f * (float)((rest + 255) / 256) / (float)share);
     return t;
 }
 static long i8_tiles(const I8Cost &c, int M, int N) { return (long)((M + c.bt - 1) / c.bt) * ((N + c.bn - 1) / c.bn); }
@@ -608,7 +613,6 @@ static int launch_gemm_i8(const I8Args &a, hipStream_t s)
     case I8_256x128:   return launch_i8_tiles<E, T256x128>(a, s);
     case I8_128x192:   return launch_i8_tiles<E, T128x192>(a, s);
     case I8_128x128:   return launch_i8_tiles<E, T128x128>(a, s);
-    case I8_128x128_8: return launch_i8_tiles<E, T128x128_8>(a, s);
     case I8_64x128:    return launch_i8_tiles<E, T64x128>(a, s);
     case I8_S64x32:    return launch_i8_split<E, S64x32>(a, s);
     case I8_S32x48:    return launch_i8_split<E, S32x48>(a, s);
@@ -617,12 +621,15 @@ static int launch_gemm_i8(const I8Args &a, hipStream_t s)
     case I8_S16x32:    return launch_i8_split<E, S16x32>(a, s);
     case I8_TWO:       return launch_i8_two_tiles<E, T256x256, T128x192>(a, i8_whole_columns(a.M, a.N), s);
     }
-    /* Rows of up to 1 KB are one trip of a wave: four rows a wave, no exchange.  Longer ones are shared by two or four waves of a
-     * block, so that a launch of few rows has all its bytes in flight at once: one token, 4096 x 11008 7.6 us (a wave for four rows 11.4);
-     * but 151936 x 896 20.0 and not 27.7. */
-    if (a.M == 1) return a.K <= 1024 ? launch_i8_stream<E, 1, 4, 1, 1>(a, s) : a.K <= 2048 ? launch_i8_stream<E, 1, 4, 2, 1>(a, s) : launch_i8_stream<E, 1, 4, 2, 2>(a, s);
-    if (a.M == 2) return a.K <= 1024 ? launch_i8_stream<E, 2, 4, 1, 1>(a, s) : launch_i8_stream<E, 2, 4, 1, 4>(a, s);
-    return a.K <= 1024 ? launch_i8_stream<E, 4, 4, 1, 1>(a, s) : launch_i8_stream<E, 4, 4, 1, 4>(a, s);
+    /* Rows of up to 1 KB are one trip of a wave: four rows a wave, no exchange.  Longer ones are shared by the waves of a block, so that
+     * a launch has its bytes in flight at once however few rows it has.  us at one token, rows x K, (rows a wave, KB a trip, waves of a
+     * row) 4, 1, 1 | 4, 1, 2 | 2, 2, 4 | 2, 4, 4: 151936 x 896 20.6 | 20.2 | 46 | 67, 32000 x 2048 12.1 | 10.9 | 11.0 | 11.6, 11008 x 4096 10.7 | 8.8 |
+     * 7.8 | 8.4, 4096 x 11008 11.2 | 10.3 | 8.8 | 8.6. */
+    const int kb = (a.K + 1023) / 1024;
+    if (a.M == 1) return kb <= 1 ? launch_i8_stream<E, 1, 4, 1, 1>(a, s) : kb <= 2 ? launch_i8_stream<E, 1, 4, 1, 2>(a, s)
+                       : kb <= 8 ? launch_i8_stream<E, 1, 2, 2, 4>(a, s) : launch_i8_stream<E, 1, 2, 4, 4>(a, s);
+    if (a.M == 2) return kb <= 1 ? launch_i8_stream<E, 2, 4, 1, 1>(a, s) : launch_i8_stream<E, 2, 2, 2, 4>(a, s);
+    return kb <= 1 ? launch_i8_stream<E, 4, 4, 1, 1>(a, s) : launch_i8_stream<E, 4, 4, 1, 4>(a, s);
 }
 
 extern "C" int ckq_launch_gemm_i8(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,

@@ -309,8 +309,8 @@ def test_matmul_tail_of_k(M):
 
 
 # the kernels that a call may be sent to (ckq_launch_i8_kernel), by the tokens and the rows of their tiles
-KERNELS = [(256, 256), (256, 128), (128, 192), (128, 128), (128, 128), (64, 128), (64, 32), (32, 48), (32, 32), (16, 16), (16, 32)]
-TWO, STREAM = 11, 12
+KERNELS = [(256, 256), (256, 128), (128, 192), (128, 128), (64, 128), (64, 32), (32, 48), (32, 32), (16, 16), (16, 32)]
+TWO, STREAM = 10, 11
 
 
 @pytest.fixture
