@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(64 * T::NW) gemm_i8_split_kernel(I8Args a, int
 #pragma unroll
                 for (int n = 0; n < RN; ++n) acc[i][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fb[n], fa[i], acc[i][n], 0, 0, 0);
         }
-        asm volatile("" ::: "memory");                        /* the next copies into this slot come after its reads, which the multiplications have waited for */
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    /* the next copies into this slot come after its reads */
         slot = slot + 1 == S ? 0 : slot + 1;
     }
 

@@ -280,7 +280,9 @@ def dev_quantize_i8(x, out=None):
     dev, stream = _i8_where()
     rows, k, ldx = _i8_rows(x, "x", dev)
     q, scale, ldq, sp = _i8_out(out, rows, k, x, dev)
-    check(lib().ckq_quantize_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, q.data_ptr(), ldq, sp, rows, k, stream), "ckq_quantize_i8_dev")
+    rc = lib().ckq_quantize_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, q.data_ptr(), ldq, sp, rows, k, stream)
+    if rc:
+        check(rc, "ckq_quantize_i8_dev")
     return q, scale
 
 
@@ -291,7 +293,9 @@ def dev_dequantize_i8(q, scale, dtype=None, out=None):
     sp = _i8_floats(scale, "scale", dev, rows)
     y = out if out is not None else _torch.empty(rows, k, dtype=dtype or _torch.float32, device=q.device)
     ldy = _i8_rows(y, "out", dev, (rows, k), dtype)[2]
-    check(lib().ckq_dequantize_i8_dev(q.data_ptr(), ldq, sp, _i8_type(y.dtype), y.data_ptr(), ldy, rows, k, stream), "ckq_dequantize_i8_dev")
+    rc = lib().ckq_dequantize_i8_dev(q.data_ptr(), ldq, sp, _i8_type(y.dtype), y.data_ptr(), ldy, rows, k, stream)
+    if rc:
+        check(rc, "ckq_dequantize_i8_dev")
     return y
 
 
@@ -312,8 +316,9 @@ def dev_rmsnorm_i8(x, gamma, eps=1e-6, residual=None, residual_out=None, out=Non
         rp, op = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise CkqError("residual_out without a residual")
-    check(lib().ckq_rmsnorm_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, rp, op, ldr, gp, eps, q.data_ptr(), ldq, sp, rows, k, stream),
-          "ckq_rmsnorm_i8_dev")
+    rc = lib().ckq_rmsnorm_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, rp, op, ldr, gp, eps, q.data_ptr(), ldq, sp, rows, k, stream)
+    if rc:
+        check(rc, "ckq_rmsnorm_i8_dev")
     return (q, scale) if residual is None else (q, scale, residual_out)
 
 
@@ -324,8 +329,9 @@ def dev_swiglu_i8(gate, up, out=None):
     if _i8_rows(up, "up", dev, (rows, k), gate.dtype)[2] != ld:
         raise CkqError("gate and up need one pitch")
     q, scale, ldq, sp = _i8_out(out, rows, k, gate, dev)
-    check(lib().ckq_swiglu_i8_dev(_i8_type(gate.dtype), gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, sp, rows, k, stream),
-          "ckq_swiglu_i8_dev")
+    rc = lib().ckq_swiglu_i8_dev(_i8_type(gate.dtype), gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, sp, rows, k, stream)
+    if rc:
+        check(rc, "ckq_swiglu_i8_dev")
     return q, scale
 
 
@@ -345,8 +351,9 @@ def dev_gemm_nt_i8(a, sa, b, sb, bias=None, dtype=None, out=None):
     bp = None if bias is None else _i8_floats(bias, "bias", dev, N)
     c = out if out is not None else _torch.empty(M, N, dtype=dtype or _torch.float32, device=b.device)
     ldc = _i8_rows(c, "out", dev, (M, N), dtype)[2]
-    check(lib().ckq_gemm_nt_i8_dev(a.data_ptr(), lda, sap, b.data_ptr(), ldb, sbp, bp, _i8_type(c.dtype), c.data_ptr(), ldc, M, N, K, stream),
-          "ckq_gemm_nt_i8_dev")
+    rc = lib().ckq_gemm_nt_i8_dev(a.data_ptr(), lda, sap, b.data_ptr(), ldb, sbp, bp, _i8_type(c.dtype), c.data_ptr(), ldc, M, N, K, stream)
+    if rc:
+        check(rc, "ckq_gemm_nt_i8_dev")
     return c
 
 

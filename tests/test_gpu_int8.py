@@ -260,14 +260,20 @@ def test_swiglu_far_gates():
 # ---- matmul ------------------------------------------------------------------------------------
 
 def check_matmul(c, a, sa, b, sb, bias):
-    """The sum is exact; it is converted, scaled twice, the bias added (U each) and the result rounded to its type."""
+    """The sum is exact; it is converted, scaled twice, the bias added (U each) and the result rounded to its type: to an infinity
+    from half a step beyond the type's largest value on (65520 in half precision, whose last step is 32)."""
     T = c.dtype
     p = (a.double() @ b.double().t()) * sa.double()[:, None] * sb.double()
     want = p if bias is None else p + bias.double()
     got = c.double()
     tol = 3 * U * 1.01 * p.abs() + (U + half_step(T)) * 1.01 * (want.abs() + 3 * U * p.abs()) + (2.0 ** -25 if T == torch.float16 else 0)
     off = (got - want).abs()
-    assert (off <= tol).all(), (off / tol.clamp_min(1e-30)).max().item()
+    top = torch.finfo(T).max * (1 + half_step(T) / 2)
+    beyond = want.abs() - 4 * U * p.abs() - 4 * U * want.abs() >= top
+    near = want.abs() + 4 * U * p.abs() + 4 * U * want.abs() >= top
+    assert (got[beyond] == torch.sign(want[beyond]) * float("inf")).all()
+    fine = (off <= tol) | beyond | (near & got.isinf())
+    assert fine.all(), (off / tol.clamp_min(1e-30)).max().item()
 
 
 def matmul_case(M, N, K, t, bias, seed=1, pitch_a=0, pitch_b=0, pitch_c=0):
@@ -396,6 +402,55 @@ def test_matmul_unaligned_results():
             out = pitched(torch.zeros(M, N).to(t), 1, 1)
             P.dev_gemm_nt_i8(a, sa, b, sb, out=out)
             assert torch.equal(out, P.dev_gemm_nt_i8(a, sa, b, sb, dtype=t))
+
+
+def test_launches_in_parts():
+    """More rows than one launch has (2^22 of a matmul, 2^21 of the producers)."""
+    a, b = codes(2, 16, 1), codes((1 << 22) + 37, 16, 2)
+    sa, sb, bias = torch.rand(2, device="cuda"), torch.rand(b.shape[0], device="cuda"), torch.rand(b.shape[0], device="cuda")
+    check_matmul(P.dev_gemm_nt_i8(a[:1], sa[:1], b, sb, bias), a[:1], sa[:1], b, sb, bias)
+    c = P.dev_gemm_nt_i8(b, sb, a, sa, dtype=torch.float16)
+    check_matmul(c, b, sb, a, sa, None)
+    x = torch.randn((1 << 21) + 3, 9, device="cuda")
+    q, s = P.dev_quantize_i8(x)
+    for part in (slice(0, 50), slice((1 << 21) - 7, None)):
+        q2, s2 = P.dev_quantize_i8(x[part].contiguous())
+        assert torch.equal(q[part], q2) and torch.equal(s[part], s2)
+    res = torch.ones_like(x)
+    qn, sn, h = P.dev_rmsnorm_i8(x, torch.ones(9, device="cuda"), residual=res)
+    q2, s2, h2 = P.dev_rmsnorm_i8(x[-9:].contiguous(), torch.ones(9, device="cuda"), residual=res[-9:].contiguous())
+    assert torch.equal(qn[-9:], q2) and torch.equal(sn[-9:], s2) and torch.equal(h, x + res) and torch.equal(h[-9:], h2)
+
+
+def test_offsets_beyond_32_bits():
+    """Rows whose distance from the first does not fit in 32 bits of elements."""
+    far = (1 << 30) + 24
+    x = torch.empty(4 * far, dtype=torch.float16, device="cuda").as_strided((5, 100), (far - 100, 1))
+    x.copy_(normal(5, 100, 1).half())
+    q = torch.empty(4 * far, dtype=torch.int8, device="cuda").as_strided((5, 100), (far - 100, 1))
+    q, s = P.dev_quantize_i8(x, out=(q, torch.empty(5, device="cuda")))
+    q2, s2 = P.dev_quantize_i8(x.contiguous())
+    assert torch.equal(q, q2) and torch.equal(s, s2)
+    y = P.dev_dequantize_i8(q, s, out=x)
+    assert torch.equal(y.contiguous(), P.dev_dequantize_i8(q2, s2, dtype=torch.float16))
+    r = P.dev_rmsnorm_i8(x, torch.ones(100, device="cuda"), residual=x, residual_out=x)
+    r2 = P.dev_rmsnorm_i8(y2 := P.dev_dequantize_i8(q2, s2, dtype=torch.float16), torch.ones(100, device="cuda"), residual=y2)
+    assert all(torch.equal(u.contiguous(), v) for u, v in zip(r, r2))
+    del x, q, y, r
+    pitch = 1 << 22                                           # the longest that a matmul's operands may have
+    big = torch.empty(1100 * pitch, dtype=torch.int8, device="cuda")
+    a = big.as_strided((1100, 200), (pitch, 1))
+    a.copy_(codes(1100, 200, 3))
+    b, sa, sb = codes(70, 200, 4), torch.rand(1100, device="cuda"), torch.rand(70, device="cuda")
+    check_matmul(P.dev_gemm_nt_i8(a, sa, b, sb), a, sa, b, sb, None)
+    check_matmul(P.dev_gemm_nt_i8(b, sb, a, sa), b, sb, a, sa, None)
+    check_matmul(P.dev_gemm_nt_i8(b[:3], sb[:3], a, sa), b[:3], sb[:3], a, sa, None)
+    out = torch.empty(3 * far, dtype=torch.float16, device="cuda").as_strided((4, 1100), (far - 1100, 1))
+    for rows in (1, 4):
+        P.dev_gemm_nt_i8(b[:rows], sb[:rows], a, sa, out=out[:rows])
+        check_matmul(out[:rows], b[:rows], sb[:rows], a, sa, None)
+    P.dev_gemm_nt_i8(codes(4, 200, 9), sb[:4], a, sa, out=out)
+    check_matmul(out, codes(4, 200, 9), sb[:4], a, sa, None)
 
 
 def test_front_ends_refuse_on_the_device():
