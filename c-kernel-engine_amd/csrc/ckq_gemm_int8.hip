@@ -1,17 +1,27 @@
 /*
  * ckq_gemm_int8.hip - matrix product of int8 rows with one scale each (one a token, one a channel):
  *
- *   C[m][n] = T((sa[m] * sb[n]) * (float) sum_k A[m][k] B[n][k]  (+ bias[n]))
+ *   C[m][n] = T((sa[m] * (float) sum_k A[m][k] B[n][k]) * sb[n]  (+ bias[n]))
  *
- * The sum is exact in int32 for k <= 131071 (128 * 128 * k < 2^31), so no order of it, and no split, changes a bit.
+ * The sum is exact in int32 for k <= 131071 (128 * 128 * k < 2^31), so no order of it, and no split, changes a bit, and what follows it
+ * is the same few fp32 operations everywhere: a token's results have the same bits whichever kernel computes them, alone or
+ * among thousands.
+ *
+ * Three forms:
+ * - gemm_i8_stream_kernel, up to four tokens: rows streamed once, v_dot4_i32_i8.  Bound by memory: 11008 x 4096 at one token 7.8 us,
+ *   5.8 TB/s; a kernel that only reads those bytes takes 7.3.
+ * - gemm_i8_split_kernel, a few to some hundred tokens: small tiles, K split among the waves of a block, which exchange their sums once.
+ *   Bound by memory where rows are read once (13 x 4096 x 11008 9.5 us, 4.8 TB/s), beyond by what a CU can load, some 55 bytes a cycle (both
+ *   operands of every tile: 333 x 1001 x 4847, 231 tiles, 390 KB a CU).
+ * - gemm_i8_tile_kernel, tiles of 64 x 128 to 256 x 256 on all waves of a block, v_mfma_i32_32x32x32_i8.  The largest are bound by the matrix
+ *   cores at the clock that the power limit leaves them (8192 x 8192 x 8192: 2430 TOPS, matrix cores busy in 71 % of the cycles at
+ *   1.6 GHz; the published 5 POP/s are at 2.4), the smaller ones by the loads of a CU: a step of 128 x 128 has 512 cycles of
+ *   multiplications and 32 KB, 600 cycles.
+ * All operands reach the matrix cores through LDS: 16 rows x 64 bytes an instruction, as the matrix cores want them in registers, load at 16 bytes a
+ * cycle and CU; whole lines at 55.
  */
 #include "ckq_gemm_common.hpp"
 #include <atomic>
-
-template <int T> struct I8Out;
-template <> struct I8Out<CKQ_T_F32>  { typedef float type; };
-template <> struct I8Out<CKQ_T_BF16> { typedef __bf16 type; };
-template <> struct I8Out<CKQ_T_F16>  { typedef _Float16 type; };
 
 struct I8Args {
     const int8_t *A, *B;
@@ -21,7 +31,13 @@ struct I8Args {
     int           M, N, K;
 };
 
-__device__ __forceinline__ float i8_scaled(int sum, float sa, float sb) { return (sa * (float)sum) * sb; }
+/* Uncontracted, so that every kernel has the same bits. */
+__device__ __forceinline__ float i8_result(int sum, float sa, float sb, bool with_bias, float bias)
+{
+#pragma clang fp contract(off)
+    const float v = (sa * (float)sum) * sb;
+    return with_bias ? v + bias : v;
+}
 
 /* ---- tiles through LDS ---------------------------------------------------------------------------------------------- */
 
@@ -61,16 +77,9 @@ __device__ __forceinline__ void i8_store_rows(const I8Args &a, const uint8_t *su
         const int e = e0 + lane, row = e / PER, c = 8 * (e % PER), t = t0 + row, n8 = n + c, left = a.N - n8;
         const ckq_v4i *s = reinterpret_cast<const ckq_v4i *>(sums + row * pitch + 4 * c);
         const ckq_v4f *fb = reinterpret_cast<const ckq_v4f *>(sb + c), *fc = reinterpret_cast<const ckq_v4f *>(bias + c);
-        float v[8];
-#pragma unroll
-        for (int r = 0; r < 8; ++r) v[r] = i8_scaled(s[r >> 2][r & 3], sa[row], fb[r >> 2][r & 3]);
-        if (a.bias) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r) v[r] += fc[r >> 2][r & 3];
-        }
         i8_out8<E> o;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) o.v[r] = (E)v[r];
+        for (int r = 0; r < 8; ++r) o.v[r] = (E)i8_result(s[r >> 2][r & 3], sa[row], fb[r >> 2][r & 3], a.bias != nullptr, fc[r >> 2][r & 3]);
         if (t >= a.M || left <= 0) continue;
         E *out = (E *)a.C + (size_t)t * a.ldc + n8;
         if (left >= 8) i8_put(out, o);
@@ -409,10 +418,7 @@ __global__ void __launch_bounds__(64 * T::NW) gemm_i8_split_kernel(I8Args a, int
     }
     i8_out8<E> o;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) {
-        const float v = i8_scaled(r < 4 ? s0[r] : s1[r - 4], sa, sb[r]);
-        o.v[r] = (E)(a.bias ? v + bias[r] : v);
-    }
+    for (int r = 0; r < 8; ++r) o.v[r] = (E)i8_result(r < 4 ? s0[r] : s1[r - 4], sa, sb[r], a.bias != nullptr, bias[r]);
     E *out = (E *)a.C + (size_t)t * a.ldc + n8;
     if (left >= 8) i8_put(out, o);
     else {
@@ -433,9 +439,11 @@ static int launch_i8_split(const I8Args &a, hipStream_t s)
 
 /* ---- few tokens: rows streamed ----------------------------------------------------------------------------------------- */
 
-/* MT tokens; a wave has R rows and every KS-th piece of KU KB of K; 4 waves a block. */
+/* MT tokens; a wave has R rows and every KS-th piece of KU KB of K; 4 waves a block.  Rows are loaded non-temporally: a decode step goes through
+ * more weights than any cache holds (nine matrices of 11008 x 4096 in turn 8.45 us each and 8.93 otherwise, 4096 x 11008 9.0 and 9.6; three, which fit the
+ * 256 MB cache, 8.25 and 8.03). */
 template <class E, int MT, int R, int KU, int KS>
-__global__ void __launch_bounds__(256) gemv_i8_kernel(I8Args a)
+__global__ void __launch_bounds__(256) gemm_i8_stream_kernel(I8Args a)
 {
     constexpr int G = 4 / KS;
     __shared__ int red[KS > 1 ? 4 * R * MT : 1];
@@ -517,25 +525,31 @@ __global__ void __launch_bounds__(256) gemv_i8_kernel(I8Args a)
 #pragma unroll
         for (int t = 0; t < MT; ++t) sum = lane == r + R * t ? acc[r][t] : sum;
     if (!job) return;
-    const float v = i8_scaled(sum, sa, sb);
-    ((E *)a.C)[(size_t)tok * a.ldc + n] = (E)(a.bias ? v + bias : v);
+    ((E *)a.C)[(size_t)tok * a.ldc + n] = (E)i8_result(sum, sa, sb, a.bias != nullptr, bias);
 }
 
 template <class E, int MT, int R, int KU, int KS>
 static int launch_i8_stream(const I8Args &a, hipStream_t s)
 {
     constexpr int per = 4 / KS * R;
-    hipLaunchKernelGGL((gemv_i8_kernel<E, MT, R, KU, KS>), dim3((unsigned)((a.N + per - 1) / per)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((gemm_i8_stream_kernel<E, MT, R, KU, KS>), dim3((unsigned)((a.N + per - 1) / per)), dim3(256), 0, s, a);
     return (int)hipGetLastError();
 }
 
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */
 
+/* Waves, stages and the places of reads and copies as measured, us.  256 x 256, 8192 x 8192 x 8192: copies over the first half of a step 453,
+ * all at its start 463, over three quarters 466, over all of it 471; four waves of 128 x 128 each 470 to 590.  128 x 128, 1024 x 4096 x 4096: three stages,
+ * reads behind the first multiplication 22.3, four stages 22.6, reads spread 23.0, four waves 22.7.  128 x 192, 512 x 11008 x 4096: 27.2 to 28.0 for any place, two
+ * stages or four waves 29 and more.  64 x 128, 125 x 11008 x 4096: four stages 14.7, five 14.8, six 15.9. */
 typedef I8Tile<2, 4, 4, 2, 2, 2, 3> T256x256;
 typedef I8Tile<4, 2, 2, 2, 3, 4, 2> T256x128;
 typedef I8Tile<4, 2, 1, 3, 3, 4, 2> T128x192;
-typedef I8Tile<4, 2, 1, 2, 4, 4, 2> T128x128;
-typedef I8Tile<2, 4, 1, 1, 5, 4, 1> T64x128;
+typedef I8Tile<4, 2, 1, 2, 3, 4, 1> T128x128;
+typedef I8Tile<2, 4, 1, 1, 4, 4, 1> T64x128;
+/* Split tiles.  13 x 4096 x 11008: 16 x 16 of eight waves, two stages 10.0, three 10.3, four 10.4; of sixteen 10.5, of four with four stages 10.4; 16 x 32 of four
+ * 11.0.  13 x 22016 x 4096: 16 x 32 of four waves, two stages 16.1 (three blocks share a CU), three 17.4, four 19; 16 x 16 19.0.  333 x 1001 x 4847: 32 x 48 of
+ * four waves, two stages 9.1, three 9.5, of eight 9.1; 32 x 64 10.1. */
 typedef I8Split<4, 2, 4, 2> S64x32;
 typedef I8Split<4, 3, 2, 2> S32x48;                   /* two blocks a CU */
 typedef I8Split<4, 2, 2, 2> S32x32;                   /* two */
@@ -548,8 +562,8 @@ enum { I8_256x256, I8_256x128, I8_128x192, I8_128x128, I8_64x128, I8_S64x32, I8_
 /* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all
  * places have a block; a last round of fewer steps faster, for the most part by how many blocks share a CU, a fifth by how many there
  * are in all (L2, power).  Fitted to 239 sizes of 5 to 2048 tokens (64 to 32000 rows, K 64 to 11008; operands from the 256 MB cache, as three
- * sets in turn leave them), each kernel within 4 to 9 % (rms); the kernel so chosen is 0.9 % slower than the best of all on average, 1.20
- * times at worst.  Without one of them: 1.1 to 2.6 % on average, 1.2 to 1.5 times at worst. */
+ * sets in turn leave them), each kernel within 4 to 9 % (rms).  On 271 other sizes the kernel so chosen is 0.6 % slower than the best of all on average,
+ * 1.26 times at worst; without one of them 0.8 to 3.2 % on average (without 64 x 32: 0.6, but 1.31 times at worst). */
 struct I8Cost { int bt, bn, places, split; float t0, t_tile, step; };
 static const I8Cost i8_costs[I8_TILINGS] = {
     {256, 256, 256, 1, 1.50f, 7.74f, 1.452f},
@@ -585,7 +599,7 @@ static int i8_whole_columns(int M, int N)
 static std::atomic<int> g_i8_kernel{-1};
 extern "C" void ckq_launch_set_i8_kernel(int kernel) { g_i8_kernel.store(kernel < 0 || kernel > I8_STREAM ? -1 : kernel); }
 
-/* Up to four tokens rows are streamed (gemv_i8_kernel): 11008 x 4096 at one token 7.4 us, at four 9.6; the split tiles 9.5 at any number up to 16. */
+/* Up to four tokens rows are streamed (gemm_i8_stream_kernel): 11008 x 4096 at one token 7.4 us, at four 9.6; the split tiles 9.5 at any number up to 16. */
 extern "C" int ckq_launch_i8_kernel(int M, int N, int K)
 {
     const int forced = g_i8_kernel.load();

@@ -343,6 +343,23 @@ def test_matmul_every_kernel_tail_of_k(kernel, which):
         matmul_case(5, 37, K, "f32", bias=False, seed=K)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,N,K", [(4, 300, 1100), (150, 333, 2049)])
+def test_matmul_every_kernel_has_the_same_bits(kernel, M, N, K, t):
+    """And a token the same results alone, in any company."""
+    a, b = codes(M, K, 1), codes(N, K, 2)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    sa, sb, bias = (torch.rand(n, device="cuda", generator=g) for n in (M, N, N))
+    want = [P.dev_gemm_nt_i8(a, sa, b, sb, v, dtype=TYPES[t]) for v in (None, bias)]
+    for which in range(len(KERNELS)):
+        kernel(which)
+        for v, w in zip((None, bias), want):
+            assert torch.equal(P.dev_gemm_nt_i8(a, sa, b, sb, v, dtype=TYPES[t]), w), which
+    kernel(-1)
+    for rows in (slice(0, 1), slice(1, 3), slice(0, 4), slice(M // 2, M), slice(0, min(M, 17))):
+        assert torch.equal(P.dev_gemm_nt_i8(a[rows], sa[rows], b, sb, bias, dtype=TYPES[t]), want[1][rows])
+
+
 @pytest.mark.parametrize("M,N,K", [(4000, 4300, 130), (2048, 8193, 128), (8100, 2100, 200)])
 def test_matmul_two_sizes_of_tiles(kernel, M, N, K):
     kernel(TWO)
