@@ -28,17 +28,29 @@ template <> struct RowType<CKQ_T_F16>  { typedef _Float16 type; };
 template <class E> struct __attribute__((packed, aligned(sizeof(E)))) row8 { E v[8]; };
 struct __attribute__((packed, aligned(1))) row8q { u32 v[2]; };
 
+/* The same as loaded, in whole registers. */
+template <class E> struct raw8 { u32 w[2 * sizeof(E)]; };
 template <class E>
-__device__ __forceinline__ void load8(float (&f)[8], const E *p, int left)
+__device__ __forceinline__ raw8<E> fetch8(const E *p, int left)
 {
-    if (left >= 8) {
-        const row8<E> r = *reinterpret_cast<const row8<E> *>(p);
+    struct __attribute__((packed, aligned(sizeof(E)))) at { raw8<E> r; };
+    if (left >= 8) return reinterpret_cast<const at *>(p)->r;
+    raw8<E> r;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = (float)r.v[i];
-    } else {
+    for (int i = 0; i < 2 * (int)sizeof(E); ++i) r.w[i] = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < left ? (float)p[i] : 0.0f;
-    }
+    for (int i = 0; i < 8; ++i)
+        if (i < left) {
+            if constexpr (sizeof(E) == 4) r.w[i] = __builtin_bit_cast(u32, p[i]);
+            else                          r.w[i / 2] |= (u32)__builtin_bit_cast(uint16_t, p[i]) << (16 * (i & 1));
+        }
+    return r;
+}
+template <class E>
+__device__ __forceinline__ float raw_value(const raw8<E> &r, int i)
+{
+    if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, r.w[i]);
+    else return (float)__builtin_bit_cast(E, (uint16_t)(r.w[i / 2] >> (16 * (i & 1))));
 }
 template <class E>
 __device__ __forceinline__ void store8(E *p, const float (&f)[8], int left)
@@ -67,38 +79,43 @@ struct RowsArgs {
     int          rows, k;
 };
 
-/* The values of vector `v` (eight elements) of a row, rmsnorm's without its factor r; `ss` collects the squares. */
-template <int OP, class E, bool AGAIN>
-__device__ __forceinline__ void row_values(float (&f)[8], const RowsArgs &a, const E *x, const E *y, E *h, int v, float &ss)
+/* What the values of a vector (eight elements) are made of. */
+template <class E> struct RowParts { raw8<E> x, y; raw8<float> g; };
+
+template <int OP, class E>
+__device__ __forceinline__ void row_fetch(RowParts<E> &p, const RowsArgs &a, const E *x, const E *y, int v)
 {
     const int left = a.k - 8 * v;
-    if (OP == ROWS_RMSNORM && AGAIN && y) {
-        load8(f, (const E *)h + 8 * v, left);          /* this thread wrote them; x + residual may be gone by now */
-    } else {
-        load8(f, x + 8 * v, left);
-        if (OP == ROWS_SWIGLU || (OP == ROWS_RMSNORM && y)) {
-            float g[8];
-            load8(g, y + 8 * v, left);
+    p.x = fetch8(x + 8 * v, left);
+    if (OP != ROWS_QUANTIZE && y) p.y = fetch8(y + 8 * v, left);
+    if (OP == ROWS_RMSNORM) p.g = fetch8(a.gamma + 8 * v, left);
+}
+
+/* The values themselves, rmsnorm's without the row's factor r; `ss` collects the squares.  x + residual goes to h, where it is not null. */
+template <int OP, class E>
+__device__ __forceinline__ void row_values(float (&f)[8], const RowParts<E> &p, bool with_y, E *h, int left, float &ss)
+{
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (OP == ROWS_SWIGLU) {
-                    /* v_exp_f32 and v_rcp_f32, an ulp each: what they are off is 2^-22 of a value that is about to
-                     * be rounded to one part in 254 of the row's largest */
-                    const float e = __builtin_amdgcn_exp2f(f[i] * -1.44269504f);
-                    f[i] = f[i] * __builtin_amdgcn_rcpf(1.0f + e) * g[i];
-                } else
-                    f[i] = (float)(E)(f[i] + g[i]);    /* the norm is of the stream as it is stored */
-            }
-            if (OP == ROWS_RMSNORM) store8(h + 8 * v, f, left);
+    for (int i = 0; i < 8; ++i) f[i] = raw_value<E>(p.x, i);
+    if (OP == ROWS_SWIGLU) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            /* v_exp_f32 and v_rcp_f32, an ulp each: what they are off is 2^-22 of a value that is about to be rounded to one part
+             * in 254 of the row's largest */
+            const float e = __builtin_amdgcn_exp2f(f[i] * -1.44269504f);
+            f[i] = f[i] * __builtin_amdgcn_rcpf(1.0f + e) * raw_value<E>(p.y, i);
         }
     }
     if (OP == ROWS_RMSNORM) {
-        float g[8];
-        load8(g, a.gamma + 8 * v, left);
+        if (with_y) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = (float)(E)(f[i] + raw_value<E>(p.y, i));         /* the norm is of the stream as it is stored */
+            if (h) store8(h, f, left);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             ss = __builtin_fmaf(f[i], f[i], ss);
-            f[i] *= g[i];
+            f[i] *= raw_value<float>(p.g, i);
         }
     }
 }
@@ -144,17 +161,30 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
     float f[NV > 0 ? NV : 1][8], ss = 0.0f;
     u32 top = 0;
     if (NV > 0) {
+        /* A vector's loads are under way together, gamma's too, before the store to h (which may be x or the residual, so that the compiler moves none
+         * across it): one row of 4096 3.0 -> 2.7 us.  Those of two vectors and more only in the quantizer (2048 x 11008 in fp32 18.6 -> 17.6): elsewhere
+         * their registers cost waves (norm of 2048 x 4096 in bf16 10.8 -> 12.6, SwiGLU of 2048 x 11008 20.1 -> 21.6). */
+        constexpr int CH = OP == ROWS_QUANTIZE && NV > 0 ? NV : 1;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int v = first + i * step;
-            if (v < nvec) {
-                row_values<OP, E, false>(f[i], a, x, y, h, v, ss);
-                top = top_bits(f[i], top);
+        for (int c = 0; c < NV; c += CH) {
+            RowParts<E> p[CH];
+#pragma unroll
+            for (int i = 0; i < CH; ++i)
+                if (first + (c + i) * step < nvec) row_fetch<OP>(p[i], a, x, y, first + (c + i) * step);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int v = first + (c + i) * step;
+                if (v < nvec) {
+                    row_values<OP>(f[c + i], p[i], y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, ss);
+                    top = top_bits(f[c + i], top);
+                }
             }
         }
     } else
         for (int v = first; v < nvec; v += step) {
-            row_values<OP, E, false>(f[0], a, x, y, h, v, ss);
+            RowParts<E> p;
+            row_fetch<OP>(p, a, x, y, v);
+            row_values<OP>(f[0], p, y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, ss);
             top = top_bits(f[0], top);
         }
 
@@ -184,8 +214,13 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
 
     int8_t *q = a.q + (size_t)row * a.ldq;
     auto put = [&](const float (&e)[8], int v) {
-        u32 p[2] = {0u, 0u};
-        if (finite) q8_round(e, inv, p);
+        /* 1.5 * 2^23 + e inv, rounded once: the nearest integer (ties to even) in the low bits, |e inv| <= 127 (1 + 2^-22) */
+        u32 b[8], p[2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = __builtin_bit_cast(u32, __builtin_fmaf(e[i], inv, 12582912.0f));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            p[i] = !finite ? 0u : __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0c0c0400u) | __builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x04000c0cu);
         const int left = a.k - 8 * v;
         if (left >= 8) {
             row8q o;
@@ -206,14 +241,18 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
         }
     } else
         for (int v = first; v < nvec; v += step) {
-            row_values<OP, E, true>(f[0], a, x, y, h, v, ss);
+            RowParts<E> p;
+            /* x + residual again from where this thread has stored it: x or the residual may be gone by now */
+            const bool stored = OP == ROWS_RMSNORM && y;
+            row_fetch<OP>(p, a, stored ? (const E *)h : x, OP == ROWS_RMSNORM ? nullptr : y, v);
+            row_values<OP, E>(f[0], p, false, nullptr, a.k - 8 * v, ss);
             put(f[0], v);
         }
 }
 
 /* Waves of a row: as few as leave a thread three vectors (24 elements), so that loads, reduction and stores of several rows share
  * a CU; where every row has a CU to itself, as many as leave it one.  us with 2 | 4 | 8 | 16 waves a row: norm of 2048 x 4096 in bf16 13.2 |
- * 11.9 | 13.2 | 15.4, SwiGLU of 2048 x 11008 31.0 | 21.3 | 20.4 | 20.9, quantizer of 11008 x 4096 in fp32 34.1 | 32.1 | 31.8 | 38.0 and of
+ * 11.9 | 13.2 | 15.4 (10.8 with four since), SwiGLU of 2048 x 11008 31.0 | 21.3 | 20.4 | 20.9, quantizer of 11008 x 4096 in fp32 34.1 | 32.1 | 31.8 | 38.0 and of
  * 11008 x 896 9.3 | 10.2 | 14.9 | 29.3 (one wave 8.7); SwiGLU of 93 x 4863 in fp32 5.1 | 4.3 | 4.2 | 3.7.  Bound by memory beyond a few hundred
  * rows: 4.9 to 7 TB/s of what is read and written (a copy has 4.8 beyond the caches), and by the latency of one trip below. */
 static int rows_waves(int nvec, int rows)
