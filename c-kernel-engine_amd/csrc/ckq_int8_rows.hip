@@ -142,6 +142,13 @@ __device__ __forceinline__ float wave_sum(float v)
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, group_sum<64>(v)), 63));
 }
 
+__device__ __forceinline__ u32 rounded_bits(float e, float inv)
+{
+#pragma clang fp contract(off)
+    const float p = e * inv;
+    return __builtin_bit_cast(u32, p + 12582912.0f);
+}
+
 /* NV > 0: `wpr` waves have a row, each thread at most NV vectors of it, held in registers between the two passes (k <= 512 wpr NV);
  * NV = 0: rows of any length, read again for the second pass. */
 template <int OP, class E, int NV>
@@ -214,10 +221,11 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
 
     int8_t *q = a.q + (size_t)row * a.ldq;
     auto put = [&](const float (&e)[8], int v) {
-        /* 1.5 * 2^23 + e inv, rounded once: the nearest integer (ties to even) in the low bits, |e inv| <= 127 (1 + 2^-22) */
+        /* e inv in fp32, plus 1.5 * 2^23: the nearest integer (ties to even) in the low bits, |e inv| <= 127 (1 + 2^-22).  Not in one multiply-add,
+         * which would round 63.5 less a rounding of inv the other way: quants are those of the formula in fp32, operation by operation. */
         u32 b[8], p[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = __builtin_bit_cast(u32, __builtin_fmaf(e[i], inv, 12582912.0f));
+        for (int i = 0; i < 8; ++i) b[i] = rounded_bits(e[i], inv);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             p[i] = !finite ? 0u : __builtin_amdgcn_perm(b[4 * i + 1], b[4 * i], 0x0c0c0400u) | __builtin_amdgcn_perm(b[4 * i + 3], b[4 * i + 2], 0x04000c0cu);
