@@ -90,23 +90,26 @@ __device__ __forceinline__ void i8_store_rows(const I8Args &a, const uint8_t *su
         }
     }
 }
-/* WT x WN waves, each 32 TT tokens x 32 TN rows, S stages in LDS; SP, FM: see `multiply`. */
-template <int WT_, int WN_, int TT_, int TN_, int S_, int SP_, int FM_> struct I8Tile {
-    static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, S = S_, SP = SP_, FM = FM_;
-    static constexpr int NW = WT * WN, BT = 32 * TT * WT, BN = 32 * TN * WN, KS = 128, STAGE = (BT + BN) * KS;
-    static constexpr int NCA = BT / 8 / NW, NCB = BN / 8 / NW;           /* copies of a wave a step: eight rows each */
+/* WT x WN waves that multiply, each 32 TT tokens x 32 TN rows; NP others that copy, or none (the former do it then); S stages in LDS; FM: see
+ * `multiply`. */
+template <int WT_, int WN_, int TT_, int TN_, int NP_, int S_, int FM_> struct I8Tile {
+    static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NP = NP_, S = S_, FM = FM_;
+    static constexpr int NW = WT * WN, BT = 32 * TT * WT, BN = 32 * TN * WN, KS = 128, STAGE = (BT + BN) * KS, WAVES = NW + NP;
+    static constexpr int NCW = NP ? NP : NW, NCA = BT / 8 / NCW, NCB = BN / 8 / NCW;   /* waves that copy, copies of each a step: eight rows */
     static constexpr int PITCH = 32 * TN * 4 + 16;                       /* of a token's sums in LDS */
     static constexpr int SCALES = S * STAGE > NW * 32 * PITCH ? S * STAGE : NW * 32 * PITCH, LDS = SCALES + 4 * (BT + 2 * BN);
-    static_assert(NW % 2 == 0 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole copies");
+    static_assert(NCW % 2 == 0 && BT % (8 * NCW) == 0 && BN % (8 * NCW) == 0, "whole copies");
     static_assert(BT % 64 == 0 && BN % 64 == 0, "whole copies of the scales");
+    static_assert(NP || S == 2, "waves that copy and multiply have a step under way");
+    static_assert((S - 1) * (NCA + NCB) < 64 && FM <= TT * TN && LDS <= 160 * 1024, "what a wave can count, a place among the multiplications, one block");
 };
 
 template <class E, class T>
 __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t *lds)
 {
-    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, S = T::S, SP = T::SP, FM = T::FM, NW = T::NW, BT = T::BT, BN = T::BN, KS = T::KS, STAGE = T::STAGE, NCA = T::NCA;
-    constexpr int NC = T::NCA + T::NCB, NM = TT * TN, NF = TT + TN, PITCH = T::PITCH;
-    const int lane = threadIdx.x & 63, wave = wave_in_block();
+    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NP = T::NP, S = T::S, FM = T::FM, NW = T::NW, BT = T::BT, BN = T::BN, KS = T::KS, STAGE = T::STAGE, NCA = T::NCA;
+    constexpr int NCW = T::NCW, NC = T::NCA + T::NCB, NM = TT * TN, NF = TT + TN, PITCH = T::PITCH;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), cw = NP ? wave - NW : wave;
     const ckq_v4i rsa = gemm_buffer((const uint8_t *)a.A + (size_t)m0 * a.lda), rsb = gemm_buffer((const uint8_t *)a.B + (size_t)n0 * a.ldb);
     const u32 base = lds_address(lds);
     const int niter = (a.K + KS - 1) / KS, last = niter - 1, tail = a.K - last * KS;      /* bytes of the last step, 1 .. 128 */
@@ -114,21 +117,25 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
     /* a copy takes eight rows of 128 bytes; the chunk of 16 that a lane fetches is the one that belongs in its place, c ^ (row / 2 % 8):
      * sixteen rows' chunks c, which a phase of a read of 16 bytes a lane takes, then lie on all 64 banks once (c ^ (row % 8): twice, 8.3 cycles a read and not 4.2) */
     u32 ofs[NC];
-    const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+    const int chunk = (lane & 7) ^ ((4 * cw + (lane >> 4)) & 7);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int row = 8 * (wave + NW * (i < NCA ? i : i - NCA)) + (lane >> 3);
+        const int row = 8 * (cw + NCW * (i < NCA ? i : i - NCA)) + (lane >> 3);
         ofs[i] = i < NCA ? (u32)min(row, a.M - 1 - m0) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb;
         ofs[i] += 16u * (u32)chunk;
     }
     auto copy = [&](int i, int it, int buf) {
         /* chunks behind the row's last are read from its start; the tokens' are zeroed (clear_tail) */
         const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
-        const u32 dst = base + (u32)(buf * STAGE + 1024 * (wave + NW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * KS));
+        const u32 dst = base + (u32)(buf * STAGE + 1024 * (cw + NCW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * KS));
         lds_copy16(i < NCA ? rsa : rsb, dst, o, it * KS);
     };
-    auto clear_tail = [&](int buf) {
-        for (int e = threadIdx.x; e < BT * 8; e += 64 * NW) {
+    auto copy_step = [&](int it, int buf) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) copy(c, it, buf);
+    };
+    auto clear_tail = [&](int buf) {                           /* all waves; then they meet */
+        for (int e = threadIdx.x; e < BT * 8; e += 64 * T::WAVES) {
             const int row = e >> 3, left = tail - 16 * ((e & 7) ^ ((row >> 1) & 7));
             if (left >= 16) continue;
             ckq_v4i *p = reinterpret_cast<ckq_v4i *>(lds + buf * STAGE + 16 * e);
@@ -140,7 +147,48 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
             }
             *p = v;
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
     };
+
+    /* the scales and the bias, BT, BN and BN floats, behind the stages: fetched first, used last */
+    float *scales = reinterpret_cast<float *>(lds + T::SCALES);
+    if (cw >= 0)
+        for (int i = cw; i < (BT + 2 * BN) / 64; i += NCW) {
+            const bool tok = i < BT / 64, ch = i < (BT + BN) / 64;
+            const float *p = tok ? a.sa : ch ? a.sb : a.bias;
+            if (!p) continue;
+            const int e = 64 * i + lane - (tok ? 0 : ch ? BT : BT + BN);
+            lds_copy4(gemm_buffer((const uint8_t *)(p + (tok ? m0 : n0))), base + (u32)T::SCALES + 256u * (u32)i, 4u * (u32)min(e, tok ? a.M - 1 - m0 : a.N - 1 - n0), 0);
+        }
+
+    /* Step `it` has stage it % S.  A step's last operands are read before its last quarter is multiplied; the barrier is there, so
+     * that no wave waits with nothing to multiply: all have step it's operands in registers, and step it + 1 has arrived; from there on the
+     * stage takes the copies of step it + S. */
+    if (NP > 0 && wave >= NW) {
+        /* A copy holds its wave until the address unit has taken it, 16 cycles and more, and with it whatever the wave would
+         * have multiplied; waves that do nothing else take that from the others (us without | with them: 512 x 11008 x 4096 27.2 | 24.2, 1024 x 4096 x 4096 22.3 |
+         * 19.1, 125 x 11008 x 4096 14.8 | 13.0). */
+#pragma unroll
+        for (int st = 0; st < S; ++st)
+            if (st < niter) copy_step(st, st);
+        if (niter >= S) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * NC) : "memory");
+        else            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (last == 0 && tail < KS) clear_tail(0);
+        int buf = 0;
+        for (int it = 0; it < niter; ++it) {
+            const int next = buf + 1 == S ? 0 : buf + 1;
+            if (it + S - 1 < niter) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * NC) : "memory");
+            else                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (it + 1 == last && tail < KS) clear_tail(next);
+            if (it + S < niter) copy_step(it + S, buf);
+            buf = next;
+        }
+        __syncthreads();
+        return;
+    }
 
     /* where a lane's operands are: row lane % 32 of a group of 32, bytes 16 (lane / 32) of the 32 of a multiplication */
     const int wt = wave / WN, wn = wave % WN, half = lane >> 5;
@@ -163,12 +211,10 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
         else if (f <= TT) fa[to][f - 1] = *reinterpret_cast<const ckq_v4i *>(p + ra[kk] + 32 * KS * (f - 1));
         else              fb[to][f - TT] = *reinterpret_cast<const ckq_v4i *>(p + rb[kk] + 32 * KS * (f - TT));
     };
-    /* The multiplications of 32 bytes of K; among the first FM of them the reads of the next 32 bytes' operands, and over the
-     * first SP quarters of a step the copies of a later one: a copy holds its wave until the address unit has taken it, 16
-     * cycles, and a burst of all waves' copies leaves the matrix cores idle for their sum; the last of them has to arrive in
-     * what is left of the step where there are two stages. */
+    /* The multiplications of 32 bytes of K; among the first FM of them the reads of the next 32 bytes' operands, and, where these waves
+     * copy too, over the first half of a step the copies of the next: a burst of all waves' copies leaves the matrix cores idle for
+     * their sum, and the last of them has to arrive in what is left of the step. */
     auto multiply = [&](int from, int quarter, int it, int buf, int fbuf, int fkk) {
-        const bool more = it < niter;
 #pragma unroll
         for (int m = 0; m < NM; ++m) {
             const int j = m / TT, i = m % TT;
@@ -178,59 +224,34 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
                 if (f * FM / NF == m && fbuf >= 0) fetch(from ^ 1, fbuf, fkk, f);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
-                if (c * NM * SP / NC == quarter * NM + m && more) copy(c, it, buf);
+                if (NP == 0 && c * NM * 2 / NC == quarter * NM + m && it < niter) copy(c, it, buf);
             __builtin_amdgcn_sched_barrier(0);                 /* or the compiler moves the reads to where they are used, and waits for each */
         }
     };
 
-    /* the scales and the bias, BT, BN and BN floats, behind the stages: fetched first, used last */
-    float *scales = reinterpret_cast<float *>(lds + T::SCALES);
-    for (int i = wave; i < (BT + 2 * BN) / 64; i += NW) {
-        const bool tok = i < BT / 64, ch = i < (BT + BN) / 64;
-        const float *p = tok ? a.sa : ch ? a.sb : a.bias;
-        if (!p) continue;
-        const int e = 64 * i + lane - (tok ? 0 : ch ? BT : BT + BN);
-        lds_copy4(gemm_buffer((const uint8_t *)(p + (tok ? m0 : n0))), base + (u32)T::SCALES + 256u * (u32)i, 4u * (u32)min(e, tok ? a.M - 1 - m0 : a.N - 1 - n0), 0);
+    if (NP == 0) {
+        copy_step(0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-
-    /* Step `it` has stage it % S.  A step's last operands are read before its last quarter is multiplied; the barrier is there, so
-     * that no wave waits with nothing to multiply, and from there on the stage takes the copies of step it + S. */
-#pragma unroll
-    for (int st = 0; st < S - 1; ++st)
-        if (st < niter) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) copy(c, st, st);
-        }
-    /* the first step is here once no more than the S - 2 behind it are in flight, where there are as many */
-    if (S > 2 && niter >= S - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * NC) : "memory");
-    else                         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    if (last == 0 && tail < KS) {
-        clear_tail(0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-    }
-    if (S - 1 < niter) {
+    if (last == 0 && tail < KS) clear_tail(0);
+    if (NP == 0 && niter > 1) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
-            if (c * SP / NC == 0) copy(c, S - 1, S - 1);
+            if (c * 2 < NC) copy(c, 1, 1);
     }
 #pragma unroll
     for (int f = 0; f < NF; ++f) fetch(0, 0, 0, f);
     int buf = 0;
     for (int it = 0; it < niter; ++it) {
-        const int next = buf + 1 == S ? 0 : buf + 1, prev = buf == 0 ? S - 1 : buf - 1;
+        const int next = buf + 1 == S ? 0 : buf + 1;
 #pragma unroll
-        for (int kk = 0; kk < 3; ++kk) multiply(kk & 1, kk + 1, it + S - 1, prev, buf, kk + 1);
-        if (S > 2 && it + S - 1 < niter) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * NC) : "memory");
-        else                             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        for (int kk = 0; kk < 3; ++kk) multiply(kk & 1, kk + 1, it + 1, next, buf, kk + 1);
+        if (NP == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        if (it + 1 == last && tail < KS) {
-            clear_tail(next);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-        }
-        multiply(1, 0, it + S, buf, it < last ? next : -1, 0);
+        if (it + 1 == last && tail < KS) clear_tail(next);
+        multiply(1, 0, it + 2, buf, it < last ? next : -1, 0);
         buf = next;
     }
 
@@ -255,7 +276,7 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
 }
 
 template <class E, class T>
-__global__ void __launch_bounds__(64 * T::NW) gemm_i8_tile_kernel(I8Args a, int ntt, int nnt)
+__global__ void __launch_bounds__(64 * T::WAVES) gemm_i8_tile_kernel(I8Args a, int ntt, int nnt)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
     int tt, nt;
@@ -264,9 +285,9 @@ __global__ void __launch_bounds__(64 * T::NW) gemm_i8_tile_kernel(I8Args a, int 
 
 /* The first nnt1 columns of tiles of T1, `blocks1` blocks of them, and the rows that they leave in tiles of T2. */
 template <class E, class T1, class T2>
-__global__ void __launch_bounds__(64 * T1::NW) gemm_i8_two_tiles_kernel(I8Args a, int ntt1, int nnt1, int blocks1, int ntt2, int nnt2)
+__global__ void __launch_bounds__(64 * T1::WAVES) gemm_i8_two_tiles_kernel(I8Args a, int ntt1, int nnt1, int blocks1, int ntt2, int nnt2)
 {
-    static_assert(T1::NW == T2::NW, "one size of block");
+    static_assert(T1::WAVES == T2::WAVES, "one size of block");
     __shared__ __attribute__((aligned(16))) uint8_t lds[T1::LDS > T2::LDS ? T1::LDS : T2::LDS];
     int tt, nt;
     if ((int)blockIdx.x < blocks1) {
@@ -280,7 +301,7 @@ static int launch_i8_tiles(const I8Args &a, hipStream_t s)
 {
     const int ntt = (a.M + T::BT - 1) / T::BT, nnt = (a.N + T::BN - 1) / T::BN;
     if ((long)ntt * nnt > 0x3fffff) return CKQ_EINVAL;       /* results beyond any memory */
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<E, T>), dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::NW), 0, s, a, ntt, nnt);
+    hipLaunchKernelGGL((gemm_i8_tile_kernel<E, T>), dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::WAVES), 0, s, a, ntt, nnt);
     return (int)hipGetLastError();
 }
 template <class E, class T1, class T2>
@@ -288,7 +309,7 @@ static int launch_i8_two_tiles(const I8Args &a, int nnt1, hipStream_t s)
 {
     const int ntt1 = (a.M + T1::BT - 1) / T1::BT, ntt2 = (a.M + T2::BT - 1) / T2::BT, nnt2 = (a.N - nnt1 * T1::BN + T2::BN - 1) / T2::BN;
     const int blocks1 = gemm_blocks(ntt1, nnt1);
-    hipLaunchKernelGGL((gemm_i8_two_tiles_kernel<E, T1, T2>), dim3((unsigned)(blocks1 + gemm_blocks(ntt2, nnt2))), dim3(64u * T1::NW), 0, s,
+    hipLaunchKernelGGL((gemm_i8_two_tiles_kernel<E, T1, T2>), dim3((unsigned)(blocks1 + gemm_blocks(ntt2, nnt2))), dim3(64u * T1::WAVES), 0, s,
                        a, ntt1, nnt1, blocks1, ntt2, nnt2);
     return (int)hipGetLastError();
 }
@@ -538,44 +559,46 @@ static int launch_i8_stream(const I8Args &a, hipStream_t s)
 
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */
 
-/* Waves, stages and the places of reads and copies as measured, us.  256 x 256, 8192 x 8192 x 8192: copies over the first half of a step 453,
- * all at its start 463, over three quarters 466, over all of it 471; four waves of 128 x 128 each 470 to 590.  128 x 128, 1024 x 4096 x 4096: three stages,
- * reads behind the first multiplication 22.3, four stages 22.6, reads spread 23.0, four waves 22.7.  128 x 192, 512 x 11008 x 4096: 27.2 to 28.0 for any place, two
- * stages or four waves 29 and more.  64 x 128, 125 x 11008 x 4096: four stages 14.7, five 14.8, six 15.9. */
-typedef I8Tile<2, 4, 4, 2, 2, 2, 3> T256x256;
-typedef I8Tile<4, 2, 2, 2, 3, 4, 2> T256x128;
-typedef I8Tile<4, 2, 1, 3, 3, 4, 2> T128x192;
-typedef I8Tile<4, 2, 1, 2, 3, 4, 1> T128x128;
-typedef I8Tile<2, 4, 1, 1, 4, 4, 1> T64x128;
+/* Stages and waves as measured, us.  What waves that only copy gain: see i8_tile; none at 256 x 256, where the eight that multiply need 216 registers and a block
+ * of twelve waves has 168 each (sixteen waves of 64 x 64 are no faster: 8192 x 8192 x 8192 470 with eight, 477).  1024 x 4096 x 4096, 128 x 128: four waves multiplying 64 x 64 each, three stages 21.7, four 22.1,
+ * with two to copy 23.4; eight multiplying 32 x 64 22.8.  2048 x 4096 x 4096, 256 x 128: eight and four waves, three stages 35.5, two 37.1.  125 x 11008 x 4096, 64 x 128:
+ * four stages 13.2, five 13.4, three 13.9.  500 x 2000 x 2000, 64 x 64: four stages, so that two blocks share a CU, 8.4; six 8.8. */
+typedef I8Tile<2, 4, 4, 2, 0, 2, 3> T256x256;
+typedef I8Tile<4, 2, 2, 3, 4, 2, 5> T256x192;
+typedef I8Tile<4, 2, 2, 2, 4, 3, 2> T256x128;
+typedef I8Tile<2, 2, 2, 3, 4, 3, 3> T128x192;
+typedef I8Tile<2, 2, 2, 2, 4, 3, 3> T128x128;
+typedef I8Tile<2, 2, 1, 2, 4, 4, 2> T64x128;
+typedef I8Tile<2, 2, 1, 1, 4, 4, 1> T64x64;                 /* two blocks a CU */
 /* Split tiles.  13 x 4096 x 11008: 16 x 16 of eight waves, two stages 10.0, three 10.3, four 10.4; of sixteen 10.5, of four with four stages 10.4; 16 x 32 of four
  * 11.0.  13 x 22016 x 4096: 16 x 32 of four waves, two stages 16.1 (three blocks share a CU), three 17.4, four 19; 16 x 16 19.0.  333 x 1001 x 4847: 32 x 48 of
  * four waves, two stages 9.1, three 9.5, of eight 9.1; 32 x 64 10.1. */
-typedef I8Split<4, 2, 4, 2> S64x32;
 typedef I8Split<4, 3, 2, 2> S32x48;                   /* two blocks a CU */
 typedef I8Split<4, 2, 2, 2> S32x32;                   /* two */
 typedef I8Split<8, 1, 1, 2> S16x16;                   /* two */
 typedef I8Split<4, 2, 1, 2> S16x32;                   /* three */
 
-enum { I8_256x256, I8_256x128, I8_128x192, I8_128x128, I8_64x128, I8_S64x32, I8_S32x48, I8_S32x32, I8_S16x16, I8_S16x32, I8_TILINGS,
+enum { I8_256x256, I8_256x192, I8_256x128, I8_128x192, I8_128x128, I8_64x128, I8_64x64, I8_S32x48, I8_S32x32, I8_S16x16, I8_S16x32, I8_TILINGS,
        I8_TWO = I8_TILINGS, I8_STREAM };
 
 /* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all
  * places have a block; a last round of fewer steps faster, for the most part by how many blocks share a CU, a fifth by how many there
- * are in all (L2, power).  Fitted to 239 sizes of 5 to 2048 tokens (64 to 32000 rows, K 64 to 11008; operands from the 256 MB cache, as three
- * sets in turn leave them), each kernel within 4 to 9 % (rms).  On 271 other sizes the kernel so chosen is 0.6 % slower than the best of all on average,
- * 1.26 times at worst; without one of them 0.8 to 3.2 % on average (without 64 x 32: 0.6, but 1.31 times at worst). */
+ * are in all (L2, power).  Fitted to 512 sizes of 5 to 2048 tokens (64 to 32000 rows, K 64 to 11008; operands from the 256 MB cache, as three
+ * sets in turn leave them), each kernel within 5 to 9 % (rms).  Fitted to half of the sizes, the kernel so chosen is on the other half 0.7 % slower than the
+ * best of all on average, 1.13 times at worst; without one of them it is 0.8 to 4 % on average. */
 struct I8Cost { int bt, bn, places, split; float t0, t_tile, step; };
 static const I8Cost i8_costs[I8_TILINGS] = {
-    {256, 256, 256, 1, 1.50f, 7.74f, 1.452f},
-    {256, 128, 256, 1, 1.50f, 4.90f, 0.850f},
-    {128, 192, 256, 1, 1.50f, 4.08f, 0.740f},
-    {128, 128, 256, 1, 1.50f, 3.16f, 0.587f},
-    {64, 128, 256, 1, 1.50f, 2.32f, 0.441f},
-    {64, 32, 256, 4, 1.77f, 1.62f, 0.546f},
-    {32, 48, 512, 4, 2.27f, 1.06f, 0.941f},
-    {32, 32, 512, 4, 2.44f, 0.90f, 0.708f},
-    {16, 16, 512, 8, 2.44f, 1.05f, 0.552f},
-    {16, 32, 768, 4, 2.82f, 0.60f, 0.810f},
+    {256, 256, 256, 1, 1.50f, 7.97f, 1.493f},
+    {256, 192, 256, 1, 1.50f, 7.57f, 1.136f},
+    {256, 128, 256, 1, 1.50f, 5.56f, 0.806f},
+    {128, 192, 256, 1, 1.50f, 6.21f, 0.663f},
+    {128, 128, 256, 1, 1.50f, 4.36f, 0.520f},
+    {64, 128, 256, 1, 1.50f, 2.86f, 0.387f},
+    {64, 64, 512, 1, 1.98f, 1.91f, 0.501f},
+    {32, 48, 512, 4, 2.15f, 1.14f, 0.889f},
+    {32, 32, 512, 4, 2.29f, 1.02f, 0.662f},
+    {16, 16, 512, 8, 2.35f, 1.02f, 0.559f},
+    {16, 32, 768, 4, 2.71f, 0.64f, 0.797f},
 };
 
 static float i8_rounds(const I8Cost &c, long tiles, int K)
@@ -599,12 +622,16 @@ static int i8_whole_columns(int M, int N)
 static std::atomic<int> g_i8_kernel{-1};
 extern "C" void ckq_launch_set_i8_kernel(int kernel) { g_i8_kernel.store(kernel < 0 || kernel > I8_STREAM ? -1 : kernel); }
 
-/* Up to four tokens rows are streamed (gemm_i8_stream_kernel): 11008 x 4096 at one token 7.4 us, at four 9.6; the split tiles 9.5 at any number up to 16. */
+/* Rows are streamed (gemm_i8_stream_kernel) for one token or two, and for four where a row is one trip of a wave; at more the dot products, which
+ * use four multiplications of an instruction, become the bound (us streamed | split tiles: two tokens, 11008 x 4096 8.5 | 8.8, 151936 x 896 21.1 | 28.7;
+ * four, 151936 x 896 24.6 | 29.0, 11008 x 896 4.5 | 3.6, 32000 x 1500 15.5 | 9.7, 11008 x 4096 10.2 | 8.9, 11008 x 11008 23.6 | 25.5). */
+static bool i8_streams(int M, int K) { return M <= 2 || (M <= 4 && K <= 1024); }
+
 extern "C" int ckq_launch_i8_kernel(int M, int N, int K)
 {
     const int forced = g_i8_kernel.load();
-    if (forced >= 0 && (forced != I8_STREAM || M <= 4) && (forced != I8_TWO || i8_whole_columns(M, N) > 0)) return forced;
-    if (M <= 4) return I8_STREAM;
+    if (forced >= 0 && (forced != I8_STREAM || i8_streams(M, K)) && (forced != I8_TWO || i8_whole_columns(M, N) > 0)) return forced;
+    if (i8_streams(M, K)) return I8_STREAM;
     int best = 0;
     float t = 1e30f;
     for (int i = 0; i < I8_TILINGS; ++i) {
@@ -624,11 +651,12 @@ static int launch_gemm_i8(const I8Args &a, hipStream_t s)
 {
     switch (ckq_launch_i8_kernel(a.M, a.N, a.K)) {
     case I8_256x256:   return launch_i8_tiles<E, T256x256>(a, s);
+    case I8_256x192:   return launch_i8_tiles<E, T256x192>(a, s);
     case I8_256x128:   return launch_i8_tiles<E, T256x128>(a, s);
     case I8_128x192:   return launch_i8_tiles<E, T128x192>(a, s);
     case I8_128x128:   return launch_i8_tiles<E, T128x128>(a, s);
     case I8_64x128:    return launch_i8_tiles<E, T64x128>(a, s);
-    case I8_S64x32:    return launch_i8_split<E, S64x32>(a, s);
+    case I8_64x64:     return launch_i8_tiles<E, T64x64>(a, s);
     case I8_S32x48:    return launch_i8_split<E, S32x48>(a, s);
     case I8_S32x32:    return launch_i8_split<E, S32x32>(a, s);
     case I8_S16x16:    return launch_i8_split<E, S16x16>(a, s);
@@ -642,8 +670,8 @@ static int launch_gemm_i8(const I8Args &a, hipStream_t s)
     const int kb = (a.K + 1023) / 1024;
     if (a.M == 1) return kb <= 1 ? launch_i8_stream<E, 1, 4, 1, 1>(a, s) : kb <= 2 ? launch_i8_stream<E, 1, 4, 1, 2>(a, s)
                        : kb <= 8 ? launch_i8_stream<E, 1, 2, 2, 4>(a, s) : launch_i8_stream<E, 1, 2, 4, 4>(a, s);
-    if (a.M == 2) return kb <= 1 ? launch_i8_stream<E, 2, 4, 1, 1>(a, s) : launch_i8_stream<E, 2, 2, 2, 4>(a, s);
-    return kb <= 1 ? launch_i8_stream<E, 4, 4, 1, 1>(a, s) : launch_i8_stream<E, 4, 4, 1, 4>(a, s);
+    if (a.M == 2) return kb <= 1 ? launch_i8_stream<E, 2, 4, 1, 1>(a, s) : kb <= 2 ? launch_i8_stream<E, 2, 4, 1, 2>(a, s) : launch_i8_stream<E, 2, 2, 2, 4>(a, s);
+    return launch_i8_stream<E, 4, 4, 1, 1>(a, s);
 }
 
 extern "C" int ckq_launch_gemm_i8(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,

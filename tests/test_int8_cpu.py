@@ -97,15 +97,16 @@ def test_front_ends_refuse_what_a_pointer_cannot_tell():
 
 
 def test_kernel_of_a_matmul(L):
-    """Up to four tokens stream; then the cheapest by the estimate, which has to be one of the kernels at every size."""
-    assert all(L.ckq_launch_i8_kernel(M, N, K) == 11 for M in (1, 2, 3, 4) for N in (1, 5000, 151936) for K in (1, 896, 131071))
+    """One or two tokens stream, four if rows are short; then the cheapest by the estimate, which has to be one of the kernels at every size."""
+    assert all(L.ckq_launch_i8_kernel(M, N, K) == 12 for N in (1, 5000, 151936) for M, K in ((1, 1), (1, 131071), (2, 896), (2, 131071), (3, 1024), (4, 1)))
+    assert all(L.ckq_launch_i8_kernel(M, N, 1025) < 12 for M in (3, 4) for N in (1, 5000, 151936))
     seen = {L.ckq_launch_i8_kernel(M, N, K) for M in (5, 12, 16, 17, 40, 64, 100, 128, 200, 333, 512, 800, 1024, 1500, 2048, 5000) for N in (1, 64, 200, 512, 896, 1001, 1504, 2048, 3500, 4096, 4864, 8000, 11008, 17000, 28000, 151936)
             for K in (1, 64, 200, 512, 896, 1500, 2048, 4096, 4847, 11008, 131071)}
-    assert seen == set(range(11)), seen
-    assert L.ckq_launch_i8_kernel(2048, 11008, 4096) == 10          # 344 tiles of 256 x 256: 256 of them, the rest smaller
+    assert seen == set(range(12)), seen
+    assert L.ckq_launch_i8_kernel(2048, 11008, 4096) == 11          # 344 tiles of 256 x 256: 256 of them, the rest smaller
     assert L.ckq_launch_i8_kernel(2048, 8192, 4096) == 0            # one round of them
-    assert L.ckq_launch_i8_kernel(1 << 22, 1 << 22, 64) in range(11)
-    for forced in range(12):
+    assert L.ckq_launch_i8_kernel(1 << 22, 1 << 22, 64) in range(12)
+    for forced in range(13):
         L.ckq_launch_set_i8_kernel(forced)
-        assert L.ckq_launch_i8_kernel(2048, 11008, 4096) == (forced if forced != 11 else 10)
+        assert L.ckq_launch_i8_kernel(2048, 11008, 4096) == (forced if forced != 12 else 11)
     L.ckq_launch_set_i8_kernel(-1)
