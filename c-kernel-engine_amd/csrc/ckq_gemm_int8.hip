@@ -308,6 +308,7 @@ template <class E, class T1, class T2>
 static int launch_i8_two_tiles(const I8Args &a, int nnt1, hipStream_t s)
 {
     const int ntt1 = (a.M + T1::BT - 1) / T1::BT, ntt2 = (a.M + T2::BT - 1) / T2::BT, nnt2 = (a.N - nnt1 * T1::BN + T2::BN - 1) / T2::BN;
+    if ((long)ntt1 * nnt1 + (long)ntt2 * nnt2 > 0x3fffff) return CKQ_EINVAL;
     const int blocks1 = gemm_blocks(ntt1, nnt1);
     hipLaunchKernelGGL((gemm_i8_two_tiles_kernel<E, T1, T2>), dim3((unsigned)(blocks1 + gemm_blocks(ntt2, nnt2))), dim3(64u * T1::WAVES), 0, s,
                        a, ntt1, nnt1, blocks1, ntt2, nnt2);

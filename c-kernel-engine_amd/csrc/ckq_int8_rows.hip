@@ -100,10 +100,11 @@ __device__ __forceinline__ void row_values(float (&f)[8], const RowParts<E> &p, 
     if (OP == ROWS_SWIGLU) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            /* v_exp_f32 and v_rcp_f32, an ulp each: what they are off is 2^-22 of a value that is about to be rounded to one part
-             * in 254 of the row's largest */
+            /* v_exp_f32 and v_rcp_f32, an ulp each: what they and the exponent's rounding are off is (2 + |gate|) 2^-23 of a value that is about to
+             * be rounded to one part in 254 of the row's largest.  A quarter of both sides of the fraction, so that the reciprocal of no finite sum is below
+             * the normal numbers, where the instruction has zeros: those values count where up is large enough. */
             const float e = __builtin_amdgcn_exp2f(f[i] * -1.44269504f);
-            f[i] = f[i] * __builtin_amdgcn_rcpf(1.0f + e) * raw_value<E>(p.y, i);
+            f[i] = 0.25f * f[i] * __builtin_amdgcn_rcpf(__builtin_fmaf(0.25f, e, 0.25f)) * raw_value<E>(p.y, i);
         }
     }
     if (OP == ROWS_RMSNORM) {
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
     /* an infinity or a NaN in the row; the squares' sum beyond fp32 (r = 0); a row of zeros and no eps (r infinite) */
     const bool finite = ftop * r < __builtin_inff() && r > 0.0f;
     const float amax = fmaxf(ftop * r, 0x1p-100f);
-    const float inv = 127.0f / amax * r;
+    const float inv = fminf(127.0f / amax * r, 0x1.fffffep127f);     /* gamma of zeros after squares without an eps: 0 * inv has to be 0 */
     if (first == 0) a.scale[row] = finite ? amax / 127.0f : top >= 0x7f800000u ? ftop : r > 0.0f ? ftop * r : __builtin_nanf("");
 
     int8_t *q = a.q + (size_t)row * a.ldq;

@@ -220,6 +220,14 @@ def test_rmsnorm_pitches_zero_rows_and_rows_that_are_not_finite(k):
         assert (q == 0).all() and s.isnan().all()
 
 
+@pytest.mark.parametrize("k", [9, 600, 40000])
+def test_rmsnorm_of_small_rows_without_eps(k):
+    x = normal(3, k, k) * 2.0 ** -60
+    for gamma in (torch.zeros(k), torch.rand(k, generator=torch.Generator().manual_seed(k)) + 0.5):
+        q, s = P.dev_rmsnorm_i8(x.cuda(), gamma.cuda(), 0.0)
+        check_norm(q, s, x, gamma, 0.0)
+
+
 # ---- SwiGLU ----------------------------------------------------------------------------------
 
 def check_swiglu(q, s, gate, up):
@@ -245,6 +253,15 @@ def test_swiglu(t, rows, k):
     gate, up = both[:, :k].contiguous().cuda(), both[:, k:].contiguous().cuda()
     q2, s2 = P.dev_swiglu_i8(gate, up)
     assert torch.equal(q, q2) and torch.equal(s, s2)
+
+
+def test_swiglu_far_gates_count_where_up_is_large():
+    """1 + exp(-gate) up to the end of fp32, whose reciprocal is below its normal numbers."""
+    for rows, k in ((3, 40), (2, 20000)):
+        gate = -86.0 - 2.7 * torch.rand(rows, k, generator=torch.Generator().manual_seed(k))
+        up = normal(rows, k, k + 1) * 2.0 ** 120
+        q, s = P.dev_swiglu_i8(gate.cuda(), up.cuda())
+        check_swiglu(q, s, gate, up)
 
 
 def test_swiglu_far_gates():
