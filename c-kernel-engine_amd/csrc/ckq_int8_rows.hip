@@ -30,12 +30,22 @@ struct __attribute__((packed, aligned(1))) row8q { u32 v[2]; };
 
 /* The same as loaded, in whole registers. */
 template <class E> struct raw8 { u32 w[2 * sizeof(E)]; };
-template <class E>
+typedef u32 rows_u4 __attribute__((ext_vector_type(4)));
+typedef rows_u4 __attribute__((aligned(2))) rows_u4_at_2;    /* one load of 16 bytes, wherever it falls */
+template <class E, bool ONCE = false>                        /* ONCE: read for the last time, kept in no cache */
 __device__ __forceinline__ raw8<E> fetch8(const E *p, int left)
 {
-    struct __attribute__((packed, aligned(sizeof(E)))) at { raw8<E> r; };
-    if (left >= 8) return reinterpret_cast<const at *>(p)->r;
     raw8<E> r;
+    if (left >= 8) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(E) / 2; ++i) {
+            const rows_u4_at_2 *at = reinterpret_cast<const rows_u4_at_2 *>(p) + i;
+            const rows_u4 v = ONCE ? __builtin_nontemporal_load(at) : *at;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r.w[4 * i + j] = v[j];
+        }
+        return r;
+    }
 #pragma unroll
     for (int i = 0; i < 2 * (int)sizeof(E); ++i) r.w[i] = 0;
 #pragma unroll
@@ -82,12 +92,12 @@ struct RowsArgs {
 /* What the values of a vector (eight elements) are made of. */
 template <class E> struct RowParts { raw8<E> x, y; raw8<float> g; };
 
-template <int OP, class E>
+template <int OP, bool ONCE, class E>
 __device__ __forceinline__ void row_fetch(RowParts<E> &p, const RowsArgs &a, const E *x, const E *y, int v)
 {
     const int left = a.k - 8 * v;
-    p.x = fetch8(x + 8 * v, left);
-    if (OP != ROWS_QUANTIZE && y) p.y = fetch8(y + 8 * v, left);
+    p.x = fetch8<E, ONCE>(x + 8 * v, left);
+    if (OP != ROWS_QUANTIZE && y) p.y = fetch8<E, ONCE>(y + 8 * v, left);
     if (OP == ROWS_RMSNORM) p.g = fetch8(a.gamma + 8 * v, left);
 }
 
@@ -173,12 +183,17 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
          * across it): one row of 4096 3.0 -> 2.7 us.  Those of two vectors and more only in the quantizer (2048 x 11008 in fp32 18.6 -> 17.6): elsewhere
          * their registers cost waves (norm of 2048 x 4096 in bf16 10.8 -> 12.6, SwiGLU of 2048 x 11008 20.1 -> 21.6). */
         constexpr int CH = OP == ROWS_QUANTIZE && NV > 0 ? NV : 1;
+        /* What is quantized and a SwiGLU's halves are read for the last time, non-temporally, which leaves the caches to the quants: SwiGLU between the
+         * two matmuls of an MLP of 4096 x 11008, at 2048 tokens 36 -> 25 us, at 4096 60 -> 42, the same at 128 to 1024 and at 8192; quantizer and what reads the quants, 11008 x 4096
+         * in fp32 70 -> 64.  What lies in a cache anyway loses 2 to 4 % (SwiGLU of 512 x 11008 and its
+         * reader, three sets in turn, 12.2 -> 12.7).  A residual stream has later readers (norm of 2048 x 4096 and its reader 17.6 -> 22.7). */
+        constexpr bool ONCE = OP != ROWS_RMSNORM;
 #pragma unroll
         for (int c = 0; c < NV; c += CH) {
             RowParts<E> p[CH];
 #pragma unroll
             for (int i = 0; i < CH; ++i)
-                if (first + (c + i) * step < nvec) row_fetch<OP>(p[i], a, x, y, first + (c + i) * step);
+                if (first + (c + i) * step < nvec) row_fetch<OP, ONCE>(p[i], a, x, y, first + (c + i) * step);
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 const int v = first + (c + i) * step;
@@ -191,7 +206,7 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
     } else
         for (int v = first; v < nvec; v += step) {
             RowParts<E> p;
-            row_fetch<OP>(p, a, x, y, v);
+            row_fetch<OP, false>(p, a, x, y, v);
             row_values<OP>(f[0], p, y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, ss);
             top = top_bits(f[0], top);
         }
@@ -253,7 +268,7 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
             RowParts<E> p;
             /* x + residual again from where this thread has stored it: x or the residual may be gone by now */
             const bool stored = OP == ROWS_RMSNORM && y;
-            row_fetch<OP>(p, a, stored ? (const E *)h : x, OP == ROWS_RMSNORM ? nullptr : y, v);
+            row_fetch<OP, false>(p, a, stored ? (const E *)h : x, OP == ROWS_RMSNORM ? nullptr : y, v);
             row_values<OP, E>(f[0], p, false, nullptr, a.k - 8 * v, ss);
             put(f[0], v);
         }
