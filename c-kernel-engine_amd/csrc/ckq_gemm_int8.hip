@@ -66,38 +66,35 @@ template <class E> __device__ __forceinline__ void i8_put(E *out, const i8_out8<
     for (int i = 0; i < (int)(sizeof(o) / 16); ++i) __builtin_nontemporal_store(w.v[i], reinterpret_cast<i8_u4_at_2 *>(out) + i);
 }
 
-/* A wave: the sums of 32 tokens (from t0) x ROWS rows (from n) at `sums`, `pitch` bytes a token, scaled and stored, eight rows a lane;
- * sa, sb, bias: the scales of those tokens and of those rows, and their bias, in LDS too. */
-template <class E, int ROWS>
-__device__ __forceinline__ void i8_store_rows(const I8Args &a, const uint8_t *sums, int pitch, const float *sa, const float *sb, const float *bias, int t0, int n, int lane)
+/* Eight rows' sums of a token, scaled and stored to C[t][n ..]; sums, scales and bias in LDS. */
+template <class E>
+__device__ __forceinline__ void i8_store8(const I8Args &a, const void *sums, float sa, const float *sb, const float *bias, int t, int n)
 {
-    constexpr int PER = ROWS / 8;                             /* lanes of a token */
+    const ckq_v4i *s = reinterpret_cast<const ckq_v4i *>(sums);
+    const ckq_v4f *fb = reinterpret_cast<const ckq_v4f *>(sb), *fc = reinterpret_cast<const ckq_v4f *>(bias);
+    const int left = a.N - n;
+    i8_out8<E> o;
 #pragma unroll
-    for (int e0 = 0; e0 < 32 * PER; e0 += 64) {
-        const int e = e0 + lane, row = e / PER, c = 8 * (e % PER), t = t0 + row, n8 = n + c, left = a.N - n8;
-        const ckq_v4i *s = reinterpret_cast<const ckq_v4i *>(sums + row * pitch + 4 * c);
-        const ckq_v4f *fb = reinterpret_cast<const ckq_v4f *>(sb + c), *fc = reinterpret_cast<const ckq_v4f *>(bias + c);
-        i8_out8<E> o;
+    for (int r = 0; r < 8; ++r) o.v[r] = (E)i8_result(s[r >> 2][r & 3], sa, fb[r >> 2][r & 3], a.bias != nullptr, fc[r >> 2][r & 3]);
+    if (t >= a.M || left <= 0) return;
+    E *out = (E *)a.C + (size_t)t * a.ldc + n;
+    if (left >= 8) i8_put(out, o);
+    else {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) o.v[r] = (E)i8_result(s[r >> 2][r & 3], sa[row], fb[r >> 2][r & 3], a.bias != nullptr, fc[r >> 2][r & 3]);
-        if (t >= a.M || left <= 0) continue;
-        E *out = (E *)a.C + (size_t)t * a.ldc + n8;
-        if (left >= 8) i8_put(out, o);
-        else {
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (r < left) out[r] = o.v[r];
-        }
+        for (int r = 0; r < 8; ++r)
+            if (r < left) out[r] = o.v[r];
     }
 }
+
 /* WT x WN waves that multiply, each 32 TT tokens x 32 TN rows; NP others that copy, or none (the former do it then); S stages in LDS; FM: see
  * `multiply`. */
 template <int WT_, int WN_, int TT_, int TN_, int NP_, int S_, int FM_> struct I8Tile {
     static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NP = NP_, S = S_, FM = FM_;
     static constexpr int NW = WT * WN, BT = 32 * TT * WT, BN = 32 * TN * WN, KS = 128, STAGE = (BT + BN) * KS, WAVES = NW + NP;
     static constexpr int NCW = NP ? NP : NW, NCA = BT / 8 / NCW, NCB = BN / 8 / NCW;   /* waves that copy, copies of each a step: eight rows */
-    static constexpr int PITCH = 32 * TN * 4 + 16;                       /* of a token's sums in LDS */
-    static constexpr int SCALES = S * STAGE > NW * 32 * PITCH ? S * STAGE : NW * 32 * PITCH, LDS = SCALES + 4 * (BT + 2 * BN);
+    /* the sums on their way out, in the stages' place, 32 tokens a wave and round (see `finish`), all of them in one if they fit */
+    static constexpr int PITCH = (NP ? BN : 32 * TN) * 4 + 16, ROUND = 32 * (NP ? WT : NW) * PITCH, AT_ONCE = NP && TT * ROUND <= S * STAGE ? TT : 1;
+    static constexpr int SCALES = S * STAGE > ROUND ? S * STAGE : ROUND, LDS = SCALES + 4 * (BT + 2 * BN);
     static_assert(NCW % 2 == 0 && BT % (8 * NCW) == 0 && BN % (8 * NCW) == 0, "whole copies");
     static_assert(BT % 64 == 0 && BN % 64 == 0, "whole copies of the scales");
     static_assert(NP || S == 2, "waves that copy and multiply have a step under way");
@@ -107,7 +104,7 @@ template <int WT_, int WN_, int TT_, int TN_, int NP_, int S_, int FM_> struct I
 template <class E, class T>
 __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t *lds)
 {
-    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NP = T::NP, S = T::S, FM = T::FM, NW = T::NW, BT = T::BT, BN = T::BN, KS = T::KS, STAGE = T::STAGE, NCA = T::NCA;
+    constexpr int WT = T::WT, WN = T::WN, TT = T::TT, TN = T::TN, NP = T::NP, S = T::S, FM = T::FM, NW = T::NW, BT = T::BT, BN = T::BN, KS = T::KS, STAGE = T::STAGE, NCA = T::NCA;
     constexpr int NCW = T::NCW, NC = T::NCA + T::NCB, NM = TT * TN, NF = TT + TN, PITCH = T::PITCH;
     const int lane = threadIdx.x & 63, wave = wave_in_block(), cw = NP ? wave - NW : wave;
     const ckq_v4i rsa = gemm_buffer((const uint8_t *)a.A + (size_t)m0 * a.lda), rsb = gemm_buffer((const uint8_t *)a.B + (size_t)n0 * a.ldb);
@@ -162,6 +159,27 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
             lds_copy4(gemm_buffer((const uint8_t *)(p + (tok ? m0 : n0))), base + (u32)T::SCALES + 256u * (u32)i, 4u * (u32)min(e, tok ? a.M - 1 - m0 : a.N - 1 - n0), 0);
         }
 
+    /* The sums through LDS, where nothing is read or copied any more, so that a lane has eight rows' results of one token and a token's leave in whole lines.  The
+     * waves that copied store too (four and four waves, 128 x 192: 0.9 us of 27.1 at 512 x 11008 x 4096); eight that are alone have a piece each and wait for no
+     * other (256 x 256: 43.2 us, together 45.6 at 512 x 4096 x 4096).  `put` brings a round's sums there. */
+    auto finish = [&](auto &&put) {
+        constexpr int PER = (NP ? T::BN : 32 * TN) / 8, JOBS = 32 * PER * (NP ? WT * T::AT_ONCE : 1);
+#pragma unroll
+        for (int round = 0; round < TT; round += T::AT_ONCE) {
+            if (NP && round) __syncthreads();
+            put(round);
+            if (NP) __syncthreads();
+            else    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll 2
+            for (int e = NP ? threadIdx.x : lane; e < JOBS; e += NP ? 64 * T::WAVES : 64) {
+                const int row = e / PER, c = 8 * (e % PER) + (NP ? 0 : 32 * TN * (wave % WN)), k = row / (32 * WT), w = NP ? row / 32 % WT : wave / WN;
+                const int tok = 32 * (TT * w + round + k) + row % 32;
+                i8_store8<E>(a, lds + (NP ? row : 32 * wave + row) * PITCH + 4 * (8 * (e % PER)), scales[tok], scales + BT + c, scales + BT + T::BN + c, m0 + tok, n0 + c);
+            }
+            if (!NP) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    };
+
     /* Step `it` has stage it % S.  A step's last operands are read before its last quarter is multiplied; the barrier is there, so
      * that no wave waits with nothing to multiply: all have step it's operands in registers, and step it + 1 has arrived; from there on the
      * stage takes the copies of step it + S. */
@@ -186,7 +204,7 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
             if (it + S < niter) copy_step(it + S, buf);
             buf = next;
         }
-        __syncthreads();
+        finish([](int) {});
         return;
     }
 
@@ -255,24 +273,18 @@ __device__ __forceinline__ void i8_tile(const I8Args &a, int m0, int n0, uint8_t
         buf = next;
     }
 
-    /* sums, 32 tokens at a time through LDS, so that a lane has eight rows' results of one token side by side and a token's leave in
-     * whole lines: every wave has its own piece, behind everything that is still read from the last step's stage */
-    __syncthreads();
-    uint8_t *mine = lds + wave * 32 * PITCH;
-    const int nw = n0 + 32 * TN * wn;
+    finish([&](int round) {
 #pragma unroll
-    for (int i = 0; i < TT; ++i) {
-        const int t0 = m0 + 32 * (TT * wt + i);
+        for (int k = 0; k < T::AT_ONCE; ++k)
 #pragma unroll
-        for (int j = 0; j < TN; ++j)
+            for (int j = 0; j < TN; ++j)
 #pragma unroll
-            for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<ckq_v4i *>(mine + (lane & 31) * PITCH + 4 * (32 * j + 8 * g + 4 * half)) =
-                    ckq_v4i{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        i8_store_rows<E, 32 * TN>(a, mine, PITCH, scales + t0 - m0, scales + BT + nw - n0, scales + BT + T::BN + nw - n0, t0, nw, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+                for (int g = 0; g < 4; ++g) {
+                    const ckq_v16i &c = acc[round + k][j];
+                    *reinterpret_cast<ckq_v4i *>(lds + (32 * (NP ? WT * k + wt : wave) + (lane & 31)) * PITCH + 4 * (32 * ((NP ? TN * wn : 0) + j) + 8 * g + 4 * half)) =
+                        ckq_v4i{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
+                }
+    });
 }
 
 template <class E, class T>
