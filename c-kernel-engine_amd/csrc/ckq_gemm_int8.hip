@@ -8,17 +8,18 @@
  * among thousands.
  *
  * Three forms:
- * - gemm_i8_stream_kernel, up to four tokens: rows streamed once, v_dot4_i32_i8.  Bound by memory: 11008 x 4096 at one token 7.8 us,
+ * - gemm_i8_stream_kernel, one or two tokens (four of short rows): rows streamed once, v_dot4_i32_i8.  Bound by memory: 11008 x 4096 at one token 7.8 us,
  *   5.8 TB/s; a kernel that only reads those bytes takes 7.3.
  * - gemm_i8_split_kernel, a few to some hundred tokens: small tiles, K split among the waves of a block, which exchange their sums once.
- *   Bound by memory where rows are read once (13 x 4096 x 11008 9.5 us, 4.8 TB/s), beyond by what a CU can load, some 55 bytes a cycle (both
- *   operands of every tile: 333 x 1001 x 4847, 231 tiles, 390 KB a CU).
- * - gemm_i8_tile_kernel, tiles of 64 x 128 to 256 x 256 on all waves of a block, v_mfma_i32_32x32x32_i8.  The largest are bound by the matrix
+ *   Bound by memory where rows are read once (13 x 4096 x 11008 9.5 us, 4.8 TB/s), beyond by what a CU can load, 64 bytes a cycle at best (both
+ *   operands of every tile: 333 x 1001 x 4847, 231 tiles, 390 KB a CU, 3 us of 9.1, of which a launch takes 3.3).
+ * - gemm_i8_tile_kernel, tiles of 64 x 64 to 256 x 256 on all waves of a block, v_mfma_i32_32x32x32_i8.  The largest are bound by the matrix
  *   cores at the clock that the power limit leaves them (8192 x 8192 x 8192: 2430 TOPS, matrix cores busy in 71 % of the cycles at
- *   1.6 GHz; the published 5 POP/s are at 2.4), the smaller ones by the loads of a CU: a step of 128 x 128 has 512 cycles of
- *   multiplications and 32 KB, 600 cycles.
+ *   1.6 GHz; the published 5 POP/s are at 2.4).  The smaller ones have a step's copies (40 KB of 128 x 192, 640 cycles at 64 bytes) beside its multiplications
+ *   (768 cycles) and come near the longer of the two while few CUs work (0.43 us a step, the multiplications alone 0.37), not with all of them
+ *   (512 x 11008 x 4096 0.63, the copies alone 0.41); a launch, the first copies and the last stores are 6 of its 26 us.
  * All operands reach the matrix cores through LDS: 16 rows x 64 bytes an instruction, as the matrix cores want them in registers, load at 16 bytes a
- * cycle and CU; whole lines at 55.
+ * cycle and CU.
  */
 #include "ckq_gemm_common.hpp"
 #include <atomic>
@@ -597,21 +598,21 @@ enum { I8_256x256, I8_256x192, I8_256x128, I8_128x192, I8_128x128, I8_64x128, I8
 /* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all
  * places have a block; a last round of fewer steps faster, for the most part by how many blocks share a CU, a fifth by how many there
  * are in all (L2, power).  Fitted to 512 sizes of 5 to 2048 tokens (64 to 32000 rows, K 64 to 11008; operands from the 256 MB cache, as three
- * sets in turn leave them), each kernel within 5 to 9 % (rms).  Fitted to half of the sizes, the kernel so chosen is on the other half 0.7 % slower than the
- * best of all on average, 1.13 times at worst; without one of them it is 0.8 to 4 % on average. */
+ * sets in turn leave them), each kernel within 4 to 8 % (rms).  Fitted to half of the sizes, the kernel so chosen is on the other half 0.8 % slower than the
+ * best of all on average, 1.25 times at worst; without one of them it is 0.9 to 4 % on average. */
 struct I8Cost { int bt, bn, places, split; float t0, t_tile, step; };
 static const I8Cost i8_costs[I8_TILINGS] = {
-    {256, 256, 256, 1, 1.50f, 7.97f, 1.493f},
-    {256, 192, 256, 1, 1.50f, 7.57f, 1.136f},
-    {256, 128, 256, 1, 1.50f, 5.56f, 0.806f},
-    {128, 192, 256, 1, 1.50f, 6.21f, 0.663f},
-    {128, 128, 256, 1, 1.50f, 4.36f, 0.520f},
-    {64, 128, 256, 1, 1.50f, 2.86f, 0.387f},
-    {64, 64, 512, 1, 1.98f, 1.91f, 0.501f},
-    {32, 48, 512, 4, 2.15f, 1.14f, 0.889f},
-    {32, 32, 512, 4, 2.29f, 1.02f, 0.662f},
-    {16, 16, 512, 8, 2.35f, 1.02f, 0.559f},
-    {16, 32, 768, 4, 2.71f, 0.64f, 0.797f},
+    {256, 256, 256, 1, 1.50f, 7.40f, 1.490f},
+    {256, 192, 256, 1, 1.50f, 6.74f, 1.173f},
+    {256, 128, 256, 1, 1.50f, 5.13f, 0.816f},
+    {128, 192, 256, 1, 1.50f, 4.84f, 0.677f},
+    {128, 128, 256, 1, 1.50f, 3.45f, 0.522f},
+    {64, 128, 256, 1, 1.50f, 2.54f, 0.399f},
+    {64, 64, 512, 1, 1.97f, 1.79f, 0.504f},
+    {32, 48, 512, 4, 2.16f, 1.14f, 0.890f},
+    {32, 32, 512, 4, 2.29f, 1.02f, 0.660f},
+    {16, 16, 512, 8, 2.36f, 1.03f, 0.553f},
+    {16, 32, 768, 4, 2.72f, 0.64f, 0.799f},
 };
 
 static float i8_rounds(const I8Cost &c, long tiles, int K)
