@@ -1466,33 +1466,6 @@ int ckq_gemm_nt_f32act_dev(int fmt, const float *A, const void *B, const float *
     return ckq_launch_gemv(k, C, B, A, bias, N, K, M, ldc, 0, N, NULL, stream);
 }
 
-int ckq_quantize_i8_dev(ckq_ck_dtype type, const void *x, long ldx, int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
-{
-    return ckq_launch_quantize_i8((int)type, x, ldx, q, ldq, scale, rows, k, stream);
-}
-
-int ckq_dequantize_i8_dev(const int8_t *q, long ldq, const float *scale, ckq_ck_dtype type, void *y, long ldy, int rows, int k, void *stream)
-{
-    return ckq_launch_dequantize_i8(q, ldq, scale, (int)type, y, ldy, rows, k, stream);
-}
-
-int ckq_rmsnorm_i8_dev(ckq_ck_dtype type, const void *x, long ldx, const void *residual, void *sum, long ldr, const float *gamma, float eps,
-                       int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
-{
-    return ckq_launch_rmsnorm_i8((int)type, x, ldx, residual, sum, ldr, gamma, eps, q, ldq, scale, rows, k, stream);
-}
-
-int ckq_swiglu_i8_dev(ckq_ck_dtype type, const void *gate, const void *up, long ld, int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
-{
-    return ckq_launch_swiglu_i8((int)type, gate, up, ld, q, ldq, scale, rows, k, stream);
-}
-
-int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,
-                       ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream)
-{
-    return ckq_launch_gemm_i8(A, lda, sa, B, ldb, sb, bias, (int)type, C, ldc, M, N, K, stream);
-}
-
 static int ranges_overlap(const void *a, size_t na, const void *b, size_t nb) { return ckq_ranges_overlap(a, na, b, nb); }
 
 /* Entries i and j of a sequence can share a launch when they have one format,
