@@ -48,7 +48,7 @@ def test_rmsnorm_refusals(L):
         return L.ckq_rmsnorm_i8_dev(t, x, ldx, residual, out, ldr, gamma, ctypes.c_float(eps), q, ldq, scale, rows, k, None)
 
     for bad in ({"x": None}, {"gamma": None}, {"q": None}, {"scale": None}, {"residual": None}, {"out": None}, {"rows": 0}, {"k": 0},
-                {"ldx": 63}, {"ldr": 63}, {"ldq": 63}, {"eps": -1e-5}, {"eps": float("nan")}):
+                {"ldx": 63}, {"ldr": 63}, {"ldq": 63}, {"eps": -1e-5}, {"eps": float("nan")}, {"eps": float("inf")}):
         assert norm(**bad) == EINVAL, bad
     assert norm(t=5) == EFORMAT
     for bad in ({"x": odd(1)}, {"residual": odd(1)}, {"out": odd(1)}, {"gamma": odd(2)}, {"scale": odd(2)}, {"t": F32, "residual": odd(2)}):
