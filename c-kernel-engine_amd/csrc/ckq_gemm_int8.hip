@@ -22,6 +22,7 @@
  * cycle and CU.
  */
 #include "ckq_gemm_common.hpp"
+#include "ckq_int8.hpp"
 #include <atomic>
 
 struct I8Args {
@@ -314,8 +315,7 @@ static int launch_i8_tiles(const I8Args &a, hipStream_t s)
 {
     const int ntt = (a.M + T::BT - 1) / T::BT, nnt = (a.N + T::BN - 1) / T::BN;
     if ((long)ntt * nnt > 0x3fffff) return CKQ_EINVAL;       /* results beyond any memory */
-    hipLaunchKernelGGL((gemm_i8_tile_kernel<E, T>), dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::WAVES), 0, s, a, ntt, nnt);
-    return (int)hipGetLastError();
+    return i8_launch(gemm_i8_tile_kernel<E, T>, dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::WAVES), s, a, ntt, nnt);
 }
 template <class E, class T1, class T2>
 static int launch_i8_two_tiles(const I8Args &a, int nnt1, hipStream_t s)
@@ -323,9 +323,7 @@ static int launch_i8_two_tiles(const I8Args &a, int nnt1, hipStream_t s)
     const int ntt1 = (a.M + T1::BT - 1) / T1::BT, ntt2 = (a.M + T2::BT - 1) / T2::BT, nnt2 = (a.N - nnt1 * T1::BN + T2::BN - 1) / T2::BN;
     if ((long)ntt1 * nnt1 + (long)ntt2 * nnt2 > 0x3fffff) return CKQ_EINVAL;
     const int blocks1 = gemm_blocks(ntt1, nnt1);
-    hipLaunchKernelGGL((gemm_i8_two_tiles_kernel<E, T1, T2>), dim3((unsigned)(blocks1 + gemm_blocks(ntt2, nnt2))), dim3(64u * T1::WAVES), 0, s,
-                       a, ntt1, nnt1, blocks1, ntt2, nnt2);
-    return (int)hipGetLastError();
+    return i8_launch(gemm_i8_two_tiles_kernel<E, T1, T2>, dim3((unsigned)(blocks1 + gemm_blocks(ntt2, nnt2))), dim3(64u * T1::WAVES), s, a, ntt1, nnt1, blocks1, ntt2, nnt2);
 }
 
 /* ---- K split among the waves of a block ------------------------------------------------------------------------------ */
@@ -468,8 +466,7 @@ static int launch_i8_split(const I8Args &a, hipStream_t s)
 {
     const int ntt = (a.M + T::BT - 1) / T::BT, nnt = (a.N + T::BN - 1) / T::BN;
     if ((long)ntt * nnt > 0x3fffff) return CKQ_EINVAL;       /* results beyond any memory */
-    hipLaunchKernelGGL((gemm_i8_split_kernel<E, T>), dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::NW), 0, s, a, ntt, nnt);
-    return (int)hipGetLastError();
+    return i8_launch(gemm_i8_split_kernel<E, T>, dim3((unsigned)gemm_blocks(ntt, nnt)), dim3(64u * T::NW), s, a, ntt, nnt);
 }
 
 /* ---- few tokens: rows streamed ----------------------------------------------------------------------------------------- */
@@ -567,8 +564,7 @@ template <class E, int MT, int R, int KU, int KS>
 static int launch_i8_stream(const I8Args &a, hipStream_t s)
 {
     constexpr int per = 4 / KS * R;
-    hipLaunchKernelGGL((gemm_i8_stream_kernel<E, MT, R, KU, KS>), dim3((unsigned)((a.N + per - 1) / per)), dim3(256), 0, s, a);
-    return (int)hipGetLastError();
+    return i8_launch(gemm_i8_stream_kernel<E, MT, R, KU, KS>, dim3((unsigned)((a.N + per - 1) / per)), dim3(256), s, a);
 }
 
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */

@@ -15,6 +15,7 @@
  * bit patterns, where NaN > inf > everything else, and no order of lanes or waves can lose one.
  */
 #include "ckq_device.hpp"
+#include "ckq_int8.hpp"
 #include "ckq_launch.h"
 
 enum { ROWS_QUANTIZE, ROWS_RMSNORM, ROWS_SWIGLU };
@@ -297,11 +298,8 @@ static int launch_rows(RowsArgs a, hipStream_t s)
         const int left = a.rows, now = min(left, 1 << 21);
         a.rows = now;
         const dim3 grid((unsigned)(wpr == 1 ? (now + 3) / 4 : now));
-        if (per <= 1)      hipLaunchKernelGGL((rows_i8_kernel<OP, E, 1>), grid, block, 0, s, a, wpr);
-        else if (per <= 2) hipLaunchKernelGGL((rows_i8_kernel<OP, E, 2>), grid, block, 0, s, a, wpr);
-        else if (per <= 4) hipLaunchKernelGGL((rows_i8_kernel<OP, E, 4>), grid, block, 0, s, a, wpr);
-        else               hipLaunchKernelGGL((rows_i8_kernel<OP, E, 0>), grid, block, 0, s, a, wpr);
-        const int rc = (int)hipGetLastError();
+        const int rc = per <= 1 ? i8_launch(rows_i8_kernel<OP, E, 1>, grid, block, s, a, wpr) : per <= 2 ? i8_launch(rows_i8_kernel<OP, E, 2>, grid, block, s, a, wpr)
+                     : per <= 4 ? i8_launch(rows_i8_kernel<OP, E, 4>, grid, block, s, a, wpr) : i8_launch(rows_i8_kernel<OP, E, 0>, grid, block, s, a, wpr);
         if (rc || left == now) return rc;
         a.x = (const E *)a.x + (size_t)now * a.ldx;
         if (a.y) a.y = (const E *)a.y + (size_t)now * a.ldy;
@@ -393,12 +391,9 @@ extern "C" int ckq_launch_dequantize_i8(const int8_t *q, long ldq, const float *
         const int n = min(rows - row, most);
         const int8_t *qr = q + (size_t)row * ldq;
         const dim3 grid((unsigned)(((size_t)n * nvec + 255) / 256)), block(256);
-        switch (type) {
-        case CKQ_T_F32:  hipLaunchKernelGGL(dequantize_i8_kernel<float>, grid, block, 0, s, qr, ldq, scale + row, (float *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec); break;
-        case CKQ_T_BF16: hipLaunchKernelGGL(dequantize_i8_kernel<__bf16>, grid, block, 0, s, qr, ldq, scale + row, (__bf16 *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec); break;
-        default:         hipLaunchKernelGGL(dequantize_i8_kernel<_Float16>, grid, block, 0, s, qr, ldq, scale + row, (_Float16 *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec); break;
-        }
-        const int rc = (int)hipGetLastError();
+        const int rc = type == CKQ_T_F32  ? i8_launch(dequantize_i8_kernel<float>, grid, block, s, qr, ldq, scale + row, (float *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec)
+                     : type == CKQ_T_BF16 ? i8_launch(dequantize_i8_kernel<__bf16>, grid, block, s, qr, ldq, scale + row, (__bf16 *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec)
+                                          : i8_launch(dequantize_i8_kernel<_Float16>, grid, block, s, qr, ldq, scale + row, (_Float16 *)y + (size_t)row * ldy, ldy, (u32)n, k, nvec);
         if (rc) return rc;
         row += n;
     }
