@@ -203,28 +203,23 @@ def dev_gemm_nt_f32act(fmt, A_t, B_t, bias_t, M, N, K, out=None):
 
 
 # ---- rows of int8 with one scale each ---------------------------------------------
-# A decode step makes these calls one by one, each for a kernel of a few microseconds, so their checks are kept
-# to one look at a tensor's shape, strides, type and device each.
+# A decode step makes these calls one by one, each for a kernel of a few microseconds.  So a call looks at a tensor's
+# shape, strides, type and device once each, in one expression without calls of functions in Python (a matmul's checks 0.6 us less);
+# what that expression does not take goes to _i8_refuse, which looks again and says why.
 
-_torch, _started, _device, _raw_stream, _I8_TYPES = None, None, None, None, {}
+_torch, _INT8, _F32, _started, _device, _raw_stream, _I8_TYPES = None, None, None, None, None, None, {}
 
 
 def _i8_torch():
     """torch, and what every call needs of it, once: an import statement in each call costs it 0.3 us a time, a chain of names 0.05."""
-    global _torch, _started, _device, _raw_stream
+    global _torch, _INT8, _F32, _started, _device, _raw_stream
     import torch
+    _INT8, _F32 = torch.int8, torch.float32
     _I8_TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})   # CKDataType values
     _started = torch.cuda.is_initialized
     _device, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
     _torch = torch
     return torch
-
-
-def _i8_type(t):
-    v = _I8_TYPES.get(t)
-    if v is None:
-        raise CkqError("rows of %s: float32, bfloat16 or float16 are taken" % t)
-    return v
 
 
 def _i8_where():
@@ -240,30 +235,26 @@ def _i8_where():
     return dev, _raw_stream(dev)
 
 
-def _i8_rows(t, what, dev, shape=None, dtype=None):
-    """Checks a 2-d tensor of rows on device `dev`, elements of a row side by side; returns rows, their length and their pitch in
-    elements.  A single row has any stride in torch: its pitch counts as its length."""
-    s = t.shape
-    if len(s) != 2 or (shape is not None and s != shape):
-        raise CkqError("%s has the shape %s, not %s" % (what, tuple(s), "rows x k" if shape is None else tuple(shape)))
-    if dtype is not None and t.dtype is not dtype:
-        raise CkqError("%s is %s, not %s" % (what, t.dtype, dtype))
-    if t.get_device() != dev:
-        raise CkqError("%s is on %s, not on the current device" % (what, t.device))
-    rows, k = s
-    pitch, step = t.stride()
-    if step != 1 and k > 1:
-        raise CkqError("%s: the elements of a row have to lie side by side" % what)
-    return rows, k, pitch if rows > 1 else k
-
-
-def _i8_floats(t, what, dev, n):
-    """A contiguous vector of n floats on device `dev`: its address."""
-    if t.dtype is not _torch.float32 or t.shape != (n,) or not t.is_contiguous():
-        raise CkqError("%s has to be %d contiguous float32" % (what, n))
-    if t.get_device() != dev:
-        raise CkqError("%s is on %s, not on the current device" % (what, t.device))
-    return t.data_ptr()
+def _i8_refuse(dev, rows, floats):
+    """Says what is wrong with a call: rows, 2-d tensors (tensor, name, shape or None, type; None: one of floats), elements of a row side by
+    side; floats, contiguous float32 vectors (tensor, name, shape).  All on device `dev`."""
+    for t, what, shape, dtype in rows:
+        if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+            raise CkqError("%s has the shape %s, not %s" % (what, tuple(t.shape), "rows x k" if shape is None else tuple(shape)))
+        if dtype is None and t.dtype not in _I8_TYPES:
+            raise CkqError("%s is %s: float32, bfloat16 or float16 are taken" % (what, t.dtype))
+        if dtype is not None and t.dtype is not dtype:
+            raise CkqError("%s is %s, not %s" % (what, t.dtype, dtype))
+        if t.get_device() != dev:
+            raise CkqError("%s is on %s, not on the current device" % (what, t.device))
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise CkqError("%s: the elements of a row have to lie side by side" % what)
+    for t, what, shape in floats:
+        if t.dtype is not _F32 or t.shape != shape or not t.is_contiguous():
+            raise CkqError("%s has to be contiguous float32 of the shape %s" % (what, tuple(shape)))
+        if t.get_device() != dev:
+            raise CkqError("%s is on %s, not on the current device" % (what, t.device))
+    raise CkqError("two tensors of this call need one pitch")
 
 
 def empty_i8(rows, k, device="cuda"):
@@ -272,18 +263,29 @@ def empty_i8(rows, k, device="cuda"):
     return torch.empty(rows, -(-k // 16) * 16, dtype=torch.int8, device=device)[:, :k]
 
 
-def _i8_out(out, rows, k, x, dev):
-    q, scale = out if out is not None else (empty_i8(rows, k, x.device), _torch.empty(rows, dtype=_torch.float32, device=x.device))
-    ldq = _i8_rows(q, "q", dev, (rows, k), _torch.int8)[2]
-    return q, scale, ldq, _i8_floats(scale, "scale", dev, rows)
+def _i8_new(x):
+    if x.dim() != 2:
+        raise CkqError("a tensor of the shape %s, not rows x k" % (tuple(x.shape),))
+    return empty_i8(*x.shape, x.device), _torch.empty(x.shape[0], dtype=_F32, device=x.device)
 
+
+# A single row has any stride in torch: its pitch counts as its length.
 
 def dev_quantize_i8(x, out=None):
     """Rows of x [rows, k] in 8 bits: (q int8 [rows, k], scale float32 [rows])."""
     dev, stream = _i8_where()
-    rows, k, ldx = _i8_rows(x, "x", dev)
-    q, scale, ldq, sp = _i8_out(out, rows, k, x, dev)
-    rc = lib().ckq_quantize_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, q.data_ptr(), ldq, sp, rows, k, stream)
+    q, scale = out if out is not None else _i8_new(x)
+    shape, kind = x.shape, _I8_TYPES.get(x.dtype)
+    if (len(shape) != 2 or q.shape != shape or kind is None or q.dtype is not _INT8 or scale.dtype is not _F32 or scale.shape != shape[:1]
+            or not scale.is_contiguous() or not x.get_device() == q.get_device() == scale.get_device() == dev):
+        _i8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _INT8)], [(scale, "scale", shape[:1])])
+    rows, k = shape
+    (ldx, ex), (ldq, eq) = x.stride(), q.stride()
+    if (ex != 1 or eq != 1) and k > 1:
+        _i8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _INT8)], [])
+    if rows == 1:
+        ldx = ldq = k
+    rc = lib().ckq_quantize_i8_dev(kind, x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr(), rows, k, stream)
     if rc:
         check(rc, "ckq_quantize_i8_dev")
     return q, scale
@@ -292,11 +294,20 @@ def dev_quantize_i8(x, out=None):
 def dev_dequantize_i8(q, scale, dtype=None, out=None):
     """scale * q as rows of dtype (float32), or into `out`."""
     dev, stream = _i8_where()
-    rows, k, ldq = _i8_rows(q, "q", dev, None, _torch.int8)
-    sp = _i8_floats(scale, "scale", dev, rows)
-    y = out if out is not None else _torch.empty(rows, k, dtype=dtype or _torch.float32, device=q.device)
-    ldy = _i8_rows(y, "out", dev, (rows, k), dtype)[2]
-    rc = lib().ckq_dequantize_i8_dev(q.data_ptr(), ldq, sp, _i8_type(y.dtype), y.data_ptr(), ldy, rows, k, stream)
+    shape = q.shape
+    y = out if out is not None else _torch.empty(shape, dtype=dtype or _F32, device=q.device)
+    t = y.dtype
+    kind = _I8_TYPES.get(t)
+    if (len(shape) != 2 or y.shape != shape or kind is None or (dtype is not None and t is not dtype) or q.dtype is not _INT8 or scale.dtype is not _F32
+            or scale.shape != shape[:1] or not scale.is_contiguous() or not q.get_device() == scale.get_device() == y.get_device() == dev):
+        _i8_refuse(dev, [(q, "q", None, _INT8), (y, "out", shape, None), (y, "out", shape, dtype)], [(scale, "scale", shape[:1])])
+    rows, k = shape
+    (ldq, eq), (ldy, ey) = q.stride(), y.stride()
+    if (eq != 1 or ey != 1) and k > 1:
+        _i8_refuse(dev, [(q, "q", None, _INT8), (y, "out", shape, None)], [])
+    if rows == 1:
+        ldq = ldy = k
+    rc = lib().ckq_dequantize_i8_dev(q.data_ptr(), ldq, scale.data_ptr(), kind, y.data_ptr(), ldy, rows, k, stream)
     if rc:
         check(rc, "ckq_dequantize_i8_dev")
     return y
@@ -306,20 +317,33 @@ def dev_rmsnorm_i8(x, gamma, eps=1e-6, residual=None, residual_out=None, out=Non
     """RMSNorm(x (+ residual)) * gamma in 8 bits: (q, scale), or (q, scale, x + residual) with a residual; residual_out
     may be the residual itself, or x."""
     dev, stream = _i8_where()
-    rows, k, ldx = _i8_rows(x, "x", dev)
-    gp = _i8_floats(gamma, "gamma", dev, k)
-    q, scale, ldq, sp = _i8_out(out, rows, k, x, dev)
-    ldr, rp, op = 0, None, None
+    q, scale = out if out is not None else _i8_new(x)
+    shape, t = x.shape, x.dtype
+    kind = _I8_TYPES.get(t)
+    if (len(shape) != 2 or q.shape != shape or kind is None or q.dtype is not _INT8 or scale.dtype is not _F32 or gamma.dtype is not _F32
+            or scale.shape != shape[:1] or gamma.shape != shape[1:] or not scale.is_contiguous() or not gamma.is_contiguous()
+            or not x.get_device() == q.get_device() == scale.get_device() == gamma.get_device() == dev):
+        _i8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _INT8)], [(scale, "scale", shape[:1]), (gamma, "gamma", shape[1:])])
+    rows, k = shape
+    (ldx, ex), (ldq, eq) = x.stride(), q.stride()
+    ldr, rp, hp = 0, None, None
     if residual is not None:
-        ldr = _i8_rows(residual, "residual", dev, (rows, k), x.dtype)[2]
         if residual_out is None:
-            residual_out = _torch.empty_strided(residual.shape, residual.stride(), dtype=x.dtype, device=x.device)
-        if _i8_rows(residual_out, "residual_out", dev, (rows, k), x.dtype)[2] != ldr:
-            raise CkqError("residual and residual_out need one pitch")
-        rp, op = residual.data_ptr(), residual_out.data_ptr()
+            residual_out = _torch.empty_strided(residual.shape, residual.stride(), dtype=t, device=x.device)
+        if (residual.shape != shape or residual_out.shape != shape or residual.dtype is not t or residual_out.dtype is not t
+                or not residual.get_device() == residual_out.get_device() == dev):
+            _i8_refuse(dev, [(residual, "residual", shape, t), (residual_out, "residual_out", shape, t)], [])
+        (ldr, er), (ldh, eh) = residual.stride(), residual_out.stride()
+        if (er != 1 or eh != 1) and k > 1 or ldr != ldh and rows > 1:
+            _i8_refuse(dev, [(residual, "residual", shape, t), (residual_out, "residual_out", shape, t)], [])
+        rp, hp = residual.data_ptr(), residual_out.data_ptr()
     elif residual_out is not None:
         raise CkqError("residual_out without a residual")
-    rc = lib().ckq_rmsnorm_i8_dev(_i8_type(x.dtype), x.data_ptr(), ldx, rp, op, ldr, gp, eps, q.data_ptr(), ldq, sp, rows, k, stream)
+    if (ex != 1 or eq != 1) and k > 1:
+        _i8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _INT8)], [])
+    if rows == 1:
+        ldx = ldq = ldr = k
+    rc = lib().ckq_rmsnorm_i8_dev(kind, x.data_ptr(), ldx, rp, hp, ldr, gamma.data_ptr(), eps, q.data_ptr(), ldq, scale.data_ptr(), rows, k, stream)
     if rc:
         check(rc, "ckq_rmsnorm_i8_dev")
     return (q, scale) if residual is None else (q, scale, residual_out)
@@ -328,11 +352,19 @@ def dev_rmsnorm_i8(x, gamma, eps=1e-6, residual=None, residual_out=None, out=Non
 def dev_swiglu_i8(gate, up, out=None):
     """SiLU(gate) * up in 8 bits: (q, scale); gate and up have one pitch (halves of one tensor, say)."""
     dev, stream = _i8_where()
-    rows, k, ld = _i8_rows(gate, "gate", dev)
-    if _i8_rows(up, "up", dev, (rows, k), gate.dtype)[2] != ld:
-        raise CkqError("gate and up need one pitch")
-    q, scale, ldq, sp = _i8_out(out, rows, k, gate, dev)
-    rc = lib().ckq_swiglu_i8_dev(_i8_type(gate.dtype), gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, sp, rows, k, stream)
+    q, scale = out if out is not None else _i8_new(gate)
+    shape, t = gate.shape, gate.dtype
+    kind = _I8_TYPES.get(t)
+    if (len(shape) != 2 or q.shape != shape or up.shape != shape or kind is None or up.dtype is not t or q.dtype is not _INT8 or scale.dtype is not _F32
+            or scale.shape != shape[:1] or not scale.is_contiguous() or not gate.get_device() == up.get_device() == q.get_device() == scale.get_device() == dev):
+        _i8_refuse(dev, [(gate, "gate", None, None), (up, "up", shape, t), (q, "q", shape, _INT8)], [(scale, "scale", shape[:1])])
+    rows, k = shape
+    (ld, eg), (ldu, eu), (ldq, eq) = gate.stride(), up.stride(), q.stride()
+    if (eg != 1 or eu != 1 or eq != 1) and k > 1 or ldu != ld and rows > 1:
+        _i8_refuse(dev, [(gate, "gate", None, None), (up, "up", shape, t), (q, "q", shape, _INT8)], [])
+    if rows == 1:
+        ld = ldq = k
+    rc = lib().ckq_swiglu_i8_dev(kind, gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), rows, k, stream)
     if rc:
         check(rc, "ckq_swiglu_i8_dev")
     return q, scale
@@ -342,19 +374,31 @@ def dev_gemm_nt_i8(a, sa, b, sb, bias=None, dtype=None, out=None):
     """C [M, N] = sa[m] * sb[n] * (a b^T) (+ bias[n]): int8 rows a [M, K] (tokens), b [N, K] (channels); C of dtype (float32),
     or into `out`."""
     dev, stream = _i8_where()
-    M, K, lda = _i8_rows(a, "a", dev, None, _torch.int8)
-    N, Kb, ldb = _i8_rows(b, "b", dev, None, _torch.int8)
-    if Kb != K:
-        raise CkqError("a and b have rows of %d and %d" % (K, Kb))
+    of_a, of_b = a.shape, b.shape
+    if len(of_a) != 2 or len(of_b) != 2 or of_a[1] != of_b[1]:
+        _i8_refuse(dev, [(a, "a", None, _INT8), (b, "b", (of_b[0], of_a[1]) if a.dim() == b.dim() == 2 else None, _INT8)], [])
+    M, K = of_a
+    N = of_b[0]
+    c = out if out is not None else _torch.empty(M, N, dtype=dtype or _F32, device=b.device)
+    t = c.dtype
+    kind = _I8_TYPES.get(t)
+    if (c.shape != (M, N) or kind is None or (dtype is not None and t is not dtype) or a.dtype is not _INT8 or b.dtype is not _INT8 or sa.dtype is not _F32 or sb.dtype is not _F32
+            or sa.shape != (M,) or sb.shape != (N,) or not sa.is_contiguous() or not sb.is_contiguous()
+            or not a.get_device() == b.get_device() == c.get_device() == sa.get_device() == sb.get_device() == dev):
+        _i8_refuse(dev, [(a, "a", None, _INT8), (b, "b", None, _INT8), (c, "out", (M, N), None), (c, "out", (M, N), dtype)], [(sa, "sa", (M,)), (sb, "sb", (N,))])
+    bp = None
+    if bias is not None:
+        if bias.dtype is not _F32 or bias.shape != (N,) or not bias.is_contiguous() or bias.get_device() != dev:
+            _i8_refuse(dev, [], [(bias, "bias", (N,))])
+        bp = bias.data_ptr()
+    (lda, ea), (ldb, eb), (ldc, ec) = a.stride(), b.stride(), c.stride()
+    if (ea != 1 or eb != 1) and K > 1 or ec != 1 and N > 1:
+        _i8_refuse(dev, [(a, "a", None, _INT8), (b, "b", None, _INT8), (c, "out", (M, N), None)], [])
     if M == 1:
-        lda = -(-K // 16) * 16
+        lda, ldc = -(-K // 16) * 16, N
     if N == 1:
         ldb = -(-K // 16) * 16
-    sap, sbp = _i8_floats(sa, "sa", dev, M), _i8_floats(sb, "sb", dev, N)
-    bp = None if bias is None else _i8_floats(bias, "bias", dev, N)
-    c = out if out is not None else _torch.empty(M, N, dtype=dtype or _torch.float32, device=b.device)
-    ldc = _i8_rows(c, "out", dev, (M, N), dtype)[2]
-    rc = lib().ckq_gemm_nt_i8_dev(a.data_ptr(), lda, sap, b.data_ptr(), ldb, sbp, bp, _i8_type(c.dtype), c.data_ptr(), ldc, M, N, K, stream)
+    rc = lib().ckq_gemm_nt_i8_dev(a.data_ptr(), lda, sa.data_ptr(), b.data_ptr(), ldb, sb.data_ptr(), bp, kind, c.data_ptr(), ldc, M, N, K, stream)
     if rc:
         check(rc, "ckq_gemm_nt_i8_dev")
     return c
