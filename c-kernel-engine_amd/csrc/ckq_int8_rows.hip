@@ -31,9 +31,10 @@ struct __attribute__((packed, aligned(1))) row8q { u32 v[2]; };
 
 /* The same as loaded, in whole registers. */
 template <class E> struct raw8 { u32 w[2 * sizeof(E)]; };
+typedef float rows_f4 __attribute__((ext_vector_type(4)));
 typedef u32 rows_u4 __attribute__((ext_vector_type(4)));
 typedef rows_u4 __attribute__((aligned(2))) rows_u4_at_2;    /* one load of 16 bytes, wherever it falls */
-template <class E, bool ONCE = false>                        /* ONCE: read for the last time, kept in no cache */
+template <bool ONCE, class E>                                /* ONCE: read for the last time, kept in no cache */
 __device__ __forceinline__ raw8<E> fetch8(const E *p, int left)
 {
     raw8<E> r;
@@ -57,6 +58,22 @@ __device__ __forceinline__ raw8<E> fetch8(const E *p, int left)
         }
     return r;
 }
+/* The elements from `drop` (0 .. 7) on, and zeros. */
+template <class E>
+__device__ __forceinline__ void drop_first(raw8<E> &r, int drop)
+{
+    constexpr int N = 2 * sizeof(E), PER = 4 / sizeof(E);    /* dwords, elements of one */
+    if (PER == 2 && (drop & 1)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.w[i] = r.w[i] >> 16 | (i + 1 < N ? r.w[i + 1] << 16 : 0u);
+    }
+#pragma unroll
+    for (int by = 1; by < N; by *= 2)
+        if (drop & (by * PER)) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) r.w[i] = i + by < N ? r.w[i + by] : 0u;
+        }
+}
 template <class E>
 __device__ __forceinline__ float raw_value(const raw8<E> &r, int i)
 {
@@ -71,6 +88,7 @@ __device__ __forceinline__ void store8(E *p, const float (&f)[8], int left)
 #pragma unroll
         for (int i = 0; i < 8; ++i) r.v[i] = (E)f[i];
         *reinterpret_cast<row8<E> *>(p) = r;
+        asm volatile("");                                    /* or what both branches store is moved behind them, in pieces */
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -97,9 +115,25 @@ template <int OP, bool ONCE, class E>
 __device__ __forceinline__ void row_fetch(RowParts<E> &p, const RowsArgs &a, const E *x, const E *y, int v)
 {
     const int left = a.k - 8 * v;
-    p.x = fetch8<E, ONCE>(x + 8 * v, left);
-    if (OP != ROWS_QUANTIZE && y) p.y = fetch8<E, ONCE>(y + 8 * v, left);
-    if (OP == ROWS_RMSNORM) p.g = fetch8(a.gamma + 8 * v, left);
+    p.x = fetch8<ONCE>(x + 8 * v, left);
+    if (OP != ROWS_QUANTIZE && y) p.y = fetch8<ONCE>(y + 8 * v, left);
+    if (OP == ROWS_RMSNORM) p.g = fetch8<false>(a.gamma + 8 * v, left);
+}
+
+/* The same of a row of eight elements and more: its last vector, where it is not whole, is cut out of the row's last eight elements, so that every lane has the same
+ * loads.  (Some of those eight may be written by the lane before it, if the sum goes where x is: these are dropped.) */
+template <int OP, bool ONCE, class E>
+__device__ __forceinline__ void row_fetch_even(RowParts<E> &p, const RowsArgs &a, const E *x, const E *y, int v)
+{
+    const int at = min(8 * v, a.k - 8), drop = 8 * v - at;
+    p.x = fetch8<ONCE>(x + at, 8);
+    if (OP != ROWS_QUANTIZE && y) p.y = fetch8<ONCE>(y + at, 8);
+    if (OP == ROWS_RMSNORM) p.g = fetch8<false>(a.gamma + at, 8);
+    if ((a.k & 7) && drop) {
+        drop_first(p.x, drop);
+        if (OP != ROWS_QUANTIZE && y) drop_first(p.y, drop);
+        if (OP == ROWS_RMSNORM) drop_first(p.g, drop);
+    }
 }
 
 /* The values themselves, rmsnorm's without the row's factor r; `ss` collects the squares.  x + residual goes to h, where it is not null. */
@@ -149,6 +183,15 @@ __device__ __forceinline__ u32 wave_top(u32 v)
     v = max(v, (u32)dpp_get<0x143, 0xC>((int)v));
     return (u32)__builtin_amdgcn_readlane((int)v, 63);
 }
+/* Of the first sixteen lanes alone. */
+__device__ __forceinline__ u32 row_top(u32 v)
+{
+    v = max(v, (u32)dpp_get<0xB1>((int)v));
+    v = max(v, (u32)dpp_get<0x4E>((int)v));
+    v = max(v, (u32)dpp_get<0x141>((int)v));
+    v = max(v, (u32)dpp_get<0x140>((int)v));
+    return (u32)__builtin_amdgcn_readlane((int)v, 0);
+}
 __device__ __forceinline__ float wave_sum(float v)
 {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, group_sum<64>(v)), 63));
@@ -162,11 +205,18 @@ __device__ __forceinline__ u32 rounded_bits(float e, float inv)
 }
 
 /* NV > 0: `wpr` waves have a row, each thread at most NV vectors of it, held in registers between the two passes (k <= 512 wpr NV);
- * NV = 0: rows of any length, read again for the second pass. */
+ * NV = 0: rows of any length, read again for the second pass: those longer than 32768, of sixteen waves each, and those shorter than eight.
+ *
+ * A row's squares are added in an order that its length alone decides, so that its results have the same bits alone and in any batch, though the
+ * number of rows decides how many waves share it: each group of 512 elements by one wave, in the tree of its lanes; groups whose numbers differ by a multiple of
+ * sixteen in turn; these sums, at most sixteen, in turn.  (NV = 0: each thread's elements, its wave's threads, the waves.)  It costs a wave of several groups a reduction for each of
+ * them, nothing that shows beside the memory (us with one reduction a wave | now: norm in bf16 of 2048 x 4096 11.2 | 11.2, of 2048 x 8192 25.5 | 24.7, of one row of
+ * 4096 2.73 | 2.69).
+ */
 template <int OP, class E, int NV>
 __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
 {
-    __shared__ float red_ss[16];
+    __shared__ __attribute__((aligned(16))) float red_ss[NV == 4 ? 32 : 16];
     __shared__ u32   red_top[16];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), nw = blockDim.x >> 6;
     const int row = __builtin_amdgcn_readfirstlane(wpr == 1 ? (int)blockIdx.x * nw + wave : (int)blockIdx.x);
@@ -177,8 +227,10 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
     E *h = a.h ? (E *)a.h + (size_t)row * a.ldh : nullptr;
     const int nvec = (a.k >> 3) + ((a.k & 7) != 0), first = wpr == 1 ? lane : (int)threadIdx.x, step = 64 * wpr;
 
-    float f[NV > 0 ? NV : 1][8], ss = 0.0f;
+    float f[NV > 0 ? NV : 1][8], sq[NV > 0 ? NV : 1], ss = 0.0f;
     u32 top = 0;
+#pragma unroll
+    for (int i = 0; i < (NV > 0 ? NV : 1); ++i) sq[i] = 0.0f;
     if (NV > 0) {
         /* A vector's loads are under way together, gamma's too, before the store to h (which may be x or the residual, so that the compiler moves none
          * across it): one row of 4096 3.0 -> 2.7 us.  Those of two vectors and more only in the quantizer (2048 x 11008 in fp32 18.6 -> 17.6): elsewhere
@@ -191,6 +243,16 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
         constexpr bool ONCE = OP != ROWS_RMSNORM;
 #pragma unroll
         for (int c = 0; c < NV; c += CH) {
+            if (CH == 1) {
+                const int v = first + c * step;
+                if (v < nvec) {
+                    RowParts<E> p;
+                    row_fetch_even<OP, ONCE>(p, a, x, y, v);
+                    row_values<OP>(f[c], p, y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, sq[c]);
+                    top = top_bits(f[c], top);
+                }
+                continue;
+            }
             RowParts<E> p[CH];
 #pragma unroll
             for (int i = 0; i < CH; ++i)
@@ -199,7 +261,7 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
             for (int i = 0; i < CH; ++i) {
                 const int v = first + (c + i) * step;
                 if (v < nvec) {
-                    row_values<OP>(f[c + i], p[i], y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, ss);
+                    row_values<OP>(f[c + i], p[i], y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, sq[c + i]);
                     top = top_bits(f[c + i], top);
                 }
             }
@@ -208,24 +270,50 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
         for (int v = first; v < nvec; v += step) {
             RowParts<E> p;
             row_fetch<OP, false>(p, a, x, y, v);
-            row_values<OP>(f[0], p, y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, ss);
+            row_values<OP>(f[0], p, y != nullptr, h ? h + 8 * v : nullptr, a.k - 8 * v, sq[0]);
             top = top_bits(f[0], top);
         }
 
     top = wave_top(top);
-    if (OP == ROWS_RMSNORM) ss = wave_sum(ss);
+    if (OP == ROWS_RMSNORM) {
+#pragma unroll
+        for (int i = 0; i < (NV > 0 ? NV : 1); ++i) sq[i] = wave_sum(sq[i]);
+    }
+    if (wpr == 1 || wpr == 16) {                             /* a wave has all groups of a row, or those that differ by multiples of sixteen */
+#pragma unroll
+        for (int i = 0; i < (NV > 0 ? NV : 1); ++i) ss += sq[i];
+    }
     if (wpr > 1) {
+        const int groups = wpr == 16 ? 16 : (NV > 0 ? NV : 1) * wpr;                  /* more than 16: three a wave of eight */
         if (lane == 0) {
             red_top[wave] = top;
-            if (OP == ROWS_RMSNORM) red_ss[wave] = ss;
+            if (OP == ROWS_RMSNORM && wpr == 16) red_ss[wave] = ss;
+            if (OP == ROWS_RMSNORM && wpr < 16) {
+#pragma unroll
+                for (int i = 0; i < (NV > 0 ? NV : 1); ++i) red_ss[wave + i * wpr] = sq[i];
+            }
         }
         __syncthreads();
-        top = 0;
-        ss = 0.0f;
-        for (int w = 0; w < nw; ++w) {                       /* in the same order for every wave */
-            top = max(top, red_top[w]);
-            if (OP == ROWS_RMSNORM) ss += red_ss[w];
+        /* the reads together: a loop over the waves waits for each by itself */
+        const u32 tops = (lane & 15) < nw ? red_top[lane & 15] : 0u;
+        if (OP == ROWS_RMSNORM) {
+            const rows_f4 *red = reinterpret_cast<const rows_f4 *>(red_ss);
+            rows_f4 col[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) col[i] = red[i];
+            if (NV == 4 && groups > 16) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) col[i] += red[4 + i];
+            }
+            ss = col[0][0] + col[0][1];
+            if (groups > 2) ss = ss + col[0][2] + col[0][3];
+            if (groups > 4) ss = ss + col[1][0] + col[1][1] + col[1][2] + col[1][3];
+            if (groups > 8) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss += col[2 + i / 4][i % 4];
+            }
         }
+        top = row_top(tops);
     }
 
     const float ftop = __builtin_bit_cast(float, top);
@@ -270,7 +358,7 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
             /* x + residual again from where this thread has stored it: x or the residual may be gone by now */
             const bool stored = OP == ROWS_RMSNORM && y;
             row_fetch<OP, false>(p, a, stored ? (const E *)h : x, OP == ROWS_RMSNORM ? nullptr : y, v);
-            row_values<OP, E>(f[0], p, false, nullptr, a.k - 8 * v, ss);
+            row_values<OP>(f[0], p, false, (E *)nullptr, a.k - 8 * v, ss);
             put(f[0], v);
         }
 }
@@ -291,7 +379,7 @@ template <int OP, class E>
 static int launch_rows(RowsArgs a, hipStream_t s)
 {
     const int nvec = a.k / 8 + (a.k % 8 != 0);
-    const int wpr = rows_waves(nvec, a.rows), per = (nvec - 1) / (64 * wpr) + 1;
+    const int wpr = rows_waves(nvec, a.rows), per = a.k < 8 ? 5 : (nvec - 1) / (64 * wpr) + 1;    /* 5: any length */
     const dim3 block(wpr == 1 ? 256u : 64u * (unsigned)wpr);
     /* a launch has fewer than 2^32 threads */
     for (;;) {

@@ -220,6 +220,22 @@ def test_rmsnorm_pitches_zero_rows_and_rows_that_are_not_finite(k):
         assert (q == 0).all() and s.isnan().all()
 
 
+# lengths on both sides of each change of the waves that share a row, of few rows and of more than 256
+SWITCHES = [512, 513, 1024, 1025, 1536, 1537, 2049, 3000, 3080, 4096, 4097, 6144, 6145, 8192, 8193, 11008, 12288, 12289, 16385, 24577, 32768, 32769]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k", SWITCHES)
+def test_rmsnorm_has_the_same_bits_in_any_batch(t, k):
+    """The number of rows decides how many waves share one, and nothing of what they compute."""
+    x, res = normal(300, k, k).to(TYPES[t]).cuda(), normal(300, k, k + 1).to(TYPES[t]).cuda()
+    gamma = (torch.rand(k, generator=torch.Generator().manual_seed(k)) + 0.25).cuda()
+    q, s, h = P.dev_rmsnorm_i8(x, gamma, 1e-6, residual=res)
+    for rows in (slice(0, 256), slice(0, 257), slice(7, 8), slice(290, 300)):
+        q1, s1, h1 = P.dev_rmsnorm_i8(x[rows], gamma, 1e-6, residual=res[rows])
+        assert torch.equal(s1, s[rows]) and torch.equal(q1, q[rows]) and torch.equal(h1, h[rows]), rows
+
+
 @pytest.mark.parametrize("k", [9, 600, 40000])
 def test_rmsnorm_of_small_rows_without_eps(k):
     x = normal(3, k, k) * 2.0 ** -60
