@@ -319,11 +319,8 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
     const float ftop = __builtin_bit_cast(float, top);
     const float r = OP == ROWS_RMSNORM ? 1.0f / sqrtf(ss / (float)a.k + a.eps) : 1.0f;
     /* an infinity or a NaN in the row; the squares' sum beyond fp32 (r = 0); a row of zeros and no eps (r infinite) */
-    const bool finite = ftop * r < __builtin_inff() && r > 0.0f;
-    const float amax = fmaxf(ftop * r, 0x1p-100f);
-    const float inv = fminf(127.0f / amax * r, 0x1.fffffep127f);     /* gamma of zeros after squares without an eps: 0 * inv has to be 0 */
-    if (first == 0) a.scale[row] = finite ? amax / 127.0f : top >= 0x7f800000u ? ftop : r > 0.0f ? ftop * r : __builtin_nanf("");
-
+    bool finite = ftop * r < __builtin_inff() && r > 0.0f;
+    float amax = fmaxf(ftop * r, 0x1p-100f), inv = fminf(127.0f / amax * r, 0x1.fffffep127f);      /* gamma of zeros: 0 * inv has to be 0 */
     int8_t *q = a.q + (size_t)row * a.ldq;
     auto put = [&](const float (&e)[8], int v) {
         /* e inv in fp32, plus 1.5 * 2^23: the nearest integer (ties to even) in the low bits, |e inv| <= 127 (1 + 2^-22).  Not in one multiply-add,
@@ -346,6 +343,81 @@ __global__ void __launch_bounds__(1024) rows_i8_kernel(RowsArgs a, int wpr)
                 if (i < left) q[8 * v + i] = (int8_t)sbyte(p[i >> 2], i & 3);
         }
     };
+    if (OP == ROWS_RMSNORM && (r > 0x1p26f || (r > 0.0f && top != 0 && ftop < 0x1p-100f))) {
+        /* So small (rms and sqrt(eps) under 2^-26, or sum * gamma under 2^-100) that squares or sum * gamma may be below what fp32 holds: the row again from memory, the
+         * larger of its largest element and sqrt(eps) made one half to one, in the order of the formula.  All waves of a row come here or none. */
+        const E *src = y ? (const E *)h : x;
+        const int groups = (nvec + 63) >> 6, w0 = wpr == 1 ? 0 : wave;
+        auto each = [&](int g, auto &&use) {                 /* this lane's vector of a group, if there is one: its elements, and gamma's */
+            const int v = 64 * g + lane;
+            if (v >= nvec) return;
+            const int left = a.k - 8 * v;
+            use(fetch8<false>(src + 8 * v, left), fetch8<false>(a.gamma + 8 * v, left), v);
+        };
+        auto meet = [&](u32 t) {                             /* largest of the row */
+            t = wave_top(t);
+            if (wpr == 1) return t;
+            __syncthreads();                                 /* what was there has been read */
+            if (lane == 0) red_top[wave] = t;
+            __syncthreads();
+            return row_top((lane & 15) < nw ? red_top[lane & 15] : 0u);
+        };
+        u32 t = 0;
+        for (int g = w0; g < groups; g += wpr)
+            each(g, [&](const raw8<E> &e, const raw8<float> &, int) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t = max(t, __builtin_bit_cast(u32, raw_value<E>(e, i)) & 0x7fffffffu);
+            });
+        const float big = fmaxf(__builtin_bit_cast(float, meet(t)), sqrtf(a.eps));
+        const int up = max(0, -__builtin_amdgcn_frexp_expf(big));
+        float sum = 0.0f;
+        for (int c = w0; c < 16; c += wpr) {                 /* in the order of above */
+            float part = 0.0f;
+            for (int g = c; g < groups; g += 16) {
+                float s = 0.0f;
+                each(g, [&](const raw8<E> &e, const raw8<float> &, int) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float b = __builtin_ldexpf(raw_value<E>(e, i), up);
+                        s = __builtin_fmaf(b, b, s);
+                    }
+                });
+                part += wave_sum(s);
+            }
+            if (wpr == 1) sum += part;
+            else if (lane == 0) red_ss[c] = part;
+        }
+        if (wpr > 1) {
+            __syncthreads();
+            for (int c = 0; c < 16; ++c) sum += red_ss[c];
+        }
+        const float rs = 1.0f / sqrtf(sum / (float)a.k + __builtin_ldexpf(a.eps, 2 * up));
+        auto values = [&](float (&o)[8], const raw8<E> &e, const raw8<float> &g) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = __builtin_ldexpf(raw_value<E>(e, i), up) * rs * raw_value<float>(g, i);
+        };
+        t = 0;
+        for (int g = w0; g < groups; g += wpr)
+            each(g, [&](const raw8<E> &e, const raw8<float> &gm, int) {
+                float o[8];
+                values(o, e, gm);
+                t = top_bits(o, t);
+            });
+        t = meet(t);
+        const float most = __builtin_bit_cast(float, t);
+        finite = big > 0.0f && most < __builtin_inff();      /* zeros and no eps: no norm */
+        amax = fmaxf(most, 0x1p-100f);
+        inv = 127.0f / amax;
+        if (first == 0) a.scale[row] = finite ? amax / 127.0f : big > 0.0f ? most : __builtin_nanf("");
+        for (int g = w0; g < groups; g += wpr)
+            each(g, [&](const raw8<E> &e, const raw8<float> &gm, int v) {
+                float o[8];
+                values(o, e, gm);
+                put(o, v);
+            });
+        return;
+    }
+    if (first == 0) a.scale[row] = finite ? amax / 127.0f : top >= 0x7f800000u ? ftop : r > 0.0f ? ftop * r : __builtin_nanf("");
     if (NV > 0) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {

@@ -244,6 +244,56 @@ def test_rmsnorm_of_small_rows_without_eps(k):
         check_norm(q, s, x, gamma, 0.0)
 
 
+SMALL = [(2.0 ** -60, 2.0 ** -65, 0.0), (2.0 ** -60, 2.0 ** -80, 0.0), (2.0 ** -74, 1.0, 0.0), (2.0 ** -100, 2.0 ** 60, 0.0), (2.0 ** -118, 1.0, 0.0), (1.0, 2.0 ** -104, 1e-6),
+         (2.0 ** -60, 1.0, 1e-30), (2.0 ** -100, 2.0 ** 40, 1e-38), (2.0 ** -110, 2.0 ** 100, 2.0 ** -140), (2.0 ** -45, 2.0 ** -90, 2.0 ** -90)]
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("size,gsize,eps", SMALL)
+def test_rmsnorm_of_rows_whose_squares_or_products_are_below_fp32(t, size, gsize, eps):
+    """The same bounds as of any row, with and without a residual, in place, and the same bits in any batch."""
+    for k in (5, 256, 1001, 4096, 11001, 40000):
+        x = (normal(300 if k < 5000 else 3, k, k) * size).to(TYPES[t])
+        gamma = (torch.rand(k, generator=torch.Generator().manual_seed(k)) + 0.5) * gsize
+        x[1] *= 2.0 ** 20 if size < 1 else 1.0
+        q, s = P.dev_rmsnorm_i8(x.cuda(), gamma.cuda(), eps)
+        check_norm(q, s, x, gamma, eps)
+        for rows in (slice(0, 1), slice(1, 3)):
+            q1, s1 = P.dev_rmsnorm_i8(x[rows].cuda(), gamma.cuda(), eps)
+            assert torch.equal(q1, q[rows]) and torch.equal(s1, s[rows])
+        half = (x.double() / 2).to(TYPES[t])
+        into = half[:3].cuda()
+        q2, s2, h2 = P.dev_rmsnorm_i8(half[:3].cuda(), gamma.cuda(), eps, residual=into, residual_out=into)
+        check_norm(q2, s2, h2.cpu(), gamma, eps)
+
+
+def test_rmsnorm_of_small_rows_in_half_precision():
+    for size, gsize in ((2.0 ** -20, 2.0 ** -100), (2.0 ** -22, 2.0 ** -80), (1.0, 2.0 ** -102)):
+        for k in (300, 9000):
+            x = (normal(3, k, k) * size).half()
+            gamma = (torch.rand(k, generator=torch.Generator().manual_seed(k)) + 0.5) * gsize
+            q, s = P.dev_rmsnorm_i8(x.cuda(), gamma.cuda(), 0.0)
+            check_norm(q, s, x, gamma, 0.0)
+
+
+@pytest.mark.parametrize("k", [7, 512, 3000, 12000, 40000])
+def test_rmsnorm_zeros_and_infinities_among_small_rows(k):
+    x = normal(6, k, k) * 2.0 ** -80
+    x[1] = 0
+    x[2, 1] = float("inf")
+    x[3, k - 1] = float("nan")
+    ones = torch.ones(k)
+    q, s = (v.cpu() for v in P.dev_rmsnorm_i8(x.cuda(), ones.cuda(), 0.0))
+    assert (q[1:4] == 0).all() and s[1].isnan() and not s[2].isfinite() and s[3].isnan()
+    check_norm(q[[0, 4, 5]], s[[0, 4, 5]], x[[0, 4, 5]], ones, 0.0)
+    q, s = (v.cpu() for v in P.dev_rmsnorm_i8(x.cuda(), ones.cuda(), 2.0 ** -120))      # zeros over sqrt(eps)
+    assert (q[1] == 0).all() and s[1] == np.float32(TINY / 127)
+    for bad in (float("nan"), float("inf")):
+        ones[0] = bad
+        q, s = (v.cpu() for v in P.dev_rmsnorm_i8(x[4:].cuda(), ones.cuda(), 0.0))
+        assert (q == 0).all() and not s.isfinite().any()
+
+
 # ---- SwiGLU ----------------------------------------------------------------------------------
 
 def check_swiglu(q, s, gate, up):
