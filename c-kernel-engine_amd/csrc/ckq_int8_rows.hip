@@ -496,6 +496,7 @@ extern "C" int ckq_launch_rmsnorm_i8(int type, const void *x, long ldx, const vo
                                      int8_t *q, long ldq, float *scale, int rows, int k, void *stream)
 {
     if (!x || !gamma || !q || !scale || rows <= 0 || k <= 0 || ldx < k || ldq < k) return CKQ_EINVAL;
+    if (sum == x && ldr != ldx && rows > 1) return CKQ_EINVAL;        /* rows would be overwritten before they are read */
     if (!residual != !sum || (residual && ldr < k) || !(eps >= 0.0f && eps < __builtin_inff())) return CKQ_EINVAL;
     if (!row_size(type)) return CKQ_EFORMAT;
     if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)sum) % row_size(type) || ((uintptr_t)scale | (uintptr_t)gamma) % 4) return CKQ_EROWS;

@@ -296,7 +296,7 @@ int ckq_gemm_nt_f32act_dev(int fmt, const float *A, const void *B, const float *
  * ckq_dequantize_i8_dev: y = scale * q, rounded to the type.
  * ckq_rmsnorm_i8_dev: sum = x + residual, rounded to the type (`residual` and `sum` both NULL: there is none, and the norm is of
  * x); then sum * (1 / sqrt(mean of sum^2 + eps)) * gamma in 8 bits as above (eps finite and >= 0, else CKQ_EINVAL).  residual and sum have one pitch, ldr; sum may be
- * residual itself, or x (with ldr = ldx).  Squares are summed in fp32: a row whose sum of squares, or whose sum * gamma, exceeds fp32
+ * residual itself, or x (with ldr = ldx, else CKQ_EINVAL).  Squares are summed in fp32: a row whose sum of squares, or whose sum * gamma, exceeds fp32
  * gets a scale that is not finite, and zeros as its quants, as does a row of zeros without an eps.  Rows, gamma and eps may be as small as their types hold.
  * ckq_swiglu_i8_dev: gate / (1 + exp(-gate)) * up in 8 bits as above (0 under -88.72, where exp(-gate) exceeds fp32); gate and up have one pitch, ld, so that both may be halves
  * of one row (the output of a projection that holds the rows of both).

@@ -244,6 +244,16 @@ def test_rmsnorm_of_small_rows_without_eps(k):
         check_norm(q, s, x, gamma, 0.0)
 
 
+def test_rmsnorm_in_place_of_x_in_a_single_row():
+    """Which has no pitch: any will do."""
+    x, res, gamma = normal(1, 500, 1).cuda(), normal(1, 500, 2).cuda(), torch.ones(500, device="cuda")
+    q, s, h = P.dev_rmsnorm_i8(x, gamma, residual=res)
+    assert ckq.lib().ckq_rmsnorm_i8_dev(0, x.data_ptr(), 500, res.data_ptr(), x.data_ptr(), 700, gamma.data_ptr(), 1e-6, q.zero_().data_ptr(), q.stride(0), s.data_ptr(), 1, 500,
+                                        torch.cuda.current_stream().cuda_stream) == 0
+    q1, s1 = P.dev_rmsnorm_i8(h, gamma)
+    assert torch.equal(x, h) and torch.equal(q, q1) and torch.equal(s, s1)
+
+
 SMALL = [(2.0 ** -60, 2.0 ** -65, 0.0), (2.0 ** -60, 2.0 ** -80, 0.0), (2.0 ** -74, 1.0, 0.0), (2.0 ** -100, 2.0 ** 60, 0.0), (2.0 ** -118, 1.0, 0.0), (1.0, 2.0 ** -104, 1e-6),
          (2.0 ** -60, 1.0, 1e-30), (2.0 ** -100, 2.0 ** 40, 1e-38), (2.0 ** -110, 2.0 ** 100, 2.0 ** -140), (2.0 ** -45, 2.0 ** -90, 2.0 ** -90)]
 

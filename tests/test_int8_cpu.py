@@ -55,6 +55,12 @@ def test_rmsnorm_refusals(L):
         assert norm(**bad) == EROWS, bad
 
 
+def test_rmsnorm_refuses_a_sum_that_lies_across_the_rows_of_x(L):
+    """`sum` may be x only with one pitch, where each row lies in its own place."""
+    for ldx, ldr in ((64, 80), (128, 64)):
+        assert L.ckq_rmsnorm_i8_dev(F16, P, ldx, odd(1 << 20), P, ldr, P, ctypes.c_float(1e-5), P, 64, P, 2, 64, None) == EINVAL
+
+
 def test_swiglu_refusals(L):
     def swiglu(t=BF16, gate=P, up=P, ld=128, q=P, ldq=64, scale=P, rows=2, k=64):
         return L.ckq_swiglu_i8_dev(t, gate, up, ld, q, ldq, scale, rows, k, None)
