@@ -588,16 +588,13 @@ typedef I8Split<4, 2, 2, 2> S32x32;                   /* two */
 typedef I8Split<8, 1, 1, 2> S16x16;                   /* two */
 typedef I8Split<4, 2, 1, 2> S16x32;                   /* three */
 
-enum { I8_256x256, I8_256x192, I8_256x128, I8_128x192, I8_128x128, I8_64x128, I8_64x64, I8_S32x48, I8_S32x32, I8_S16x16, I8_S16x32, I8_TILINGS,
-       I8_TWO = I8_TILINGS, I8_STREAM };
-
 /* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all
  * places have a block; a last round of fewer steps faster, for the most part by how many blocks share a CU, a fifth by how many there
  * are in all (L2, power).  Fitted to 512 sizes of 5 to 2048 tokens (64 to 32000 rows, K 64 to 11008; operands from the 256 MB cache, as three
  * sets in turn leave them), each kernel within 4 to 8 % (rms).  Fitted to half of the sizes, the kernel so chosen is on the other half 0.8 % slower than the
  * best of all on average, 1.25 times at worst; without one of them it is 0.9 to 4 % on average. */
 struct I8Cost { int bt, bn, places, split; float t0, t_tile, step; };
-static const I8Cost i8_costs[I8_TILINGS] = {
+static const I8Cost i8_costs[CKQ_I8_TILINGS] = {
     {256, 256, 256, 1, 1.50f, 7.40f, 1.490f},
     {256, 192, 256, 1, 1.50f, 6.74f, 1.173f},
     {256, 128, 256, 1, 1.50f, 5.13f, 0.816f},
@@ -630,7 +627,7 @@ static int i8_whole_columns(int M, int N)
 }
 
 static std::atomic<int> g_i8_kernel{-1};
-extern "C" void ckq_launch_set_i8_kernel(int kernel) { g_i8_kernel.store(kernel < 0 || kernel > I8_STREAM ? -1 : kernel); }
+extern "C" void ckq_launch_set_i8_kernel(int kernel) { g_i8_kernel.store(kernel < 0 || kernel > CKQ_I8_STREAM ? -1 : kernel); }
 
 /* Rows are streamed (gemm_i8_stream_kernel) for one token or two, and for four where a row is one trip of a wave; at more the dot products, which
  * use four multiplications of an instruction, become the bound (us streamed | split tiles: two tokens, 11008 x 4096 8.5 | 8.8, 151936 x 896 21.1 | 28.7;
@@ -640,18 +637,18 @@ static bool i8_streams(int M, int K) { return M <= 2 || (M <= 4 && K <= 1024); }
 extern "C" int ckq_launch_i8_kernel(int M, int N, int K)
 {
     const int forced = g_i8_kernel.load();
-    if (forced >= 0 && (forced != I8_STREAM || i8_streams(M, K)) && (forced != I8_TWO || i8_whole_columns(M, N) > 0)) return forced;
-    if (i8_streams(M, K)) return I8_STREAM;
+    if (forced >= 0 && (forced != CKQ_I8_STREAM || i8_streams(M, K)) && (forced != CKQ_I8_TWO || i8_whole_columns(M, N) > 0)) return forced;
+    if (i8_streams(M, K)) return CKQ_I8_STREAM;
     int best = 0;
     float t = 1e30f;
-    for (int i = 0; i < I8_TILINGS; ++i) {
+    for (int i = 0; i < CKQ_I8_TILINGS; ++i) {
         const float ti = i8_costs[i].t0 + i8_rounds(i8_costs[i], i8_tiles(i8_costs[i], M, N), K);
         if (ti < t) { t = ti; best = i; }
     }
     const int cols = i8_whole_columns(M, N);
     if (cols > 0 && 256 * cols < N) {
-        const I8Cost &a = i8_costs[I8_256x256], &b = i8_costs[I8_128x192];
-        if (a.t0 + i8_rounds(a, (long)((M + 255) / 256) * cols, K) + i8_rounds(b, i8_tiles(b, M, N - 256 * cols), K) < t) best = I8_TWO;
+        const I8Cost &a = i8_costs[CKQ_I8_256x256], &b = i8_costs[CKQ_I8_128x192];
+        if (a.t0 + i8_rounds(a, (long)((M + 255) / 256) * cols, K) + i8_rounds(b, i8_tiles(b, M, N - 256 * cols), K) < t) best = CKQ_I8_TWO;
     }
     return best;
 }
@@ -660,18 +657,18 @@ template <class E>
 static int launch_gemm_i8(const I8Args &a, hipStream_t s)
 {
     switch (ckq_launch_i8_kernel(a.M, a.N, a.K)) {
-    case I8_256x256:   return launch_i8_tiles<E, T256x256>(a, s);
-    case I8_256x192:   return launch_i8_tiles<E, T256x192>(a, s);
-    case I8_256x128:   return launch_i8_tiles<E, T256x128>(a, s);
-    case I8_128x192:   return launch_i8_tiles<E, T128x192>(a, s);
-    case I8_128x128:   return launch_i8_tiles<E, T128x128>(a, s);
-    case I8_64x128:    return launch_i8_tiles<E, T64x128>(a, s);
-    case I8_64x64:     return launch_i8_tiles<E, T64x64>(a, s);
-    case I8_S32x48:    return launch_i8_split<E, S32x48>(a, s);
-    case I8_S32x32:    return launch_i8_split<E, S32x32>(a, s);
-    case I8_S16x16:    return launch_i8_split<E, S16x16>(a, s);
-    case I8_S16x32:    return launch_i8_split<E, S16x32>(a, s);
-    case I8_TWO:       return launch_i8_two_tiles<E, T256x256, T128x192>(a, i8_whole_columns(a.M, a.N), s);
+    case CKQ_I8_256x256:   return launch_i8_tiles<E, T256x256>(a, s);
+    case CKQ_I8_256x192:   return launch_i8_tiles<E, T256x192>(a, s);
+    case CKQ_I8_256x128:   return launch_i8_tiles<E, T256x128>(a, s);
+    case CKQ_I8_128x192:   return launch_i8_tiles<E, T128x192>(a, s);
+    case CKQ_I8_128x128:   return launch_i8_tiles<E, T128x128>(a, s);
+    case CKQ_I8_64x128:    return launch_i8_tiles<E, T64x128>(a, s);
+    case CKQ_I8_64x64:     return launch_i8_tiles<E, T64x64>(a, s);
+    case CKQ_I8_S32x48:    return launch_i8_split<E, S32x48>(a, s);
+    case CKQ_I8_S32x32:    return launch_i8_split<E, S32x32>(a, s);
+    case CKQ_I8_S16x16:    return launch_i8_split<E, S16x16>(a, s);
+    case CKQ_I8_S16x32:    return launch_i8_split<E, S16x32>(a, s);
+    case CKQ_I8_TWO:       return launch_i8_two_tiles<E, T256x256, T128x192>(a, i8_whole_columns(a.M, a.N), s);
     }
     /* Rows of up to 1 KB are one trip of a wave: four rows a wave, no exchange.  Longer ones are shared by the waves of a block, so that
      * a launch has its bytes in flight at once however few rows it has.  us at one token, rows x K, (rows a wave, KB a trip, waves of a

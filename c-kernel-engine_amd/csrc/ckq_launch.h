@@ -166,6 +166,13 @@ int ckq_launch_rmsnorm_i8(int type, const void *x, long ldx, const void *residua
 int ckq_launch_swiglu_i8(int type, const void *gate, const void *up, long ld, int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
 int ckq_launch_gemm_i8(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,
                        int type, void *C, long ldc, int M, int N, int K, void *stream);
+/* Which kernel takes a product of M x N x K: tiles of so many tokens x rows (S: with K split among a block's waves), two sizes of tiles in a launch, or
+ * the rows streamed.  Host arithmetic; exported for the test of the rules. */
+enum { CKQ_I8_256x256, CKQ_I8_256x192, CKQ_I8_256x128, CKQ_I8_128x192, CKQ_I8_128x128, CKQ_I8_64x128, CKQ_I8_64x64, CKQ_I8_S32x48, CKQ_I8_S32x32, CKQ_I8_S16x16, CKQ_I8_S16x32,
+       CKQ_I8_TILINGS, CKQ_I8_TWO = CKQ_I8_TILINGS, CKQ_I8_STREAM };
+int ckq_launch_i8_kernel(int M, int N, int K);
+/* -1 = by shape (default), else that kernel wherever it can take the product, in all calls of the process. */
+void ckq_launch_set_i8_kernel(int kernel);
 
 /* Plain device copy kernel (calibration of the memory counters / roofline). */
 int ckq_launch_copy(void *dst, const void *src, size_t bytes, void *stream);

@@ -3,6 +3,8 @@ kernel is launched here."""
 import ctypes
 import importlib
 import os
+import re
+import subprocess
 
 import pytest
 
@@ -16,6 +18,12 @@ def L():
     if not os.path.exists(ckq.lib_path()):
         ckq.build()
     return ckq.lib()
+
+
+@pytest.fixture(autouse=True)
+def _kernel_by_shape(L):
+    yield
+    L.ckq_launch_set_i8_kernel(-1)
 
 
 P = ctypes.c_void_p(4096)
@@ -116,3 +124,12 @@ def test_kernel_of_a_matmul(L):
         L.ckq_launch_set_i8_kernel(forced)
         assert L.ckq_launch_i8_kernel(2048, 11008, 4096) == (forced if forced != 12 else 11)
     L.ckq_launch_set_i8_kernel(-1)
+
+
+def test_exported_launches_are_declared(L):
+    """What the library exports of its kernels' interface stands in ckq_launch.h, the switches of the tests too."""
+    text = open(os.path.join(ckq.api.CSRC, "ckq_launch.h")).read()
+    names = subprocess.run(["nm", "-D", "--defined-only", ckq.lib_path()], capture_output=True, text=True, check=True).stdout.split()
+    launches = {n for n in names if n.startswith("ckq_launch_")}
+    assert len(launches) > 20
+    assert not {n for n in launches if not re.search(r"\b%s\(" % n, text)}
