@@ -257,6 +257,10 @@ def _i8_refuse(dev, rows, floats):
     raise CkqError("two tensors of this call need one pitch")
 
 
+def _i8_too_many(*sizes):
+    raise CkqError("sizes %s: the library takes 2^31 - 1 at most (ctypes would pass their lowest 32 bits)" % (sizes,))
+
+
 def empty_i8(rows, k, device="cuda"):
     """int8 [rows, k] whose rows begin at multiples of 16 bytes, as dev_gemm_nt_i8 takes them."""
     torch = _torch or _i8_torch()
@@ -280,6 +284,8 @@ def dev_quantize_i8(x, out=None):
             or not scale.is_contiguous() or not x.get_device() == q.get_device() == scale.get_device() == dev):
         _i8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _INT8)], [(scale, "scale", shape[:1])])
     rows, k = shape
+    if (rows | k) >> 31:
+        _i8_too_many(rows, k)
     (ldx, ex), (ldq, eq) = x.stride(), q.stride()
     if (ex != 1 or eq != 1) and k > 1:
         _i8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _INT8)], [])
@@ -302,6 +308,8 @@ def dev_dequantize_i8(q, scale, dtype=None, out=None):
             or scale.shape != shape[:1] or not scale.is_contiguous() or not q.get_device() == scale.get_device() == y.get_device() == dev):
         _i8_refuse(dev, [(q, "q", None, _INT8), (y, "out", shape, None), (y, "out", shape, dtype)], [(scale, "scale", shape[:1])])
     rows, k = shape
+    if (rows | k) >> 31:
+        _i8_too_many(rows, k)
     (ldq, eq), (ldy, ey) = q.stride(), y.stride()
     if (eq != 1 or ey != 1) and k > 1:
         _i8_refuse(dev, [(q, "q", None, _INT8), (y, "out", shape, None)], [])
@@ -325,6 +333,8 @@ def dev_rmsnorm_i8(x, gamma, eps=1e-6, residual=None, residual_out=None, out=Non
             or not x.get_device() == q.get_device() == scale.get_device() == gamma.get_device() == dev):
         _i8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _INT8)], [(scale, "scale", shape[:1]), (gamma, "gamma", shape[1:])])
     rows, k = shape
+    if (rows | k) >> 31:
+        _i8_too_many(rows, k)
     (ldx, ex), (ldq, eq) = x.stride(), q.stride()
     ldr, rp, hp = 0, None, None
     if residual is not None:
@@ -359,6 +369,8 @@ def dev_swiglu_i8(gate, up, out=None):
             or scale.shape != shape[:1] or not scale.is_contiguous() or not gate.get_device() == up.get_device() == q.get_device() == scale.get_device() == dev):
         _i8_refuse(dev, [(gate, "gate", None, None), (up, "up", shape, t), (q, "q", shape, _INT8)], [(scale, "scale", shape[:1])])
     rows, k = shape
+    if (rows | k) >> 31:
+        _i8_too_many(rows, k)
     (ld, eg), (ldu, eu), (ldq, eq) = gate.stride(), up.stride(), q.stride()
     if (eg != 1 or eu != 1 or eq != 1) and k > 1 or ldu != ld and rows > 1:
         _i8_refuse(dev, [(gate, "gate", None, None), (up, "up", shape, t), (q, "q", shape, _INT8)], [])
@@ -379,6 +391,8 @@ def dev_gemm_nt_i8(a, sa, b, sb, bias=None, dtype=None, out=None):
         _i8_refuse(dev, [(a, "a", None, _INT8), (b, "b", (of_b[0], of_a[1]) if a.dim() == b.dim() == 2 else None, _INT8)], [])
     M, K = of_a
     N = of_b[0]
+    if (M | N | K) >> 31:
+        _i8_too_many(M, N, K)
     c = out if out is not None else _torch.empty(M, N, dtype=dtype or _F32, device=b.device)
     t = c.dtype
     kind = _I8_TYPES.get(t)

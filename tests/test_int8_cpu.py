@@ -110,6 +110,37 @@ def test_front_ends_refuse_what_a_pointer_cannot_tell():
     assert par.empty_i8(3, 33, device="cpu").shape == (3, 33) and par.empty_i8(3, 33, device="cpu").stride() == (48, 1)
 
 
+def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
+    """ctypes passes the lowest 32 bits of an int: 2^32 + 16 rows would be 16.  Memory that nothing touches, and a library that nothing reaches."""
+    import torch
+    par, err = ckq.parity, ckq.CkqError
+    if torch.cuda.is_available():
+        pytest.skip("the memory of a host without a device is meant")
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: 0
+    monkeypatch.setattr(par, "lib", Library)
+    monkeypatch.setattr(par, "_i8_where", lambda: (-1, None))            # the device of host tensors
+    par._i8_torch()
+    f, q = torch.zeros(64), torch.zeros(64, dtype=torch.int8)
+    assert par.dev_quantize_i8(f.view(4, 16))[0].shape == (4, 16)        # sizes as they should be get through
+    for shape in (((1 << 32) + 16, 1), (1, (1 << 32) + 16), (1 << 31, 1), (1, 1 << 31)):
+        rows, k = shape
+        x, y = torch.empty(shape, dtype=torch.bfloat16), torch.empty(shape, dtype=torch.int8)
+        out = (y, torch.empty(rows))
+        gamma = torch.empty(k)
+        for call in (lambda: par.dev_quantize_i8(x, out=out), lambda: par.dev_dequantize_i8(*out, out=x), lambda: par.dev_swiglu_i8(x, x, out=out),
+                     lambda: par.dev_rmsnorm_i8(x, gamma, out=out)):
+            with pytest.raises(err, match="2\\^31"):
+                call()
+    many = torch.empty((1 << 32) + 32, dtype=torch.int8)
+    far, few, scales = many.as_strided(((1 << 32) + 16, 16), (1, 1)), q.view(4, 16), torch.empty((1 << 32) + 16)
+    for call in (lambda: par.dev_gemm_nt_i8(far, scales, few, f[:4], out=scales), lambda: par.dev_gemm_nt_i8(few, f[:4], far, scales, out=scales)):
+        with pytest.raises(err, match="2\\^31"):
+            call()
+
+
 def test_kernel_of_a_matmul(L):
     """One or two tokens stream, four if rows are short; then the cheapest by the estimate, which has to be one of the kernels at every size."""
     assert all(L.ckq_launch_i8_kernel(M, N, K) == 12 for N in (1, 5000, 151936) for M, K in ((1, 1), (1, 131071), (2, 896), (2, 131071), (3, 1024), (4, 1)))
