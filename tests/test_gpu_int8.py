@@ -6,6 +6,7 @@ value; a result of type T adds half a step of T.  A quant is the nearest integer
 127 times what the fp32 operations before the rounding put on t (their number is at each test)."""
 import importlib
 import os
+import threading
 
 import numpy as np
 import pytest
@@ -350,6 +351,62 @@ def test_swiglu_far_gates():
     assert (q == 0).all() and s.isnan().all()
 
 
+# ---- more than 256 rows: fewer waves share a row, with two to four vectors a thread ------------------
+
+def norm_chain(k):
+    """Longest chain of additions of a row's sum of squares, a function of its length alone: a thread's elements, the tree of a wave,
+    groups of 512 sixteen apart, and up to sixteen of these sums; rows that are read twice: a thread's elements, the tree, the waves."""
+    nvec, groups = -(-k // 8), -(-k // 512)
+    return 8 * -(-nvec // 1024) + 6 + 16 if k < 8 or k > 32768 else 8 + 6 + -(-groups // 16) + min(16, groups)
+
+
+def check_many_norm(q, s, h, gamma, eps):
+    check_codes(q, s, norm64(h, gamma, eps), 6 * U, ((norm_chain(h.shape[1]) + 2) / 2 + 2 + 4) * U)
+
+
+MANY = SWITCHES + [5, 100, 777, 1531, 2001, 3071, 5999, 9001, 12281, 20001]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k", MANY)
+def test_quantize_many_rows(t, k):
+    x = normal(259, k, k, 3.0).to(TYPES[t])
+    q, s = P.dev_quantize_i8(x.cuda())
+    check_codes(q, s, x.double(), 2 * U, U)
+    base = torch.full((259, k + 5), 77, dtype=torch.int8, device="cuda")
+    q2, s2 = P.dev_quantize_i8(pitched(x, 3, 1), out=(base[:, :k], torch.empty_like(s)))
+    assert torch.equal(q, q2) and torch.equal(s, s2) and (base[:, k:] == 77).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k", MANY)
+def test_rmsnorm_many_rows(t, k):
+    T, rows = TYPES[t], 258
+    x, res = normal(rows, k, 3 * k).to(T), normal(rows, k, 5 * k, 2.0).to(T)
+    gamma = torch.rand(k, generator=torch.Generator().manual_seed(k)) + 0.25
+    q, s, h = P.dev_rmsnorm_i8(x.cuda(), gamma.cuda(), 1e-5, residual=res.cuda())
+    want = x.double() + res.double()
+    assert ((h.cpu().double() - want).abs() <= (U + half_step(T) * (1 + U)) * want.abs()).all()
+    check_many_norm(q, s, h.cpu(), gamma, 1e-5)
+    for out in (P.dev_rmsnorm_i8(h, gamma.cuda(), 1e-5), P.dev_rmsnorm_i8(pitched(h.cpu(), 5, 3), gamma.cuda(), 1e-5)):
+        assert torch.equal(out[0], q) and torch.equal(out[1], s)
+    for into in ("x", "residual"):                            # in place, at a pitch
+        xd, rd = pitched(x, 3, 1), pitched(res, 3, 1)
+        q1, s1, h1 = P.dev_rmsnorm_i8(xd, gamma.cuda(), 1e-5, residual=rd, residual_out=xd if into == "x" else rd)
+        assert torch.equal(q1, q) and torch.equal(s1, s) and torch.equal(h1, h), into
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("k", MANY)
+def test_swiglu_many_rows(t, k):
+    both = normal(257, 2 * k, 7 * k, 3.0).to(TYPES[t])
+    d = both.cuda()
+    q, s = P.dev_swiglu_i8(d[:, :k], d[:, k:])
+    check_swiglu(q, s, both[:, :k], both[:, k:])
+    q2, s2 = P.dev_swiglu_i8(d[40:41, :k], d[40:41, k:])
+    assert torch.equal(q2, q[40:41]) and torch.equal(s2, s[40:41])
+
+
 # ---- matmul ------------------------------------------------------------------------------------
 
 def check_matmul(c, a, sa, b, sb, bias):
@@ -458,6 +515,21 @@ def test_matmul_two_sizes_of_tiles(kernel, M, N, K):
     kernel(TWO)
     assert ckq.lib().ckq_launch_i8_kernel(M, N, K) == TWO
     matmul_case(M, N, K, "bf16", bias=True)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,N,K", [(2048, 8500, 4096), (2040, 11008, 1111), (300, 40000, 2049)])
+def test_matmul_two_sizes_of_tiles_over_long_rows(kernel, M, N, K, t):
+    """And the bits of a launch of one size."""
+    kernel(TWO)
+    assert ckq.lib().ckq_launch_i8_kernel(M, N, K) == TWO
+    c = matmul_case(M, N, K, t, bias=True, pitch_a=1, pitch_c=1)
+    for which in (0, 3, 9):
+        kernel(which)
+        a, b = codes(M, K, 1, -(-K // 16) * 16 + 16), codes(N, K, 2)
+        g = torch.Generator().manual_seed(3)
+        sa, sb = (torch.rand(M, generator=g) * 0.01 + 0.001).cuda(), (torch.rand(N, generator=g) * 0.01 + 0.001).cuda()
+        assert torch.equal(P.dev_gemm_nt_i8(a, sa, b, sb, torch.randn(N, generator=g).cuda(), dtype=TYPES[t]), c), which
 
 
 @pytest.mark.parametrize("K", [1, 15, 16, 17, 100, 1008, 1023, 1024, 1025, 1040, 2047, 2048, 2049, 4095, 4097, 6000, 8191, 8193, 11008])
@@ -646,3 +718,24 @@ def test_mlp_captured_replayed_and_on_two_streams(M):
                 assert torch.equal(got, w)
         again = m.run()                                       # eager work between the replays
         assert all(torch.equal(a, b) for a, b in zip(again, want))
+
+
+def test_two_host_threads_on_streams_of_their_own():
+    layers = [Mlp(M, 512, 1000, torch.bfloat16, seed=10 * M) for M in (1, 40)]
+    wants = [m.run() for m in layers]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(layer, want):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                if not all(torch.equal(a, b) for a, b in zip(layer.run(), want)):
+                    failed.append(layer)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=pair) for pair in zip(layers, wants)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed
