@@ -8,16 +8,16 @@
  * among thousands.
  *
  * Three forms:
- * - gemm_i8_stream_kernel, one or two tokens (four of short rows): rows streamed once, v_dot4_i32_i8.  Bound by memory: 11008 x 4096 at one token 7.8 us,
- *   5.8 TB/s; a kernel that only reads those bytes takes 7.3.
+ * - gemm_i8_stream_kernel, one or two tokens (four of short rows): rows streamed once, v_dot4_i32_i8.  Bound by memory: 11008 x 4096 at one token 7.8 us
+ *   with three sets in turn, which the 256 MB cache holds, 5.8 TB/s (a kernel that only reads those bytes takes 7.3), and 8.4 with nine, which it does not.
  * - gemm_i8_split_kernel, a few to some hundred tokens: small tiles, K split among the waves of a block, which exchange their sums once.
- *   Bound by memory where rows are read once (13 x 4096 x 11008 9.5 us, 4.8 TB/s), beyond by what a CU can load, 64 bytes a cycle at best (both
+ *   Bound by memory where rows are read once (13 x 4096 x 11008 9.5 us, 4.8 TB/s, with three sets in turn, 13.2 with nine), beyond by what a CU can load, 64 bytes a cycle at best (both
  *   operands of every tile: 333 x 1001 x 4847, 231 tiles, 390 KB a CU, 3 us of 9.1, of which a launch takes 3.3).
  * - gemm_i8_tile_kernel, tiles of 64 x 64 to 256 x 256 on all waves of a block, v_mfma_i32_32x32x32_i8.  The largest are bound by the matrix
- *   cores at the clock that the power limit leaves them (8192 x 8192 x 8192: 2430 TOPS, matrix cores busy in 71 % of the cycles at
- *   1.6 GHz; the published 5 POP/s are at 2.4).  The smaller ones have a step's copies (40 KB of 128 x 192, 640 cycles at 64 bytes) beside its multiplications
- *   (768 cycles) and come near the longer of the two while few CUs work (0.43 us a step, the multiplications alone 0.37), not with all of them
- *   (512 x 11008 x 4096 0.63, the copies alone 0.41); a launch, the first copies and the last stores are 6 of its 26 us.
+ *   cores at the clock that the power limit leaves them (8192 x 8192 x 8192: 464 us, 2370 TOPS, matrix cores busy in 71 % of the cycles at
+ *   1.6 GHz; the published 5 POP/s are at 2.4).  The smaller ones have a step's copies (40 KB of 128 x 192, 640 cycles at 64 bytes) and reads of LDS beside its multiplications
+ *   (768 cycles) and come near the longest of these while few CUs work (0.43 us a step, the multiplications alone 0.37), not with all of them
+ *   (512 x 11008 x 4096 0.63: without copies 0.52, without reads too 0.39, the copies alone 0.41); a launch, the first copies and the last stores are 6 of its 26 us.
  * All operands reach the matrix cores through LDS: 16 rows x 64 bytes an instruction, as the matrix cores want them in registers, load at 16 bytes a
  * cycle and CU.
  */
@@ -570,7 +570,7 @@ static int launch_i8_stream(const I8Args &a, hipStream_t s)
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */
 
 /* Stages and waves as measured, us.  What waves that only copy gain: see i8_tile; none at 256 x 256, where the eight that multiply need 216 registers and a block
- * of twelve waves has 168 each (sixteen waves of 64 x 64 are no faster: 8192 x 8192 x 8192 470 with eight, 477).  1024 x 4096 x 4096, 128 x 128: four waves multiplying 64 x 64 each, three stages 21.7, four 22.1,
+ * of twelve waves has 168 each (sixteen waves of 64 x 64 are no faster: 8192 x 8192 x 8192 1.5 % slower).  1024 x 4096 x 4096, 128 x 128: four waves multiplying 64 x 64 each, three stages 21.7, four 22.1,
  * with two to copy 23.4; eight multiplying 32 x 64 22.8.  2048 x 4096 x 4096, 256 x 128: eight and four waves, three stages 35.5, two 37.1.  125 x 11008 x 4096, 64 x 128:
  * four stages 13.2, five 13.4, three 13.9.  500 x 2000 x 2000, 64 x 64: four stages, so that two blocks share a CU, 8.4; six 8.8. */
 typedef I8Tile<2, 4, 4, 2, 0, 2, 3> T256x256;
@@ -592,7 +592,8 @@ typedef I8Split<4, 2, 1, 2> S16x32;                   /* three */
  * places have a block; a last round of fewer steps faster, for the most part by how many blocks share a CU, a fifth by how many there
  * are in all (L2, power).  Fitted to 512 sizes of 5 to 2048 tokens (64 to 32000 rows, K 64 to 11008; operands from the 256 MB cache, as three
  * sets in turn leave them), each kernel within 4 to 8 % (rms).  Fitted to half of the sizes, the kernel so chosen is on the other half 0.8 % slower than the
- * best of all on average, 1.25 times at worst; without one of them it is 0.9 to 4 % on average. */
+ * best of all on average, 1.25 times at worst; without one of them it is 0.9 to 4 % on average.  With weights from memory (28 sizes of 3 to 128 tokens, more sets in turn than the cache holds)
+ * 0.9 % and 1.15 times. */
 struct I8Cost { int bt, bn, places, split; float t0, t_tile, step; };
 static const I8Cost i8_costs[CKQ_I8_TILINGS] = {
     {256, 256, 256, 1, 1.50f, 7.40f, 1.490f},

@@ -288,7 +288,8 @@ int ckq_gemm_nt_f32act_dev(int fmt, const float *A, const void *B, const float *
  * model's projections: weights with a scale a channel (N rows), activations with a scale a token (M rows).  No counterpart in
  * the reference.  `type` of the floats is CKQ_CK_DTYPE_FP32, _BF16 or _FP16, anything else is CKQ_EFORMAT (-3); rows of
  * floats lie ld elements apart, rows of int8 ld bytes, at least their length (else CKQ_EINVAL, -1).  Floats are aligned to their own
- * size, else CKQ_EROWS (-8).  Nothing is allocated, no scratch is shared between calls, and every call may be captured.
+ * size, else CKQ_EROWS (-8).  Scales, gamma and bias are fp32 with every type.  There is at least one row, and one element in it (else CKQ_EINVAL).
+ * Nothing is allocated, no scratch is shared between calls, and every call may be captured.  A row's results have the same bits alone and in any batch.
  *
  * ckq_quantize_i8_dev: a = max(largest |x| of the row, 2^-100), q = RNE(x * (127 / a)), scale = a / 127, in fp32.  A row with a
  * NaN or an infinity gets that as its scale (NaN if there is one) and zeros as its quants.  Bytes of q behind a row's k-th stay
@@ -298,10 +299,11 @@ int ckq_gemm_nt_f32act_dev(int fmt, const float *A, const void *B, const float *
  * x); then sum * (1 / sqrt(mean of sum^2 + eps)) * gamma in 8 bits as above (eps finite and >= 0, else CKQ_EINVAL).  residual and sum have one pitch, ldr; sum may be
  * residual itself, or x (with ldr = ldx, else CKQ_EINVAL).  Squares are summed in fp32: a row whose sum of squares, or whose sum * gamma, exceeds fp32
  * gets a scale that is not finite, and zeros as its quants, as does a row of zeros without an eps.  Rows, gamma and eps may be as small as their types hold.
- * ckq_swiglu_i8_dev: gate / (1 + exp(-gate)) * up in 8 bits as above (0 under -88.72, where exp(-gate) exceeds fp32); gate and up have one pitch, ld, so that both may be halves
+ * ckq_swiglu_i8_dev: gate / (1 + exp(-gate)) * up in 8 bits as above (0 under -88.72, where exp(-gate) exceeds fp32; the function is (4 + |gate|) 2^-23 of its
+ * value off at most for gates under 0, and so is the scale of a row whose largest has such a gate); gate and up have one pitch, ld, so that both may be halves
  * of one row (the output of a projection that holds the rows of both).
- * ckq_gemm_nt_i8_dev: C[m*ldc + n] = sa[m] * sb[n] * (sum over k of A[m][k] * B[n][k]) (+ bias[n]), the sum exact in int32, the
- * rest in fp32, rounded once to the type of C.  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are,
+ * ckq_gemm_nt_i8_dev: C[m*ldc + n] = (sa[m] * (sum over k of A[m][k] * B[n][k])) * sb[n] (+ bias[n]), the sum exact in int32, the
+ * rest in fp32 in this order, rounded once to the type of C.  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are,
  * multiples of 16 bytes, pitches at most 4 MiB, K at most 131071 (else CKQ_EROWS).  K may be odd: of the 16 bytes that hold a
  * row's last, those behind it may be read and are not used. */
 int ckq_quantize_i8_dev(ckq_ck_dtype type, const void *x, long ldx, int8_t *q, long ldq, float *scale, int rows, int k, void *stream);
