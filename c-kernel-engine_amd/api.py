@@ -132,6 +132,16 @@ _SIGS = {
     "ckq_rmsnorm_i8_dev": (_i, [_i, _vp, _l, _vp, _vp, _l, _vp, _c.c_float, _vp, _l, _vp, _i, _i, _vp]),
     "ckq_swiglu_i8_dev": (_i, [_i, _vp, _vp, _l, _vp, _l, _vp, _i, _i, _vp]),
     "ckq_gemm_nt_i8_dev": (_i, [_vp, _l, _vp, _vp, _l, _vp, _vp, _i, _vp, _l, _i, _i, _i, _vp]),
+    "ckq_quantize_f8_dev": (_i, [_i, _vp, _l, _vp, _l, _vp, _l, _i, _i, _vp]),
+    "ckq_dequantize_f8_dev": (_i, [_vp, _l, _vp, _l, _i, _vp, _l, _i, _i, _vp]),
+    "ckq_swiglu_f8_dev": (_i, [_i, _vp, _vp, _l, _vp, _l, _vp, _l, _i, _i, _vp]),
+    "ckq_gemm_nt_f8_dev": (_i, [_vp, _l, _vp, _l, _vp, _l, _vp, _l, _vp, _i, _vp, _l, _i, _i, _i, _vp]),
+    "ckq_gemm_nt_f8_experts_dev": (_i, [_vp, _l, _vp, _l, _vp, _l, _l, _vp, _l, _l, _vp, _vp, _i, _i, _vp, _l, _i, _i, _i, _vp]),
+    "ckq_moe_sort_dev": (_i, [_vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
+    "ckq_moe_gather_dev": (_i, [_i, _vp, _l, _vp, _vp, _l, _i, _i, _i, _i, _vp]),
+    "ckq_moe_gather_f8_dev": (_i, [_i, _vp, _l, _vp, _vp, _l, _vp, _l, _i, _i, _i, _i, _vp]),
+    "ckq_moe_combine_dev": (_i, [_i, _vp, _l, _vp, _vp, _vp, _l, _i, _i, _i, _i, _vp]),
+    "ckq_moe_combine_backward_dev": (_i, [_i, _vp, _l, _vp, _l, _vp, _vp, _vp, _l, _vp, _i, _i, _i, _i, _vp]),
     "ckq_matmul_sequence_dev": (_i, [_vp, _i, _i, _vp]),
     "ckq_subblock_dots_dev": (_i, [_i, _vp, _vp, _vp, _i, _i, _vp]),
     "ckq_subblock_dots_tokens_dev": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _vp]),

@@ -119,7 +119,7 @@ const char *ckq_error_string(int code)
     case CKQ_EINVAL: return "invalid argument (NULL pointer or non-positive dimension)";
     case CKQ_ESHAPE: return "K is not a multiple of the quantization block size";
     case CKQ_EFORMAT: return "unknown weight format";
-    case CKQ_EROWS: return "int8 rows: pointers and pitches of a matmul's operands have to be multiples of 16 bytes, pitches at most 4 MiB, K at most 131071; floats have to be aligned to their size";
+    case CKQ_EROWS: return "rows of int8 or e4m3: pointers and pitches of a matmul's operands have to be multiples of 16 bytes, pitches at most 4 MiB, K of int8 at most 131071; numbers have to be aligned to their size";
     case CKQ_ENODUMP: return "the integer dumps of the exactness tests are built into libckernel_quant_hip_dump.so, not into this library";
     case CKQ_ESCRATCH: return "the call is of a size that ckq_gemm_nt_noalloc_dev counts with more scratch than it holds (4 MiB); use ckq_gemm_nt_dev or fewer tokens per call";
     default: return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown error";

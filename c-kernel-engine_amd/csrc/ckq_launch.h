@@ -20,7 +20,7 @@ extern "C" {
 #define CKQ_EFORMAT (-3)  /* unknown format tag */
 #define CKQ_ESCRATCH (-4) /* the call is counted with more scratch than the entry point that allocates nothing holds */
 #define CKQ_ENOGROUP (-7) /* internal: a grouped GEMM launch was declined; the caller launches the matrices one by one */
-#define CKQ_EROWS (-8)    /* rows of int8, or the floats beside them, that are not as the kernels take them (ckernel_quant_hip.h) */
+#define CKQ_EROWS (-8)    /* rows of int8 or e4m3, or the numbers beside them, that are not as the kernels take them (ckernel_quant_hip.h) */
 #define CKQ_ENODUMP (-6)  /* the integer dumps are compiled into libckernel_quant_hip_dump.so only */
 /* 1 in the test library (same sources, same templates, plus the DUMP instantiations that also
  * store the integers behind every output); 0 in the product library, which stays smaller for it. */
@@ -173,6 +173,26 @@ enum { CKQ_I8_256x256, CKQ_I8_256x192, CKQ_I8_256x128, CKQ_I8_128x192, CKQ_I8_12
 int ckq_launch_i8_kernel(int M, int N, int K);
 /* -1 = by shape (default), else that kernel wherever it can take the product, in all calls of the process. */
 void ckq_launch_set_i8_kernel(int kernel);
+
+/* Rows in e4m3 with one scale for each 128 elements, and tokens sorted by expert (ckq_f8_rows.hip, ckq_gemm_f8.hip, ckq_moe.hip).  See ckernel_quant_hip.h for what
+ * they compute and take. */
+#define CKQ_MOE_EXPERTS_MAX 65535
+#define CKQ_MOE_SLOTS_MAX (1l << 30)
+int ckq_launch_quantize_f8(int type, const void *x, long ldx, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
+int ckq_launch_dequantize_f8(const uint8_t *q, long ldq, const float *scale, long lds, int type, void *y, long ldy, int rows, int k, void *stream);
+int ckq_launch_swiglu_f8(int type, const void *gate, const void *up, long ld, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
+int ckq_launch_gemm_f8(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, const float *sb, long ldsb, const float *bias,
+                       int type, void *C, long ldc, int M, int N, int K, void *stream);
+int ckq_launch_gemm_f8_experts(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, long eb, const float *sb, long ldsb, long esb,
+                               const float *bias, const int32_t *offsets, int experts, int type, void *C, long ldc, int M, int N, int K, void *stream);
+int ckq_launch_moe_sort(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets, int32_t *order, int32_t *position, void *stream);
+int ckq_launch_moe_gather(int type, const void *x, long ldx, const int32_t *position, void *y, long ldy, int tokens, int choices, int rows, int k, void *stream);
+int ckq_launch_moe_gather_f8(int type, const void *x, long ldx, const int32_t *position, uint8_t *q, long ldq, float *scale, long lds,
+                             int tokens, int choices, int rows, int k, void *stream);
+int ckq_launch_moe_combine(int type, const void *y, long ldy, const int32_t *position, const float *weights, void *out, long ldo,
+                           int tokens, int choices, int rows, int k, void *stream);
+int ckq_launch_moe_combine_backward(int type, const void *dout, long ldd, const void *y, long ldy, const int32_t *position, const float *weights,
+                                    void *dy, long lddy, float *dweights, int tokens, int choices, int rows, int k, void *stream);
 
 /* Plain device copy kernel (calibration of the memory counters / roofline). */
 int ckq_launch_copy(void *dst, const void *src, size_t bytes, void *stream);

@@ -1,0 +1,217 @@
+/*
+ * ckq_moe.hip - tokens sorted by expert and back.  Token t has `choices` slots, s = t * choices + j, each with the number of an expert
+ * (none: anything outside 0 .. experts - 1) and, on the way back, a weight.
+ *
+ *   sort      slots in the order of their experts, those of one expert as they come: offsets[e] = slots of experts under e,
+ *             order[p] = slot, position[s] = p (none: -1, and -1 in order from offsets[experts] on)
+ *   gather    y[position[s]] = x[s / choices]
+ *   combine   out[t] = T(sum_j w[s] y[position[s]]), in fp32, j in turn; without weights, the gradient of gather
+ *   backward  dy[position[s]] = T(w[s] dout[t]),  dw[s] = sum_i dout[t][i] y[position[s]][i]
+ *
+ * No atomics: every result has one order of operations, whatever runs when.  Bound by memory but for a few tokens, where a launch is.
+ */
+#include "ckq_device.hpp"
+#include "ckq_int8.hpp"
+#include "ckq_launch.h"
+#include "ckq_rows.hpp"
+
+/* ---- sort ---------------------------------------------------------------------------------------------------------- */
+
+/* A block has an expert, the last one what has none.  Each goes through all slots twice: it counts those that belong before its own, and its own in each
+ * wave's run of slots; then it writes its own where they belong.  No scratch memory, one launch, and the order of the slots
+ * is kept without a sort; the slots' 4 bytes come from the caches. */
+__global__ void __launch_bounds__(1024) moe_sort_kernel(const int32_t *__restrict__ ids, int slots, int experts, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
+                                                        int32_t *__restrict__ position)
+{
+    __shared__ int before[16], mine[16];
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), nw = blockDim.x >> 6, e = blockIdx.x;
+    const int run = ((slots - 1) / (64 * nw) + 1) * 64;         /* slots of a wave */
+    const long from = (long)wave * run;
+    const int first = (int)min(from, (long)slots), end = (int)min(from + run, (long)slots);
+    int less = 0, same = 0;
+    for (int s = first + lane; s < end; s += 64) {
+        const u32 id = (u32)ids[s];
+        less += id < (u32)e;
+        same += e < experts ? id == (u32)e : id >= (u32)e;
+    }
+    less = group_sum<64>(less);
+    same = group_sum<64>(same);
+    if (lane == 63) {
+        before[wave] = less;
+        mine[wave] = same;
+    }
+    __syncthreads();
+    int at = 0, all = 0;
+    for (int w = 0; w < nw; ++w) {
+        all += before[w];
+        at += before[w] + (w < wave ? mine[w] : 0);
+    }
+    if (threadIdx.x == 0) offsets[e] = all;
+    for (int s0 = first; s0 < end; s0 += 64) {
+        const int s = s0 + lane;
+        const u32 id = s < end ? (u32)ids[s] : 0;
+        const bool own = s < end && (e < experts ? id == (u32)e : id >= (u32)e);
+        const unsigned long long m = __ballot(own);
+        const int p = at + __builtin_amdgcn_mbcnt_hi((u32)(m >> 32), __builtin_amdgcn_mbcnt_lo((u32)m, 0));
+        if (own) {
+            order[p] = e < experts ? s : -1;
+            position[s] = e < experts ? p : -1;
+        }
+        at += __popcll(m);
+    }
+}
+
+extern "C" int ckq_launch_moe_sort(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets, int32_t *order, int32_t *position, void *stream)
+{
+    if (!ids || !offsets || !order || !position || tokens <= 0 || choices <= 0 || experts <= 0) return CKQ_EINVAL;
+    if ((long)tokens * choices > CKQ_MOE_SLOTS_MAX || experts > CKQ_MOE_EXPERTS_MAX) return CKQ_EINVAL;
+    if (((uintptr_t)ids | (uintptr_t)offsets | (uintptr_t)order | (uintptr_t)position) % 4) return CKQ_EROWS;
+    const int slots = tokens * choices;
+    return i8_launch(moe_sort_kernel, dim3((u32)experts + 1), dim3(slots <= 256 ? 64 : slots <= 2048 ? 256 : 1024), (hipStream_t)stream, ids, slots, experts, offsets, order, position);
+}
+
+/* ---- rows there and back ------------------------------------------------------------------------------------------- */
+
+struct MoeArgs {
+    const void    *x;        /* gather: tokens' rows; combine: experts' rows; backward: the gradient of combine's output */
+    const void    *y;        /* backward: experts' rows */
+    void          *out;
+    const int32_t *position;
+    const float   *w;        /* or null */
+    float         *dw;
+    long           ldx, ldy, ldo;
+    int            tokens, choices, rows, k;
+};
+
+/* Eight elements a thread. */
+template <class E>
+__global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
+{
+    const u32 i = blockIdx.x * 256 + threadIdx.x, t = i / nvec, v = i - t * nvec;
+    if (t >= (u32)a.tokens) return;
+    const int left = a.k - 8 * (int)v;
+    const raw8<E> r = fetch8<false>((const E *)a.x + (size_t)t * a.ldx + 8 * (size_t)v, left);
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = raw_value<E>(r, j);
+    for (int j = 0; j < a.choices; ++j) {
+        const int p = a.position[(size_t)t * a.choices + j];
+        if ((u32)p < (u32)a.rows) store8((E *)a.out + (size_t)p * a.ldo + 8 * (size_t)v, f, left);
+    }
+}
+
+template <class E>
+__global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
+{
+    const u32 i = blockIdx.x * 256 + threadIdx.x, t = i / nvec, v = i - t * nvec;
+    if (t >= (u32)a.tokens) return;
+    const int left = a.k - 8 * (int)v;
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+    for (int j = 0; j < a.choices; ++j) {
+        const int p = a.position[(size_t)t * a.choices + j];
+        if ((u32)p >= (u32)a.rows) continue;
+        const float w = a.w ? a.w[(size_t)t * a.choices + j] : 1.0f;
+        const raw8<E> r = fetch8<false>((const E *)a.x + (size_t)p * a.ldx + 8 * (size_t)v, left);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) f[c] = __builtin_fmaf(w, raw_value<E>(r, c), f[c]);
+    }
+    store8((E *)a.out + (size_t)t * a.ldo + 8 * (size_t)v, f, left);
+}
+
+/* A block has a token.  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
+template <class E>
+__global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
+{
+    __shared__ float red[4];
+    const size_t t = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = wave_in_block();
+    const E *d = (const E *)a.x + t * a.ldx;
+    for (int j = 0; j < a.choices; ++j) {
+        const size_t s = t * a.choices + j;
+        const int p = a.position[s];
+        const bool there = (u32)p < (u32)a.rows;
+        const float w = a.w[s];
+        float sum = 0.0f;
+        if (there)
+            for (long v = 8l * threadIdx.x; v < a.k; v += 2048) {
+                const int left = a.k - (int)v;
+                const raw8<E> g = fetch8<false>(d + v, left), y = fetch8<false>((const E *)a.y + (size_t)p * a.ldy + v, left);
+                float f[8];
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    sum = __builtin_fmaf(raw_value<E>(g, c), raw_value<E>(y, c), sum);
+                    f[c] = w * raw_value<E>(g, c);
+                }
+                store8((E *)a.out + (size_t)p * a.ldo + v, f, left);
+            }
+        sum = group_sum<64>(sum);
+        __syncthreads();
+        if (lane == 63) red[wave] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) a.dw[s] = red[0] + red[1] + red[2] + red[3];
+    }
+}
+
+/* The launches of all tokens: one has fewer than 2^32 threads. */
+template <class E, class L>
+static int moe_each(MoeArgs a, bool out_by_token, size_t threads, L &&launch)
+{
+    const int most = (int)min((size_t)a.tokens, max((size_t)1, ((size_t)1 << 31) / threads));
+    for (int left = a.tokens;;) {
+        const int now = min(left, most);
+        a.tokens = now;
+        const int rc = launch(a);
+        if (rc || left == now) return rc;
+        left -= now;
+        a.position += (size_t)now * a.choices;
+        if (a.w) a.w += (size_t)now * a.choices;
+        if (a.dw) a.dw += (size_t)now * a.choices;
+        if (out_by_token) a.out = (E *)a.out + (size_t)now * a.ldo;
+        else              a.x = (const E *)a.x + (size_t)now * a.ldx;
+    }
+}
+
+enum { MOE_GATHER, MOE_COMBINE, MOE_BACKWARD };
+template <int OP, class E>
+static int launch_moe(const MoeArgs &a, hipStream_t s)
+{
+    const u32 nvec = (u32)(a.k / 8 + (a.k % 8 != 0));
+    return moe_each<E>(a, OP == MOE_COMBINE, OP == MOE_BACKWARD ? 256 : nvec, [&](const MoeArgs &b) {
+        if (OP == MOE_BACKWARD) return i8_launch(moe_combine_backward_kernel<E>, dim3((u32)b.tokens), dim3(256), s, b);
+        const dim3 grid((u32)(((size_t)b.tokens * nvec + 255) / 256));
+        return i8_launch(OP == MOE_GATHER ? moe_gather_kernel<E> : moe_combine_kernel<E>, grid, dim3(256), s, b, nvec);
+    });
+}
+template <int OP>
+static int launch_moe(int type, const MoeArgs &a, void *stream)
+{
+    if (a.tokens <= 0 || a.choices <= 0 || a.rows <= 0 || a.k <= 0) return CKQ_EINVAL;
+    const int size = row_size(type);
+    if (!size) return CKQ_EFORMAT;
+    if (((uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.out) % size || ((uintptr_t)a.position | (uintptr_t)a.w | (uintptr_t)a.dw) % 4) return CKQ_EROWS;
+    const hipStream_t s = (hipStream_t)stream;
+    return type == CKQ_T_F32 ? launch_moe<OP, float>(a, s) : type == CKQ_T_BF16 ? launch_moe<OP, __bf16>(a, s) : launch_moe<OP, _Float16>(a, s);
+}
+
+extern "C" int ckq_launch_moe_gather(int type, const void *x, long ldx, const int32_t *position, void *y, long ldy, int tokens, int choices, int rows, int k, void *stream)
+{
+    if (!x || !position || !y || ldx < k || ldy < k) return CKQ_EINVAL;
+    return launch_moe<MOE_GATHER>(type, {x, nullptr, y, position, nullptr, nullptr, ldx, 0, ldy, tokens, choices, rows, k}, stream);
+}
+
+extern "C" int ckq_launch_moe_combine(int type, const void *y, long ldy, const int32_t *position, const float *weights, void *out, long ldo,
+                                      int tokens, int choices, int rows, int k, void *stream)
+{
+    if (!y || !position || !out || ldy < k || ldo < k) return CKQ_EINVAL;
+    return launch_moe<MOE_COMBINE>(type, {y, nullptr, out, position, weights, nullptr, ldy, 0, ldo, tokens, choices, rows, k}, stream);
+}
+
+extern "C" int ckq_launch_moe_combine_backward(int type, const void *dout, long ldd, const void *y, long ldy, const int32_t *position, const float *weights,
+                                               void *dy, long lddy, float *dweights, int tokens, int choices, int rows, int k, void *stream)
+{
+    if (!dout || !y || !position || !weights || !dy || !dweights || ldd < k || ldy < k || lddy < k) return CKQ_EINVAL;
+    if (dy == y && lddy != ldy && rows > 1) return CKQ_EINVAL;        /* rows would be overwritten before they are read */
+    return launch_moe<MOE_BACKWARD>(type, {dout, y, dy, position, weights, dweights, ldd, ldy, lddy, tokens, choices, rows, k}, stream);
+}

@@ -207,14 +207,14 @@ def dev_gemm_nt_f32act(fmt, A_t, B_t, bias_t, M, N, K, out=None):
 # shape, strides, type and device once each, in one expression without calls of functions in Python (a matmul's checks 0.6 us less);
 # what that expression does not take goes to _i8_refuse, which looks again and says why.
 
-_torch, _INT8, _F32, _started, _device, _raw_stream, _I8_TYPES = None, None, None, None, None, None, {}
+_torch, _INT8, _F8, _I32, _F32, _started, _device, _raw_stream, _I8_TYPES = None, None, None, None, None, None, None, None, {}
 
 
 def _i8_torch():
     """torch, and what every call needs of it, once: an import statement in each call costs it 0.3 us a time, a chain of names 0.05."""
-    global _torch, _INT8, _F32, _started, _device, _raw_stream
+    global _torch, _INT8, _F8, _I32, _F32, _started, _device, _raw_stream
     import torch
-    _INT8, _F32 = torch.int8, torch.float32
+    _INT8, _F8, _I32, _F32 = torch.int8, torch.float8_e4m3fn, torch.int32, torch.float32
     _I8_TYPES.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})   # CKDataType values
     _started = torch.cuda.is_initialized
     _device, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -416,6 +416,310 @@ def dev_gemm_nt_i8(a, sa, b, sb, bias=None, dtype=None, out=None):
     if rc:
         check(rc, "ckq_gemm_nt_i8_dev")
     return c
+
+
+# ---- rows in e4m3 with one scale for each 128 elements, tokens sorted by expert --------------
+# The manner of the int8 rows above: one expression of checks a call, the reasons of a refusal looked for afterwards.
+# Scales are float32 [rows, groups] whose first index runs fastest (those of a group side by side), as empty_f8 makes them.
+
+def _f8_refuse(dev, rows, scales=(), wholes=()):
+    """Says what is wrong with a call: rows as _i8_refuse takes them; scales (tensor, name, shape), float32, the first index fastest; wholes,
+    contiguous tensors (tensor, name, shape, type).  All on device `dev`."""
+    for t, what, shape in scales:
+        if t.dtype is not _F32 or tuple(t.shape) != tuple(shape):
+            raise CkqError("%s has to be float32 of the shape %s, not %s %s" % (what, tuple(shape), t.dtype, tuple(t.shape)))
+        if t.get_device() != dev:
+            raise CkqError("%s is on %s, not on the current device" % (what, t.device))
+        if (t.shape[0] > 1 and t.stride(0) != 1) or (t.shape[1] > 1 and t.stride(1) < t.shape[0]):
+            raise CkqError("%s: the scales of a group have to lie side by side (empty_f8 makes them so)" % what)
+    for t, what, shape, dtype in wholes:
+        if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+            raise CkqError("%s has to be contiguous %s of the shape %s, not %s %s" % (what, dtype, tuple(shape), t.dtype, tuple(t.shape)))
+        if t.get_device() != dev:
+            raise CkqError("%s is on %s, not on the current device" % (what, t.device))
+    _i8_refuse(dev, rows, [])
+
+
+def empty_f8(rows, k, device="cuda"):
+    """(codes, scales) for rows of k: float8_e4m3fn [rows, k] whose rows begin at multiples of 16 bytes, as dev_gemm_nt_f8 takes them, and float32
+    [rows, ceil(k / 128)] with the scales of a group side by side."""
+    torch = _torch or _i8_torch()
+    return (torch.empty(rows, -(-k // 16) * 16, dtype=torch.float8_e4m3fn, device=device)[:, :k],
+            torch.empty(-(-k // 128), rows, dtype=torch.float32, device=device).t())
+
+
+def _f8_new(x, rows=None):
+    if x.dim() != 2:
+        raise CkqError("a tensor of the shape %s, not rows x k" % (tuple(x.shape),))
+    return empty_f8(x.shape[0] if rows is None else rows, x.shape[1], x.device)
+
+
+def _f8_side(scale, rows, groups):
+    """The pitch of scales [rows, groups], 0 where they do not lie as the library takes them."""
+    if scale.dtype is not _F32 or scale.shape != (rows, groups):
+        return 0
+    s0, s1 = scale.stride()
+    if groups == 1:
+        s1 = rows
+    return s1 if (s0 == 1 or rows == 1) and s1 >= rows else 0
+
+
+def dev_quantize_f8(x, out=None):
+    """Rows of x [rows, k] in e4m3: (q float8_e4m3fn [rows, k], scale float32 [rows, ceil(k / 128)])."""
+    dev, stream = _i8_where()
+    q, scale = out if out is not None else _f8_new(x)
+    shape, kind = x.shape, _I8_TYPES.get(x.dtype)
+    if (len(shape) != 2 or q.shape != shape or kind is None or q.dtype is not _F8 or not x.get_device() == q.get_device() == scale.get_device() == dev):
+        _f8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _F8)], [(scale, "scale", (shape[0], -(-shape[-1] // 128)))])
+    rows, k = shape
+    if (rows | k) >> 31:
+        _i8_too_many(rows, k)
+    lds = _f8_side(scale, rows, -(-k // 128))
+    (ldx, ex), (ldq, eq) = x.stride(), q.stride()
+    if (ex != 1 or eq != 1) and k > 1 or not lds:
+        _f8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _F8)], [(scale, "scale", (rows, -(-k // 128)))])
+    if rows == 1:
+        ldx = ldq = k
+    rc = lib().ckq_quantize_f8_dev(kind, x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr(), lds, rows, k, stream)
+    if rc:
+        check(rc, "ckq_quantize_f8_dev")
+    return q, scale
+
+
+def dev_dequantize_f8(q, scale, dtype=None, out=None):
+    """scale * q as rows of dtype (float32), or into `out`."""
+    dev, stream = _i8_where()
+    shape = q.shape
+    y = out if out is not None else _torch.empty(shape, dtype=dtype or _F32, device=q.device)
+    kind = _I8_TYPES.get(y.dtype)
+    if (len(shape) != 2 or y.shape != shape or kind is None or (dtype is not None and y.dtype is not dtype) or q.dtype is not _F8
+            or not q.get_device() == scale.get_device() == y.get_device() == dev):
+        _f8_refuse(dev, [(q, "q", None, _F8), (y, "out", shape, None), (y, "out", shape, dtype)], [(scale, "scale", (shape[0], -(-shape[-1] // 128)))])
+    rows, k = shape
+    if (rows | k) >> 31:
+        _i8_too_many(rows, k)
+    lds = _f8_side(scale, rows, -(-k // 128))
+    (ldq, eq), (ldy, ey) = q.stride(), y.stride()
+    if (eq != 1 or ey != 1) and k > 1 or not lds:
+        _f8_refuse(dev, [(q, "q", None, _F8), (y, "out", shape, None)], [(scale, "scale", (rows, -(-k // 128)))])
+    if rows == 1:
+        ldq = ldy = k
+    rc = lib().ckq_dequantize_f8_dev(q.data_ptr(), ldq, scale.data_ptr(), lds, kind, y.data_ptr(), ldy, rows, k, stream)
+    if rc:
+        check(rc, "ckq_dequantize_f8_dev")
+    return y
+
+
+def dev_swiglu_f8(gate, up, out=None):
+    """SiLU(gate) * up in e4m3: (q, scale); gate and up have one pitch (halves of one tensor, say)."""
+    dev, stream = _i8_where()
+    q, scale = out if out is not None else _f8_new(gate)
+    shape, t = gate.shape, gate.dtype
+    kind = _I8_TYPES.get(t)
+    if (len(shape) != 2 or q.shape != shape or up.shape != shape or kind is None or up.dtype is not t or q.dtype is not _F8
+            or not gate.get_device() == up.get_device() == q.get_device() == scale.get_device() == dev):
+        _f8_refuse(dev, [(gate, "gate", None, None), (up, "up", shape, t), (q, "q", shape, _F8)], [(scale, "scale", (shape[0], -(-shape[-1] // 128)))])
+    rows, k = shape
+    if (rows | k) >> 31:
+        _i8_too_many(rows, k)
+    lds = _f8_side(scale, rows, -(-k // 128))
+    (ld, eg), (ldu, eu), (ldq, eq) = gate.stride(), up.stride(), q.stride()
+    if (eg != 1 or eu != 1 or eq != 1) and k > 1 or ldu != ld and rows > 1 or not lds:
+        _f8_refuse(dev, [(gate, "gate", None, None), (up, "up", shape, t), (q, "q", shape, _F8)], [(scale, "scale", (rows, -(-k // 128)))])
+    if rows == 1:
+        ld = ldq = k
+    rc = lib().ckq_swiglu_f8_dev(kind, gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), lds, rows, k, stream)
+    if rc:
+        check(rc, "ckq_swiglu_f8_dev")
+    return q, scale
+
+
+def dev_gemm_nt_f8(a, sa, b, sb, bias=None, dtype=None, out=None):
+    """C [M, N] = a b^T (+ bias[n]) of the values that the codes stand for: float8_e4m3fn rows a [M, K] (tokens) with scales sa [M, ceil(K / 128)], b [N, K]
+    (channels) with float32 scales sb [ceil(N / 128), ceil(K / 128)]; C of dtype (float32), or into `out`."""
+    dev, stream = _i8_where()
+    of_a, of_b = a.shape, b.shape
+    if len(of_a) != 2 or len(of_b) != 2 or of_a[1] != of_b[1]:
+        _f8_refuse(dev, [(a, "a", None, _F8), (b, "b", (of_b[0], of_a[1]) if a.dim() == b.dim() == 2 else None, _F8)])
+    M, K = of_a
+    N = of_b[0]
+    if (M | N | K) >> 31:
+        _i8_too_many(M, N, K)
+    G, blocks = -(-K // 128), -(-N // 128)
+    c = out if out is not None else _torch.empty(M, N, dtype=dtype or _F32, device=b.device)
+    t = c.dtype
+    kind = _I8_TYPES.get(t)
+    ldsa = _f8_side(sa, M, G)
+    if (c.shape != (M, N) or kind is None or (dtype is not None and t is not dtype) or a.dtype is not _F8 or b.dtype is not _F8 or not ldsa
+            or sb.dtype is not _F32 or sb.shape != (blocks, G) or not sb.is_contiguous()
+            or not a.get_device() == b.get_device() == c.get_device() == sa.get_device() == sb.get_device() == dev):
+        _f8_refuse(dev, [(a, "a", None, _F8), (b, "b", None, _F8), (c, "out", (M, N), None), (c, "out", (M, N), dtype)], [(sa, "sa", (M, G))], [(sb, "sb", (blocks, G), _F32)])
+    bp = None
+    if bias is not None:
+        if bias.dtype is not _F32 or bias.shape != (N,) or not bias.is_contiguous() or bias.get_device() != dev:
+            _i8_refuse(dev, [], [(bias, "bias", (N,))])
+        bp = bias.data_ptr()
+    (lda, ea), (ldb, eb), (ldc, ec) = a.stride(), b.stride(), c.stride()
+    if (ea != 1 or eb != 1) and K > 1 or ec != 1 and N > 1:
+        _f8_refuse(dev, [(a, "a", None, _F8), (b, "b", None, _F8), (c, "out", (M, N), None)])
+    if M == 1:
+        lda, ldc = -(-K // 16) * 16, N
+    if N == 1:
+        ldb = -(-K // 16) * 16
+    rc = lib().ckq_gemm_nt_f8_dev(a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, sb.data_ptr(), G, bp, kind, c.data_ptr(), ldc, M, N, K, stream)
+    if rc:
+        check(rc, "ckq_gemm_nt_f8_dev")
+    return c
+
+
+def dev_gemm_nt_f8_experts(a, sa, b, sb, offsets, bias=None, dtype=None, out=None):
+    """Rows offsets[e] .. offsets[e + 1] - 1 of C [M, N] as dev_gemm_nt_f8 has them with b[e], sb[e], bias[e]: b float8_e4m3fn [E, N, K], sb float32 [E, ceil(N / 128),
+    ceil(K / 128)], bias float32 [E, N], offsets int32 [E + 1].  Rows that no expert has stay as they are in `out`."""
+    dev, stream = _i8_where()
+    of_a, of_b = a.shape, b.shape
+    if len(of_a) != 2 or len(of_b) != 3 or of_a[1] != of_b[2]:
+        raise CkqError("a of the shape %s and b of the shape %s, not rows x k and experts x rows x k" % (tuple(of_a), tuple(of_b)))
+    M, K = of_a
+    E, N = of_b[:2]
+    if (M | N | K | E) >> 31:
+        _i8_too_many(M, N, K, E)
+    G, blocks = -(-K // 128), -(-N // 128)
+    c = out if out is not None else _torch.empty(M, N, dtype=dtype or _F32, device=b.device)
+    t = c.dtype
+    kind = _I8_TYPES.get(t)
+    ldsa = _f8_side(sa, M, G)
+    if (c.shape != (M, N) or kind is None or (dtype is not None and t is not dtype) or a.dtype is not _F8 or b.dtype is not _F8 or not ldsa
+            or sb.dtype is not _F32 or sb.shape != (E, blocks, G) or not sb.is_contiguous() or offsets.dtype is not _I32 or offsets.shape != (E + 1,) or not offsets.is_contiguous()
+            or not a.get_device() == b.get_device() == c.get_device() == sa.get_device() == sb.get_device() == offsets.get_device() == dev):
+        _f8_refuse(dev, [(a, "a", None, _F8), (b[0] if E else b, "b[e]", None, _F8), (c, "out", (M, N), None), (c, "out", (M, N), dtype)], [(sa, "sa", (M, G))],
+                   [(sb, "sb", (E, blocks, G), _F32), (offsets, "offsets", (E + 1,), _I32)])
+    bp = None
+    if bias is not None:
+        if bias.dtype is not _F32 or bias.shape != (E, N) or not bias.is_contiguous() or bias.get_device() != dev:
+            _f8_refuse(dev, [], [], [(bias, "bias", (E, N), _F32)])
+        bp = bias.data_ptr()
+    (lda, ea), (per, ldb, eb), (ldc, ec) = a.stride(), b.stride(), c.stride()
+    if (ea != 1 or eb != 1) and K > 1 or ec != 1 and N > 1:
+        _f8_refuse(dev, [(a, "a", None, _F8), (b[0], "b[e]", None, _F8), (c, "out", (M, N), None)])
+    if M == 1:
+        lda, ldc = -(-K // 16) * 16, N
+    if N == 1:
+        ldb = -(-K // 16) * 16
+    if E == 1:
+        per = 0
+    rc = lib().ckq_gemm_nt_f8_experts_dev(a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, per, sb.data_ptr(), G, blocks * G, bp, offsets.data_ptr(), E, kind,
+                                          c.data_ptr(), ldc, M, N, K, stream)
+    if rc:
+        check(rc, "ckq_gemm_nt_f8_experts_dev")
+    return c
+
+
+def dev_moe_sort(ids, experts, out=None):
+    """Slots (t, j) of ids int32 [tokens, choices] in the order of their experts, those of one expert as they come: (offsets int32 [experts + 1], order int32 [tokens * choices],
+    position int32 [tokens, choices]); -1 in position, and at the end of order, for ids outside 0 .. experts - 1."""
+    dev, stream = _i8_where()
+    shape = ids.shape
+    if len(shape) != 2 or experts < 1:
+        raise CkqError("ids of the shape %s, not tokens x choices, or %s experts" % (tuple(shape), experts))
+    T, c = shape
+    if out is None:
+        out = (_torch.empty(experts + 1, dtype=_I32, device=ids.device), _torch.empty(T * c, dtype=_I32, device=ids.device), _torch.empty(T, c, dtype=_I32, device=ids.device))
+    offsets, order, position = out
+    if (not ids.dtype is offsets.dtype is order.dtype is position.dtype is _I32 or offsets.shape != (experts + 1,) or order.shape != (T * c,) or position.shape != shape
+            or not (ids.is_contiguous() and offsets.is_contiguous() and order.is_contiguous() and position.is_contiguous())
+            or not ids.get_device() == offsets.get_device() == order.get_device() == position.get_device() == dev):
+        _f8_refuse(dev, [], [], [(ids, "ids", shape, _I32), (offsets, "offsets", (experts + 1,), _I32), (order, "order", (T * c,), _I32), (position, "position", shape, _I32)])
+    if (T | c | experts) >> 31:
+        _i8_too_many(T, c, experts)
+    rc = lib().ckq_moe_sort_dev(ids.data_ptr(), T, c, experts, offsets.data_ptr(), order.data_ptr(), position.data_ptr(), stream)
+    if rc:
+        check(rc, "ckq_moe_sort_dev")
+    return out
+
+
+def _moe_shapes(x, tokens_of, position, others, weights=()):
+    """What a call of rows there and back takes: x [tokens_of or any rows, k] of floats, position int32 [tokens, choices], others (tensor, name, rows or None) of x's
+    type and width, weights (tensor, name) like position.  Returns the device's number for the library's checks of types."""
+    dev, _ = _i8_where()
+    shape, kind = x.shape, _I8_TYPES.get(x.dtype)
+    ok = (len(shape) == 2 and position.dim() == 2 and kind is not None and position.dtype is _I32 and position.is_contiguous() and x.get_device() == position.get_device() == dev
+          and (x.stride(1) == 1 or shape[1] <= 1) and (tokens_of is None or shape[0] == tokens_of))
+    for t, _, rows in others:
+        ok = ok and t.dim() == 2 and t.dtype is x.dtype and t.shape[1] == shape[1] and (rows is None or t.shape[0] == rows) and (t.stride(1) == 1 or shape[1] <= 1) and t.get_device() == dev
+    for t, _ in weights:
+        ok = ok and t.dtype is _F32 and t.shape == position.shape and t.is_contiguous() and t.get_device() == dev
+    if not ok:
+        if position.dim() != 2:
+            raise CkqError("position has the shape %s, not tokens x choices" % (tuple(position.shape),))
+        _f8_refuse(dev, [(x, "rows", None if tokens_of is None else (tokens_of, x.shape[-1]), None)]
+                   + [(t, what, (t.shape[0] if rows is None else rows, x.shape[-1]), x.dtype) for t, what, rows in others], [],
+                   [(position, "position", position.shape, _I32)] + [(t, what, position.shape, _F32) for t, what in weights])
+    if (shape[0] | shape[1] | position.shape[0] | position.shape[1]) >> 31:
+        _i8_too_many(*shape, *position.shape)
+    return kind
+
+
+def _pitch(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def dev_moe_gather(x, position, out=None):
+    """y[position[t][j]] = x[t]: x [tokens, k], position as dev_moe_sort has it; y [tokens * choices, k], or into the rows of `out`.  Rows that have no slot stay as they are."""
+    if out is None and x.dim() == position.dim() == 2:
+        out = (_torch or _i8_torch()).empty(position.numel(), x.shape[1], dtype=x.dtype, device=x.device)
+    kind = _moe_shapes(x, position.shape[0], position, [(out, "out", None)])
+    T, c = position.shape
+    rc = lib().ckq_moe_gather_dev(kind, x.data_ptr(), _pitch(x), position.data_ptr(), out.data_ptr(), _pitch(out), T, c, out.shape[0], x.shape[1], _i8_where()[1])
+    if rc:
+        check(rc, "ckq_moe_gather_dev")
+    return out
+
+
+def dev_moe_gather_f8(x, position, out=None):
+    """The same in e4m3: (q [tokens * choices, k], scale)."""
+    q, scale = out if out is not None else _f8_new(x, position.numel())
+    kind = _moe_shapes(x, position.shape[0], position, [])
+    dev, stream = _i8_where()
+    k = x.shape[1]
+    rows = q.shape[0]
+    lds = _f8_side(scale, rows, -(-k // 128))
+    if rows >> 31:
+        _i8_too_many(rows)
+    if q.dim() != 2 or q.shape[1] != k or q.dtype is not _F8 or (q.stride(1) != 1 and k > 1) or not lds or not q.get_device() == scale.get_device() == dev:
+        _f8_refuse(dev, [(q, "q", (rows, k), _F8)], [(scale, "scale", (rows, -(-k // 128)))])
+    T, c = position.shape
+    rc = lib().ckq_moe_gather_f8_dev(kind, x.data_ptr(), _pitch(x), position.data_ptr(), q.data_ptr(), _pitch(q), scale.data_ptr(), lds, T, c, rows, k, stream)
+    if rc:
+        check(rc, "ckq_moe_gather_f8_dev")
+    return q, scale
+
+
+def dev_moe_combine(y, position, weights=None, out=None):
+    """out[t] = sum over j of weights[t][j] * y[position[t][j]]: [tokens, k].  Without weights (ones) the gradient of dev_moe_gather."""
+    if out is None and y.dim() == position.dim() == 2:
+        out = (_torch or _i8_torch()).empty(position.shape[0], y.shape[1], dtype=y.dtype, device=y.device)
+    kind = _moe_shapes(y, None, position, [(out, "out", position.shape[0])], [(weights, "weights")] if weights is not None else ())
+    T, c = position.shape
+    rc = lib().ckq_moe_combine_dev(kind, y.data_ptr(), _pitch(y), position.data_ptr(), weights.data_ptr() if weights is not None else None, out.data_ptr(), _pitch(out),
+                                   T, c, y.shape[0], y.shape[1], _i8_where()[1])
+    if rc:
+        check(rc, "ckq_moe_combine_dev")
+    return out
+
+
+def dev_moe_combine_backward(dout, y, position, weights, out=None):
+    """Of dout [tokens, k], the gradient of dev_moe_combine's result: (dy, of y's shape, dweights float32 [tokens, choices]).  Rows of dy that have no slot stay as they
+    are; dy may be y."""
+    if out is None:
+        out = (_torch or _i8_torch()).empty_strided(y.shape, y.stride(), dtype=y.dtype, device=y.device), _torch.empty(position.shape, dtype=_torch.float32, device=y.device)
+    dy, dw = out
+    kind = _moe_shapes(dout, position.shape[0], position, [(y, "y", None), (dy, "dy", y.shape[0])], [(weights, "weights"), (dw, "dweights")])
+    T, c = position.shape
+    rc = lib().ckq_moe_combine_backward_dev(kind, dout.data_ptr(), _pitch(dout), y.data_ptr(), _pitch(y), position.data_ptr(), weights.data_ptr(), dy.data_ptr(), _pitch(dy),
+                                            dw.data_ptr(), T, c, y.shape[0], y.shape[1], _i8_where()[1])
+    if rc:
+        check(rc, "ckq_moe_combine_backward_dev")
+    return dy, dw
 
 
 def dev_subblock_dots(fmt, W_t, x_t, M, K):

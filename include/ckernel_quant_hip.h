@@ -314,6 +314,54 @@ int ckq_swiglu_i8_dev(ckq_ck_dtype type, const void *gate, const void *up, long 
 int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t *B, long ldb, const float *sb, const float *bias,
                        ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream);
 
+/* Rows in 8-bit floating point (e4m3: four bits of exponent, three of mantissa, no infinities, largest 448) with one fp32 scale for each group of 128
+ * elements: the value of q[row][i] is scale[i / 128][row] * q[row][i].  The last group of a row may be shorter.  The scales of one group lie
+ * side by side: scale[g * lds + row], lds at least the number of rows, so that a tile of tokens finds its own together.  Weights have one scale for each block of 128 rows x 128 elements,
+ * block by block as checkpoints hold them: sb[(n / 128) * ldsb + k / 128].  No counterpart in the reference.  Types, pitches, alignment of floats and errors as with
+ * the rows of int8 above; nothing is allocated, no scratch is shared between calls, every call may be captured, and the same call has the same bits each time.
+ *
+ * ckq_quantize_f8_dev: a = max(largest |x| of the group, 2^-100), q = the e4m3 value nearest to 448 x / a (the quotient rounded correctly to fp32, ties of codes
+ * to even), scale = a / 448.  A group with a NaN or an infinity gets that as its scale (NaN if there is one) and zeros as its codes.  Bytes of q behind
+ * a row's k-th stay as they are.
+ * ckq_dequantize_f8_dev: y = scale * q, rounded to the type.
+ * ckq_swiglu_f8_dev: gate / (1 + exp(-gate)) * up in 8 bits as above (the function as exact as ckq_swiglu_i8_dev's); gate and up have one pitch, ld.
+ * ckq_gemm_nt_f8_dev: C[m*ldc + n] = sum over groups g of (sa[g*ldsa + m] * sb[(n/128)*ldsb + g]) * (sum over k in g of A[m][k] * B[n][k]) (+ bias[n]), in
+ * fp32, rounded once to the type of C.  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are, multiples of 16 bytes, pitches at
+ * most 4 MiB (else CKQ_EROWS).  K may be any number: of the 16 bytes that hold a row's last, those behind it may be read and are not used.  The gradient of the
+ * activations is the same product with the transposed codes and scales of the weights.
+ * ckq_gemm_nt_f8_experts_dev: the same of rows sorted by expert, each expert with a matrix, scales and bias of its own: rows offsets[e] .. offsets[e + 1] - 1 of A and C
+ * with B + e * eb, sb + e * esb and bias + e * N (eb a multiple of 16).  offsets are on the device, experts + 1 of them, from 0 on and none less than the one before
+ * (what lies outside 0 .. M counts as the nearest of these); an expert may have no rows, and rows of C that no expert has stay as they are. */
+int ckq_quantize_f8_dev(ckq_ck_dtype type, const void *x, long ldx, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
+int ckq_dequantize_f8_dev(const uint8_t *q, long ldq, const float *scale, long lds, ckq_ck_dtype type, void *y, long ldy, int rows, int k, void *stream);
+int ckq_swiglu_f8_dev(ckq_ck_dtype type, const void *gate, const void *up, long ld, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
+int ckq_gemm_nt_f8_dev(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, const float *sb, long ldsb, const float *bias,
+                       ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream);
+int ckq_gemm_nt_f8_experts_dev(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, long eb, const float *sb, long ldsb, long esb,
+                               const float *bias, const int32_t *offsets, int experts, ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream);
+
+/* Tokens sorted by expert and back, around the product above.  Each token has `choices` slots, s = t * choices + j: ids[s] is the number of an expert (anything outside
+ * 0 .. experts - 1: the slot has none, a padded token, say, or an expert of another device), weights[s] what its result counts.  The same expert may be there twice.  At most 65535 experts and 2^30
+ * slots, at least one token, choice, expert and element (else CKQ_EINVAL); integers are int32.  No atomics: the same bits each time.
+ *
+ * ckq_moe_sort_dev: slots in the order of their experts, those of one expert as they come: offsets[e] = number of slots of experts under e (experts + 1 of them),
+ * order[p] = the slot at place p (-1 from offsets[experts] on), position[s] = the place of slot s (-1: none).
+ * In what follows y has `rows` rows, and a position outside 0 .. rows - 1 counts as none.  No two slots have one position.
+ * ckq_moe_gather_dev: y[position[s]] = x[s / choices]; other rows of y stay as they are.
+ * ckq_moe_gather_f8_dev: the same in 8 bits, as ckq_quantize_f8_dev has them (lds at least `rows`).
+ * ckq_moe_combine_dev: out[t] = sum over j of weights[s] * y[position[s]], in fp32, j in turn, rounded once; zeros where a token has no slot with a place.  weights NULL: ones - the
+ * gradient of gather, of the experts' rows' gradients.
+ * ckq_moe_combine_backward_dev: of dout, the gradient of combine's result: dy[position[s]] = weights[s] * dout[t], rounded to the type (other rows stay as they are; dy may be y itself, with
+ * one pitch, else CKQ_EINVAL), and dweights[s] = sum over i of dout[t][i] * y[position[s]][i] in fp32 (0 where there is no place). */
+int ckq_moe_sort_dev(const int32_t *ids, int tokens, int choices, int experts, int32_t *offsets, int32_t *order, int32_t *position, void *stream);
+int ckq_moe_gather_dev(ckq_ck_dtype type, const void *x, long ldx, const int32_t *position, void *y, long ldy, int tokens, int choices, int rows, int k, void *stream);
+int ckq_moe_gather_f8_dev(ckq_ck_dtype type, const void *x, long ldx, const int32_t *position, uint8_t *q, long ldq, float *scale, long lds,
+                          int tokens, int choices, int rows, int k, void *stream);
+int ckq_moe_combine_dev(ckq_ck_dtype type, const void *y, long ldy, const int32_t *position, const float *weights, void *out, long ldo,
+                        int tokens, int choices, int rows, int k, void *stream);
+int ckq_moe_combine_backward_dev(ckq_ck_dtype type, const void *dout, long ldd, const void *y, long ldy, const int32_t *position, const float *weights,
+                                 void *dy, long lddy, float *dweights, int tokens, int choices, int rows, int k, void *stream);
+
 /* A list of steps enqueued back-to-back, the whole list `repeat` times: the
  * per-token chain of a decoder layer (norm -> Q8_K -> Q/K/V ... -> down) is one
  * such list.  A matmul entry (fmt = a ckq_format weight tag) computes

@@ -1,0 +1,135 @@
+"""CPU checks of the entry points of e4m3 rows and of tokens sorted by expert: what they refuse, before anything touches a device, and with
+which code.  No kernel is launched here."""
+import ctypes
+import importlib
+import os
+
+import pytest
+
+ckq = importlib.import_module("c-kernel-engine_amd")
+EINVAL, EFORMAT, EROWS = -1, -3, -8
+F32, BF16, F16 = 0, 1, 2
+
+
+@pytest.fixture(scope="module")
+def L():
+    if not os.path.exists(ckq.lib_path()):
+        ckq.build()
+    return ckq.lib()
+
+
+P = ctypes.c_void_p(4096)
+
+
+def odd(n):
+    return ctypes.c_void_p(4096 + n)
+
+
+def refuses(call, invalid, format_, rows):
+    for bad in invalid:
+        assert call(**bad) == EINVAL, bad
+    for bad in format_:
+        assert call(**bad) == EFORMAT, bad
+    for bad in rows:
+        assert call(**bad) == EROWS, bad
+
+
+TYPES_THAT_ARE_NONE = [{"t": t} for t in (-1, 3, 7, 9, 13)]
+
+
+def test_rows_refusals(L):
+    def quantize(t=BF16, x=P, ldx=64, q=P, ldq=64, scale=P, lds=2, rows=2, k=64):
+        return L.ckq_quantize_f8_dev(t, x, ldx, q, ldq, scale, lds, rows, k, None)
+
+    def dequantize(q=P, ldq=64, scale=P, lds=2, t=BF16, y=P, ldy=64, rows=2, k=64):
+        return L.ckq_dequantize_f8_dev(q, ldq, scale, lds, t, y, ldy, rows, k, None)
+
+    def swiglu(t=BF16, gate=P, up=P, ld=128, q=P, ldq=64, scale=P, lds=2, rows=2, k=64):
+        return L.ckq_swiglu_f8_dev(t, gate, up, ld, q, ldq, scale, lds, rows, k, None)
+
+    sizes = [{"rows": 0}, {"rows": -1}, {"k": 0}, {"k": -5}, {"lds": 1}, {"ldq": 63}, {"q": None}, {"scale": None}]
+    refuses(quantize, sizes + [{"x": None}, {"ldx": 63}], TYPES_THAT_ARE_NONE, [{"x": odd(1)}, {"scale": odd(2)}, {"t": F32, "x": odd(2)}])
+    refuses(dequantize, sizes + [{"y": None}, {"ldy": 63}], TYPES_THAT_ARE_NONE, [{"y": odd(1)}, {"scale": odd(2)}, {"t": F32, "y": odd(2)}])
+    refuses(swiglu, sizes + [{"gate": None}, {"up": None}, {"ld": 63}], TYPES_THAT_ARE_NONE, [{"gate": odd(1)}, {"up": odd(1)}, {"scale": odd(1)}, {"t": F32, "up": odd(2)}])
+
+
+def test_matmul_refusals(L):
+    def gemm(a=P, lda=64, sa=P, ldsa=2, b=P, ldb=64, sb=P, ldsb=1, bias=P, t=BF16, c=P, ldc=32, M=2, N=32, K=50):
+        return L.ckq_gemm_nt_f8_dev(a, lda, sa, ldsa, b, ldb, sb, ldsb, bias, t, c, ldc, M, N, K, None)
+
+    def experts(a=P, lda=64, sa=P, ldsa=2, b=P, ldb=64, eb=2048, sb=P, ldsb=1, esb=1, bias=P, o=P, E=3, t=BF16, c=P, ldc=32, M=2, N=32, K=50):
+        return L.ckq_gemm_nt_f8_experts_dev(a, lda, sa, ldsa, b, ldb, eb, sb, ldsb, esb, bias, o, E, t, c, ldc, M, N, K, None)
+
+    invalid = [{"a": None}, {"sa": None}, {"b": None}, {"sb": None}, {"c": None}, {"M": 0}, {"N": 0}, {"K": 0}, {"M": -1}, {"K": 65}, {"lda": 48}, {"ldb": 48}, {"ldc": 31}, {"ldsa": 1},
+               {"ldsb": 0}, {"K": 129, "lda": 144, "ldb": 144}]
+    rows = [{"a": odd(8)}, {"b": odd(4)}, {"lda": 72}, {"ldb": 50}, {"lda": (1 << 22) + 16}, {"ldb": 1 << 30}, {"c": odd(1)}, {"t": F32, "c": odd(2)}, {"sa": odd(2)}, {"sb": odd(1)}, {"bias": odd(3)}]
+    refuses(gemm, invalid, TYPES_THAT_ARE_NONE, rows)
+    refuses(experts, invalid + [{"o": None}, {"E": 0}, {"E": -2}, {"E": 65536}, {"eb": -16}, {"esb": -1}], TYPES_THAT_ARE_NONE, rows + [{"eb": 2040}, {"o": odd(2)}])
+    assert b"16 bytes" in L.ckq_error_string(EROWS)
+
+
+def test_sort_and_rows_there_and_back_refusals(L):
+    def sort(ids=P, T=2, c=2, E=3, offsets=P, order=P, position=P):
+        return L.ckq_moe_sort_dev(ids, T, c, E, offsets, order, position, None)
+
+    refuses(sort, [{"ids": None}, {"offsets": None}, {"order": None}, {"position": None}, {"T": 0}, {"c": 0}, {"E": 0}, {"T": -1}, {"E": 65536}, {"T": 1 << 20, "c": 1025}, {"T": (1 << 31) - 1, "c": (1 << 31) - 1}],
+            [], [{"ids": odd(1)}, {"offsets": odd(2)}, {"order": odd(2)}, {"position": odd(2)}])
+
+    def gather(t=BF16, x=P, ldx=64, pos=P, y=P, ldy=64, T=2, c=2, rows=4, k=64):
+        return L.ckq_moe_gather_dev(t, x, ldx, pos, y, ldy, T, c, rows, k, None)
+
+    def gather_f8(t=BF16, x=P, ldx=64, pos=P, q=P, ldq=64, scale=P, lds=4, T=2, c=2, rows=4, k=64):
+        return L.ckq_moe_gather_f8_dev(t, x, ldx, pos, q, ldq, scale, lds, T, c, rows, k, None)
+
+    def combine(t=BF16, y=P, ldy=64, pos=P, w=P, out=P, ldo=64, T=2, c=2, rows=4, k=64):
+        return L.ckq_moe_combine_dev(t, y, ldy, pos, w, out, ldo, T, c, rows, k, None)
+
+    def backward(t=BF16, dout=P, ldd=64, y=P, ldy=64, pos=P, w=P, dy=P, lddy=64, dw=P, T=2, c=2, rows=4, k=64):
+        return L.ckq_moe_combine_backward_dev(t, dout, ldd, y, ldy, pos, w, dy, lddy, dw, T, c, rows, k, None)
+
+    sizes = [{"T": 0}, {"c": 0}, {"rows": 0}, {"k": 0}, {"T": -1}, {"k": -1}, {"pos": None}]
+    refuses(gather, sizes + [{"x": None}, {"y": None}, {"ldx": 63}, {"ldy": 63}], TYPES_THAT_ARE_NONE, [{"x": odd(1)}, {"y": odd(1)}, {"pos": odd(2)}, {"t": F32, "y": odd(2)}])
+    refuses(gather_f8, sizes + [{"x": None}, {"q": None}, {"scale": None}, {"ldx": 63}, {"ldq": 63}, {"lds": 3}], TYPES_THAT_ARE_NONE, [{"x": odd(1)}, {"scale": odd(1)}, {"pos": odd(2)}])
+    refuses(combine, sizes + [{"y": None}, {"out": None}, {"ldy": 63}, {"ldo": 63}], TYPES_THAT_ARE_NONE, [{"y": odd(1)}, {"out": odd(1)}, {"pos": odd(2)}, {"w": odd(2)}])
+    refuses(backward, sizes + [{"dout": None}, {"y": None}, {"w": None}, {"dy": None}, {"dw": None}, {"ldd": 63}, {"ldy": 63}, {"lddy": 63}, {"lddy": 80}], TYPES_THAT_ARE_NONE,
+            [{"dout": odd(1)}, {"y": odd(1)}, {"dy": odd(1)}, {"pos": odd(2)}, {"w": odd(2)}, {"dw": odd(1)}])
+
+
+def test_front_ends_refuse_what_a_pointer_cannot_tell():
+    import torch
+    par, err = ckq.parity, ckq.CkqError
+    x, pos = torch.zeros(3, 32), torch.zeros(3, 2, dtype=torch.int32)
+    if not torch.cuda.is_available():
+        for call in (lambda: par.dev_quantize_f8(x), lambda: par.dev_moe_sort(pos, 4), lambda: par.dev_moe_gather(x, pos), lambda: par.dev_moe_combine(x, pos)):
+            with pytest.raises(err, match="not on the current device"):
+                call()
+    for call in (lambda: par.dev_quantize_f8(x[0]), lambda: par.dev_swiglu_f8(x[0], x[0]), lambda: par.dev_moe_sort(pos[0], 4), lambda: par.dev_moe_gather(x, pos[0]),
+                 lambda: par.dev_moe_gather_f8(x[0], pos), lambda: par.dev_gemm_nt_f8_experts(x, x, x, x, pos)):
+        with pytest.raises(err, match="shape"):
+            call()
+    q, s = par.empty_f8(3, 200, device="cpu")
+    assert q.shape == (3, 200) and q.stride() == (208, 1) and s.shape == (3, 2) and s.stride() == (1, 3) and q.dtype == torch.float8_e4m3fn
+
+
+def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
+    """ctypes passes the lowest 32 bits of an int: 2^32 + 16 rows would be 16.  Memory that nothing touches, and a library that nothing reaches."""
+    import torch
+    par, err = ckq.parity, ckq.CkqError
+    if torch.cuda.is_available():
+        pytest.skip("the memory of a host without a device is meant")
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: 0
+    monkeypatch.setattr(par, "lib", Library)
+    monkeypatch.setattr(par, "_i8_where", lambda: (-1, None))            # the device of host tensors
+    par._i8_torch()
+    many = (1 << 32) + 16
+    f, q, s = torch.empty(many, 1), torch.empty(many, 1, dtype=torch.float8_e4m3fn), torch.empty(1, many).t()
+    assert par.dev_quantize_f8(torch.zeros(4, 16))[0].shape == (4, 16)   # sizes as they should be get through
+    for call in (lambda: par.dev_quantize_f8(f, out=(q, s)), lambda: par.dev_dequantize_f8(q, s, out=f), lambda: par.dev_swiglu_f8(f, f, out=(q, s)),
+                 lambda: par.dev_gemm_nt_f8(q, s, q[:2], torch.empty(1, 1), out=f.view(many, 1).expand(many, 2)),
+                 lambda: par.dev_moe_sort(torch.empty(many, 1, dtype=torch.int32), 2), lambda: par.dev_moe_combine(f, torch.zeros(1, 1, dtype=torch.int32)),
+                 lambda: par.dev_moe_gather_f8(f[:2], torch.zeros(2, 1, dtype=torch.int32), out=(q, s))):
+        with pytest.raises(err, match="2\\^31"):
+            call()
