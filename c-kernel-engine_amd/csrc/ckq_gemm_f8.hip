@@ -13,6 +13,7 @@
 #include "ckq_gemm_common.hpp"
 #include "ckq_int8.hpp"
 #include "ckq_rows.hpp"
+#include <atomic>
 
 typedef _Float16 f8_v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 f8_v8h __attribute__((ext_vector_type(8)));
@@ -27,53 +28,70 @@ struct F8Args {
     int            M, N, K, experts;
 };
 
-/* Which rows the t-th tile of BT rows has: expert e, rows m0 .. mend - 1.  All lanes of a wave. */
-__device__ __forceinline__ bool f8_rows(const F8Args &a, int t, int BT, int &e, int &m0, int &mend)
+/* ---- which tile ---------------------------------------------------------------------------------------------------- */
+
+/* Inclusive sums over a wave's lanes. */
+__device__ __forceinline__ int wave_scan(int v)
 {
-    if (!a.offsets) {
-        e = 0;
-        m0 = t * BT;
-        mend = a.M;
-        return m0 < a.M;
-    }
+    v += dpp_get<0x111>(v);                                    /* row_shr 1, 2, 4, 8 */
+    v += dpp_get<0x112>(v);
+    v += dpp_get<0x114>(v);
+    v += dpp_get<0x118>(v);
+    v += dpp_get<0x142, 0xA>(v);                               /* row_bcast 15, 31 */
+    v += dpp_get<0x143, 0xC>(v);
+    return v;
+}
+
+struct F8Tile { int e, m0, mend, nt; };                        /* expert, rows m0 .. mend - 1 of A, tile of weight rows */
+
+/* Which tile of BT rows x a tile of weight rows the `id`-th block has.  Tiles are dealt to the XCDs in equal runs (gemm_deal), and in the order of a run eight
+ * tiles of rows lie beside each other for every tile of weight rows, so that the tiles an XCD works on at a time share both operands in its L2.  Of experts, the
+ * tiles that there are are counted first, from the offsets: 64 experts at a time, one a lane. */
+__device__ __forceinline__ bool f8_tile(const F8Args &a, int id, int BT, int nnt, F8Tile &w)
+{
     const int lane = threadIdx.x & 63;
+    int ntt = (a.M + BT - 1) / BT, lo = 0, hi = 0, sum = 0, n = 0;
+    auto chunk = [&](int e0) {                                 /* the tiles of experts e0 .. e0 + 63 */
+        const int i = min(e0 + lane, a.experts - 1);
+        lo = max(0, min(a.offsets[i], a.M));
+        hi = max(lo, min(a.offsets[i + 1], a.M));
+        n = e0 + lane < a.experts ? (hi - lo + BT - 1) / BT : 0;
+        sum = wave_scan(n);
+        return __builtin_amdgcn_readlane(sum, 63);
+    };
+    if (a.offsets) {
+        ntt = 0;
+        const int most = a.M / BT + min(a.M, a.experts);       /* that the launch counts with: offsets may be anything */
+        for (int e0 = 0; e0 < a.experts; e0 += 64) ntt = min(ntt + chunk(e0), most);
+    }
+    const int t = ntt ? gemm_deal(id, ntt * nnt) : -1;
+    if (t < 0) return false;
+    const int band = t / (8 * nnt), in = t - band * 8 * nnt, wide = min(8, ntt - 8 * band);
+    w.nt = in / wide;
+    const int tt = 8 * band + in - w.nt * wide;
+    w.e = 0;
+    w.m0 = tt * BT;
+    w.mend = a.M;
+    if (!a.offsets) return true;
     int before = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 64) {
-        const int i = min(e0 + lane, a.experts - 1);
-        const int lo = max(0, min(a.offsets[i], a.M)), hi = max(lo, min(a.offsets[i + 1], a.M));
-        const int n = e0 + lane < a.experts ? (hi - lo + BT - 1) / BT : 0;
-        int sum = n;
-        for (int d = 1; d < 64; d *= 2) {
-            const int other = __shfl_up(sum, d);
-            if (lane >= d) sum += other;
-        }
-        const unsigned long long m = __ballot(before + sum > t);
-        if (m) {
-            const int l = __ffsll((long long)m) - 1;
-            e = __builtin_amdgcn_readfirstlane(e0 + l);
-            m0 = __builtin_amdgcn_readlane(lo + (t - before - (sum - n)) * BT, l);
-            mend = __builtin_amdgcn_readlane(hi, l);
+        const int all = a.experts <= 64 ? __builtin_amdgcn_readlane(sum, 63) : chunk(e0);
+        if (before + all > tt) {
+            const int l = __ffsll((long long)__ballot(before + sum > tt)) - 1;
+            w.e = e0 + l;
+            w.m0 = __builtin_amdgcn_readlane(lo + (tt - before - (sum - n)) * BT, l);
+            w.mend = __builtin_amdgcn_readlane(hi, l);
             return true;
         }
-        before += __builtin_amdgcn_readlane(sum, 63);
+        before += all;
     }
     return false;
 }
 
-/* Sixteen bytes of a row from k on, zeros behind its last. */
-__device__ __forceinline__ ckq_v4i f8_chunk(const uint8_t *row, int k, int K)
-{
-    ckq_v4i v = {0, 0, 0, 0};
-    if (k < K) v = *reinterpret_cast<const ckq_v4i *>(row + k);
-    if (K - k < 16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = K - k - 4 * i;
-            v[i] = n >= 4 ? v[i] : n <= 0 ? 0 : v[i] & (int)((1u << (8 * n)) - 1u);
-        }
-    }
-    return v;
-}
+/* Blocks that have all tiles there can be: an expert's last tile may be one row. */
+static long f8_most_tiles(const F8Args &a, int BT) { return a.offsets ? (long)a.M / BT + min(a.M, a.experts) : ((long)a.M + BT - 1) / BT; }
+
+/* ---- operands and results -------------------------------------------------------------------------------------------- */
 
 /* Eight codes as fp16. */
 __device__ __forceinline__ f8_v8h f8_half(int lo, int hi)
@@ -83,57 +101,348 @@ __device__ __forceinline__ f8_v8h f8_half(int lo, int hi)
     return f8_v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-/* 16 tokens x 64 rows a wave, operands straight from memory. */
+template <class E> struct __attribute__((packed, aligned(sizeof(E)))) f8_out8 { E v[8]; };
+
+/* Eight rows' results of a token to C[t][n ..], non-temporally: they are not read again by the launch that writes them. */
 template <class E>
-__global__ void __launch_bounds__(256) gemm_f8_kernel(F8Args a, int nnt)
+__device__ __forceinline__ void f8_store8(const F8Args &a, const float *bias, const float (&f)[8], int t, int n)
 {
-    const int lane = threadIdx.x & 63, wave = wave_in_block();
-    const int tt = (int)blockIdx.x / nnt, n0 = ((int)blockIdx.x - tt * nnt) * 256 + 64 * wave;
-    int e, m0, mend;
-    if (!f8_rows(a, tt, 16, e, m0, mend) || n0 >= a.N) return;
-    const uint8_t *B = a.B + (size_t)e * a.eb;
-    const float *sb = a.sb + (size_t)e * a.esb, *bias = a.bias ? a.bias + (size_t)e * a.N : nullptr;
-    const int tok = min(m0 + (lane & 15), mend - 1);
-    const uint8_t *pa = a.A + (size_t)tok * a.lda, *pb[4];
+    const int left = a.N - n;
+    f8_out8<E> o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) pb[j] = B + (size_t)min(n0 + 16 * j + (lane & 15), a.N - 1) * a.ldb;
-    f8_v4f acc[4];
+    for (int r = 0; r < 8; ++r) o.v[r] = (E)(bias ? f[r] + bias[min(n + r, a.N - 1)] : f[r]);
+    E *out = (E *)a.C + (size_t)t * a.ldc + n;
+    if (left >= 8) {
+        struct { rows_u4 v[sizeof(o) / 16]; } w = __builtin_bit_cast(decltype(w), o);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int g = 0; g * 128 < a.K; ++g) {
-        const int k = 128 * g + 32 * (lane >> 4);
-        const ckq_v4i x0 = f8_chunk(pa, k, a.K), x1 = f8_chunk(pa, k + 16, a.K);
-        const f8_v8h x[4] = {f8_half(x0[0], x0[1]), f8_half(x0[2], x0[3]), f8_half(x1[0], x1[1]), f8_half(x1[2], x1[3])};
-        const float s = a.sa[(size_t)g * a.ldsa + tok] * sb[(size_t)(n0 >> 7) * a.ldsb + g];
+        for (int i = 0; i < (int)(sizeof(o) / 16); ++i) __builtin_nontemporal_store(w.v[i], reinterpret_cast<rows_u4_at_2 *>(out) + i);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const ckq_v4i w0 = f8_chunk(pb[j], k, a.K), w1 = f8_chunk(pb[j], k + 16, a.K);
-            f8_v4f p = {0.0f, 0.0f, 0.0f, 0.0f};
-            p = __builtin_amdgcn_mfma_f32_16x16x32_f16(f8_half(w0[0], w0[1]), x[0], p, 0, 0, 0);
-            p = __builtin_amdgcn_mfma_f32_16x16x32_f16(f8_half(w0[2], w0[3]), x[1], p, 0, 0, 0);
-            p = __builtin_amdgcn_mfma_f32_16x16x32_f16(f8_half(w1[0], w1[1]), x[2], p, 0, 0, 0);
-            p = __builtin_amdgcn_mfma_f32_16x16x32_f16(f8_half(w1[2], w1[3]), x[3], p, 0, 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] = __builtin_fmaf(s, p[i], acc[j][i]);
-        }
+        for (int r = 0; r < 8; ++r)
+            if (r < left) out[r] = o.v[r];
     }
-    if (m0 + (lane & 15) >= mend) return;
-    E *out = (E *)a.C + (size_t)tok * a.ldc;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
+}
+
+/* Zeros in the bytes behind `tail` of the step of 128 whose `rows` rows lie at p, chunks of 16 swizzled (f8_place): both operands', since a byte there may
+ * be a NaN.  `threads` threads. */
+__device__ __forceinline__ void f8_clear_tail(uint8_t *p, int rows, int tail, int thread, int threads)
+{
+    for (int e = thread; e < rows * 8; e += threads) {
+        const int row = e >> 3, left = tail - 16 * ((e & 7) ^ ((row >> 1) & 7));
+        if (left >= 16) continue;
+        ckq_v4i *q = reinterpret_cast<ckq_v4i *>(p + 16 * e);
+        ckq_v4i v = *q;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int n = n0 + 16 * j + 4 * (lane >> 4) + i;
-            if (n < a.N) out[n] = (E)(acc[j][i] + (bias ? bias[n] : 0.0f));
+            const int n = left - 4 * i;
+            v[i] = n >= 4 ? v[i] : n <= 0 ? 0 : v[i] & (int)((1u << (8 * n)) - 1u);
         }
+        *q = v;
+    }
+}
+
+/* ---- tiles on the fp16 instructions ----------------------------------------------------------------------------------- */
+
+/* WT x WN waves, each 32 TT tokens x 32 TN rows.  A step is a group of 128; its codes come to LDS as they are, eight rows of 128 bytes a copy, the chunk of 16 that a
+ * lane fetches is the one that belongs in its place, c ^ (row / 2 % 8), so that a read of 16 bytes a lane meets all banks once. */
+template <int WT_, int WN_, int TT_, int TN_> struct F8Half {
+    static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NW = WT * WN, BT = 32 * TT * WT, BN = 32 * TN * WN, S = 2;
+    static constexpr int CODES = (BT + BN) * 128, STAGE = CODES + 4 * BT + 256, NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
+    static constexpr int PITCH = 32 * TN * 4 + 16, OUT = NW * 32 * PITCH, LDS = S * STAGE > OUT ? S * STAGE : OUT;
+    static_assert(BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BN == 64 || BN == 128), "whole copies; one block of scales");
+    static_assert(LDS <= 80 * 1024, "two blocks a CU");
+};
+
+template <class E, class T>
+__global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, int nnt)
+{
+    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NW = T::NW, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = T::NC, NCA = T::NCA, PITCH = T::PITCH;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
+    F8Tile w;
+    if (!f8_tile(a, blockIdx.x, BT, nnt, w)) return;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), n0 = w.nt * BN, mrows = w.mend - w.m0;
+    const float *sb = a.sb + (size_t)w.e * a.esb + (size_t)(n0 >> 7) * a.ldsb;
+    const ckq_v4i rsa = gemm_buffer(a.A + (size_t)w.m0 * a.lda), rsb = gemm_buffer(a.B + (size_t)w.e * a.eb + (size_t)n0 * a.ldb);
+    const u32 base = lds_address(lds);
+    const int niter = (a.K + 127) / 128, last = niter - 1, tail = a.K - last * 128;
+    u32 ofs[NC];
+    const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int row = 8 * (wave + NW * (i < NCA ? i : i - NCA)) + (lane >> 3);
+        ofs[i] = (i < NCA ? (u32)min(row, mrows - 1) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
+    }
+    auto copy_step = [&](int it, int buf) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            /* chunks behind the row's last are read from its start, and zeroed (f8_clear_tail) */
+            const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
+            lds_copy16(i < NCA ? rsa : rsb, base + (u32)(buf * STAGE + 1024 * (wave + NW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * 128)), o, it * 128);
+        }
+        if (wave < BT / 64) lds_copy4(gemm_buffer((const uint8_t *)(a.sa + (size_t)it * a.ldsa + w.m0)), base + (u32)(buf * STAGE + T::CODES + 256 * wave), 4u * (u32)min(64 * wave + lane, mrows - 1), 0);
+        if (wave == NW - 1) lds_copy4(gemm_buffer((const uint8_t *)(sb + it)), base + (u32)(buf * STAGE + T::CODES + 4 * BT), 0, 0);
+    };
+    const int wt = wave / WN, wn = wave % WN, half = lane >> 5;
+    u32 ra[4], rb[4];
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk) {
+        const u32 pos = 16u * (u32)((2 * kk + half) ^ ((lane >> 1) & 7));
+        ra[kk] = (u32)(32 * TT * wt + (lane & 31)) * 128 + pos;
+        rb[kk] = (u32)(BT + 32 * TN * wn + (lane & 31)) * 128 + pos;
+    }
+    ckq_v16f acc[TT][TN];
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = ckq_v16f{};
+    copy_step(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    for (int it = 0; it < niter; ++it) {
+        const int buf = it & 1;
+        uint8_t *p = lds + buf * STAGE;
+        if (it == last && tail < 128) {
+            f8_clear_tail(p, BT + BN, tail, threadIdx.x, 64 * NW);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+        }
+        if (it < last) copy_step(it + 1, buf ^ 1);
+        ckq_v16f part[TT][TN];
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            f8_v8h fa[TT][2], fb[TN][2];
+#pragma unroll
+            for (int i = 0; i < TT; ++i) {
+                const ckq_v4i v = *reinterpret_cast<const ckq_v4i *>(p + ra[kk] + 32 * 128 * i);
+                fa[i][0] = f8_half(v[0], v[1]);
+                fa[i][1] = f8_half(v[2], v[3]);
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const ckq_v4i v = *reinterpret_cast<const ckq_v4i *>(p + rb[kk] + 32 * 128 * j);
+                fb[j][0] = f8_half(v[0], v[1]);
+                fb[j][1] = f8_half(v[2], v[3]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < TN; ++j)
+#pragma unroll
+                    for (int i = 0; i < TT; ++i)
+                        part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[j][h], fa[i][h], kk == 0 && h == 0 ? ckq_v16f{} : part[i][j], 0, 0, 0);
+        }
+        const float *sc = reinterpret_cast<const float *>(p + T::CODES);
+        const float s1 = sc[BT];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            const float s = sc[32 * (TT * wt + i) + (lane & 31)] * s1;
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_fmaf(s, part[i][j][r], acc[i][j][r]);
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    }
+    /* Through LDS, each wave by itself, 32 tokens at a time, so that a lane has eight rows' results of a token and a token's leave in whole lines. */
+    const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
+    uint8_t *mine = lds + wave * 32 * PITCH;
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f8_v4f *>(mine + (lane & 31) * PITCH + 4 * (32 * j + 8 * g + 4 * half)) = f8_v4f{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int e = lane; e < 32 * 4 * TN; e += 64) {
+            const int row = e / (4 * TN), c = 8 * (e % (4 * TN)), t = w.m0 + 32 * (TT * wt + i) + row, n = n0 + 32 * TN * wn + c;
+            float f[8];
+            const f8_v4f *q = reinterpret_cast<const f8_v4f *>(mine + row * PITCH + 4 * c);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) f[r] = q[r >> 2][r & 3];
+            if (t < w.mend && n < a.N) f8_store8<E>(a, bias, f, t, n);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+template <class E, class T>
+static int launch_f8_half(const F8Args &a, hipStream_t s)
+{
+    const int nnt = (a.N + T::BN - 1) / T::BN;
+    const long tiles = f8_most_tiles(a, T::BT) * nnt;
+    if (tiles >= 1l << 23) return CKQ_EINVAL;
+    return i8_launch(gemm_f8_half_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
+}
+
+/* ---- K split among the waves of a block -------------------------------------------------------------------------------- */
+
+/* 16 TG tokens x 16 RN rows a block of NW waves; every wave has all of the tile and each NW-th group of K, through S stages of its own, so that nothing is waited for
+ * but its own copies until the waves' sums meet at the end, in the order of the waves. */
+template <int NW_, int RN_, int TG_, int S_> struct F8Split {
+    static constexpr int NW = NW_, RN = RN_, TG = TG_, S = S_, BT = 16 * TG, BN = 16 * RN, CODES = (BT + BN) * 128, STAGE = CODES + 512, PITCH = BN * 4 + 16, NC = 2 * (RN + TG);
+    static constexpr int LDS = NW * (S * STAGE > BT * PITCH ? S * STAGE : BT * PITCH);
+    static_assert(LDS <= 160 * 1024 && BT <= 64 && 128 % BN == 0, "one block fits; one copy of scales, one block of them");
+};
+
+template <class E, class T>
+__global__ void __launch_bounds__(64 * T::NW) gemm_f8_split_kernel(F8Args a, int nnt)
+{
+    constexpr int NW = T::NW, RN = T::RN, TG = T::TG, S = T::S, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = T::NC, PITCH = T::PITCH;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
+    F8Tile w;
+    if (!f8_tile(a, blockIdx.x, BT, nnt, w)) return;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), n0 = w.nt * BN, mrows = w.mend - w.m0;
+    const float *sb = a.sb + (size_t)w.e * a.esb + (size_t)(n0 >> 7) * a.ldsb;
+    const ckq_v4i rsa = gemm_buffer(a.A + (size_t)w.m0 * a.lda), rsb = gemm_buffer(a.B + (size_t)w.e * a.eb + (size_t)n0 * a.ldb);
+    uint8_t *mine = lds + wave * S * STAGE;
+    const u32 base = lds_address(mine);
+    const int niter = (a.K + 127) / 128, last = niter - 1, tail = a.K - last * 128, steps = wave < niter ? (niter - 1 - wave) / NW + 1 : 0;
+    u32 ofs[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int cr = 8 * (i < 2 * TG ? i : i - 2 * TG) + (lane >> 3), chunk = (lane & 7) ^ ((cr >> 1) & 7);
+        ofs[i] = (i < 2 * TG ? (u32)min(cr, mrows - 1) * (u32)a.lda : (u32)min(cr, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
+    }
+    auto copy = [&](int j, int slot) {
+        const int it = wave + NW * j;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int cr = 8 * (i < 2 * TG ? i : i - 2 * TG) + (lane >> 3), chunk = (lane & 7) ^ ((cr >> 1) & 7);
+            const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
+            lds_copy16(i < 2 * TG ? rsa : rsb, base + (u32)(slot * STAGE + 1024 * i), o, it * 128);
+        }
+        lds_copy4(gemm_buffer((const uint8_t *)(a.sa + (size_t)it * a.ldsa + w.m0)), base + (u32)(slot * STAGE + T::CODES), 4u * (u32)min(lane, mrows - 1), 0);
+        lds_copy4(gemm_buffer((const uint8_t *)(sb + it)), base + (u32)(slot * STAGE + T::CODES + 256), 0, 0);
+    };
+    f8_v4f acc[TG][RN];
+#pragma unroll
+    for (int i = 0; i < TG; ++i)
+#pragma unroll
+        for (int j = 0; j < RN; ++j) acc[i][j] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < S - 1; ++j)
+        if (j < steps) copy(j, j);
+    int slot = 0;
+    for (int j = 0; j < steps; ++j) {
+        const int it = wave + NW * j;
+        if (j + S - 1 < steps) {
+            copy(j + S - 1, slot == 0 ? S - 1 : slot - 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * (NC + 2)) : "memory");
+        } else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        uint8_t *p = mine + slot * STAGE;
+        if (it == last && tail < 128) {
+            f8_clear_tail(p, BT + BN, tail, lane, 64);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        const float *sc = reinterpret_cast<const float *>(p + T::CODES);
+        float s[TG];
+#pragma unroll
+        for (int i = 0; i < TG; ++i) s[i] = sc[16 * i + (lane & 15)] * sc[64];
+        f8_v4f part[TG][RN];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int c = 4 * kk + (lane >> 4);
+            const u32 at = (u32)((lane & 15) * 128 + 16 * (c ^ ((lane >> 1) & 7)));
+            f8_v8h fa[TG][2], fb[RN][2];
+#pragma unroll
+            for (int i = 0; i < TG; ++i) {
+                const ckq_v4i v = *reinterpret_cast<const ckq_v4i *>(p + at + 16 * 128 * i);
+                fa[i][0] = f8_half(v[0], v[1]);
+                fa[i][1] = f8_half(v[2], v[3]);
+            }
+#pragma unroll
+            for (int i = 0; i < RN; ++i) {
+                const ckq_v4i v = *reinterpret_cast<const ckq_v4i *>(p + at + (BT + 16 * i) * 128);
+                fb[i][0] = f8_half(v[0], v[1]);
+                fb[i][1] = f8_half(v[2], v[3]);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < TG; ++i)
+#pragma unroll
+                    for (int n = 0; n < RN; ++n)
+                        part[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[n][h], fa[i][h], kk == 0 && h == 0 ? f8_v4f{0.0f, 0.0f, 0.0f, 0.0f} : part[i][n], 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < TG; ++i)
+#pragma unroll
+            for (int n = 0; n < RN; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][n][r] = __builtin_fmaf(s[i], part[i][n][r], acc[i][n][r]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");    /* the next copies into this slot come after its reads */
+        slot = slot + 1 == S ? 0 : slot + 1;
+    }
+    /* the waves' sums meet in LDS; eight rows of a token a thread */
+    __syncthreads();
+    uint8_t *red = lds + wave * BT * PITCH;
+#pragma unroll
+    for (int i = 0; i < TG; ++i)
+#pragma unroll
+        for (int n = 0; n < RN; ++n)
+            *reinterpret_cast<f8_v4f *>(red + (16 * i + (lane & 15)) * PITCH + 4 * (16 * n + 4 * (lane >> 4))) = acc[i][n];
+    __syncthreads();
+    constexpr int PER = BN / 8, JOBS = BT * PER;
+    static_assert(JOBS <= 64 * NW, "a job a thread");
+    const int row = (int)threadIdx.x / PER, col = 8 * ((int)threadIdx.x % PER), t = w.m0 + row, n = n0 + col;
+    if ((int)threadIdx.x >= JOBS || t >= w.mend || n >= a.N) return;
+    float f[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) f[r] = 0.0f;
+#pragma unroll
+    for (int v = 0; v < NW; ++v) {
+        const f8_v4f *q = reinterpret_cast<const f8_v4f *>(lds + v * BT * PITCH + row * PITCH + 4 * col);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) f[r] += q[r >> 2][r & 3];
+    }
+    f8_store8<E>(a, a.bias ? a.bias + (size_t)w.e * a.N : nullptr, f, t, n);
+}
+
+template <class E, class T>
+static int launch_f8_split(const F8Args &a, hipStream_t s)
+{
+    const int nnt = (a.N + T::BN - 1) / T::BN;
+    const long tiles = f8_most_tiles(a, T::BT) * nnt;
+    if (tiles >= 1l << 23) return CKQ_EINVAL;
+    return i8_launch(gemm_f8_split_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
+}
+
+/* ---- which kernel ------------------------------------------------------------------------------------------------------ */
+
+typedef F8Half<2, 2, 2, 2> H128x128;
+typedef F8Half<2, 2, 1, 1> H64x64;
+typedef F8Half<2, 2, 1, 2> H64x128;
+typedef F8Split<4, 2, 2, 2> S32x32;
+typedef F8Split<4, 2, 1, 2> S16x32;
+typedef F8Split<8, 1, 1, 2> S16x16;
+
+static std::atomic<int> g_f8_kernel{-1};
+extern "C" void ckq_launch_set_f8_kernel(int kernel) { g_f8_kernel.store(kernel < 0 || kernel >= CKQ_F8_KERNELS ? -1 : kernel); }
+
+/* Which kernel takes a product of M rows for `experts` matrices (0: no offsets), N x K each. */
+extern "C" int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts)
+{
+    const int forced = g_f8_kernel.load();
+    if (forced >= 0) return forced;
+    const int rows = experts ? (M + experts - 1) / experts : M;
+    return rows > 64 ? CKQ_F8_H128x128 : rows > 32 ? CKQ_F8_H64x64 : rows > 16 ? CKQ_F8_S32x32 : CKQ_F8_S16x32;
 }
 
 template <class E>
-static int launch_gemm_f8(const F8Args &a, hipStream_t s)
+static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
 {
-    const int ntt = a.offsets ? a.M / 16 + min(a.M, a.experts) : (a.M + 15) / 16, nnt = (a.N + 255) / 256;
-    if ((long)ntt * nnt >= 1l << 24) return CKQ_EINVAL;
-    return i8_launch(gemm_f8_kernel<E>, dim3((u32)(ntt * nnt)), dim3(256), s, a, nnt);
+    switch (ckq_launch_f8_kernel(type, a.M, a.N, a.K, a.offsets ? a.experts : 0)) {
+    case CKQ_F8_H128x128: return launch_f8_half<E, H128x128>(a, s);
+    case CKQ_F8_H64x128:  return launch_f8_half<E, H64x128>(a, s);
+    case CKQ_F8_H64x64:   return launch_f8_half<E, H64x64>(a, s);
+    case CKQ_F8_S32x32:   return launch_f8_split<E, S32x32>(a, s);
+    case CKQ_F8_S16x32:   return launch_f8_split<E, S16x32>(a, s);
+    default:              return launch_f8_split<E, S16x16>(a, s);
+    }
 }
 
 static int f8_gemm(const F8Args &a, int type, void *stream)
@@ -145,7 +454,7 @@ static int f8_gemm(const F8Args &a, int type, void *stream)
     if (((uintptr_t)a.A | (uintptr_t)a.B) % 16 || a.lda % 16 || a.ldb % 16 || a.eb % 16 || a.lda > CKQ_I8_PITCH_MAX || a.ldb > CKQ_I8_PITCH_MAX) return CKQ_EROWS;
     if ((uintptr_t)a.C % size || ((uintptr_t)a.sa | (uintptr_t)a.sb | (uintptr_t)a.bias | (uintptr_t)a.offsets) % 4) return CKQ_EROWS;
     const hipStream_t s = (hipStream_t)stream;
-    return type == CKQ_T_F32 ? launch_gemm_f8<float>(a, s) : type == CKQ_T_BF16 ? launch_gemm_f8<__bf16>(a, s) : launch_gemm_f8<_Float16>(a, s);
+    return type == CKQ_T_F32 ? launch_gemm_f8<float>(a, type, s) : type == CKQ_T_BF16 ? launch_gemm_f8<__bf16>(a, type, s) : launch_gemm_f8<_Float16>(a, type, s);
 }
 
 extern "C" int ckq_launch_gemm_f8(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, const float *sb, long ldsb, const float *bias,
