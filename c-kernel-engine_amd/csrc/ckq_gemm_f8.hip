@@ -15,6 +15,7 @@
 #include "ckq_rows.hpp"
 #include <atomic>
 
+typedef int   f8_v8i __attribute__((ext_vector_type(8)));
 typedef _Float16 f8_v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 f8_v8h __attribute__((ext_vector_type(8)));
 typedef float f8_v4f __attribute__((ext_vector_type(4)));
@@ -277,6 +278,162 @@ static int launch_f8_half(const F8Args &a, hipStream_t s)
     return i8_launch(gemm_f8_half_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
 }
 
+/* ---- tiles on the e4m3 instructions ------------------------------------------------------------------------------------ */
+
+/* WT x WN waves, each 16 TT tokens x 16 TN rows; a group's product is one multiplication, 16 x 16 x 128, whose four sums a lane scales and adds while the next ones are
+ * multiplied. */
+template <int WT_, int WN_, int TT_, int TN_, int PERCU_> struct F8Core {
+    static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NW = WT * WN, BT = 16 * TT * WT, BN = 16 * TN * WN, PERCU = PERCU_;
+    static constexpr int CODES = (BT + BN) * 128, SB = CODES + 4 * BT, STAGE = SB + 256 * ((BN + 127) / 128), NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
+    static constexpr int PITCH = 16 * TN * 4 + 16, OUT = NW * 16 * PITCH, LDS = 2 * STAGE > OUT ? 2 * STAGE : OUT;
+    static_assert(BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && BT / 64 + BN / 128 <= NW && BT % 64 == 0 && (BN == 64 || BN % 128 == 0) && 128 % (16 * TN) == 0, "whole copies; a wave's rows in one block of scales");
+    static_assert(LDS <= 160 * 1024 / PERCU, "they fit");
+};
+
+template <class E, class T>
+__global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core_kernel(F8Args a, int nnt)
+{
+    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NW = T::NW, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = T::NC, NCA = T::NCA, PITCH = T::PITCH, NB = (BN + 127) / 128;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
+    F8Tile w;
+    if (!f8_tile(a, blockIdx.x, BT, nnt, w)) return;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), n0 = w.nt * BN, mrows = w.mend - w.m0;
+    const ckq_v4i rsa = gemm_buffer(a.A + (size_t)w.m0 * a.lda), rsb = gemm_buffer(a.B + (size_t)w.e * a.eb + (size_t)n0 * a.ldb);
+    const u32 base = lds_address(lds);
+    const int niter = (a.K + 127) / 128, last = niter - 1, tail = a.K - last * 128;
+    u32 ofs[NC];
+    const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int row = 8 * (wave + NW * (i < NCA ? i : i - NCA)) + (lane >> 3);
+        ofs[i] = (i < NCA ? (u32)min(row, mrows - 1) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
+    }
+    auto copy = [&](int i, int it, int buf) {
+        const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
+        lds_copy16(i < NCA ? rsa : rsb, base + (u32)(buf * STAGE + 1024 * (wave + NW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * 128)), o, it * 128);
+    };
+    auto copy_scales = [&](int it, int buf) {
+        if (wave < BT / 64) lds_copy4(gemm_buffer((const uint8_t *)(a.sa + (size_t)it * a.ldsa + w.m0)), base + (u32)(buf * STAGE + T::CODES + 256 * wave), 4u * (u32)min(64 * wave + lane, mrows - 1), 0);
+        else if (wave - BT / 64 < NB)
+            lds_copy4(gemm_buffer((const uint8_t *)(a.sb + (size_t)w.e * a.esb + (size_t)min((n0 >> 7) + wave - BT / 64, (a.N - 1) >> 7) * a.ldsb + it)), base + (u32)(buf * STAGE + T::SB + 256 * (wave - BT / 64)), 0, 0);
+    };
+    const int wt = wave / WN, wn = wave % WN;
+    u32 ra[2], rb[2];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+        const u32 pos = 16u * (u32)((4 * kk + (lane >> 4)) ^ ((lane >> 1) & 7));
+        ra[kk] = (u32)(16 * TT * wt + (lane & 15)) * 128 + pos;
+        rb[kk] = (u32)(BT + 16 * TN * wn + (lane & 15)) * 128 + pos;
+    }
+    auto read = [&](int buf, const u32 (&r)[2], int f) {
+        const uint8_t *p = lds + buf * STAGE + 16 * 128 * f;
+        const ckq_v4i lo = *reinterpret_cast<const ckq_v4i *>(p + r[0]), hi = *reinterpret_cast<const ckq_v4i *>(p + r[1]);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    };
+    f8_v4f acc[TT][TN];
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
+
+#pragma unroll
+    for (int i = 0; i < NC; ++i) copy(i, 0, 0);
+    copy_scales(0, 0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (last == 0 && tail < 128) {
+        f8_clear_tail(lds, BT + BN, tail, threadIdx.x, 64 * NW);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    }
+    f8_v8i fa[2], fb[TN];
+    float sa[TT], sb;
+    auto read_scales = [&](int buf) {
+        const float *sc = reinterpret_cast<const float *>(lds + buf * STAGE + T::CODES);
+        sb = sc[BT + 64 * (16 * TN * wn >> 7)];
+#pragma unroll
+        for (int i = 0; i < TT; ++i) sa[i] = sc[16 * (TT * wt + i) + (lane & 15)];
+    };
+#pragma unroll
+    for (int j = 0; j < TN; ++j) fb[j] = read(0, rb, j);
+    fa[0] = read(0, ra, 0);
+    read_scales(0);
+    const f8_v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int it = 0; it < niter; ++it) {
+        const int buf = it & 1;
+        f8_v4f part[2];
+        float s[2];
+        auto scaled = [&](int m) {                             /* the sums of the m-th multiplication of the step */
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[m / TN][m % TN][r] = __builtin_fmaf(s[m / TN & 1], part[m & 1][r], acc[m / TN][m % TN][r]);
+            asm volatile("" : "+v"(acc[m / TN][m % TN]));     /* here, and not all of them behind the last branch of the step */
+        };
+#pragma unroll
+        for (int i = 0; i < TT; ++i) {
+            s[i & 1] = sa[i] * sb;
+            if (i + 1 < TT) fa[(i + 1) & 1] = read(buf, ra, i + 1);
+            else {
+                /* all have this step's operands in registers, and the next ones have arrived */
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                if (it + 1 == last && tail < 128) {
+                    f8_clear_tail(lds + (buf ^ 1) * STAGE, BT + BN, tail, threadIdx.x, 64 * NW);
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const int m = i * TN + j;
+                part[m & 1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i & 1], zero, 0, 0, 0, 0, 0, 0);
+                if (m > 0) scaled(m - 1);
+                if (i + 1 == TT && it < last) {
+                    fb[j] = read(buf ^ 1, rb, j);
+                    if (j == 0) fa[TT & 1] = read(buf ^ 1, ra, 0);
+                }
+                /* the copies of the next step, one at a time: a copy holds its wave until the address unit has taken it */
+                constexpr int SPAN = TT * TN * 5 / 8;          /* all of them before the wait */
+                static_assert(SPAN <= (TT - 1) * TN, "the wait is at the last tokens");
+                if (m == 0 && it < last) copy_scales(it + 1, buf ^ 1);
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+                    if (c * SPAN / NC == m && it < last) copy(c, it + 1, buf ^ 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        scaled(TT * TN - 1);
+        if (it < last) read_scales(buf ^ 1);
+    }
+    const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
+    uint8_t *mine = lds + wave * 16 * PITCH;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) *reinterpret_cast<f8_v4f *>(mine + (lane & 15) * PITCH + 4 * (16 * j + 4 * (lane >> 4))) = acc[i][j];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int e = lane; e < 16 * 2 * TN; e += 64) {
+            const int row = e / (2 * TN), c = 8 * (e % (2 * TN)), t = w.m0 + 16 * (TT * wt + i) + row, n = n0 + 16 * TN * wn + c;
+            float f[8];
+            const f8_v4f *q = reinterpret_cast<const f8_v4f *>(mine + row * PITCH + 4 * c);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) f[r] = q[r >> 2][r & 3];
+            if (t < w.mend && n < a.N) f8_store8<E>(a, bias, f, t, n);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
+}
+
+template <class E, class T>
+static int launch_f8_core(const F8Args &a, hipStream_t s)
+{
+    const int nnt = (a.N + T::BN - 1) / T::BN;
+    const long tiles = f8_most_tiles(a, T::BT) * nnt;
+    if (tiles >= 1l << 23) return CKQ_EINVAL;
+    return i8_launch(gemm_f8_core_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
+}
+
 /* ---- K split among the waves of a block -------------------------------------------------------------------------------- */
 
 /* 16 TG tokens x 16 RN rows a block of NW waves; every wave has all of the tile and each NW-th group of K, through S stages of its own, so that nothing is waited for
@@ -413,6 +570,9 @@ static int launch_f8_split(const F8Args &a, hipStream_t s)
 
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */
 
+typedef F8Core<2, 4, 8, 4, 1> C256x256;
+typedef F8Core<4, 2, 4, 4, 1> C256x128;
+typedef F8Core<2, 2, 4, 4, 2> C128x128;
 typedef F8Half<2, 2, 2, 2> H128x128;
 typedef F8Half<2, 2, 1, 1> H64x64;
 typedef F8Half<2, 2, 1, 2> H64x128;
@@ -439,6 +599,9 @@ static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
     case CKQ_F8_H128x128: return launch_f8_half<E, H128x128>(a, s);
     case CKQ_F8_H64x128:  return launch_f8_half<E, H64x128>(a, s);
     case CKQ_F8_H64x64:   return launch_f8_half<E, H64x64>(a, s);
+    case CKQ_F8_C256x256: return launch_f8_core<E, C256x256>(a, s);
+    case CKQ_F8_C256x128: return launch_f8_core<E, C256x128>(a, s);
+    case CKQ_F8_C128x128: return launch_f8_core<E, C128x128>(a, s);
     case CKQ_F8_S32x32:   return launch_f8_split<E, S32x32>(a, s);
     case CKQ_F8_S16x32:   return launch_f8_split<E, S16x32>(a, s);
     default:              return launch_f8_split<E, S16x16>(a, s);

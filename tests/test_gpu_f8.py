@@ -425,6 +425,35 @@ def test_experts(t, M, N, K, counts):
         check_experts(out, a, sa, b, sb, offsets, bias)
 
 
+KERNELS = range(9)              # CKQ_F8_* of ckq_launch.h
+CORES = (6, 7, 8)               # those on the e4m3 instructions
+
+
+@pytest.fixture
+def kernel(request):
+    ckq.lib().ckq_launch_set_f8_kernel(request.param)
+    yield request.param
+    ckq.lib().ckq_launch_set_f8_kernel(-1)
+
+
+@pytest.mark.parametrize("kernel", KERNELS, indirect=True)
+@pytest.mark.parametrize("M,N,K", [(1, 3, 16), (1, 128, 128), (2, 129, 127), (5, 300, 640), (17, 257, 384), (65, 130, 65), (129, 255, 1000), (200, 700, 2000), (257, 513, 896), (333, 1001, 1111), (520, 384, 129)])
+def test_matmul_on_every_kernel(kernel, M, N, K):
+    a, sa, b, sb = codes(M, K, M + K, -(-K // 16) * 16 + 32), side(M, K, M, 3), codes(N, K, N + K), blocks(N, K, N)
+    bias = normal(1, N, N)[0].cuda() if M % 2 else None
+    for t in TYPES.values():
+        c = P.dev_gemm_nt_f8(a, sa, b, sb, bias, dtype=t)
+        check_matmul(c, a, sa, b, sb, bias, cores=kernel in CORES)
+        assert torch.equal(c, P.dev_gemm_nt_f8(a, sa, b, sb, bias, dtype=t))
+
+
+@pytest.mark.parametrize("kernel", KERNELS, indirect=True)
+@pytest.mark.parametrize("M,N,K,counts", EXPERTS)
+def test_experts_on_every_kernel(kernel, M, N, K, counts):
+    a, sa, b, sb, offsets, bias, out = experts(M, N, K, counts, torch.bfloat16, M % 2)
+    check_experts(out, a, sa, b, sb, offsets, bias, cores=kernel in CORES)
+
+
 def test_experts_of_one_matrix_and_of_offsets_out_of_range():
     a, sa, b, sb = codes(40, 200, 1), side(40, 200, 2), codes(130, 200, 3), blocks(130, 200, 4)
     # experts side by side in one tensor whose rows are further apart, one matrix for all of them
