@@ -14,6 +14,7 @@
 #include "ckq_int8.hpp"
 #include "ckq_rows.hpp"
 #include <atomic>
+#include <type_traits>
 
 typedef int   f8_v8i __attribute__((ext_vector_type(8)));
 typedef _Float16 f8_v2h __attribute__((ext_vector_type(2)));
@@ -151,7 +152,7 @@ template <int WT_, int WN_, int TT_, int TN_> struct F8Half {
     static constexpr int CODES = (BT + BN) * 128, STAGE = CODES + 4 * BT + 256, NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
     static constexpr int PITCH = 32 * TN * 4 + 16, OUT = NW * 32 * PITCH, LDS = S * STAGE > OUT ? S * STAGE : OUT;
     static_assert(BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BN == 64 || BN == 128), "whole copies; one block of scales");
-    static_assert(LDS <= 80 * 1024, "two blocks a CU");
+    static_assert(LDS <= 80 * 1024 && TT <= 2, "two blocks a CU");
 };
 
 template <class E, class T>
@@ -199,57 +200,90 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
     copy_step(0, 0);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
-    for (int it = 0; it < niter; ++it) {
-        const int buf = it & 1;
-        uint8_t *p = lds + buf * STAGE;
-        if (it == last && tail < 128) {
-            f8_clear_tail(p, BT + BN, tail, threadIdx.x, 64 * NW);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-        }
-        if (it < last) copy_step(it + 1, buf ^ 1);
-        ckq_v16f part[TT][TN];
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-            f8_v8h fa[TT][2], fb[TN][2];
-#pragma unroll
-            for (int i = 0; i < TT; ++i) {
-                const ckq_v4i v = *reinterpret_cast<const ckq_v4i *>(p + ra[kk] + 32 * 128 * i);
-                fa[i][0] = f8_half(v[0], v[1]);
-                fa[i][1] = f8_half(v[2], v[3]);
-            }
-#pragma unroll
-            for (int j = 0; j < TN; ++j) {
-                const ckq_v4i v = *reinterpret_cast<const ckq_v4i *>(p + rb[kk] + 32 * 128 * j);
-                fb[j][0] = f8_half(v[0], v[1]);
-                fb[j][1] = f8_half(v[2], v[3]);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int j = 0; j < TN; ++j)
-#pragma unroll
-                    for (int i = 0; i < TT; ++i)
-                        part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fb[j][h], fa[i][h], kk == 0 && h == 0 ? ckq_v16f{} : part[i][j], 0, 0, 0);
-        }
-        const float *sc = reinterpret_cast<const float *>(p + T::CODES);
-        const float s1 = sc[BT];
-#pragma unroll
-        for (int i = 0; i < TT; ++i) {
-            const float s = sc[32 * (TT * wt + i) + (lane & 31)] * s1;
-#pragma unroll
-            for (int j = 0; j < TN; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = __builtin_fmaf(s, part[i][j][r], acc[i][j][r]);
-        }
+    auto clear_tail = [&](int buf) {
+        f8_clear_tail(lds + buf * STAGE, BT + BN, tail, threadIdx.x, 64 * NW);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    };
+    if (last == 0 && tail < 128) clear_tail(0);
+    if (last > 0) copy_step(1, 1);
+    /* All have read this step's operands, and the next ones have arrived: from here on the stage takes the copies of the step after them. */
+    auto turn = [&](int it) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-    }
+        if (it + 1 == last && tail < 128) clear_tail((it + 1) & 1);
+        if (it + 2 <= last) copy_step(it + 2, it & 1);
+    };
+    /* The steps of a wave with LIVE groups of 32 tokens.  Quarters of a step, 32 of its 128: the products of one while the codes of the next become fp16, one operand's
+     * half between two multiplications, and those of the one after it leave LDS.  A tile's sums are scaled while the next one's are made, the last tile's in the step
+     * after. */
+    auto steps = [&](auto live) {
+        constexpr int LIVE = decltype(live)::value, NF = LIVE + TN, NM = LIVE * TN;
+        f8_v8h h[2][NF][2];                                    /* operands: tokens first, then rows; quarter, halves of 16 */
+        ckq_v4i code[NF];
+        ckq_v16f part[NM];
+        float s[LIVE], tok[LIVE], row = 0.0f, s_last = 0.0f;
+        auto read = [&](int f, int it, int kk) { return *reinterpret_cast<const ckq_v4i *>(lds + (it & 1) * STAGE + (f < LIVE ? ra[kk] + 32 * 128 * f : rb[kk] + 32 * 128 * (f - LIVE))); };
+#pragma unroll
+        for (int f = 0; f < NF; ++f) code[f] = read(f, 0, 0);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            h[0][f][0] = f8_half(code[f][0], code[f][1]);
+            h[0][f][1] = f8_half(code[f][2], code[f][3]);
+            code[f] = read(f, 0, 1);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) part[NM - 1][r] = 0.0f;
+        auto scaled = [&](int t, float by) {                   /* tile t: tokens t % LIVE, rows t / LIVE */
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t % LIVE][t / LIVE][r] = __builtin_fmaf(by, part[t][r], acc[t % LIVE][t / LIVE][r]);
+            asm volatile("" : "+v"(acc[t % LIVE][t / LIVE]));
+        };
+        for (int it = 0; it < niter; ++it) {
+            const float *sc = reinterpret_cast<const float *>(lds + (it & 1) * STAGE + T::CODES);
+#pragma unroll
+            for (int i = 0; i < LIVE; ++i) tok[i] = sc[32 * (TT * wt + i) + (lane & 31)];
+            row = sc[BT];
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) {
+                if (kk == 2) turn(it);
+#pragma unroll
+                for (int m = 0; m < 2 * NM; ++m) {
+                    const int t = m >> 1, i = t % LIVE, j = t / LIVE;
+                    part[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(h[kk & 1][LIVE + j][m & 1], h[kk & 1][i][m & 1], kk == 0 && (m & 1) == 0 ? ckq_v16f{} : part[t], 0, 0, 0);
+                    if (kk == 0 && m == 1 && NM > 1) scaled(NM - 1, s_last);
+                    if (kk == 3 && (m & 1) && t > 0) scaled(t - 1, s[(t - 1) % LIVE]);
+#pragma unroll
+                    for (int u = 0; u < 2 * NF; ++u)           /* the next quarter's operands, all of them among the multiplications */
+                        if (u * 2 * NM / (2 * NF) == m) {
+                            const int f = u >> 1;
+                            h[(kk + 1) & 1][f][u & 1] = f8_half(code[f][2 * (u & 1)], code[f][2 * (u & 1) + 1]);
+                            if (u & 1) code[f] = read(f, it + (kk >= 2), (kk + 2) & 3);          /* behind the last step: anything */
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (kk == 1) {
+#pragma unroll
+                    for (int i = 0; i < LIVE; ++i) s[i] = tok[i] * row;
+                }
+            }
+            if (NM == 1) scaled(0, s[0]);
+            s_last = s[LIVE - 1];
+        }
+        if (NM > 1) scaled(NM - 1, s_last);
+    };
+    const int live = min(TT, (mrows - 32 * TT * wt + 31) >> 5);
+    if (live >= TT) steps(std::integral_constant<int, TT>{});
+    else if (TT > 1 && live == 1) steps(std::integral_constant<int, 1>{});
+    else
+        for (int it = 0; it < niter; ++it) turn(it);           /* its tokens are behind the last: it copies */
+    __syncthreads();
     /* Through LDS, each wave by itself, 32 tokens at a time, so that a lane has eight rows' results of a token and a token's leave in whole lines. */
     const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
     uint8_t *mine = lds + wave * 32 * PITCH;
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
+        if (i >= live) break;
 #pragma unroll
         for (int j = 0; j < TN; ++j)
 #pragma unroll
@@ -286,7 +320,7 @@ template <int WT_, int WN_, int TT_, int TN_, int PERCU_> struct F8Core {
     static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NW = WT * WN, BT = 16 * TT * WT, BN = 16 * TN * WN, PERCU = PERCU_;
     static constexpr int CODES = (BT + BN) * 128, SB = CODES + 4 * BT, STAGE = SB + 256 * ((BN + 127) / 128), NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
     static constexpr int PITCH = 16 * TN * 4 + 16, OUT = NW * 16 * PITCH, LDS = 2 * STAGE > OUT ? 2 * STAGE : OUT;
-    static_assert(BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && BT / 64 + BN / 128 <= NW && BT % 64 == 0 && (BN == 64 || BN % 128 == 0) && 128 % (16 * TN) == 0, "whole copies; a wave's rows in one block of scales");
+    static_assert(TT >= 3 && TN >= 2 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && BT / 64 + BN / 128 <= NW && BT % 64 == 0 && (BN == 64 || BN % 128 == 0) && 128 % (16 * TN) == 0, "whole copies; a wave's rows in one block of scales");
     static_assert(LDS <= 160 * 1024 / PERCU, "they fit");
 };
 
@@ -346,7 +380,7 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
     }
-    f8_v8i fa[2], fb[TN];
+    f8_v8i fa[3], fb[TN];
     float sa[TT], sb;
     auto read_scales = [&](int buf) {
         const float *sc = reinterpret_cast<const float *>(lds + buf * STAGE + T::CODES);
@@ -357,22 +391,23 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
 #pragma unroll
     for (int j = 0; j < TN; ++j) fb[j] = read(0, rb, j);
     fa[0] = read(0, ra, 0);
+    fa[1] = read(0, ra, 1);
     read_scales(0);
     const f8_v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int it = 0; it < niter; ++it) {
         const int buf = it & 1;
-        f8_v4f part[2];
-        float s[2];
+        f8_v4f part[3];
+        float s[TT];
         auto scaled = [&](int m) {                             /* the sums of the m-th multiplication of the step */
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[m / TN][m % TN][r] = __builtin_fmaf(s[m / TN & 1], part[m & 1][r], acc[m / TN][m % TN][r]);
+            for (int r = 0; r < 4; ++r) acc[m / TN][m % TN][r] = __builtin_fmaf(s[m / TN], part[m % 3][r], acc[m / TN][m % TN][r]);
             asm volatile("" : "+v"(acc[m / TN][m % TN]));     /* here, and not all of them behind the last branch of the step */
         };
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-            s[i & 1] = sa[i] * sb;
-            if (i + 1 < TT) fa[(i + 1) & 1] = read(buf, ra, i + 1);
-            else {
+            s[i] = sa[i] * sb;
+            if (i + 2 < TT) fa[(i + 2) % 3] = read(buf, ra, i + 2);
+            if (i + 1 == TT) {
                 /* all have this step's operands in registers, and the next ones have arrived */
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
@@ -382,18 +417,19 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
                     __builtin_amdgcn_s_barrier();
                 }
             }
+            const f8_v8i now = fa[i % 3];
 #pragma unroll
             for (int j = 0; j < TN; ++j) {
                 const int m = i * TN + j;
-                part[m & 1] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i & 1], zero, 0, 0, 0, 0, 0, 0);
-                if (m > 0) scaled(m - 1);
-                if (i + 1 == TT && it < last) {
+                part[m % 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], now, zero, 0, 0, 0, 0, 0, 0);
+                if (m > 1) scaled(m - 2);
+                if (i + 1 == TT) {                             /* behind the last step's: anything */
                     fb[j] = read(buf ^ 1, rb, j);
-                    if (j == 0) fa[TT & 1] = read(buf ^ 1, ra, 0);
+                    if (j == 0) fa[0] = read(buf ^ 1, ra, 0);
+                    if (j == 1) fa[1] = read(buf ^ 1, ra, 1);
                 }
                 /* the copies of the next step, one at a time: a copy holds its wave until the address unit has taken it */
-                constexpr int SPAN = TT * TN * 5 / 8;          /* all of them before the wait */
-                static_assert(SPAN <= (TT - 1) * TN, "the wait is at the last tokens");
+                constexpr int SPAN = TT * TN * 3 / 8;
                 if (m == 0 && it < last) copy_scales(it + 1, buf ^ 1);
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
@@ -401,8 +437,9 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        scaled(TT * TN - 2);
         scaled(TT * TN - 1);
-        if (it < last) read_scales(buf ^ 1);
+        read_scales(buf ^ 1);
     }
     const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
     uint8_t *mine = lds + wave * 16 * PITCH;
