@@ -258,6 +258,7 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
                         if (u * 2 * NM / (2 * NF) == m) {
                             const int f = u >> 1;
                             h[(kk + 1) & 1][f][u & 1] = f8_half(code[f][2 * (u & 1)], code[f][2 * (u & 1) + 1]);
+                            asm volatile("" : "+v"(h[(kk + 1) & 1][f][u & 1]));              /* here, not before its use */
                             if (u & 1) code[f] = read(f, it + (kk >= 2), (kk + 2) & 3);          /* behind the last step: anything */
                         }
                     __builtin_amdgcn_sched_barrier(0);

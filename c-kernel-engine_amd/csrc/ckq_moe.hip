@@ -17,22 +17,53 @@
 
 /* ---- sort ---------------------------------------------------------------------------------------------------------- */
 
-/* A block has an expert, the last one what has none.  Each goes through all slots twice: it counts those that belong before its own, and its own in each
- * wave's run of slots; then it writes its own where they belong.  No scratch memory, one launch, and the order of the slots
- * is kept without a sort; the slots' 4 bytes come from the caches. */
+/* Four slots of a lane that are the block's own, a bit each, and how many of the four belong to experts before it. */
+struct moe_four { u32 own; int less; };
+__device__ __forceinline__ moe_four moe_count(const u32 (&id)[4], int left, u32 e, u32 experts)
+{
+    moe_four r = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.less += i < left && id[i] < e;
+        r.own |= (u32)(i < left && (e < experts ? id[i] == e : id[i] >= experts)) << i;
+    }
+    return r;
+}
+
+/* A block has an expert, the last one what has none.  Each goes through all slots: it counts those that belong before its own, and its own in each wave's run of slots, whose
+ * places follow from that; then it writes its own.  No scratch memory, one launch, and the slots' order is kept without a sort.  A wave takes 1024 slots at a time, four a
+ * lane and load, four loads together, and remembers its own of the first 4096 in a bit each, so that up to 65536 slots are read once (us: 65536 slots of 128 experts, one slot a
+ * lane and load, read twice, 41.6). */
 __global__ void __launch_bounds__(1024) moe_sort_kernel(const int32_t *__restrict__ ids, int slots, int experts, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
                                                         int32_t *__restrict__ position)
 {
     __shared__ int before[16], mine[16];
-    const int lane = threadIdx.x & 63, wave = wave_in_block(), nw = blockDim.x >> 6, e = blockIdx.x;
-    const int run = ((slots - 1) / (64 * nw) + 1) * 64;         /* slots of a wave */
-    const long from = (long)wave * run;
-    const int first = (int)min(from, (long)slots), end = (int)min(from + run, (long)slots);
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), nw = blockDim.x >> 6;
+    const u32 e = blockIdx.x;
+    const long run = ((long)(slots - 1) / (256l * nw) + 1) * 256;  /* slots of a wave */
+    const int first = (int)min(wave * run, (long)slots), end = (int)min(wave * run + run, (long)slots);
+    auto load = [&](u32 (&id)[4], int s) {
+        if (s + 4 <= end) {
+            const rows_u4 v = *reinterpret_cast<const rows_u4_at_2 *>(ids + s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) id[i] = v[i];
+        } else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) id[i] = s + i < end ? (u32)ids[s + i] : 0u;
+    };
     int less = 0, same = 0;
-    for (int s = first + lane; s < end; s += 64) {
-        const u32 id = (u32)ids[s];
-        less += id < (u32)e;
-        same += e < experts ? id == (u32)e : id >= (u32)e;
+    unsigned long long kept = 0;
+    for (int s0 = first, b = 0; s0 < end; s0 += 1024, b += 4) {
+        u32 id[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) load(id[u], s0 + 256 * u + 4 * lane);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const moe_four f = moe_count(id[u], end - (s0 + 256 * u + 4 * lane), e, (u32)experts);
+            less += f.less;
+            same += __popc(f.own);
+            if (b < 16) kept |= (unsigned long long)f.own << (4 * (b + u));
+        }
     }
     less = group_sum<64>(less);
     same = group_sum<64>(same);
@@ -47,17 +78,30 @@ __global__ void __launch_bounds__(1024) moe_sort_kernel(const int32_t *__restric
         at += before[w] + (w < wave ? mine[w] : 0);
     }
     if (threadIdx.x == 0) offsets[e] = all;
-    for (int s0 = first; s0 < end; s0 += 64) {
-        const int s = s0 + lane;
-        const u32 id = s < end ? (u32)ids[s] : 0;
-        const bool own = s < end && (e < experts ? id == (u32)e : id >= (u32)e);
-        const unsigned long long m = __ballot(own);
-        const int p = at + __builtin_amdgcn_mbcnt_hi((u32)(m >> 32), __builtin_amdgcn_mbcnt_lo((u32)m, 0));
-        if (own) {
-            order[p] = e < experts ? s : -1;
-            position[s] = e < experts ? p : -1;
+    if (mine[wave] == 0) return;
+    for (int s0 = first, b = 0; s0 < end; s0 += 256, ++b) {
+        const int s = s0 + 4 * lane;
+        u32 own = (u32)(kept >> (4 * (b & 15))) & 15u;
+        if (b >= 16) {
+            u32 id[4];
+            load(id, s);
+            own = moe_count(id, end - s, e, (u32)experts).own;
         }
-        at += __popcll(m);
+        /* ranks: a lane's four slots follow each other, lanes in turn */
+        int p = at;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned long long m = __ballot(own >> i & 1);
+            p = __builtin_amdgcn_mbcnt_hi((u32)(m >> 32), __builtin_amdgcn_mbcnt_lo((u32)m, (u32)p));
+            at += __popcll(m);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (own >> i & 1) {
+                order[p] = e < (u32)experts ? s + i : -1;
+                position[s + i] = e < (u32)experts ? p : -1;
+                ++p;
+            }
     }
 }
 
@@ -83,6 +127,19 @@ struct MoeArgs {
     int            tokens, choices, rows, k;
 };
 
+/* Eight slots' places at a time are read before anything is done with them. */
+template <class F>
+__device__ __forceinline__ void moe_places(const MoeArgs &a, size_t t, F &&use)
+{
+    const int32_t *position = a.position + t * a.choices;
+    for (int j0 = 0; j0 < a.choices; j0 += 8) {
+        int p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = j0 + j < a.choices ? position[j0 + j] : -1;
+        use(j0, p);
+    }
+}
+
 /* Eight elements a thread. */
 template <class E>
 __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
@@ -94,64 +151,90 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = raw_value<E>(r, j);
-    for (int j = 0; j < a.choices; ++j) {
-        const int p = a.position[(size_t)t * a.choices + j];
-        if ((u32)p < (u32)a.rows) store8((E *)a.out + (size_t)p * a.ldo + 8 * (size_t)v, f, left);
-    }
+    moe_places(a, t, [&](int, const int (&p)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if ((u32)p[j] < (u32)a.rows) store8((E *)a.out + (size_t)p[j] * a.ldo + 8 * (size_t)v, f, left);
+    });
 }
 
+/* Eight elements a thread, the rows of eight slots on their way together (us, one after the other | together: 8192 tokens of 8 slots x 2048 in bf16 86.5 | now). */
 template <class E>
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
 {
     const u32 i = blockIdx.x * 256 + threadIdx.x, t = i / nvec, v = i - t * nvec;
     if (t >= (u32)a.tokens) return;
     const int left = a.k - 8 * (int)v;
+    const E *y = (const E *)a.x + 8 * (size_t)v;
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = 0.0f;
-    for (int j = 0; j < a.choices; ++j) {
-        const int p = a.position[(size_t)t * a.choices + j];
-        if ((u32)p >= (u32)a.rows) continue;
-        const float w = a.w ? a.w[(size_t)t * a.choices + j] : 1.0f;
-        const raw8<E> r = fetch8<false>((const E *)a.x + (size_t)p * a.ldx + 8 * (size_t)v, left);
+    moe_places(a, t, [&](int j0, const int (&p)[8]) {
+        float w[8];
+        raw8<E> r[8];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) f[c] = __builtin_fmaf(w, raw_value<E>(r, c), f[c]);
-    }
+        for (int j = 0; j < 8; ++j) w[j] = a.w && j0 + j < a.choices ? a.w[(size_t)t * a.choices + j0 + j] : 1.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j0 + j < a.choices) r[j] = fetch8<false>(y + (size_t)((u32)p[j] < (u32)a.rows ? p[j] : 0) * a.ldx, left);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if ((u32)p[j] < (u32)a.rows) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) f[c] = __builtin_fmaf(w[j], raw_value<E>(r[j], c), f[c]);
+            }
+    });
     store8((E *)a.out + (size_t)t * a.ldo + 8 * (size_t)v, f, left);
 }
 
-/* A block has a token.  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
+/* A block has a token, its slots four at a time.  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
 template <class E>
 __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
 {
-    __shared__ float red[4];
+    __shared__ float red[4][8];
     const size_t t = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = wave_in_block();
     const E *d = (const E *)a.x + t * a.ldx;
-    for (int j = 0; j < a.choices; ++j) {
-        const size_t s = t * a.choices + j;
-        const int p = a.position[s];
-        const bool there = (u32)p < (u32)a.rows;
-        const float w = a.w[s];
-        float sum = 0.0f;
-        if (there)
-            for (long v = 8l * threadIdx.x; v < a.k; v += 2048) {
-                const int left = a.k - (int)v;
-                const raw8<E> g = fetch8<false>(d + v, left), y = fetch8<false>((const E *)a.y + (size_t)p * a.ldy + v, left);
-                float f[8];
+    moe_places(a, t, [&](int j0, const int (&p)[8]) {
+        float w[8], sum[8];
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    sum = __builtin_fmaf(raw_value<E>(g, c), raw_value<E>(y, c), sum);
-                    f[c] = w * raw_value<E>(g, c);
-                }
-                store8((E *)a.out + (size_t)p * a.ldo + v, f, left);
+        for (int j = 0; j < 8; ++j) {
+            w[j] = j0 + j < a.choices ? a.w[t * a.choices + j0 + j] : 0.0f;
+            sum[j] = 0.0f;
+        }
+        for (long v = 8l * threadIdx.x; v < a.k; v += 2048) {
+            const int left = (int)(a.k - v);
+            const raw8<E> g = fetch8<false>(d + v, left);
+#pragma unroll
+            for (int h = 0; h < 8; h += 4) {
+                if (j0 + h >= a.choices) break;
+                raw8<E> y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (j0 + h + j < a.choices) y[j] = fetch8<false>((const E *)a.y + (size_t)((u32)p[h + j] < (u32)a.rows ? p[h + j] : 0) * a.ldy + v, left);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if ((u32)p[h + j] < (u32)a.rows) {
+                        float f[8];
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            sum[h + j] = __builtin_fmaf(raw_value<E>(g, c), raw_value<E>(y[j], c), sum[h + j]);
+                            f[c] = w[h + j] * raw_value<E>(g, c);
+                        }
+                        store8((E *)a.out + (size_t)p[h + j] * a.ldo + v, f, left);
+                    }
             }
-        sum = group_sum<64>(sum);
+        }
+        if (j0) __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float s = group_sum<64>(sum[j]);
+            if (lane == 63) red[wave][j] = s;
+        }
         __syncthreads();
-        if (lane == 63) red[wave] = sum;
-        __syncthreads();
-        if (threadIdx.x == 0) a.dw[s] = red[0] + red[1] + red[2] + red[3];
-    }
+        if ((int)threadIdx.x < 8 && j0 + (int)threadIdx.x < a.choices)
+            a.dw[t * a.choices + j0 + threadIdx.x] = red[0][threadIdx.x] + red[1][threadIdx.x] + red[2][threadIdx.x] + red[3][threadIdx.x];
+    });
 }
 
 /* The launches of all tokens: one has fewer than 2^32 threads. */

@@ -637,39 +637,35 @@ def dev_moe_sort(ids, experts, out=None):
     return out
 
 
-def _moe_shapes(x, tokens_of, position, others, weights=()):
-    """What a call of rows there and back takes: x [tokens_of or any rows, k] of floats, position int32 [tokens, choices], others (tensor, name, rows or None) of x's
-    type and width, weights (tensor, name) like position.  Returns the device's number for the library's checks of types."""
-    dev, _ = _i8_where()
-    shape, kind = x.shape, _I8_TYPES.get(x.dtype)
-    ok = (len(shape) == 2 and position.dim() == 2 and kind is not None and position.dtype is _I32 and position.is_contiguous() and x.get_device() == position.get_device() == dev
-          and (x.stride(1) == 1 or shape[1] <= 1) and (tokens_of is None or shape[0] == tokens_of))
-    for t, _, rows in others:
-        ok = ok and t.dim() == 2 and t.dtype is x.dtype and t.shape[1] == shape[1] and (rows is None or t.shape[0] == rows) and (t.stride(1) == 1 or shape[1] <= 1) and t.get_device() == dev
-    for t, _ in weights:
-        ok = ok and t.dtype is _F32 and t.shape == position.shape and t.is_contiguous() and t.get_device() == dev
-    if not ok:
-        if position.dim() != 2:
-            raise CkqError("position has the shape %s, not tokens x choices" % (tuple(position.shape),))
-        _f8_refuse(dev, [(x, "rows", None if tokens_of is None else (tokens_of, x.shape[-1]), None)]
-                   + [(t, what, (t.shape[0] if rows is None else rows, x.shape[-1]), x.dtype) for t, what, rows in others], [],
-                   [(position, "position", position.shape, _I32)] + [(t, what, position.shape, _F32) for t, what in weights])
-    if (shape[0] | shape[1] | position.shape[0] | position.shape[1]) >> 31:
-        _i8_too_many(*shape, *position.shape)
-    return kind
-
-
-def _pitch(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _moe_refuse(dev, x, tokens, position, others, weights=()):
+    """Says what is wrong with rows there and back: x [tokens (None: any), k] of floats, position int32 [tokens, choices], others (tensor, name, rows or None) of x's type and
+    width, weights (tensor, name) like position."""
+    places = position.shape
+    if len(places) != 2:
+        raise CkqError("position has the shape %s, not tokens x choices" % (tuple(places),))
+    sizes = [n for t in [x, position] + [o[0] for o in others] for n in t.shape]
+    if any(n >> 31 for n in sizes):
+        _i8_too_many(*sizes)
+    _f8_refuse(dev, [(x, "the rows", None if tokens is None or x.dim() != 2 else (tokens, x.shape[1]), None)]
+               + [(t, what, (t.shape[0] if rows is None and t.dim() else rows, x.shape[-1]), x.dtype) for t, what, rows in others], [],
+               [(position, "position", places, _I32)] + [(t, what, places, _F32) for t, what in weights])
 
 
 def dev_moe_gather(x, position, out=None):
     """y[position[t][j]] = x[t]: x [tokens, k], position as dev_moe_sort has it; y [tokens * choices, k], or into the rows of `out`.  Rows that have no slot stay as they are."""
-    if out is None and x.dim() == position.dim() == 2:
-        out = (_torch or _i8_torch()).empty(position.numel(), x.shape[1], dtype=x.dtype, device=x.device)
-    kind = _moe_shapes(x, position.shape[0], position, [(out, "out", None)])
-    T, c = position.shape
-    rc = lib().ckq_moe_gather_dev(kind, x.data_ptr(), _pitch(x), position.data_ptr(), out.data_ptr(), _pitch(out), T, c, out.shape[0], x.shape[1], _i8_where()[1])
+    dev, stream = _i8_where()
+    shape, places, t = x.shape, position.shape, x.dtype
+    if out is None and len(shape) == 2:
+        out = _torch.empty(position.numel(), shape[1], dtype=t, device=x.device)
+    into, kind = out.shape if out is not None else (), _I8_TYPES.get(t)
+    if (len(shape) != 2 or len(places) != 2 or len(into) != 2 or shape[0] != places[0] or into[1] != shape[1] or kind is None or out.dtype is not t or position.dtype is not _I32
+            or not position.is_contiguous() or not x.get_device() == position.get_device() == out.get_device() == dev):
+        _moe_refuse(dev, x, places[0] if places else 0, position, [(out, "out", None)] if out is not None else [])
+    (T, k), c, rows = shape, places[1], into[0]
+    (ldx, ex), (ldy, ey) = x.stride(), out.stride()
+    if (ex != 1 or ey != 1) and k > 1 or (T | k | c | rows) >> 31:
+        _moe_refuse(dev, x, T, position, [(out, "out", None)])
+    rc = lib().ckq_moe_gather_dev(kind, x.data_ptr(), ldx if T > 1 else k, position.data_ptr(), out.data_ptr(), ldy if rows > 1 else k, T, c, rows, k, stream)
     if rc:
         check(rc, "ckq_moe_gather_dev")
     return out
@@ -677,18 +673,22 @@ def dev_moe_gather(x, position, out=None):
 
 def dev_moe_gather_f8(x, position, out=None):
     """The same in e4m3: (q [tokens * choices, k], scale)."""
-    q, scale = out if out is not None else _f8_new(x, position.numel())
-    kind = _moe_shapes(x, position.shape[0], position, [])
     dev, stream = _i8_where()
-    k = x.shape[1]
-    rows = q.shape[0]
+    q, scale = out if out is not None else _f8_new(x, position.numel())
+    shape, places, into = x.shape, position.shape, q.shape
+    kind = _I8_TYPES.get(x.dtype)
+    if (len(shape) != 2 or len(places) != 2 or len(into) != 2 or shape[0] != places[0] or into[1] != shape[1] or kind is None or q.dtype is not _F8 or position.dtype is not _I32
+            or not position.is_contiguous() or not x.get_device() == position.get_device() == q.get_device() == scale.get_device() == dev):
+        _f8_refuse(dev, [(q, "q", (into[0], shape[-1]), _F8)], [(scale, "scale", (into[0], -(-shape[-1] // 128)))]) if q.dtype is not _F8 or into[1:] != shape[1:] else None
+        _moe_refuse(dev, x, places[0] if places else 0, position, [])
+    (T, k), c, rows = shape, places[1], into[0]
+    if (T | k | c | rows) >> 31:
+        _i8_too_many(T, k, c, rows)
     lds = _f8_side(scale, rows, -(-k // 128))
-    if rows >> 31:
-        _i8_too_many(rows)
-    if q.dim() != 2 or q.shape[1] != k or q.dtype is not _F8 or (q.stride(1) != 1 and k > 1) or not lds or not q.get_device() == scale.get_device() == dev:
-        _f8_refuse(dev, [(q, "q", (rows, k), _F8)], [(scale, "scale", (rows, -(-k // 128)))])
-    T, c = position.shape
-    rc = lib().ckq_moe_gather_f8_dev(kind, x.data_ptr(), _pitch(x), position.data_ptr(), q.data_ptr(), _pitch(q), scale.data_ptr(), lds, T, c, rows, k, stream)
+    (ldx, ex), (ldq, eq) = x.stride(), q.stride()
+    if (ex != 1 or eq != 1) and k > 1 or not lds:
+        _f8_refuse(dev, [(x, "x", shape, None), (q, "q", into, _F8)], [(scale, "scale", (rows, -(-k // 128)))])
+    rc = lib().ckq_moe_gather_f8_dev(kind, x.data_ptr(), ldx if T > 1 else k, position.data_ptr(), q.data_ptr(), ldq if rows > 1 else k, scale.data_ptr(), lds, T, c, rows, k, stream)
     if rc:
         check(rc, "ckq_moe_gather_f8_dev")
     return q, scale
@@ -696,12 +696,21 @@ def dev_moe_gather_f8(x, position, out=None):
 
 def dev_moe_combine(y, position, weights=None, out=None):
     """out[t] = sum over j of weights[t][j] * y[position[t][j]]: [tokens, k].  Without weights (ones) the gradient of dev_moe_gather."""
-    if out is None and y.dim() == position.dim() == 2:
-        out = (_torch or _i8_torch()).empty(position.shape[0], y.shape[1], dtype=y.dtype, device=y.device)
-    kind = _moe_shapes(y, None, position, [(out, "out", position.shape[0])], [(weights, "weights")] if weights is not None else ())
-    T, c = position.shape
-    rc = lib().ckq_moe_combine_dev(kind, y.data_ptr(), _pitch(y), position.data_ptr(), weights.data_ptr() if weights is not None else None, out.data_ptr(), _pitch(out),
-                                   T, c, y.shape[0], y.shape[1], _i8_where()[1])
+    dev, stream = _i8_where()
+    shape, places, t = y.shape, position.shape, y.dtype
+    if out is None and len(shape) == len(places) == 2:
+        out = _torch.empty(places[0], shape[1], dtype=t, device=y.device)
+    into, kind = out.shape if out is not None else (), _I8_TYPES.get(t)
+    if (len(shape) != 2 or len(places) != 2 or into != (places[0], shape[1]) or kind is None or out.dtype is not t or position.dtype is not _I32
+            or not position.is_contiguous() or not y.get_device() == position.get_device() == out.get_device() == dev
+            or weights is not None and (weights.dtype is not _F32 or weights.shape != places or not weights.is_contiguous() or weights.get_device() != dev)):
+        _moe_refuse(dev, y, None, position, [(out, "out", places[0] if places else 0)] if out is not None else [], [(weights, "weights")] if weights is not None else ())
+    (rows, k), (T, c) = shape, places
+    (ldy, ey), (ldo, eo) = y.stride(), out.stride()
+    if (ey != 1 or eo != 1) and k > 1 or (T | k | c | rows) >> 31:
+        _moe_refuse(dev, y, None, position, [(out, "out", T)])
+    rc = lib().ckq_moe_combine_dev(kind, y.data_ptr(), ldy if rows > 1 else k, position.data_ptr(), weights.data_ptr() if weights is not None else None, out.data_ptr(),
+                                   ldo if T > 1 else k, T, c, rows, k, stream)
     if rc:
         check(rc, "ckq_moe_combine_dev")
     return out
@@ -710,13 +719,25 @@ def dev_moe_combine(y, position, weights=None, out=None):
 def dev_moe_combine_backward(dout, y, position, weights, out=None):
     """Of dout [tokens, k], the gradient of dev_moe_combine's result: (dy, of y's shape, dweights float32 [tokens, choices]).  Rows of dy that have no slot stay as they
     are; dy may be y."""
+    dev, stream = _i8_where()
     if out is None:
-        out = (_torch or _i8_torch()).empty_strided(y.shape, y.stride(), dtype=y.dtype, device=y.device), _torch.empty(position.shape, dtype=_torch.float32, device=y.device)
+        out = _torch.empty_strided(y.shape, y.stride(), dtype=y.dtype, device=y.device), _torch.empty(position.shape, dtype=_F32, device=y.device)
     dy, dw = out
-    kind = _moe_shapes(dout, position.shape[0], position, [(y, "y", None), (dy, "dy", y.shape[0])], [(weights, "weights"), (dw, "dweights")])
-    T, c = position.shape
-    rc = lib().ckq_moe_combine_backward_dev(kind, dout.data_ptr(), _pitch(dout), y.data_ptr(), _pitch(y), position.data_ptr(), weights.data_ptr(), dy.data_ptr(), _pitch(dy),
-                                            dw.data_ptr(), T, c, y.shape[0], y.shape[1], _i8_where()[1])
+    shape, places, of_y, t = dout.shape, position.shape, y.shape, dout.dtype
+    kind = _I8_TYPES.get(t)
+    if (len(shape) != 2 or len(places) != 2 or len(of_y) != 2 or shape[0] != places[0] or of_y[1] != shape[1] or dy.shape != of_y or kind is None or not y.dtype is dy.dtype is t
+            or position.dtype is not _I32 or not weights.dtype is dw.dtype is _F32 or weights.shape != places or dw.shape != places
+            or not (position.is_contiguous() and weights.is_contiguous() and dw.is_contiguous())
+            or not dout.get_device() == y.get_device() == dy.get_device() == position.get_device() == weights.get_device() == dw.get_device() == dev):
+        _moe_refuse(dev, dout, places[0] if places else 0, position, [(y, "y", None), (dy, "dy", of_y[0] if of_y else 0)], [(weights, "weights"), (dw, "dweights")])
+    (T, k), c, rows = shape, places[1], of_y[0]
+    (ldd, ed), (ldy, ey), (ldg, eg) = dout.stride(), y.stride(), dy.stride()
+    if (ed != 1 or ey != 1 or eg != 1) and k > 1 or (T | k | c | rows) >> 31:
+        _moe_refuse(dev, dout, T, position, [(y, "y", None), (dy, "dy", rows)])
+    if rows == 1:
+        ldy = ldg = k
+    rc = lib().ckq_moe_combine_backward_dev(kind, dout.data_ptr(), ldd if T > 1 else k, y.data_ptr(), ldy, position.data_ptr(), weights.data_ptr(), dy.data_ptr(), ldg,
+                                            dw.data_ptr(), T, c, rows, k, stream)
     if rc:
         check(rc, "ckq_moe_combine_backward_dev")
     return dy, dw
