@@ -177,7 +177,7 @@ void ckq_launch_set_i8_kernel(int kernel);
 /* Rows in e4m3 with one scale for each 128 elements, and tokens sorted by expert (ckq_f8_rows.hip, ckq_gemm_f8.hip, ckq_moe.hip).  See ckernel_quant_hip.h for what
  * they compute and take. */
 #define CKQ_MOE_EXPERTS_MAX 65535
-#define CKQ_MOE_SLOTS_MAX (1l << 30)
+#define CKQ_MOE_SLOTS_MAX (1l << 29)
 int ckq_launch_quantize_f8(int type, const void *x, long ldx, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
 int ckq_launch_dequantize_f8(const uint8_t *q, long ldq, const float *scale, long lds, int type, void *y, long ldy, int rows, int k, void *stream);
 int ckq_launch_swiglu_f8(int type, const void *gate, const void *up, long ld, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);

@@ -341,7 +341,7 @@ int ckq_gemm_nt_f8_experts_dev(const uint8_t *A, long lda, const float *sa, long
                                const float *bias, const int32_t *offsets, int experts, ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream);
 
 /* Tokens sorted by expert and back, around the product above.  Each token has `choices` slots, s = t * choices + j: ids[s] is the number of an expert (anything outside
- * 0 .. experts - 1: the slot has none, a padded token, say, or an expert of another device), weights[s] what its result counts.  The same expert may be there twice.  At most 65535 experts and 2^30
+ * 0 .. experts - 1: the slot has none, a padded token, say, or an expert of another device), weights[s] what its result counts.  The same expert may be there twice.  At most 65535 experts and 2^29
  * slots, at least one token, choice, expert and element (else CKQ_EINVAL); integers are int32.  No atomics: the same bits each time.
  *
  * ckq_moe_sort_dev: slots in the order of their experts, those of one expert as they come: offsets[e] = number of slots of experts under e (experts + 1 of them),
