@@ -118,8 +118,8 @@ __device__ __forceinline__ void moe_places(const MoeArgs &a, size_t t, F &&use)
     }
 }
 
-/* Eight elements a thread. */
-template <class E>
+/* Eight elements a thread.  ONCE here and in the backward pass: what is written leaves non-temporally (moe_past_cache). */
+template <class E, bool ONCE>
 __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
 {
     const u32 i = blockIdx.x * 256 + threadIdx.x, t = i / nvec, v = i - t * nvec;
@@ -132,11 +132,12 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
     moe_places(a, t, [&](int, const int (&p)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if ((u32)p[j] < (u32)a.rows) store8((E *)a.out + (size_t)p[j] * a.ldo + 8 * (size_t)v, f, left);
+            if ((u32)p[j] < (u32)a.rows) store8<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + 8 * (size_t)v, f, left);
     });
 }
 
-/* Eight elements a thread, the rows of eight slots on their way together (us, one after the other | together: 8192 tokens of 8 slots x 2048 in bf16 86.5 | now). */
+/* Eight elements a thread, the rows of eight slots on their way together (one token of 8 slots x 2048 6.8 us one after the other, 3.7 together), non-temporally, being read for the last
+ * time, which leaves the caches to what is beside them (with a gather before it, 8192 tokens of 8 slots x 2048 in bf16 132 -> 115 us). */
 template <class E>
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
 {
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
         for (int j = 0; j < 8; ++j) w[j] = a.w && j0 + j < a.choices ? a.w[(size_t)t * a.choices + j0 + j] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j0 + j < a.choices) r[j] = fetch8<false>(y + (size_t)((u32)p[j] < (u32)a.rows ? p[j] : 0) * a.ldx, left);
+            if (j0 + j < a.choices) r[j] = fetch8<true>(y + (size_t)((u32)p[j] < (u32)a.rows ? p[j] : 0) * a.ldx, left);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if ((u32)p[j] < (u32)a.rows) {
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
 }
 
 /* A block has a token, its slots four at a time.  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
-template <class E>
+template <class E, bool ONCE>
 __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
 {
     __shared__ float red[4][8];
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
                 raw8<E> y[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (j0 + h + j < a.choices) y[j] = fetch8<false>((const E *)a.y + (size_t)((u32)p[h + j] < (u32)a.rows ? p[h + j] : 0) * a.ldy + v, left);
+                    if (j0 + h + j < a.choices) y[j] = fetch8<ONCE>((const E *)a.y + (size_t)((u32)p[h + j] < (u32)a.rows ? p[h + j] : 0) * a.ldy + v, left);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if ((u32)p[h + j] < (u32)a.rows) {
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
                             sum[h + j] = __builtin_fmaf(raw_value<E>(g, c), raw_value<E>(y[j], c), sum[h + j]);
                             f[c] = w[h + j] * raw_value<E>(g, c);
                         }
-                        store8((E *)a.out + (size_t)p[h + j] * a.ldo + v, f, left);
+                        store8<E, ONCE>((E *)a.out + (size_t)p[h + j] * a.ldo + v, f, left);
                     }
             }
         }
@@ -234,15 +235,20 @@ static int moe_each(MoeArgs a, bool out_by_token, size_t threads, L &&launch)
     }
 }
 
+/* Whether what is written, a row for each slot, is more than the 256 MB cache holds beside the rest: then it leaves non-temporally, and its reader finds it in memory either way.  us, kept | not: gather and
+ * the combine of its rows, bf16 x 2048, 67 MB 25.6 | 28.5, 134 MB 47.0 | 51.7, 252 MB 115 | 100; the backward pass and the combine of its rows, 134 MB 73.0 | 80.6. */
+static bool moe_past_cache(const MoeArgs &a, size_t size) { return (size_t)a.tokens * a.choices * a.k * size > (size_t)192 << 20; }
+
 enum { MOE_GATHER, MOE_COMBINE, MOE_BACKWARD };
 template <int OP, class E>
 static int launch_moe(const MoeArgs &a, hipStream_t s)
 {
     const u32 nvec = (u32)(a.k / 8 + (a.k % 8 != 0));
+    const bool once = moe_past_cache(a, sizeof(E));
     return moe_each<E>(a, OP == MOE_COMBINE, OP == MOE_BACKWARD ? 256 : nvec, [&](const MoeArgs &b) {
-        if (OP == MOE_BACKWARD) return i8_launch(moe_combine_backward_kernel<E>, dim3((u32)b.tokens), dim3(256), s, b);
+        if (OP == MOE_BACKWARD) return i8_launch(once ? moe_combine_backward_kernel<E, true> : moe_combine_backward_kernel<E, false>, dim3((u32)b.tokens), dim3(256), s, b);
         const dim3 grid((u32)(((size_t)b.tokens * nvec + 255) / 256));
-        return i8_launch(OP == MOE_GATHER ? moe_gather_kernel<E> : moe_combine_kernel<E>, grid, dim3(256), s, b, nvec);
+        return i8_launch(OP == MOE_COMBINE ? moe_combine_kernel<E> : once ? moe_gather_kernel<E, true> : moe_gather_kernel<E, false>, grid, dim3(256), s, b, nvec);
     });
 }
 template <int OP>

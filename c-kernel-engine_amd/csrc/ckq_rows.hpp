@@ -63,14 +63,19 @@ __device__ __forceinline__ float raw_value(const raw8<E> &r, int i)
     if constexpr (sizeof(E) == 4) return __builtin_bit_cast(float, r.w[i]);
     else return (float)__builtin_bit_cast(E, (uint16_t)(r.w[i / 2] >> (16 * (i & 1))));
 }
-template <class E>
+template <class E, bool ONCE = false>                        /* ONCE: not kept in a cache */
 __device__ __forceinline__ void store8(E *p, const float (&f)[8], int left)
 {
     if (left >= 8) {
         row8<E> r;
 #pragma unroll
         for (int i = 0; i < 8; ++i) r.v[i] = (E)f[i];
-        *reinterpret_cast<row8<E> *>(p) = r;
+        if (ONCE) {
+            struct { rows_u4 v[sizeof(E) / 2]; } w = __builtin_bit_cast(decltype(w), r);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(E) / 2; ++i) __builtin_nontemporal_store(w.v[i], reinterpret_cast<rows_u4_at_2 *>(p) + i);
+        } else
+            *reinterpret_cast<row8<E> *>(p) = r;
         asm volatile("");                                    /* or what both branches store is moved behind them, in pieces */
     } else {
 #pragma unroll
