@@ -142,6 +142,7 @@ _SIGS = {
     "ckq_moe_gather_f8_dev": (_i, [_i, _vp, _l, _vp, _vp, _l, _vp, _l, _i, _i, _i, _i, _vp]),
     "ckq_moe_combine_dev": (_i, [_i, _vp, _l, _vp, _vp, _vp, _l, _i, _i, _i, _i, _vp]),
     "ckq_moe_combine_backward_dev": (_i, [_i, _vp, _l, _vp, _l, _vp, _vp, _vp, _l, _vp, _i, _i, _i, _i, _vp]),
+    "ckq_call_dev": (_i, [_c.c_char_p]),
     "ckq_matmul_sequence_dev": (_i, [_vp, _i, _i, _vp]),
     "ckq_subblock_dots_dev": (_i, [_i, _vp, _vp, _vp, _i, _i, _vp]),
     "ckq_subblock_dots_tokens_dev": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _vp]),

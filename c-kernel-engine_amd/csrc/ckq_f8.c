@@ -1,5 +1,6 @@
 /* ckq_f8.c - the entry points of e4m3 rows with one scale for each 128 elements, and of tokens sorted by expert: no staging, no state; the launches check
  * what they take. */
+#include <string.h>
 #include "ckernel_quant_hip.h"
 #include "ckq_launch.h"
 
@@ -56,4 +57,43 @@ int ckq_moe_combine_backward_dev(ckq_ck_dtype type, const void *dout, long ldd, 
                                  void *dy, long lddy, float *dweights, int tokens, int choices, int rows, int k, void *stream)
 {
     return ckq_launch_moe_combine_backward((int)type, dout, ldd, y, ldy, position, weights, dy, lddy, dweights, tokens, choices, rows, k, stream);
+}
+
+#define PTR(T, i) ((T *)(uintptr_t)a[i])
+#define INT(i)    ((int)a[i])
+#define LONG(i)   ((long)a[i])
+
+int ckq_call_dev(const void *call)
+{
+    static const unsigned char arguments[] = {10, 10, 11, 16, 20, 8, 11, 13, 12, 15};
+    int64_t which, a[20];
+    if (!call) return CKQ_EINVAL;
+    memcpy(&which, call, 8);
+    if (which < 0 || which >= (int64_t)sizeof arguments) return CKQ_EINVAL;
+    memcpy(a, (const char *)call + 8, 8u * arguments[which]);
+    switch (which) {
+    case CKQ_CALL_QUANTIZE_F8:
+        return ckq_launch_quantize_f8(INT(0), PTR(const void, 1), LONG(2), PTR(uint8_t, 3), LONG(4), PTR(float, 5), LONG(6), INT(7), INT(8), PTR(void, 9));
+    case CKQ_CALL_DEQUANTIZE_F8:
+        return ckq_launch_dequantize_f8(PTR(const uint8_t, 0), LONG(1), PTR(const float, 2), LONG(3), INT(4), PTR(void, 5), LONG(6), INT(7), INT(8), PTR(void, 9));
+    case CKQ_CALL_SWIGLU_F8:
+        return ckq_launch_swiglu_f8(INT(0), PTR(const void, 1), PTR(const void, 2), LONG(3), PTR(uint8_t, 4), LONG(5), PTR(float, 6), LONG(7), INT(8), INT(9), PTR(void, 10));
+    case CKQ_CALL_GEMM_NT_F8:
+        return ckq_launch_gemm_f8(PTR(const uint8_t, 0), LONG(1), PTR(const float, 2), LONG(3), PTR(const uint8_t, 4), LONG(5), PTR(const float, 6), LONG(7), PTR(const float, 8), INT(9),
+                                  PTR(void, 10), LONG(11), INT(12), INT(13), INT(14), PTR(void, 15));
+    case CKQ_CALL_GEMM_NT_F8_EXPERTS:
+        return ckq_launch_gemm_f8_experts(PTR(const uint8_t, 0), LONG(1), PTR(const float, 2), LONG(3), PTR(const uint8_t, 4), LONG(5), LONG(6), PTR(const float, 7), LONG(8), LONG(9),
+                                          PTR(const float, 10), PTR(const int32_t, 11), INT(12), INT(13), PTR(void, 14), LONG(15), INT(16), INT(17), INT(18), PTR(void, 19));
+    case CKQ_CALL_MOE_SORT:
+        return ckq_launch_moe_sort(PTR(const int32_t, 0), INT(1), INT(2), INT(3), PTR(int32_t, 4), PTR(int32_t, 5), PTR(int32_t, 6), PTR(void, 7));
+    case CKQ_CALL_MOE_GATHER:
+        return ckq_launch_moe_gather(INT(0), PTR(const void, 1), LONG(2), PTR(const int32_t, 3), PTR(void, 4), LONG(5), INT(6), INT(7), INT(8), INT(9), PTR(void, 10));
+    case CKQ_CALL_MOE_GATHER_F8:
+        return ckq_launch_moe_gather_f8(INT(0), PTR(const void, 1), LONG(2), PTR(const int32_t, 3), PTR(uint8_t, 4), LONG(5), PTR(float, 6), LONG(7), INT(8), INT(9), INT(10), INT(11), PTR(void, 12));
+    case CKQ_CALL_MOE_COMBINE:
+        return ckq_launch_moe_combine(INT(0), PTR(const void, 1), LONG(2), PTR(const int32_t, 3), PTR(const float, 4), PTR(void, 5), LONG(6), INT(7), INT(8), INT(9), INT(10), PTR(void, 11));
+    default:
+        return ckq_launch_moe_combine_backward(INT(0), PTR(const void, 1), LONG(2), PTR(const void, 3), LONG(4), PTR(const int32_t, 5), PTR(const float, 6), PTR(void, 7), LONG(8), PTR(float, 9),
+                                               INT(10), INT(11), INT(12), INT(13), PTR(void, 14));
+    }
 }

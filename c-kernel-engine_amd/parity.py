@@ -6,6 +6,7 @@ Host functions take NumPy arrays and go through the drop-in (host-pointer)
 symbols; `dev_*` functions take torch CUDA tensors and go through the
 device-resident entry points on torch's current stream."""
 import ctypes
+import struct
 
 import numpy as np
 
@@ -440,6 +441,10 @@ def _f8_refuse(dev, rows, scales=(), wholes=()):
     _i8_refuse(dev, rows, [])
 
 
+# The calls go through ckq_call_dev, which number and arguments in one string of bytes: an argument costs ctypes 0.09 us and struct 0.01.
+_PACK_8, _PACK_10, _PACK_11, _PACK_12, _PACK_13, _PACK_15, _PACK_16, _PACK_20 = (struct.Struct("%dq" % (n + 1)).pack for n in (8, 10, 11, 12, 13, 15, 16, 20))
+
+
 def empty_f8(rows, k, device="cuda"):
     """(codes, scales) for rows of k: float8_e4m3fn [rows, k] whose rows begin at multiples of 16 bytes, as dev_gemm_nt_f8 takes them, and float32
     [rows, ceil(k / 128)] with the scales of a group side by side."""
@@ -480,7 +485,7 @@ def dev_quantize_f8(x, out=None):
         _f8_refuse(dev, [(x, "x", None, None), (q, "q", shape, _F8)], [(scale, "scale", (rows, -(-k // 128)))])
     if rows == 1:
         ldx = ldq = k
-    rc = lib().ckq_quantize_f8_dev(kind, x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr(), lds, rows, k, stream)
+    rc = lib().ckq_call_dev(_PACK_10(0, kind, x.data_ptr(), ldx, q.data_ptr(), ldq, scale.data_ptr(), lds, rows, k, stream))
     if rc:
         check(rc, "ckq_quantize_f8_dev")
     return q, scale
@@ -504,7 +509,7 @@ def dev_dequantize_f8(q, scale, dtype=None, out=None):
         _f8_refuse(dev, [(q, "q", None, _F8), (y, "out", shape, None)], [(scale, "scale", (rows, -(-k // 128)))])
     if rows == 1:
         ldq = ldy = k
-    rc = lib().ckq_dequantize_f8_dev(q.data_ptr(), ldq, scale.data_ptr(), lds, kind, y.data_ptr(), ldy, rows, k, stream)
+    rc = lib().ckq_call_dev(_PACK_10(1, q.data_ptr(), ldq, scale.data_ptr(), lds, kind, y.data_ptr(), ldy, rows, k, stream))
     if rc:
         check(rc, "ckq_dequantize_f8_dev")
     return y
@@ -528,7 +533,7 @@ def dev_swiglu_f8(gate, up, out=None):
         _f8_refuse(dev, [(gate, "gate", None, None), (up, "up", shape, t), (q, "q", shape, _F8)], [(scale, "scale", (rows, -(-k // 128)))])
     if rows == 1:
         ld = ldq = k
-    rc = lib().ckq_swiglu_f8_dev(kind, gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), lds, rows, k, stream)
+    rc = lib().ckq_call_dev(_PACK_11(2, kind, gate.data_ptr(), up.data_ptr(), ld, q.data_ptr(), ldq, scale.data_ptr(), lds, rows, k, stream))
     if rc:
         check(rc, "ckq_swiglu_f8_dev")
     return q, scale
@@ -554,7 +559,7 @@ def dev_gemm_nt_f8(a, sa, b, sb, bias=None, dtype=None, out=None):
             or sb.dtype is not _F32 or sb.shape != (blocks, G) or not sb.is_contiguous()
             or not a.get_device() == b.get_device() == c.get_device() == sa.get_device() == sb.get_device() == dev):
         _f8_refuse(dev, [(a, "a", None, _F8), (b, "b", None, _F8), (c, "out", (M, N), None), (c, "out", (M, N), dtype)], [(sa, "sa", (M, G))], [(sb, "sb", (blocks, G), _F32)])
-    bp = None
+    bp = 0
     if bias is not None:
         if bias.dtype is not _F32 or bias.shape != (N,) or not bias.is_contiguous() or bias.get_device() != dev:
             _i8_refuse(dev, [], [(bias, "bias", (N,))])
@@ -566,7 +571,7 @@ def dev_gemm_nt_f8(a, sa, b, sb, bias=None, dtype=None, out=None):
         lda, ldc = -(-K // 16) * 16, N
     if N == 1:
         ldb = -(-K // 16) * 16
-    rc = lib().ckq_gemm_nt_f8_dev(a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, sb.data_ptr(), G, bp, kind, c.data_ptr(), ldc, M, N, K, stream)
+    rc = lib().ckq_call_dev(_PACK_16(3, a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, sb.data_ptr(), G, bp, kind, c.data_ptr(), ldc, M, N, K, stream))
     if rc:
         check(rc, "ckq_gemm_nt_f8_dev")
     return c
@@ -593,7 +598,7 @@ def dev_gemm_nt_f8_experts(a, sa, b, sb, offsets, bias=None, dtype=None, out=Non
             or not a.get_device() == b.get_device() == c.get_device() == sa.get_device() == sb.get_device() == offsets.get_device() == dev):
         _f8_refuse(dev, [(a, "a", None, _F8), (b[0] if E else b, "b[e]", None, _F8), (c, "out", (M, N), None), (c, "out", (M, N), dtype)], [(sa, "sa", (M, G))],
                    [(sb, "sb", (E, blocks, G), _F32), (offsets, "offsets", (E + 1,), _I32)])
-    bp = None
+    bp = 0
     if bias is not None:
         if bias.dtype is not _F32 or bias.shape != (E, N) or not bias.is_contiguous() or bias.get_device() != dev:
             _f8_refuse(dev, [], [], [(bias, "bias", (E, N), _F32)])
@@ -607,8 +612,8 @@ def dev_gemm_nt_f8_experts(a, sa, b, sb, offsets, bias=None, dtype=None, out=Non
         ldb = -(-K // 16) * 16
     if E == 1:
         per = 0
-    rc = lib().ckq_gemm_nt_f8_experts_dev(a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, per, sb.data_ptr(), G, blocks * G, bp, offsets.data_ptr(), E, kind,
-                                          c.data_ptr(), ldc, M, N, K, stream)
+    rc = lib().ckq_call_dev(_PACK_20(4, a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, per, sb.data_ptr(), G, blocks * G, bp, offsets.data_ptr(), E, kind,
+                                          c.data_ptr(), ldc, M, N, K, stream))
     if rc:
         check(rc, "ckq_gemm_nt_f8_experts_dev")
     return c
@@ -631,7 +636,7 @@ def dev_moe_sort(ids, experts, out=None):
         _f8_refuse(dev, [], [], [(ids, "ids", shape, _I32), (offsets, "offsets", (experts + 1,), _I32), (order, "order", (T * c,), _I32), (position, "position", shape, _I32)])
     if (T | c | experts) >> 31:
         _i8_too_many(T, c, experts)
-    rc = lib().ckq_moe_sort_dev(ids.data_ptr(), T, c, experts, offsets.data_ptr(), order.data_ptr(), position.data_ptr(), stream)
+    rc = lib().ckq_call_dev(_PACK_8(5, ids.data_ptr(), T, c, experts, offsets.data_ptr(), order.data_ptr(), position.data_ptr(), stream))
     if rc:
         check(rc, "ckq_moe_sort_dev")
     return out
@@ -665,7 +670,7 @@ def dev_moe_gather(x, position, out=None):
     (ldx, ex), (ldy, ey) = x.stride(), out.stride()
     if (ex != 1 or ey != 1) and k > 1 or (T | k | c | rows) >> 31:
         _moe_refuse(dev, x, T, position, [(out, "out", None)])
-    rc = lib().ckq_moe_gather_dev(kind, x.data_ptr(), ldx if T > 1 else k, position.data_ptr(), out.data_ptr(), ldy if rows > 1 else k, T, c, rows, k, stream)
+    rc = lib().ckq_call_dev(_PACK_11(6, kind, x.data_ptr(), ldx if T > 1 else k, position.data_ptr(), out.data_ptr(), ldy if rows > 1 else k, T, c, rows, k, stream))
     if rc:
         check(rc, "ckq_moe_gather_dev")
     return out
@@ -688,7 +693,7 @@ def dev_moe_gather_f8(x, position, out=None):
     (ldx, ex), (ldq, eq) = x.stride(), q.stride()
     if (ex != 1 or eq != 1) and k > 1 or not lds:
         _f8_refuse(dev, [(x, "x", shape, None), (q, "q", into, _F8)], [(scale, "scale", (rows, -(-k // 128)))])
-    rc = lib().ckq_moe_gather_f8_dev(kind, x.data_ptr(), ldx if T > 1 else k, position.data_ptr(), q.data_ptr(), ldq if rows > 1 else k, scale.data_ptr(), lds, T, c, rows, k, stream)
+    rc = lib().ckq_call_dev(_PACK_13(7, kind, x.data_ptr(), ldx if T > 1 else k, position.data_ptr(), q.data_ptr(), ldq if rows > 1 else k, scale.data_ptr(), lds, T, c, rows, k, stream))
     if rc:
         check(rc, "ckq_moe_gather_f8_dev")
     return q, scale
@@ -709,8 +714,8 @@ def dev_moe_combine(y, position, weights=None, out=None):
     (ldy, ey), (ldo, eo) = y.stride(), out.stride()
     if (ey != 1 or eo != 1) and k > 1 or (T | k | c | rows) >> 31:
         _moe_refuse(dev, y, None, position, [(out, "out", T)])
-    rc = lib().ckq_moe_combine_dev(kind, y.data_ptr(), ldy if rows > 1 else k, position.data_ptr(), weights.data_ptr() if weights is not None else None, out.data_ptr(),
-                                   ldo if T > 1 else k, T, c, rows, k, stream)
+    rc = lib().ckq_call_dev(_PACK_12(8, kind, y.data_ptr(), ldy if rows > 1 else k, position.data_ptr(), weights.data_ptr() if weights is not None else 0, out.data_ptr(),
+                                   ldo if T > 1 else k, T, c, rows, k, stream))
     if rc:
         check(rc, "ckq_moe_combine_dev")
     return out
@@ -736,8 +741,8 @@ def dev_moe_combine_backward(dout, y, position, weights, out=None):
         _moe_refuse(dev, dout, T, position, [(y, "y", None), (dy, "dy", rows)])
     if rows == 1:
         ldy = ldg = k
-    rc = lib().ckq_moe_combine_backward_dev(kind, dout.data_ptr(), ldd if T > 1 else k, y.data_ptr(), ldy, position.data_ptr(), weights.data_ptr(), dy.data_ptr(), ldg,
-                                            dw.data_ptr(), T, c, rows, k, stream)
+    rc = lib().ckq_call_dev(_PACK_15(9, kind, dout.data_ptr(), ldd if T > 1 else k, y.data_ptr(), ldy, position.data_ptr(), weights.data_ptr(), dy.data_ptr(), ldg,
+                                            dw.data_ptr(), T, c, rows, k, stream))
     if rc:
         check(rc, "ckq_moe_combine_backward_dev")
     return dy, dw

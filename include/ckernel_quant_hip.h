@@ -362,6 +362,12 @@ int ckq_moe_combine_dev(ckq_ck_dtype type, const void *y, long ldy, const int32_
 int ckq_moe_combine_backward_dev(ckq_ck_dtype type, const void *dout, long ldd, const void *y, long ldy, const int32_t *position, const float *weights,
                                  void *dy, long lddy, float *dweights, int tokens, int choices, int rows, int k, void *stream);
 
+/* Any entry point from ckq_quantize_f8_dev to here, for callers whose arguments cost them one by one (ctypes: 0.09 us each): call[0] says which, its arguments
+ * follow in order, 64 bits each, pointers as integers.  CKQ_EINVAL for a number that is none of these. */
+enum { CKQ_CALL_QUANTIZE_F8, CKQ_CALL_DEQUANTIZE_F8, CKQ_CALL_SWIGLU_F8, CKQ_CALL_GEMM_NT_F8, CKQ_CALL_GEMM_NT_F8_EXPERTS, CKQ_CALL_MOE_SORT, CKQ_CALL_MOE_GATHER, CKQ_CALL_MOE_GATHER_F8,
+       CKQ_CALL_MOE_COMBINE, CKQ_CALL_MOE_COMBINE_BACKWARD };
+int ckq_call_dev(const void *call);
+
 /* A list of steps enqueued back-to-back, the whole list `repeat` times: the
  * per-token chain of a decoder layer (norm -> Q8_K -> Q/K/V ... -> down) is one
  * such list.  A matmul entry (fmt = a ckq_format weight tag) computes

@@ -95,6 +95,24 @@ def test_sort_and_rows_there_and_back_refusals(L):
             [{"dout": odd(1)}, {"y": odd(1)}, {"dy": odd(1)}, {"pos": odd(2)}, {"w": odd(2)}, {"dw": odd(1)}])
 
 
+def test_any_call_by_its_number(L):
+    """ckq_call_dev takes each entry point's arguments in its order: what that refuses, with its code."""
+    import struct
+    call = lambda *a: L.ckq_call_dev(struct.pack("%dq" % len(a), *a))
+    p, n = 4096, 0
+    good = [(BF16, p, 64, p, 64, p, 2, 2, 64, n), (p, 64, p, 2, BF16, p, 64, 2, 64, n), (BF16, p, p, 64, p, 64, p, 2, 2, 64, n), (p, 64, p, 2, p, 64, p, 1, p, BF16, p, 32, 2, 32, 64, n),
+            (p, 64, p, 2, p, 64, 2048, p, 1, 1, p, p, 3, BF16, p, 32, 2, 32, 64, n), (p, 2, 2, 3, p, p, p, n), (BF16, p, 64, p, p, 64, 2, 2, 4, 64, n), (BF16, p, 64, p, p, 64, p, 4, 2, 2, 4, 64, n),
+            (BF16, p, 64, p, p, p, 64, 2, 2, 4, 64, n), (BF16, p, 64, p, 64, p, p, p, 64, p, 2, 2, 4, 64, n)]
+    pointers = [(1, 3, 5), (0, 2, 5), (1, 2, 4, 6), (0, 2, 4, 6, 10), (0, 2, 4, 7, 11, 14), (0, 4, 5, 6), (1, 3, 4), (1, 3, 4, 6), (1, 3, 5), (1, 3, 5, 6, 7, 9)]
+    types = [0, 4, 0, 9, 13, None, 0, 0, 0, 0]
+    for which, (a, at, t) in enumerate(zip(good, pointers, types)):
+        for i in at:
+            assert call(which, *a[:i], 0, *a[i + 1:]) == EINVAL, (which, i)
+        if t is not None:
+            assert call(which, *a[:t], 5, *a[t + 1:]) == EFORMAT
+    assert call(-1, *good[4]) == EINVAL and call(10, *good[4]) == EINVAL and L.ckq_call_dev(None) == EINVAL
+
+
 def test_front_ends_refuse_what_a_pointer_cannot_tell():
     import torch
     par, err = ckq.parity, ckq.CkqError
@@ -122,7 +140,7 @@ def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
         def __getattr__(self, name):
             return lambda *a: 0
     monkeypatch.setattr(par, "lib", Library)
-    monkeypatch.setattr(par, "_i8_where", lambda: (-1, None))            # the device of host tensors
+    monkeypatch.setattr(par, "_i8_where", lambda: (-1, 0))               # the device of host tensors
     par._i8_torch()
     many = (1 << 32) + 16
     f, q, s = torch.empty(many, 1), torch.empty(many, 1, dtype=torch.float8_e4m3fn), torch.empty(1, many).t()
