@@ -321,18 +321,16 @@ template <int WT_, int WN_, int TT_, int TN_, int PERCU_> struct F8Core {
     static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NW = WT * WN, BT = 16 * TT * WT, BN = 16 * TN * WN, PERCU = PERCU_;
     static constexpr int CODES = (BT + BN) * 128, SB = CODES + 4 * BT, STAGE = SB + 256 * ((BN + 127) / 128), NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
     static constexpr int PITCH = 16 * TN * 4 + 16, OUT = NW * 16 * PITCH, LDS = 2 * STAGE > OUT ? 2 * STAGE : OUT;
-    static_assert(TT >= 3 && TN >= 2 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && BT / 64 + BN / 128 <= NW && BT % 64 == 0 && (BN == 64 || BN % 128 == 0) && 128 % (16 * TN) == 0, "whole copies; a wave's rows in one block of scales");
+    static constexpr bool EACH = 128 % (16 * TN) != 0;         /* a wave's rows may lie in two blocks of scales: one for each sixteen of them */
+    static_assert(TT >= 3 && TN >= 2 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && BT / 64 + (BN + 127) / 128 <= NW && BT % 64 == 0 && BN % 64 == 0, "whole copies, whole copies of scales");
     static_assert(LDS <= 160 * 1024 / PERCU, "they fit");
 };
 
 template <class E, class T>
-__global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core_kernel(F8Args a, int nnt)
+__device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, int n0, uint8_t *lds)
 {
-    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NW = T::NW, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = T::NC, NCA = T::NCA, PITCH = T::PITCH, NB = (BN + 127) / 128;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
-    F8Tile w;
-    if (!f8_tile(a, blockIdx.x, BT, nnt, w)) return;
-    const int lane = threadIdx.x & 63, wave = wave_in_block(), n0 = w.nt * BN, mrows = w.mend - w.m0;
+    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NW = T::NW, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = T::NC, NCA = T::NCA, PITCH = T::PITCH, NB = (BN + 127) / 128, NS = T::EACH ? TN : 1;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), mrows = w.mend - w.m0;
     const ckq_v4i rsa = gemm_buffer(a.A + (size_t)w.m0 * a.lda), rsb = gemm_buffer(a.B + (size_t)w.e * a.eb + (size_t)n0 * a.ldb);
     const u32 base = lds_address(lds);
     const int niter = (a.K + 127) / 128, last = niter - 1, tail = a.K - last * 128;
@@ -382,10 +380,14 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
         __builtin_amdgcn_s_barrier();
     }
     f8_v8i fa[3], fb[TN];
-    float sa[TT], sb;
+    float sa[TT], sb[NS];
+    int sb_at[NS];                                             /* which of the tile's blocks of scales */
+#pragma unroll
+    for (int j = 0; j < NS; ++j) sb_at[j] = BT + 64 * (((n0 & 127) + 16 * (TN * wn + j)) >> 7);
     auto read_scales = [&](int buf) {
         const float *sc = reinterpret_cast<const float *>(lds + buf * STAGE + T::CODES);
-        sb = sc[BT + 64 * (16 * TN * wn >> 7)];
+#pragma unroll
+        for (int j = 0; j < NS; ++j) sb[j] = sc[sb_at[j]];
 #pragma unroll
         for (int i = 0; i < TT; ++i) sa[i] = sc[16 * (TT * wt + i) + (lane & 15)];
     };
@@ -398,15 +400,14 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
     for (int it = 0; it < niter; ++it) {
         const int buf = it & 1;
         f8_v4f part[3];
-        float s[TT];
         auto scaled = [&](int m) {                             /* the sums of the m-th multiplication of the step */
+            const float s = sa[m / TN] * sb[m % TN % NS];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[m / TN][m % TN][r] = __builtin_fmaf(s[m / TN], part[m % 3][r], acc[m / TN][m % TN][r]);
+            for (int r = 0; r < 4; ++r) acc[m / TN][m % TN][r] = __builtin_fmaf(s, part[m % 3][r], acc[m / TN][m % TN][r]);
             asm volatile("" : "+v"(acc[m / TN][m % TN]));     /* here, and not all of them behind the last branch of the step */
         };
 #pragma unroll
         for (int i = 0; i < TT; ++i) {
-            s[i] = sa[i] * sb;
             if (i + 2 < TT) fa[(i + 2) % 3] = read(buf, ra, i + 2);
             if (i + 1 == TT) {
                 /* all have this step's operands in registers, and the next ones have arrived */
@@ -461,6 +462,35 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
         }
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
+}
+
+template <class E, class T>
+__global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core_kernel(F8Args a, int nnt)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
+    F8Tile w;
+    if (f8_tile(a, blockIdx.x, T::BT, nnt, w)) f8_core_tile<E, T>(a, w, w.nt * T::BN, lds);
+}
+
+/* One matrix: the first nnt1 columns of tiles of T1, `blocks1` blocks of them, and the rows that they leave in tiles of T2. */
+template <class E, class T1, class T2>
+__global__ void __launch_bounds__(64 * T1::NW, T1::NW / 4) gemm_f8_two_kernel(F8Args a, int nnt1, int blocks1, int nnt2)
+{
+    static_assert(T1::NW == T2::NW && T1::PERCU == 1, "one size of block");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[T1::LDS > T2::LDS ? T1::LDS : T2::LDS];
+    F8Tile w;
+    if ((int)blockIdx.x < blocks1) {
+        if (f8_tile(a, blockIdx.x, T1::BT, nnt1, w)) f8_core_tile<E, T1>(a, w, w.nt * T1::BN, lds);
+    } else if (f8_tile(a, blockIdx.x - blocks1, T2::BT, nnt2, w))
+        f8_core_tile<E, T2>(a, w, nnt1 * T1::BN + w.nt * T2::BN, lds);
+}
+template <class E, class T1, class T2>
+static int launch_f8_two(const F8Args &a, int nnt1, hipStream_t s)
+{
+    const int nnt2 = (a.N - nnt1 * T1::BN + T2::BN - 1) / T2::BN;
+    const long blocks1 = (f8_most_tiles(a, T1::BT) * nnt1 + 7) & ~7l, blocks2 = (f8_most_tiles(a, T2::BT) * nnt2 + 7) & ~7l;
+    if (blocks1 + blocks2 >= 1l << 23) return CKQ_EINVAL;
+    return i8_launch(gemm_f8_two_kernel<E, T1, T2>, dim3((u32)(blocks1 + blocks2)), dim3(64u * T1::NW), s, a, nnt1, (int)blocks1, nnt2);
 }
 
 template <class E, class T>
@@ -606,10 +636,116 @@ static int launch_f8_split(const F8Args &a, hipStream_t s)
     return i8_launch(gemm_f8_split_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
 }
 
+/* ---- one token: rows streamed ------------------------------------------------------------------------------------------ */
+
+/* A wave has R rows and every KS-th piece of KU KB of K; 4 waves a block.  A lane has sixteen elements of a group at a time: their products in pairs (v_dot2_f32_f16), times the group's scales, onto
+ * its sum.  Rows are loaded non-temporally: a decode step goes through more weights than any cache holds. */
+template <class E, int R, int KU, int KS>
+__global__ void __launch_bounds__(256) gemm_f8_stream_kernel(F8Args a)
+{
+    constexpr int G = 4 / KS;
+    static_assert(R <= 64 && 128 % R == 0, "a result a lane; rows in one block of scales");
+    __shared__ float red[KS > 1 ? 4 * R : 1];
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), part = wave % KS, n0 = ((int)blockIdx.x * G + wave / KS) * R, last_group = (a.K - 1) >> 7;
+    if (KS == 1 && n0 >= a.N) return;
+    const uint8_t *pb[R];
+    const float *sb = a.sb + (size_t)(min(n0, a.N - 1) >> 7) * a.ldsb;
+#pragma unroll
+    for (int r = 0; r < R; ++r) pb[r] = a.B + (size_t)min(n0 + r, a.N - 1) * a.ldb;
+    float acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = 0.0f;
+    for (int k0 = part * KU * 1024; k0 < a.K; k0 += KS * KU * 1024) {
+        ckq_v4i v[R][KU], x[KU];
+        float s[KU];
+        u32 at[KU];
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            at[u] = (u32)k0 + 1024u * u + 16u * (u32)lane;
+            if ((int)at[u] >= a.K) at[u] = 0;                /* zeroed below */
+        }
+#pragma unroll
+        for (int u = 0; u < KU; ++u)
+#pragma unroll
+            for (int r = 0; r < R; ++r) v[r][u] = __builtin_nontemporal_load(reinterpret_cast<const ckq_v4i *>(pb[r] + at[u]));
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            const int g = min((k0 >> 7) + 8 * u + (lane >> 3), last_group);
+            x[u] = *reinterpret_cast<const ckq_v4i *>(a.A + at[u]);
+            s[u] = a.sa[(size_t)g * a.ldsa] * sb[g];
+        }
+        if (k0 + KU * 1024 > a.K) {
+#pragma unroll
+            for (int u = 0; u < KU; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {                  /* both sides: a byte behind the last may be a NaN */
+                    const int n = a.K - (k0 + 1024 * u + 16 * lane + 4 * i), keep = n >= 4 ? -1 : n <= 0 ? 0 : (int)((1u << (8 * n)) - 1u);
+                    x[u][i] &= keep;
+#pragma unroll
+                    for (int r = 0; r < R; ++r) v[r][u][i] &= keep;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < KU; ++u) {
+            f8_v2h h[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                h[2 * i] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[u][i], 1.0f, false);
+                h[2 * i + 1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[u][i], 1.0f, true);
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    sum = __builtin_amdgcn_fdot2(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[r][u][i], 1.0f, false), h[2 * i], sum, false);
+                    sum = __builtin_amdgcn_fdot2(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v[r][u][i], 1.0f, true), h[2 * i + 1], sum, false);
+                }
+                acc[r] = __builtin_fmaf(s[u], sum, acc[r]);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, group_sum<64>(acc[r])), 63));
+    if (KS > 1) {
+        if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) red[wave * R + r] = acc[r];
+        }
+        __syncthreads();
+        if (part) return;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 1; v < KS; ++v) acc[r] += red[(wave + v) * R + r];
+    }
+    float sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) sum = lane == r ? acc[r] : sum;
+    const int n = n0 + lane;
+    if (lane < R && n < a.N) ((E *)a.C)[n] = (E)(a.bias ? sum + a.bias[n] : sum);
+}
+
+template <class E, int R, int KU, int KS>
+static int launch_f8_stream(const F8Args &a, hipStream_t s)
+{
+    constexpr int per = 4 / KS * R;
+    return i8_launch(gemm_f8_stream_kernel<E, R, KU, KS>, dim3((u32)((a.N + per - 1) / per)), dim3(256), s, a);
+}
+/* us, rows x K, (rows a wave, KB a trip, waves of a row): 11008 x 4096, 4, 1, 2 9.66 | 4, 1, 4 9.23 | 2, 2, 2 9.18 | 2, 1, 4 9.82 | 1, 2, 4 13.2; 4096 x 11008, 4, 1, 4 9.97 | 2, 1, 4 9.32 | 2, 4, 4 10.0; 11008 x 2048, 4, 1, 2 5.76 |
+ * 2, 2, 2 5.88; 4000 x 1000, 4, 1, 1 2.94 | 4, 1, 4 3.23. */
+template <class E>
+static int launch_f8_stream(const F8Args &a, hipStream_t s)
+{
+    const int kb = (a.K + 1023) / 1024;
+    return kb <= 1 ? launch_f8_stream<E, 4, 1, 1>(a, s) : kb <= 2 ? launch_f8_stream<E, 4, 1, 2>(a, s) : kb <= 4 ? launch_f8_stream<E, 2, 2, 2>(a, s) : launch_f8_stream<E, 2, 1, 4>(a, s);
+}
+
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */
 
 typedef F8Core<2, 4, 8, 4, 1> C256x256;
 typedef F8Core<4, 2, 4, 4, 1> C256x128;
+typedef F8Core<2, 4, 4, 3, 1> C128x192;
 typedef F8Core<2, 2, 4, 4, 2> C128x128;
 typedef F8Half<2, 2, 2, 2> H128x128;
 typedef F8Half<2, 2, 1, 1> H64x64;
@@ -618,6 +754,13 @@ typedef F8Split<4, 2, 2, 2> S32x32;
 typedef F8Split<4, 2, 1, 2> S16x32;
 typedef F8Split<8, 1, 1, 2> S16x16;
 
+/* Columns of 256 x 256 tiles that make whole rounds of the 256 CUs. */
+static int f8_whole_columns(int M, int N)
+{
+    const int ntt = (M + 255) / 256, nnt = (N + 255) / 256;
+    return (int)((long)ntt * nnt / 256 * 256 / ntt);
+}
+
 static std::atomic<int> g_f8_kernel{-1};
 extern "C" void ckq_launch_set_f8_kernel(int kernel) { g_f8_kernel.store(kernel < 0 || kernel >= CKQ_F8_KERNELS ? -1 : kernel); }
 
@@ -625,7 +768,8 @@ extern "C" void ckq_launch_set_f8_kernel(int kernel) { g_f8_kernel.store(kernel 
 extern "C" int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts)
 {
     const int forced = g_f8_kernel.load();
-    if (forced >= 0) return forced;
+    if (forced >= 0 && (forced != CKQ_F8_STREAM || (M == 1 && !experts)) && (forced != CKQ_F8_TWO || (!experts && f8_whole_columns(M, N) > 0))) return forced;
+    if (M == 1 && !experts) return CKQ_F8_STREAM;
     const int rows = experts ? (M + experts - 1) / experts : M;
     return rows > 64 ? CKQ_F8_H128x128 : rows > 32 ? CKQ_F8_H64x64 : rows > 16 ? CKQ_F8_S32x32 : CKQ_F8_S16x32;
 }
@@ -640,6 +784,8 @@ static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
     case CKQ_F8_C256x256: return launch_f8_core<E, C256x256>(a, s);
     case CKQ_F8_C256x128: return launch_f8_core<E, C256x128>(a, s);
     case CKQ_F8_C128x128: return launch_f8_core<E, C128x128>(a, s);
+    case CKQ_F8_TWO:      return launch_f8_two<E, C256x256, C128x192>(a, f8_whole_columns(a.M, a.N), s);
+    case CKQ_F8_STREAM:   return launch_f8_stream<E>(a, s);
     case CKQ_F8_S32x32:   return launch_f8_split<E, S32x32>(a, s);
     case CKQ_F8_S16x32:   return launch_f8_split<E, S16x32>(a, s);
     default:              return launch_f8_split<E, S16x16>(a, s);
