@@ -315,41 +315,79 @@ static int launch_f8_half(const F8Args &a, hipStream_t s)
 
 /* ---- tiles on the e4m3 instructions ------------------------------------------------------------------------------------ */
 
-/* WT x WN waves, each 16 TT tokens x 16 TN rows; a group's product is one multiplication, 16 x 16 x 128, whose four sums a lane scales and adds while the next ones are
- * multiplied. */
-template <int WT_, int WN_, int TT_, int TN_, int PERCU_> struct F8Core {
-    static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NW = WT * WN, BT = 16 * TT * WT, BN = 16 * TN * WN, PERCU = PERCU_;
-    static constexpr int CODES = (BT + BN) * 128, SB = CODES + 4 * BT, STAGE = SB + 256 * ((BN + 127) / 128), NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
-    static constexpr int PITCH = 16 * TN * 4 + 16, OUT = NW * 16 * PITCH, LDS = 2 * STAGE > OUT ? 2 * STAGE : OUT;
+/* WT x WN waves that multiply, each 16 TT tokens x 16 TN rows; a group's product is one multiplication, 16 x 16 x 128, whose four sums a lane scales and adds while the next ones are
+ * multiplied.  NP others that copy, or none (the former do it then); S stages in LDS; PERCU blocks a CU. */
+template <int WT_, int WN_, int TT_, int TN_, int NP_, int S_, int PERCU_> struct F8Core {
+    static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NP = NP_, S = S_, PERCU = PERCU_, NW = WT * WN, WAVES = NW + NP, BT = 16 * TT * WT, BN = 16 * TN * WN, NB = (BN + 127) / 128;
+    static constexpr int CODES = (BT + BN) * 128, SB = CODES + 4 * BT, STAGE = SB + 256 * NB;
+    static constexpr int CW = NP ? NP : NW, NC = (BT + BN) / 8 / CW, NCA = BT / 8 / CW, NS = (BT / 64 + NB + CW - 1) / CW;       /* waves that copy, copies of each a step: eight rows; 64 scales */
+    static constexpr int PITCH = 16 * TN * 4 + 16, OUT = NW * 16 * PITCH, LDS = S * STAGE > OUT ? S * STAGE : OUT;
     static constexpr bool EACH = 128 % (16 * TN) != 0;         /* a wave's rows may lie in two blocks of scales: one for each sixteen of them */
-    static_assert(TT >= 3 && TN >= 2 && BT % (8 * NW) == 0 && BN % (8 * NW) == 0 && BT / 64 + (BN + 127) / 128 <= NW && BT % 64 == 0 && BN % 64 == 0, "whole copies, whole copies of scales");
-    static_assert(LDS <= 160 * 1024 / PERCU, "they fit");
+    static_assert(TT >= 2 && TN >= 2 && CW % 2 == 0 && BT % (8 * CW) == 0 && BN % (8 * CW) == 0 && BT % 64 == 0 && BN % 64 == 0, "whole copies, whole copies of scales");
+    static_assert((NP || S == 2) && (S - 1) * (NC + NS) < 64 && LDS <= 160 * 1024 / PERCU, "waves that copy and multiply have a step under way; what a wave can count; they fit");
 };
 
 template <class E, class T>
 __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, int n0, uint8_t *lds)
 {
-    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NW = T::NW, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = T::NC, NCA = T::NCA, PITCH = T::PITCH, NB = (BN + 127) / 128, NS = T::EACH ? TN : 1;
-    const int lane = threadIdx.x & 63, wave = wave_in_block(), mrows = w.mend - w.m0;
+    constexpr int WN = T::WN, TT = T::TT, TN = T::TN, NP = T::NP, S = T::S, NW = T::NW, CW = T::CW, BT = T::BT, BN = T::BN, STAGE = T::STAGE, NC = T::NC, NCA = T::NCA, PITCH = T::PITCH, NS = T::EACH ? TN : 1;
+    const int lane = threadIdx.x & 63, wave = wave_in_block(), cw = NP ? wave - NW : wave, mrows = w.mend - w.m0;
     const ckq_v4i rsa = gemm_buffer(a.A + (size_t)w.m0 * a.lda), rsb = gemm_buffer(a.B + (size_t)w.e * a.eb + (size_t)n0 * a.ldb);
     const u32 base = lds_address(lds);
     const int niter = (a.K + 127) / 128, last = niter - 1, tail = a.K - last * 128;
     u32 ofs[NC];
-    const int chunk = (lane & 7) ^ ((4 * wave + (lane >> 4)) & 7);
+    const int chunk = (lane & 7) ^ ((4 * cw + (lane >> 4)) & 7);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int row = 8 * (wave + NW * (i < NCA ? i : i - NCA)) + (lane >> 3);
+        const int row = 8 * (cw + CW * (i < NCA ? i : i - NCA)) + (lane >> 3);
         ofs[i] = (i < NCA ? (u32)min(row, mrows - 1) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
     }
     auto copy = [&](int i, int it, int buf) {
         const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
-        lds_copy16(i < NCA ? rsa : rsb, base + (u32)(buf * STAGE + 1024 * (wave + NW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * 128)), o, it * 128);
+        lds_copy16(i < NCA ? rsa : rsb, base + (u32)(buf * STAGE + 1024 * (cw + CW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * 128)), o, it * 128);
     };
     auto copy_scales = [&](int it, int buf) {
-        if (wave < BT / 64) lds_copy4(gemm_buffer((const uint8_t *)(a.sa + (size_t)it * a.ldsa + w.m0)), base + (u32)(buf * STAGE + T::CODES + 256 * wave), 4u * (u32)min(64 * wave + lane, mrows - 1), 0);
-        else if (wave - BT / 64 < NB)
-            lds_copy4(gemm_buffer((const uint8_t *)(a.sb + (size_t)w.e * a.esb + (size_t)min((n0 >> 7) + wave - BT / 64, (a.N - 1) >> 7) * a.ldsb + it)), base + (u32)(buf * STAGE + T::SB + 256 * (wave - BT / 64)), 0, 0);
+#pragma unroll
+        for (int i = 0; i < T::NS; ++i) {
+            const int q = min(cw + CW * i, BT / 64 + T::NB - 1), j = q - BT / 64;         /* every wave has as many, the last ones twice */
+            const float *p = j < 0 ? a.sa + (size_t)it * a.ldsa + w.m0 : a.sb + (size_t)w.e * a.esb + (size_t)min((n0 >> 7) + j, (a.N - 1) >> 7) * a.ldsb + it;
+            lds_copy4(gemm_buffer((const uint8_t *)p), base + (u32)(buf * STAGE + (j < 0 ? T::CODES + 256 * q : T::SB + 256 * j)), j < 0 ? 4u * (u32)min(64 * q + lane, mrows - 1) : 0u, 0);
+        }
     };
+    auto copy_step = [&](int it, int buf) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) copy(i, it, buf);
+        copy_scales(it, buf);
+    };
+    auto clear_tail = [&](int buf) {                           /* all waves; then they meet */
+        f8_clear_tail(lds + buf * STAGE, BT + BN, tail, threadIdx.x, 64 * T::WAVES);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+    };
+    /* Step `it` has stage it % S.  A step's last operands are read before its last tokens are multiplied; the barrier is there: all have step it's operands in registers, and step it + 1 has
+     * arrived; from there on the stage takes the copies of step it + S. */
+    if (NP > 0 && wave >= NW) {
+        constexpr int EACH_STEP = NC + T::NS;
+#pragma unroll
+        for (int st = 0; st < S; ++st)
+            if (st < niter) copy_step(st, st);
+        if (niter >= S) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * EACH_STEP) : "memory");
+        else            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (last == 0 && tail < 128) clear_tail(0);
+        int buf = 0;
+        for (int it = 0; it < niter; ++it) {
+            const int next = buf + 1 == S ? 0 : buf + 1;
+            if (it + S - 1 < niter) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 2) * EACH_STEP) : "memory");
+            else                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            if (it + 1 == last && tail < 128) clear_tail(next);
+            if (it + S < niter) copy_step(it + S, buf);
+            buf = next;
+        }
+        __syncthreads();
+        return;
+    }
     const int wt = wave / WN, wn = wave % WN;
     u32 ra[2], rb[2];
 #pragma unroll
@@ -369,16 +407,12 @@ __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, i
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f8_v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
-#pragma unroll
-    for (int i = 0; i < NC; ++i) copy(i, 0, 0);
-    copy_scales(0, 0);
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    if (last == 0 && tail < 128) {
-        f8_clear_tail(lds, BT + BN, tail, threadIdx.x, 64 * NW);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
+    if (NP == 0) {
+        copy_step(0, 0);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
+    __builtin_amdgcn_s_barrier();
+    if (last == 0 && tail < 128) clear_tail(0);
     f8_v8i fa[3], fb[TN];
     float sa[TT], sb[NS];
     int sb_at[NS];                                             /* which of the tile's blocks of scales */
@@ -397,8 +431,9 @@ __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, i
     fa[1] = read(0, ra, 1);
     read_scales(0);
     const f8_v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    int buf = 0;
     for (int it = 0; it < niter; ++it) {
-        const int buf = it & 1;
+        const int next = buf + 1 == S ? 0 : buf + 1;
         f8_v4f part[3];
         auto scaled = [&](int m) {                             /* the sums of the m-th multiplication of the step */
             const float s = sa[m / TN] * sb[m % TN % NS];
@@ -410,14 +445,10 @@ __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, i
         for (int i = 0; i < TT; ++i) {
             if (i + 2 < TT) fa[(i + 2) % 3] = read(buf, ra, i + 2);
             if (i + 1 == TT) {
-                /* all have this step's operands in registers, and the next ones have arrived */
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                if (NP == 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                else         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
-                if (it + 1 == last && tail < 128) {
-                    f8_clear_tail(lds + (buf ^ 1) * STAGE, BT + BN, tail, threadIdx.x, 64 * NW);
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    __builtin_amdgcn_s_barrier();
-                }
+                if (it + 1 == last && tail < 128) clear_tail(next);
             }
             const f8_v8i now = fa[i % 3];
 #pragma unroll
@@ -426,22 +457,23 @@ __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, i
                 part[m % 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], now, zero, 0, 0, 0, 0, 0, 0);
                 if (m > 1) scaled(m - 2);
                 if (i + 1 == TT) {                             /* behind the last step's: anything */
-                    fb[j] = read(buf ^ 1, rb, j);
-                    if (j == 0) fa[0] = read(buf ^ 1, ra, 0);
-                    if (j == 1) fa[1] = read(buf ^ 1, ra, 1);
+                    fb[j] = read(next, rb, j);
+                    if (j == 0) fa[0] = read(next, ra, 0);
+                    if (j == 1) fa[1] = read(next, ra, 1);
                 }
                 /* the copies of the next step, one at a time: a copy holds its wave until the address unit has taken it */
                 constexpr int SPAN = TT * TN * 3 / 8;
-                if (m == 0 && it < last) copy_scales(it + 1, buf ^ 1);
+                if (NP == 0 && m == 0 && it < last) copy_scales(it + 1, next);
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
-                    if (c * SPAN / NC == m && it < last) copy(c, it + 1, buf ^ 1);
+                    if (NP == 0 && c * SPAN / NC == m && it < last) copy(c, it + 1, next);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         scaled(TT * TN - 2);
         scaled(TT * TN - 1);
-        read_scales(buf ^ 1);
+        read_scales(next);
+        buf = next;
     }
     const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
     uint8_t *mine = lds + wave * 16 * PITCH;
@@ -465,7 +497,7 @@ __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, i
 }
 
 template <class E, class T>
-__global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core_kernel(F8Args a, int nnt)
+__global__ void __launch_bounds__(64 * T::WAVES, T::WAVES * T::PERCU / 4) gemm_f8_core_kernel(F8Args a, int nnt)
 {
     __shared__ __attribute__((aligned(16))) uint8_t lds[T::LDS];
     F8Tile w;
@@ -474,9 +506,9 @@ __global__ void __launch_bounds__(64 * T::NW, T::NW * T::PERCU / 4) gemm_f8_core
 
 /* One matrix: the first nnt1 columns of tiles of T1, `blocks1` blocks of them, and the rows that they leave in tiles of T2. */
 template <class E, class T1, class T2>
-__global__ void __launch_bounds__(64 * T1::NW, T1::NW / 4) gemm_f8_two_kernel(F8Args a, int nnt1, int blocks1, int nnt2)
+__global__ void __launch_bounds__(64 * T1::WAVES, T1::WAVES / 4) gemm_f8_two_kernel(F8Args a, int nnt1, int blocks1, int nnt2)
 {
-    static_assert(T1::NW == T2::NW && T1::PERCU == 1, "one size of block");
+    static_assert(T1::WAVES == T2::WAVES && T1::PERCU == 1, "one size of block");
     __shared__ __attribute__((aligned(16))) uint8_t lds[T1::LDS > T2::LDS ? T1::LDS : T2::LDS];
     F8Tile w;
     if ((int)blockIdx.x < blocks1) {
@@ -490,7 +522,7 @@ static int launch_f8_two(const F8Args &a, int nnt1, hipStream_t s)
     const int nnt2 = (a.N - nnt1 * T1::BN + T2::BN - 1) / T2::BN;
     const long blocks1 = (f8_most_tiles(a, T1::BT) * nnt1 + 7) & ~7l, blocks2 = (f8_most_tiles(a, T2::BT) * nnt2 + 7) & ~7l;
     if (blocks1 + blocks2 >= 1l << 23) return CKQ_EINVAL;
-    return i8_launch(gemm_f8_two_kernel<E, T1, T2>, dim3((u32)(blocks1 + blocks2)), dim3(64u * T1::NW), s, a, nnt1, (int)blocks1, nnt2);
+    return i8_launch(gemm_f8_two_kernel<E, T1, T2>, dim3((u32)(blocks1 + blocks2)), dim3(64u * T1::WAVES), s, a, nnt1, (int)blocks1, nnt2);
 }
 
 template <class E, class T>
@@ -499,7 +531,7 @@ static int launch_f8_core(const F8Args &a, hipStream_t s)
     const int nnt = (a.N + T::BN - 1) / T::BN;
     const long tiles = f8_most_tiles(a, T::BT) * nnt;
     if (tiles >= 1l << 23) return CKQ_EINVAL;
-    return i8_launch(gemm_f8_core_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
+    return i8_launch(gemm_f8_core_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::WAVES), s, a, nnt);
 }
 
 /* ---- K split among the waves of a block -------------------------------------------------------------------------------- */
@@ -743,10 +775,13 @@ static int launch_f8_stream(const F8Args &a, hipStream_t s)
 
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */
 
-typedef F8Core<2, 4, 8, 4, 1> C256x256;
-typedef F8Core<4, 2, 4, 4, 1> C256x128;
-typedef F8Core<2, 4, 4, 3, 1> C128x192;
-typedef F8Core<2, 2, 4, 4, 2> C128x128;
+typedef F8Core<2, 4, 8, 4, 0, 2, 1> C256x256;
+typedef F8Core<4, 2, 4, 4, 4, 3, 1> C256x128;
+typedef F8Core<2, 2, 4, 6, 4, 3, 1> C128x192;
+typedef F8Core<2, 2, 4, 4, 4, 4, 1> C128x128;
+typedef F8Core<2, 2, 2, 4, 4, 4, 1> C64x128;
+typedef F8Core<2, 2, 2, 2, 4, 4, 2> C64x64;
+typedef F8Core<2, 2, 4, 4, 0, 2, 2> D128x128;
 typedef F8Half<2, 2, 2, 2> H128x128;
 typedef F8Half<2, 2, 1, 1> H64x64;
 typedef F8Half<2, 2, 1, 2> H64x128;
@@ -783,7 +818,11 @@ static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
     case CKQ_F8_H64x64:   return launch_f8_half<E, H64x64>(a, s);
     case CKQ_F8_C256x256: return launch_f8_core<E, C256x256>(a, s);
     case CKQ_F8_C256x128: return launch_f8_core<E, C256x128>(a, s);
+    case CKQ_F8_C128x192: return launch_f8_core<E, C128x192>(a, s);
     case CKQ_F8_C128x128: return launch_f8_core<E, C128x128>(a, s);
+    case CKQ_F8_C64x128:  return launch_f8_core<E, C64x128>(a, s);
+    case CKQ_F8_C64x64:   return launch_f8_core<E, C64x64>(a, s);
+    case CKQ_F8_D128x128: return launch_f8_core<E, D128x128>(a, s);
     case CKQ_F8_TWO:      return launch_f8_two<E, C256x256, C128x192>(a, f8_whole_columns(a.M, a.N), s);
     case CKQ_F8_STREAM:   return launch_f8_stream<E>(a, s);
     case CKQ_F8_S32x32:   return launch_f8_split<E, S32x32>(a, s);

@@ -425,8 +425,8 @@ def test_experts(t, M, N, K, counts):
         check_experts(out, a, sa, b, sb, offsets, bias)
 
 
-KERNELS = range(11)             # CKQ_F8_* of ckq_launch.h
-CORES = (6, 7, 8, 9)              # those on the e4m3 instructions
+KERNELS = range(15)             # CKQ_F8_* of ckq_launch.h
+CORES = range(6, 14)              # those on the e4m3 instructions
 
 
 @pytest.fixture
