@@ -174,15 +174,19 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
         const int row = 8 * (wave + NW * (i < NCA ? i : i - NCA)) + (lane >> 3);
         ofs[i] = (i < NCA ? (u32)min(row, mrows - 1) * (u32)a.lda : (u32)min(row, a.N - 1 - n0) * (u32)a.ldb) + 16u * (u32)chunk;
     }
+    auto copy = [&](int i, int it, int buf) {                  /* the last: scales */
+        if (i == NC) {
+            if (wave < BT / 64) lds_copy4(gemm_buffer((const uint8_t *)(a.sa + (size_t)it * a.ldsa + w.m0)), base + (u32)(buf * STAGE + T::CODES + 256 * wave), 4u * (u32)min(64 * wave + lane, mrows - 1), 0);
+            if (wave == NW - 1) lds_copy4(gemm_buffer((const uint8_t *)(sb + it)), base + (u32)(buf * STAGE + T::CODES + 4 * BT), 0, 0);
+            return;
+        }
+        /* chunks behind the row's last are read from its start, and zeroed (f8_clear_tail) */
+        const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
+        lds_copy16(i < NCA ? rsa : rsb, base + (u32)(buf * STAGE + 1024 * (wave + NW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * 128)), o, it * 128);
+    };
     auto copy_step = [&](int it, int buf) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            /* chunks behind the row's last are read from its start, and zeroed (f8_clear_tail) */
-            const u32 o = it == last && 16 * chunk >= tail ? ofs[i] - 16u * (u32)chunk : ofs[i];
-            lds_copy16(i < NCA ? rsa : rsb, base + (u32)(buf * STAGE + 1024 * (wave + NW * (i < NCA ? i : i - NCA)) + (i < NCA ? 0 : BT * 128)), o, it * 128);
-        }
-        if (wave < BT / 64) lds_copy4(gemm_buffer((const uint8_t *)(a.sa + (size_t)it * a.ldsa + w.m0)), base + (u32)(buf * STAGE + T::CODES + 256 * wave), 4u * (u32)min(64 * wave + lane, mrows - 1), 0);
-        if (wave == NW - 1) lds_copy4(gemm_buffer((const uint8_t *)(sb + it)), base + (u32)(buf * STAGE + T::CODES + 4 * BT), 0, 0);
+        for (int i = 0; i <= NC; ++i) copy(i, it, buf);
     };
     const int wt = wave / WN, wn = wave % WN, half = lane >> 5;
     u32 ra[4], rb[4];
@@ -212,7 +216,6 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         if (it + 1 == last && tail < 128) clear_tail((it + 1) & 1);
-        if (it + 2 <= last) copy_step(it + 2, it & 1);
     };
     /* The steps of a wave with LIVE groups of 32 tokens.  Quarters of a step, 32 of its 128: the products of one while the codes of the next become fp16, one operand's
      * half between two multiplications, and those of the one after it leave LDS.  A tile's sums are scaled while the next one's are made, the last tile's in the step
@@ -261,6 +264,10 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
                             asm volatile("" : "+v"(h[(kk + 1) & 1][f][u & 1]));              /* here, not before its use */
                             if (u & 1) code[f] = read(f, it + (kk >= 2), (kk + 2) & 3);          /* behind the last step: anything */
                         }
+                    constexpr int SPAN = 3 * NM;               /* the copies one at a time: a copy holds its wave until the address unit has taken it */
+#pragma unroll
+                    for (int c = 0; c <= NC; ++c)
+                        if (kk >= 2 && c * SPAN / (NC + 1) == (kk - 2) * 2 * NM + m && it + 2 <= last) copy(c, it + 2, it & 1);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (kk == 1) {
@@ -277,7 +284,10 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
     if (live >= TT) steps(std::integral_constant<int, TT>{});
     else if (TT > 1 && live == 1) steps(std::integral_constant<int, 1>{});
     else
-        for (int it = 0; it < niter; ++it) turn(it);           /* its tokens are behind the last: it copies */
+        for (int it = 0; it < niter; ++it) {                   /* its tokens are behind the last: it copies */
+            turn(it);
+            if (it + 2 <= last) copy_step(it + 2, it & 1);
+        }
     __syncthreads();
     /* Through LDS, each wave by itself, 32 tokens at a time, so that a lane has eight rows' results of a token and a token's leave in whole lines. */
     const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
