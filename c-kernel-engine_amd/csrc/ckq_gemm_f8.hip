@@ -14,6 +14,7 @@
 #include "ckq_int8.hpp"
 #include "ckq_rows.hpp"
 #include <atomic>
+#include <math.h>
 #include <type_traits>
 
 typedef int   f8_v8i __attribute__((ext_vector_type(8)));
@@ -785,21 +786,53 @@ static int launch_f8_stream(const F8Args &a, hipStream_t s)
 
 /* ---- which kernel ------------------------------------------------------------------------------------------------------ */
 
+typedef F8Half<2, 2, 2, 2> H128x128;
+typedef F8Half<2, 2, 1, 2> H64x128;
+typedef F8Half<2, 2, 1, 1> H64x64;
+typedef F8Split<8, 2, 2, 2> S32x32w8;
+typedef F8Split<4, 2, 2, 2> S32x32;
+typedef F8Split<8, 2, 1, 2> S16x32w8;
+typedef F8Split<4, 2, 1, 2> S16x32;
+typedef F8Split<8, 1, 1, 2> S16x16;
 typedef F8Core<2, 4, 8, 4, 0, 2, 1> C256x256;
 typedef F8Core<4, 2, 4, 4, 4, 3, 1> C256x128;
-typedef F8Core<2, 2, 4, 6, 4, 3, 1> C128x192;
+typedef F8Core<2, 2, 4, 6, 4, 3, 1> C128x192;            /* in two sizes of tiles */
 typedef F8Core<2, 2, 4, 4, 4, 4, 1> C128x128;
 typedef F8Core<2, 2, 2, 4, 4, 4, 1> C64x128;
 typedef F8Core<2, 2, 2, 2, 4, 4, 2> C64x64;
-typedef F8Core<2, 2, 4, 4, 0, 2, 2> D128x128;
-typedef F8Half<2, 2, 2, 2> H128x128;
-typedef F8Half<2, 2, 1, 1> H64x64;
-typedef F8Half<2, 2, 1, 2> H64x128;
-typedef F8Split<4, 2, 2, 2> S32x32;
-typedef F8Split<4, 2, 1, 2> S16x32;
-typedef F8Split<8, 1, 1, 2> S16x16;
 
-/* Columns of 256 x 256 tiles that make whole rounds of the 256 CUs. */
+/* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all places have a block; a last round of fewer blocks less, `share`
+ * of it by how many share a CU, the rest by how many there are in all.  Fitted to 700 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three sets in turn): the kernel so
+ * chosen is 1.4 % slower than the fastest on average, 1.3 times at worst; fitted to half of them, 1.2 % on the other half; over experts (400 random products, 2 to 128 of them) 2.7 % and 1.6 times. */
+struct F8Cost { int bt, bn, places, split; float t0, t_tile, step, share; };
+static const F8Cost f8_costs[CKQ_F8_TILINGS] = {
+    {128, 128, 512, 1, 0.72f, 5.47f, 1.958f, 0.89f}, {64, 128, 768, 1, 2.64f, 2.66f, 1.832f, 1.00f}, {64, 64, 1024, 1, 2.89f, 1.75f, 1.505f, 1.00f},
+    {32, 32, 256, 8, 2.16f, 2.17f, 0.814f, 0.84f},   {32, 32, 512, 4, 2.61f, 1.90f, 0.825f, 1.00f},  {16, 32, 256, 8, 2.18f, 1.80f, 0.657f, 0.77f},
+    {16, 32, 768, 4, 2.82f, 1.44f, 0.862f, 1.00f},   {16, 16, 512, 8, 2.50f, 1.50f, 0.688f, 1.00f},
+    {256, 256, 256, 1, 0.00f, 7.80f, 1.966f, 0.62f}, {256, 128, 256, 1, 0.00f, 6.90f, 0.927f, 0.64f}, {128, 128, 256, 1, 1.46f, 4.65f, 0.591f, 0.66f},
+    {64, 128, 256, 1, 1.76f, 3.16f, 0.393f, 0.70f},  {64, 64, 512, 1, 2.13f, 2.19f, 0.443f, 1.00f},
+};
+static const F8Cost f8_cost_rest = {128, 192, 256, 1, 0.00f, 12.05f, 0.519f, 0.45f};
+
+static float f8_rounds(const F8Cost &c, float tiles, int K)
+{
+    const int steps = ((K + 127) / 128 + c.split - 1) / c.split;
+    const float full = floorf(tiles / (float)c.places), rest = tiles - full * (float)c.places;
+    float t = full * (c.t_tile + (float)steps * c.step);
+    if (rest > 0.0f) t += c.t_tile + (float)steps * c.step * ((1.0f - c.share) * rest / (float)c.places + c.share * ceilf(rest / 256.0f) / ((float)c.places / 256.0f));
+    return t;
+}
+/* Tiles of M rows; of experts, which have what only the device knows, as many as if each row went to any of them alike. */
+static float f8_row_tiles(int bt, int M, int experts)
+{
+    if (!experts) return (float)((M + bt - 1) / bt);
+    const float used = (float)experts * (1.0f - powf(1.0f - 1.0f / (float)experts, (float)M)), rows = (float)M / used;
+    return rows > 0.75f * (float)bt ? used * fmaxf(1.0f, rows / (float)bt + 0.5f) : used;
+}
+static float f8_tiles(const F8Cost &c, int M, int N, int experts) { return f8_row_tiles(c.bt, M, experts) * (float)((N + c.bn - 1) / c.bn); }
+
+/* Columns of 256 x 256 tiles that make whole rounds of the 256 CUs: what they leave goes in tiles of 128 x 192, a shorter last round (2048 x 11008 x 4096: 344 tiles of 256 x 256 in two rounds 105 us; 256 of
+ * them and 240 small ones 87). */
 static int f8_whole_columns(int M, int N)
 {
     const int ntt = (M + 255) / 256, nnt = (N + 255) / 256;
@@ -807,37 +840,50 @@ static int f8_whole_columns(int M, int N)
 }
 
 static std::atomic<int> g_f8_kernel{-1};
-extern "C" void ckq_launch_set_f8_kernel(int kernel) { g_f8_kernel.store(kernel < 0 || kernel >= CKQ_F8_KERNELS ? -1 : kernel); }
+extern "C" void ckq_launch_set_f8_kernel(int kernel) { g_f8_kernel.store(kernel < 0 || kernel > CKQ_F8_STREAM ? -1 : kernel); }
 
-/* Which kernel takes a product of M rows for `experts` matrices (0: no offsets), N x K each. */
+/* The e4m3 instructions' sums, 1.5e-5 off, are taken where the result is rounded to 16 bits (bf16 2^-9, fp16 2^-12 off) and nothing but that: not for fp32 results, and not over experts, whose first product's
+ * results go through another quantizer, where each change of a value moves some of them by a sixteenth (an MLP with 32 experts in fp16: 0.0017 off the definition, with fp32 sums 0.0003).  Random products of one
+ * matrix gain 5.8 % by them on average, 2048 x 11008 x 4096 174 -> 87 us. */
 extern "C" int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts)
 {
     const int forced = g_f8_kernel.load();
-    if (forced >= 0 && (forced != CKQ_F8_STREAM || (M == 1 && !experts)) && (forced != CKQ_F8_TWO || (!experts && f8_whole_columns(M, N) > 0))) return forced;
+    const int cols = experts ? 0 : f8_whole_columns(M, N);
+    if (forced >= 0 && (forced != CKQ_F8_STREAM || (M == 1 && !experts)) && (forced != CKQ_F8_TWO || cols > 0)) return forced;
     if (M == 1 && !experts) return CKQ_F8_STREAM;
-    const int rows = experts ? (M + experts - 1) / experts : M;
-    return rows > 64 ? CKQ_F8_H128x128 : rows > 32 ? CKQ_F8_H64x64 : rows > 16 ? CKQ_F8_S32x32 : CKQ_F8_S16x32;
+    const bool cores = type != CKQ_T_F32 && !experts;
+    int best = 0;
+    float t = 1e30f;
+    for (int i = 0; i < (cores ? CKQ_F8_TILINGS : CKQ_F8_C256x256); ++i) {
+        const float ti = f8_costs[i].t0 + f8_rounds(f8_costs[i], f8_tiles(f8_costs[i], M, N, experts), K);
+        if (ti < t) { t = ti; best = i; }
+    }
+    if (cores && cols > 0 && 256 * cols < N) {
+        const F8Cost &a = f8_costs[CKQ_F8_C256x256], &b = f8_cost_rest;
+        if (a.t0 + f8_rounds(a, (float)((M + 255) / 256) * (float)cols, K) + f8_rounds(b, f8_tiles(b, M, N - 256 * cols, 0), K) < t) best = CKQ_F8_TWO;
+    }
+    return best;
 }
 
 template <class E>
 static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
 {
     switch (ckq_launch_f8_kernel(type, a.M, a.N, a.K, a.offsets ? a.experts : 0)) {
-    case CKQ_F8_H128x128: return launch_f8_half<E, H128x128>(a, s);
-    case CKQ_F8_H64x128:  return launch_f8_half<E, H64x128>(a, s);
-    case CKQ_F8_H64x64:   return launch_f8_half<E, H64x64>(a, s);
-    case CKQ_F8_C256x256: return launch_f8_core<E, C256x256>(a, s);
-    case CKQ_F8_C256x128: return launch_f8_core<E, C256x128>(a, s);
-    case CKQ_F8_C128x192: return launch_f8_core<E, C128x192>(a, s);
-    case CKQ_F8_C128x128: return launch_f8_core<E, C128x128>(a, s);
-    case CKQ_F8_C64x128:  return launch_f8_core<E, C64x128>(a, s);
-    case CKQ_F8_C64x64:   return launch_f8_core<E, C64x64>(a, s);
-    case CKQ_F8_D128x128: return launch_f8_core<E, D128x128>(a, s);
-    case CKQ_F8_TWO:      return launch_f8_two<E, C256x256, C128x192>(a, f8_whole_columns(a.M, a.N), s);
-    case CKQ_F8_STREAM:   return launch_f8_stream<E>(a, s);
-    case CKQ_F8_S32x32:   return launch_f8_split<E, S32x32>(a, s);
-    case CKQ_F8_S16x32:   return launch_f8_split<E, S16x32>(a, s);
-    default:              return launch_f8_split<E, S16x16>(a, s);
+    case CKQ_F8_H128x128:    return launch_f8_half<E, H128x128>(a, s);
+    case CKQ_F8_H64x128:     return launch_f8_half<E, H64x128>(a, s);
+    case CKQ_F8_H64x64:      return launch_f8_half<E, H64x64>(a, s);
+    case CKQ_F8_S32x32w8:    return launch_f8_split<E, S32x32w8>(a, s);
+    case CKQ_F8_S32x32:      return launch_f8_split<E, S32x32>(a, s);
+    case CKQ_F8_S16x32w8:    return launch_f8_split<E, S16x32w8>(a, s);
+    case CKQ_F8_S16x32:      return launch_f8_split<E, S16x32>(a, s);
+    case CKQ_F8_S16x16:      return launch_f8_split<E, S16x16>(a, s);
+    case CKQ_F8_C256x256:    return launch_f8_core<E, C256x256>(a, s);
+    case CKQ_F8_C256x128:    return launch_f8_core<E, C256x128>(a, s);
+    case CKQ_F8_C128x128:    return launch_f8_core<E, C128x128>(a, s);
+    case CKQ_F8_C64x128:     return launch_f8_core<E, C64x128>(a, s);
+    case CKQ_F8_C64x64:      return launch_f8_core<E, C64x64>(a, s);
+    case CKQ_F8_TWO:         return launch_f8_two<E, C256x256, C128x192>(a, f8_whole_columns(a.M, a.N), s);
+    default:                 return launch_f8_stream<E>(a, s);
     }
 }
 

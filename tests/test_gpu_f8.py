@@ -426,7 +426,7 @@ def test_experts(t, M, N, K, counts):
 
 
 KERNELS = range(15)             # CKQ_F8_* of ckq_launch.h
-CORES = range(6, 14)              # those on the e4m3 instructions
+CORES = range(8, 14)              # those on the e4m3 instructions
 
 
 @pytest.fixture
