@@ -35,8 +35,8 @@ def dump_lib_path():
     return os.path.join(CSRC, "libckernel_quant_hip_dump.so")
 
 
-def build(targets=("synth", "hip", "dump")):
-    """Compile the host helper and the gfx950 library in-tree (hipcc
+def build(targets=("synth", "hip", "dump", "tensors")):
+    """Compile the host helper, the gfx950 library and the module that reads tensors in-tree (hipcc
     cross-compiles without a GPU)."""
     subprocess.run(["make", "-C", CSRC, "-B"] + list(targets), check=True)
 

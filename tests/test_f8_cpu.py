@@ -135,6 +135,26 @@ def test_front_ends_refuse_what_a_pointer_cannot_tell():
     assert q.shape == (3, 200) and q.stride() == (208, 1) and s.shape == (3, 2) and s.stride() == (1, 3) and q.dtype == torch.float8_e4m3fn
 
 
+def without_module(par):
+    none = par._Fast()
+    none.absent = True
+    return none
+
+
+def test_the_module_that_reads_tensors_takes_none_of_the_host(L):
+    """It is there, and whatever it is given that is not for it comes back untouched, as does a call of something that is no tensor."""
+    import torch
+    par = ckq.parity
+    m = par._load_fast()
+    names = ("quantize", "dequantize", "swiglu", "gemm", "experts", "sort", "gather", "gather_f8", "combine", "backward")
+    assert os.path.exists(os.path.join(ckq.api.CSRC, "ckq_tensors.so")) and par._fast is m and all(hasattr(m, n) for n in names)
+    x = torch.ones(3, 32)
+    for n in names:
+        for args in ((), (x,), (x,) * 7, (None,) * 7, (3, "a", 2.5, x, [x], None, x), (x.to_sparse(),) * 7, (x.to("meta"),) * 7):
+            assert getattr(m, n)(*args) == -1000
+    assert without_module(par).gemm(x) == -1000
+
+
 def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
     """ctypes passes the lowest 32 bits of an int: 2^32 + 16 rows would be 16.  Memory that nothing touches, and a library that nothing reaches."""
     import torch
@@ -145,6 +165,7 @@ def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
     class Library:
         def __getattr__(self, name):
             return lambda *a: 0
+    monkeypatch.setattr(par, "_fast", without_module(par))
     monkeypatch.setattr(par, "lib", Library)
     monkeypatch.setattr(par, "_i8_where", lambda: (-1, 0))               # the device of host tensors
     par._i8_torch()

@@ -758,6 +758,43 @@ def test_experts_captured_replayed_and_on_two_streams(T):
     assert all(torch.equal(a, b) for a, b in zip(m.run(), got))
 
 
+def test_the_same_with_and_without_the_module_that_reads_tensors(monkeypatch):
+    """Every call that it takes is made by the Python checks with the same result; what those refuse it does not take."""
+    assert P._fast.gemm() == -1000 and P._fast.__name__ == "ckq_tensors"
+    took = []
+
+    class Watch:
+        def __getattr__(self, name):
+            f = getattr(module, name)
+            return lambda *a: took.append((name, f(*a))) or took[-1][1]
+    module, none = P._fast, P._Fast()
+    none.absent = True
+
+    def everything():
+        m = Moe(9, 2, 5, 300, 77, torch.float16)
+        out = m.run()
+        a, sa, b, sb, x = codes(9, 200, 1), side(9, 200, 2, 3), codes(70, 200, 3), blocks(70, 200, 4), normal(9, 200, 5).cuda()
+        q, s, y, c = *P.empty_f8(9, 200), torch.zeros(9, 200, device="cuda"), torch.zeros(9, 70, device="cuda")
+        P.dev_quantize_f8(x, out=(q, s))
+        P.dev_dequantize_f8(q, s, out=y)
+        P.dev_gemm_nt_f8(a, sa, b, sb, sb.new_ones(70), out=c)
+        rows, dy, dw = torch.zeros(18, 300, dtype=torch.float16, device="cuda"), torch.zeros(18, 300, dtype=torch.float16, device="cuda"), torch.zeros(9, 2, device="cuda")
+        P.dev_moe_gather(m.x, m.place[2], out=rows)
+        P.dev_moe_combine_backward(m.x, m.y, m.place[2], m.w, out=(dy, dw))
+        one = P.dev_gemm_nt_f8(a[:1], sa[:1], b, sb, out=c[:1].clone())
+        return out + [v.float() for v in (q, s, y, c, rows, dy, dw, one)]
+
+    monkeypatch.setattr(P, "_fast", Watch())
+    got = everything()
+    assert {n for n, rc in took if rc == 0} == {"quantize", "dequantize", "swiglu", "gemm", "experts", "sort", "gather", "gather_f8", "combine", "backward"} and all(rc == 0 for _, rc in took)
+    monkeypatch.setattr(P, "_fast", none)
+    assert all(torch.equal(a, b) for a, b in zip(got, everything()))
+    monkeypatch.setattr(P, "_fast", Watch())
+    del took[:]
+    test_front_ends_refuse_on_the_device()
+    assert took and all(rc != 0 for _, rc in took)
+
+
 def test_two_host_threads_on_streams_of_their_own():
     layers = [Moe(T, 3, 6, 256, 200, torch.bfloat16, seed=10 * T) for T in (1, 40)]
     wants = [m.run() for m in layers]
