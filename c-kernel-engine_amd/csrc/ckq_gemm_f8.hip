@@ -793,6 +793,7 @@ typedef F8Split<8, 2, 2, 2> S32x32w8;
 typedef F8Split<4, 2, 2, 2> S32x32;
 typedef F8Split<8, 2, 1, 2> S16x32w8;
 typedef F8Split<4, 2, 1, 2> S16x32;
+typedef F8Split<2, 2, 1, 2> S16x32w2;
 typedef F8Split<8, 1, 1, 2> S16x16;
 typedef F8Core<2, 4, 8, 4, 0, 2, 1> C256x256;
 typedef F8Core<4, 2, 4, 4, 4, 3, 1> C256x128;
@@ -801,25 +802,26 @@ typedef F8Core<2, 2, 4, 4, 4, 4, 1> C128x128;
 typedef F8Core<2, 2, 2, 4, 4, 4, 1> C64x128;
 typedef F8Core<2, 2, 2, 2, 4, 4, 2> C64x64;
 
-/* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all places have a block; a last round of fewer blocks less, `share`
- * of it by how many share a CU, the rest by how many there are in all.  Fitted to 700 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three sets in turn): the kernel so
- * chosen is 1.4 % slower than the fastest on average, 1.3 times at worst; fitted to half of them, 1.2 % on the other half; over experts (400 random products, 2 to 128 of them) 2.7 % and 1.6 times. */
-struct F8Cost { int bt, bn, places, split; float t0, t_tile, step, share; };
+/* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all places have a block; in a last round of fewer blocks less, `share` of it by how
+ * many share a CU, the rest by how many there are in all, but no less than a block alone takes, `alone`.  Fitted to 700 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three
+ * sets in turn): the kernel so chosen is 1.0 % (fp32 results) and 1.2 % (16 bits) slower than the fastest on average, 1.3 times at worst, as much on one half of them when fitted to the other; over experts (500
+ * random products, 2 to 128 of them, none of which it was fitted to) 1.9 % and 1.4 times. */
+struct F8Cost { int bt, bn, places, split; float t0, t_tile, step, share, alone; };
 static const F8Cost f8_costs[CKQ_F8_TILINGS] = {
-    {128, 128, 512, 1, 0.72f, 5.47f, 1.958f, 0.89f}, {64, 128, 768, 1, 2.64f, 2.66f, 1.832f, 1.00f}, {64, 64, 1024, 1, 2.89f, 1.75f, 1.505f, 1.00f},
-    {32, 32, 256, 8, 2.16f, 2.17f, 0.814f, 0.84f},   {32, 32, 512, 4, 2.61f, 1.90f, 0.825f, 1.00f},  {16, 32, 256, 8, 2.18f, 1.80f, 0.657f, 0.77f},
-    {16, 32, 768, 4, 2.82f, 1.44f, 0.862f, 1.00f},   {16, 16, 512, 8, 2.50f, 1.50f, 0.688f, 1.00f},
-    {256, 256, 256, 1, 0.00f, 7.80f, 1.966f, 0.62f}, {256, 128, 256, 1, 0.00f, 6.90f, 0.927f, 0.64f}, {128, 128, 256, 1, 1.46f, 4.65f, 0.591f, 0.66f},
-    {64, 128, 256, 1, 1.76f, 3.16f, 0.393f, 0.70f},  {64, 64, 512, 1, 2.13f, 2.19f, 0.443f, 1.00f},
+    {128, 128, 512, 1, 0.93f, 5.28f, 1.920f, 0.90f, 0.40f}, {64, 128, 768, 1, 1.20f, 3.76f, 1.610f, 1.00f, 0.44f}, {64, 64, 1024, 1, 1.67f, 2.52f, 1.324f, 1.00f, 0.40f},
+    {32, 32, 256, 8, 2.14f, 2.18f, 0.817f, 0.84f, 0.0f},    {32, 32, 512, 4, 2.15f, 2.16f, 0.738f, 1.00f, 0.72f},  {16, 32, 256, 8, 2.19f, 1.81f, 0.660f, 0.76f, 0.0f},
+    {16, 32, 768, 4, 2.37f, 1.65f, 0.779f, 1.00f, 0.56f},   {16, 32, 1536, 2, 2.17f, 1.75f, 0.812f, 1.00f, 0.54f}, {16, 16, 512, 8, 2.39f, 1.54f, 0.646f, 1.00f, 0.60f},
+    {256, 256, 256, 1, 0.00f, 7.80f, 1.959f, 0.62f, 0.0f},  {256, 128, 256, 1, 0.00f, 6.92f, 0.913f, 0.65f, 0.0f}, {128, 128, 256, 1, 1.45f, 4.69f, 0.587f, 0.67f, 0.0f},
+    {64, 128, 256, 1, 1.71f, 3.21f, 0.391f, 0.70f, 0.0f},   {64, 64, 512, 1, 1.94f, 2.34f, 0.416f, 1.00f, 0.55f},
 };
-static const F8Cost f8_cost_rest = {128, 192, 256, 1, 0.00f, 12.05f, 0.519f, 0.45f};
+static const F8Cost f8_cost_rest = {128, 192, 256, 1, 0.00f, 12.10f, 0.514f, 0.47f, 0.0f};
 
 static float f8_rounds(const F8Cost &c, float tiles, int K)
 {
     const int steps = ((K + 127) / 128 + c.split - 1) / c.split;
-    const float full = floorf(tiles / (float)c.places), rest = tiles - full * (float)c.places;
+    const float places = (float)c.places, full = floorf(tiles / places), rest = tiles - full * places;
     float t = full * (c.t_tile + (float)steps * c.step);
-    if (rest > 0.0f) t += c.t_tile + (float)steps * c.step * ((1.0f - c.share) * rest / (float)c.places + c.share * ceilf(rest / 256.0f) / ((float)c.places / 256.0f));
+    if (rest > 0.0f) t += c.t_tile + (float)steps * c.step * fmaxf(c.alone, (1.0f - c.share) * rest / places + c.share * ceilf(rest / 256.0f) * 256.0f / places);
     return t;
 }
 /* Tiles of M rows; of experts, which have what only the device knows, as many as if each row went to any of them alike. */
@@ -876,6 +878,7 @@ static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
     case CKQ_F8_S32x32:      return launch_f8_split<E, S32x32>(a, s);
     case CKQ_F8_S16x32w8:    return launch_f8_split<E, S16x32w8>(a, s);
     case CKQ_F8_S16x32:      return launch_f8_split<E, S16x32>(a, s);
+    case CKQ_F8_S16x32w2:    return launch_f8_split<E, S16x32w2>(a, s);
     case CKQ_F8_S16x16:      return launch_f8_split<E, S16x16>(a, s);
     case CKQ_F8_C256x256:    return launch_f8_core<E, C256x256>(a, s);
     case CKQ_F8_C256x128:    return launch_f8_core<E, C256x128>(a, s);
