@@ -65,6 +65,11 @@ __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 
     if (row >= a.rows || 128l * g >= a.k) return;              /* all eight lanes */
     const int left = (int)(a.k - at);
     const E *x = (const E *)a.x + (size_t)row * a.ldx + at;
+    int to[8];                                                 /* gather: where the first eight go, under way with the row itself */
+    if (OP == F8_GATHER) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j] = a.position[(size_t)row * a.choices + min(j, a.choices - 1)];
+    }
     constexpr bool ONCE = OP != F8_GATHER;
     raw8<E> r0 = fetch8<ONCE>(x, left), r1 = fetch8<ONCE>(x + 8, left - 8);
     float v[16];
@@ -105,11 +110,15 @@ __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 
         if (l == 0) a.scale[(size_t)g * a.lds + to] = scale;
     };
     if (OP != F8_GATHER) put(row);
-    else
-        for (int j = 0; j < a.choices; ++j) {
-            const int to = a.position[(size_t)row * a.choices + j];
-            if ((u32)to < (u32)a.most) put(to);
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < a.choices && (u32)to[j] < (u32)a.most) put(to[j]);
+        for (int j = 8; j < a.choices; ++j) {
+            const int more = a.position[(size_t)row * a.choices + j];
+            if ((u32)more < (u32)a.most) put(more);
         }
+    }
 }
 
 /* As many rows beside each other as there are, 32 at most: the scales of a group leave side by side. */

@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
         if (j0) __syncthreads();
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+            if (j0 + j >= a.choices) break;
             const float s = group_sum<64>(sum[j]);
             if (lane == 63) red[wave][j] = s;
         }
