@@ -19,6 +19,7 @@
 #include "ckq_int8.hpp"
 #include "ckq_launch.h"
 #include "ckq_rows.hpp"
+#include <algorithm>
 
 enum { F8_QUANTIZE, F8_SWIGLU, F8_GATHER };
 
@@ -129,7 +130,7 @@ static int f8_rows_shift(int rows, int k)
     return rs;
 }
 /* Rows that one launch takes, for the same reason. */
-static int f8_rows_most(int rows, int rs, u32 group_tiles) { return (int)min((size_t)rows, ((size_t)1 << 23) / group_tiles << rs); }
+static int f8_rows_most(int rows, int rs, u32 group_tiles) { return (int)std::min<size_t>(rows, ((size_t)1 << 23) / group_tiles << rs); }
 
 template <int OP, class E>
 static int launch_rows_f8(F8RowsArgs a, hipStream_t s)

@@ -14,6 +14,7 @@
 #include "ckq_int8.hpp"
 #include "ckq_launch.h"
 #include "ckq_rows.hpp"
+#include <algorithm>
 
 /* ---- sort ---------------------------------------------------------------------------------------------------------- */
 
@@ -28,12 +29,12 @@ __global__ void __launch_bounds__(1024) moe_sort_kernel(const int32_t *__restric
     __shared__ int before[16], mine[16];
     const int lane = threadIdx.x & 63, wave = wave_in_block(), nw = blockDim.x >> 6;
     const u32 e = blockIdx.x;
-    const int first = (int)min((long)wave * run, (long)slots), end = (int)min((long)wave * run + run, (long)slots);
+    const int first = min(wave * run, slots), end = min(first + run, slots);
     u32 key[NV];                                               /* none: `experts`; behind the end: more than that.  No branch depends on either */
-    const __amdgpu_buffer_rsrc_t all_ids = __builtin_amdgcn_make_buffer_rsrc((void *)ids, 0, (int)(4u * (u32)slots), 0x00020000);      /* zeros behind the last */
     auto load = [&](int s0) {
+        const __amdgpu_buffer_rsrc_t rest = __builtin_amdgcn_make_buffer_rsrc((void *)(ids + s0), 0, (int)(4u * (u32)(slots - s0)), 0x00020000);      /* zeros behind the last */
 #pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = __builtin_amdgcn_raw_buffer_load_b32(all_ids, 4 * lane + 256 * i, 4 * s0, 0);
+        for (int i = 0; i < NV; ++i) key[i] = __builtin_amdgcn_raw_buffer_load_b32(rest, 4 * lane + 256 * i, 0, 0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) key[i] = min(key[i], (u32)experts);
         if (end - s0 < 64 * NV)
@@ -217,11 +218,11 @@ __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
     });
 }
 
-/* The launches of all tokens: one has fewer than 2^32 threads. */
+/* The launches of all tokens: one has fewer than 2^32 threads.  (min and max without std:: are those of int, on the host.) */
 template <class E, class L>
 static int moe_each(MoeArgs a, bool out_by_token, size_t threads, L &&launch)
 {
-    const int most = (int)min((size_t)a.tokens, max((size_t)1, ((size_t)1 << 31) / threads));
+    const int most = (int)std::min<size_t>(a.tokens, std::max<size_t>(1, ((size_t)1 << 31) / threads));
     for (int left = a.tokens;;) {
         const int now = min(left, most);
         a.tokens = now;
