@@ -18,6 +18,7 @@
 #include "ckq_int8.hpp"
 #include "ckq_launch.h"
 #include "ckq_rows.hpp"
+#include <algorithm>
 
 enum { ROWS_QUANTIZE, ROWS_RMSNORM, ROWS_SWIGLU };
 
@@ -464,7 +465,7 @@ extern "C" int ckq_launch_dequantize_i8(const int8_t *q, long ldq, const float *
     const u32 nvec = (u32)(k / 16 + (k % 16 != 0));
     const hipStream_t s = (hipStream_t)stream;
     /* a launch has fewer than 2^32 threads */
-    const int most = (int)min((size_t)rows, max((size_t)1, ((size_t)1 << 31) / nvec));
+    const int most = (int)std::min<size_t>(rows, std::max<size_t>(1, ((size_t)1 << 31) / nvec));
     for (int row = 0; row < rows;) {
         const int n = min(rows - row, most);
         const int8_t *qr = q + (size_t)row * ldq;

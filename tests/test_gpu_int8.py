@@ -604,6 +604,12 @@ def test_launches_in_parts():
     assert torch.equal(qn[-9:], q2) and torch.equal(sn[-9:], s2) and torch.equal(h, x + res) and torch.equal(h[-9:], h2)
 
 
+def test_many_short_rows_are_read_back_in_one_launch():
+    """A launch for each row would take minutes."""
+    q, s = torch.randint(-127, 128, (1 << 26, 3), device="cuda", dtype=torch.int8), torch.rand(1 << 26, device="cuda")
+    assert torch.equal(P.dev_dequantize_i8(q, s), q.float() * s[:, None])
+
+
 def test_offsets_beyond_32_bits():
     """Rows whose distance from the first does not fit in 32 bits of elements."""
     far = (1 << 30) + 24
