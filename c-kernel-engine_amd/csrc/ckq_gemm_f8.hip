@@ -27,7 +27,7 @@ struct F8Args {
     const float   *sa, *sb, *bias;
     const int32_t *offsets;                 /* experts: where each one's rows begin, experts + 1 of them; null: one matrix */
     void          *C;
-    long           lda, ldsa, ldb, eb, ldsb, esb, ldc;     /* eb, esb: from one expert's matrix and scales to the next */
+    long           lda, ldsa, ldb, eb, ldsb, esb, ebias, ldc;     /* eb, esb, ebias: from one expert's matrix, scales and bias to the next */
     int            M, N, K, experts;
 };
 
@@ -92,7 +92,9 @@ __device__ __forceinline__ bool f8_tile(const F8Args &a, int id, int BT, int nnt
 }
 
 /* Blocks that have all tiles there can be: an expert's last tile may be one row. */
-static long f8_most_tiles(const F8Args &a, int BT) { return a.offsets ? (long)a.M / BT + min(a.M, a.experts) : ((long)a.M + BT - 1) / BT; }
+enum { F8_LAUNCH_MOST = 1 << 23 };                              /* blocks of a launch stay below this: fewer than 2^32 threads */
+static long f8_most_tiles(int M, int experts, int BT) { return experts ? (long)M / BT + min(M, experts) : ((long)M + BT - 1) / BT; }
+static long f8_most_tiles(const F8Args &a, int BT) { return f8_most_tiles(a.M, a.offsets ? a.experts : 0, BT); }
 
 /* ---- operands and results -------------------------------------------------------------------------------------------- */
 
@@ -295,7 +297,7 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
         }
     __syncthreads();
     /* Through LDS, each wave by itself, 32 tokens at a time, so that a lane has eight rows' results of a token and a token's leave in whole lines. */
-    const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
+    const float *bias = a.bias ? a.bias + (size_t)w.e * a.ebias : nullptr;
     uint8_t *mine = lds + wave * 32 * PITCH;
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
@@ -324,7 +326,6 @@ static int launch_f8_half(const F8Args &a, hipStream_t s)
 {
     const int nnt = (a.N + T::BN - 1) / T::BN;
     const long tiles = f8_most_tiles(a, T::BT) * nnt;
-    if (tiles >= 1l << 23) return CKQ_EINVAL;
     return i8_launch(gemm_f8_half_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
 }
 
@@ -490,7 +491,7 @@ __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, i
         read_scales(next);
         buf = next;
     }
-    const float *bias = a.bias ? a.bias + (size_t)w.e * a.N : nullptr;
+    const float *bias = a.bias ? a.bias + (size_t)w.e * a.ebias : nullptr;
     uint8_t *mine = lds + wave * 16 * PITCH;
     __syncthreads();
 #pragma unroll
@@ -536,7 +537,6 @@ static int launch_f8_two(const F8Args &a, int nnt1, hipStream_t s)
 {
     const int nnt2 = (a.N - nnt1 * T1::BN + T2::BN - 1) / T2::BN;
     const long blocks1 = (f8_most_tiles(a, T1::BT) * nnt1 + 7) & ~7l, blocks2 = (f8_most_tiles(a, T2::BT) * nnt2 + 7) & ~7l;
-    if (blocks1 + blocks2 >= 1l << 23) return CKQ_EINVAL;
     return i8_launch(gemm_f8_two_kernel<E, T1, T2>, dim3((u32)(blocks1 + blocks2)), dim3(64u * T1::WAVES), s, a, nnt1, (int)blocks1, nnt2);
 }
 
@@ -545,7 +545,6 @@ static int launch_f8_core(const F8Args &a, hipStream_t s)
 {
     const int nnt = (a.N + T::BN - 1) / T::BN;
     const long tiles = f8_most_tiles(a, T::BT) * nnt;
-    if (tiles >= 1l << 23) return CKQ_EINVAL;
     return i8_launch(gemm_f8_core_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::WAVES), s, a, nnt);
 }
 
@@ -671,7 +670,7 @@ __global__ void __launch_bounds__(64 * T::NW) gemm_f8_split_kernel(F8Args a, int
 #pragma unroll
         for (int r = 0; r < 8; ++r) f[r] += q[r >> 2][r & 3];
     }
-    f8_store8<E, false>(a, a.bias ? a.bias + (size_t)w.e * a.N : nullptr, f, t, n);
+    f8_store8<E, false>(a, a.bias ? a.bias + (size_t)w.e * a.ebias : nullptr, f, t, n);
 }
 
 template <class E, class T>
@@ -679,7 +678,6 @@ static int launch_f8_split(const F8Args &a, hipStream_t s)
 {
     const int nnt = (a.N + T::BN - 1) / T::BN;
     const long tiles = f8_most_tiles(a, T::BT) * nnt;
-    if (tiles >= 1l << 23) return CKQ_EINVAL;
     return i8_launch(gemm_f8_split_kernel<E, T>, dim3((u32)((tiles + 7) & ~7l)), dim3(64u * T::NW), s, a, nnt);
 }
 
@@ -831,18 +829,27 @@ static float f8_rounds(const F8Cost &c, float tiles, int K)
 /* Tiles of M rows; of experts, which have what only the device knows, as many as if each row went to any of them alike. */
 static float f8_row_tiles(int bt, int M, int experts)
 {
-    if (!experts) return (float)((M + bt - 1) / bt);
+    if (!experts) return (float)((M + (long)bt - 1) / bt);
     const float used = (float)experts * (1.0f - powf(1.0f - 1.0f / (float)experts, (float)M)), rows = (float)M / used;
     return rows > 0.75f * (float)bt ? used * fmaxf(1.0f, rows / (float)bt + 0.5f) : used;
 }
-static float f8_tiles(const F8Cost &c, int M, int N, int experts) { return f8_row_tiles(c.bt, M, experts) * (float)((N + c.bn - 1) / c.bn); }
+static float f8_tiles(const F8Cost &c, int M, int N, int experts) { return f8_row_tiles(c.bt, M, experts) * (float)((N + (long)c.bn - 1) / c.bn); }
 
 /* Columns of 256 x 256 tiles that make whole rounds of the 256 CUs: what they leave goes in tiles of 128 x 192, a shorter last round (2048 x 11008 x 4096: 344 tiles of 256 x 256 in two rounds 105 us; 256 of
  * them and 240 small ones 87). */
 static int f8_whole_columns(int M, int N)
 {
-    const int ntt = (M + 255) / 256, nnt = (N + 255) / 256;
-    return (int)((long)ntt * nnt / 256 * 256 / ntt);
+    const long ntt = (M + 255l) / 256, nnt = (N + 255l) / 256;
+    return (int)(ntt * nnt / 256 * 256 / ntt);
+}
+
+/* Whether a kernel takes a product in one launch. */
+static bool f8_fits(int kernel, int M, int N, int experts)
+{
+    if (kernel == CKQ_F8_STREAM) return N <= 1 << 23;
+    const int bt = kernel == CKQ_F8_TWO ? 128 : f8_costs[kernel].bt, bn = kernel == CKQ_F8_TWO ? 192 : f8_costs[kernel].bn;
+    const long wide = (N + (long)bn - 1) / bn, tiles = kernel == CKQ_F8_TWO ? (f8_most_tiles(M, experts, bt) + 2) * (wide + 2) : f8_most_tiles(M, experts, bt) * wide;
+    return tiles < F8_LAUNCH_MOST - 16;
 }
 
 static std::atomic<int> g_f8_kernel{-1};
@@ -851,26 +858,28 @@ extern "C" void ckq_launch_set_f8_kernel(int kernel) { g_f8_kernel.store(kernel 
 /* The e4m3 instructions' sums, 1.5e-5 off, are taken where the result is rounded to 16 bits (bf16 2^-9, fp16 2^-12 off) and nothing but that: not for fp32 results, and not over experts, whose first product's
  * results go through another quantizer, where each change of a value moves some of them by a sixteenth (an MLP with 32 experts in fp16: 0.0017 off the definition, with fp32 sums 0.0003).  Random products of one
  * matrix gain 5.8 % by them on average, 2048 x 11008 x 4096 174 -> 87 us. */
+/* -1: none takes it in one launch. */
 extern "C" int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts)
 {
     const int forced = g_f8_kernel.load();
     const int cols = experts ? 0 : f8_whole_columns(M, N);
-    if (forced >= 0 && (forced != CKQ_F8_STREAM || (M == 1 && !experts)) && (forced != CKQ_F8_TWO || cols > 0)) return forced;
-    if (M == 1 && !experts) return CKQ_F8_STREAM;
+    if (forced >= 0 && (forced != CKQ_F8_STREAM || (M == 1 && !experts)) && (forced != CKQ_F8_TWO || cols > 0)) return f8_fits(forced, M, N, experts) ? forced : -1;
+    if (M == 1 && !experts) return f8_fits(CKQ_F8_STREAM, M, N, 0) ? CKQ_F8_STREAM : -1;
     const bool cores = type != CKQ_T_F32 && !experts;
-    int best = 0;
+    int best = -1;
     float t = 1e30f;
     for (int i = 0; i < (cores ? CKQ_F8_TILINGS : CKQ_F8_C256x256); ++i) {
         const float ti = f8_costs[i].t0 + f8_rounds(f8_costs[i], f8_tiles(f8_costs[i], M, N, experts), K);
-        if (ti < t) { t = ti; best = i; }
+        if (ti < t && f8_fits(i, M, N, experts)) { t = ti; best = i; }
     }
-    if (cores && cols > 0 && 256 * cols < N) {
+    if (best >= 0 && cores && cols > 0 && 256 * cols < N) {
         const F8Cost &a = f8_costs[CKQ_F8_C256x256], &b = f8_cost_rest;
-        if (a.t0 + f8_rounds(a, (float)((M + 255) / 256) * (float)cols, K) + f8_rounds(b, f8_tiles(b, M, N - 256 * cols, 0), K) < t) best = CKQ_F8_TWO;
+        if (a.t0 + f8_rounds(a, (float)((M + 255l) / 256) * (float)cols, K) + f8_rounds(b, f8_tiles(b, M, N - 256 * cols, 0), K) < t && f8_fits(CKQ_F8_TWO, M, N, 0)) best = CKQ_F8_TWO;
     }
     return best;
 }
 
+/* What one launch does not take goes in halves, of the tokens or of the weights' rows, which are whole tiles and blocks of scales; over experts of the latter only. */
 template <class E>
 static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
 {
@@ -890,8 +899,28 @@ static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
     case CKQ_F8_C64x128:     return launch_f8_core<E, C64x128>(a, s);
     case CKQ_F8_C64x64:      return launch_f8_core<E, C64x64>(a, s);
     case CKQ_F8_TWO:         return launch_f8_two<E, C256x256, C128x192>(a, f8_whole_columns(a.M, a.N), s);
-    default:                 return launch_f8_stream<E>(a, s);
+    case CKQ_F8_STREAM:      return launch_f8_stream<E>(a, s);
+    default:                 break;
     }
+    F8Args first = a, second = a;
+    if (!a.offsets && a.M > a.N) {
+        first.M = (a.M / 2 + 127) & ~127;
+        if (first.M >= a.M) return CKQ_EINVAL;
+        second.M = a.M - first.M;
+        second.A += (size_t)first.M * a.lda;
+        second.sa += first.M;
+        second.C = (E *)a.C + (size_t)first.M * a.ldc;
+    } else {
+        first.N = (a.N / 2 + 127) & ~127;
+        if (first.N >= a.N) return CKQ_EINVAL;
+        second.N = a.N - first.N;
+        second.B += (size_t)first.N * a.ldb;
+        second.sb += (size_t)(first.N / 128) * a.ldsb;
+        if (a.bias) second.bias += first.N;
+        second.C = (E *)a.C + first.N;
+    }
+    const int rc = launch_gemm_f8<E>(first, type, s);
+    return rc ? rc : launch_gemm_f8<E>(second, type, s);
 }
 
 static int f8_gemm(const F8Args &a, int type, void *stream)
@@ -909,12 +938,12 @@ static int f8_gemm(const F8Args &a, int type, void *stream)
 extern "C" int ckq_launch_gemm_f8(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, const float *sb, long ldsb, const float *bias,
                                   int type, void *C, long ldc, int M, int N, int K, void *stream)
 {
-    return f8_gemm({A, B, sa, sb, bias, nullptr, C, lda, ldsa, ldb, 0, ldsb, 0, ldc, M, N, K, 1}, type, stream);
+    return f8_gemm({A, B, sa, sb, bias, nullptr, C, lda, ldsa, ldb, 0, ldsb, 0, 0, ldc, M, N, K, 1}, type, stream);
 }
 
 extern "C" int ckq_launch_gemm_f8_experts(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, long eb, const float *sb, long ldsb, long esb,
                                           const float *bias, const int32_t *offsets, int experts, int type, void *C, long ldc, int M, int N, int K, void *stream)
 {
-    if (!offsets || experts <= 0 || experts > CKQ_MOE_EXPERTS_MAX || eb < 0 || esb < 0) return CKQ_EINVAL;
-    return f8_gemm({A, B, sa, sb, bias, offsets, C, lda, ldsa, ldb, eb, ldsb, esb, ldc, M, N, K, experts}, type, stream);
+    if (!offsets || experts <= 0 || experts > CKQ_MOE_EXPERTS_MAX || M > CKQ_MOE_SLOTS_MAX || eb < 0 || esb < 0) return CKQ_EINVAL;
+    return f8_gemm({A, B, sa, sb, bias, offsets, C, lda, ldsa, ldb, eb, ldsb, esb, N, ldc, M, N, K, experts}, type, stream);
 }

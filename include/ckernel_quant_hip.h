@@ -331,7 +331,7 @@ int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t 
  * activations is the same product with the transposed codes and scales of the weights.
  * ckq_gemm_nt_f8_experts_dev: the same of rows sorted by expert, each expert with a matrix, scales and bias of its own: rows offsets[e] .. offsets[e + 1] - 1 of A and C
  * with B + e * eb, sb + e * esb and bias + e * N (eb a multiple of 16).  offsets are on the device, experts + 1 of them, from 0 on and none less than the one before
- * (what lies outside 0 .. M counts as the nearest of these); an expert may have no rows, and rows of C that no expert has stay as they are. */
+ * (what lies outside 0 .. M counts as the nearest of these, and M is at most 2^29); an expert may have no rows, and rows of C that no expert has stay as they are. */
 int ckq_quantize_f8_dev(ckq_ck_dtype type, const void *x, long ldx, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
 int ckq_dequantize_f8_dev(const uint8_t *q, long ldq, const float *scale, long lds, ckq_ck_dtype type, void *y, long ldy, int rows, int k, void *stream);
 int ckq_swiglu_f8_dev(ckq_ck_dtype type, const void *gate, const void *up, long ld, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
@@ -346,7 +346,7 @@ int ckq_gemm_nt_f8_experts_dev(const uint8_t *A, long lda, const float *sa, long
  *
  * ckq_moe_sort_dev: slots in the order of their experts, those of one expert as they come: offsets[e] = number of slots of experts under e (experts + 1 of them),
  * order[p] = the slot at place p (-1 from offsets[experts] on), position[s] = the place of slot s (-1: none).
- * In what follows y has `rows` rows, and a position outside 0 .. rows - 1 counts as none.  No two slots have one position.
+ * In what follows y has `rows` rows, and a position outside 0 .. rows - 1 counts as none.  No two slots have one position, and what is written overlaps nothing that is read but where it says so.
  * ckq_moe_gather_dev: y[position[s]] = x[s / choices]; other rows of y stay as they are.
  * ckq_moe_gather_f8_dev: the same in 8 bits, as ckq_quantize_f8_dev has them (lds at least `rows`).
  * ckq_moe_combine_dev: out[t] = sum over j of weights[s] * y[position[s]], in fp32, j in turn, rounded once; zeros where a token has no slot with a place.  weights NULL: ones - the

@@ -454,6 +454,81 @@ def test_experts_on_every_kernel(kernel, M, N, K, counts):
     check_experts(out, a, sa, b, sb, offsets, bias, cores=kernel in CORES)
 
 
+@pytest.mark.parametrize("kernel", [8, 6, 0], indirect=True)
+def test_matmul_launches_in_parts(kernel):
+    """More tiles than one launch has blocks, of 16 x 16 and 16 x 32: whole numbers, whose sums are exact in any order."""
+    def whole(*shape):
+        return torch.randint(-4, 5, shape, device="cuda", generator=g).to(torch.float16)
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for M, N, E in ((4100, (1 << 19) + 77, 0), ((1 << 19) + 77, 4100, 0), (3000, (1 << 18) + 130, 300), (1, (1 << 24) + 9, 0)):
+        a, b, K = whole(M, 16), whole(*((E, N, 16) if E else (N, 16))), 16
+        sa, sb = torch.full((1, M), 2.0, device="cuda").t(), torch.full((*b.shape[:-2], -(-N // 128), 1), 0.25, device="cuda")
+        sa[M // 2:] = 4.0
+        sb[..., 5::3, :] = 0.5
+        bias = torch.randint(-3, 4, b.shape[:-1], device="cuda", generator=g).float()
+        out = torch.full((M, N), 7.0, device="cuda", dtype=torch.float16)
+        aw, bw = a * sa.half(), b * sb.half().repeat_interleave(128, -2)[..., :N, :]           # |sums| <= 16 * 16 * 2 + 3 in steps of 1/2: exact in fp16
+        if E:
+            counts = torch.full((E,), M // E)
+            counts[3], counts[7] = 0, 2 * (M // E)
+            offsets = torch.nn.functional.pad(counts.cumsum(0), (1, 0)).int().cuda()
+            P.dev_gemm_nt_f8_experts(a.to(F8), sa, b.to(F8), sb, offsets, bias, out=out)
+            at = [0] + counts.cumsum(0).tolist()
+            for e in range(E):
+                assert torch.equal(out[at[e]:at[e + 1]], aw[at[e]:at[e + 1]] @ bw[e].t() + bias[e].half()), e
+        else:
+            P.dev_gemm_nt_f8(a.to(F8), sa, b.to(F8), sb, bias, out=out)
+            for m in range(0, M, 1 << 16):
+                assert torch.equal(out[m:m + (1 << 16)], aw[m:m + (1 << 16)] @ bw.t() + bias.half()), m
+        del out, aw, bw
+
+
+def test_rows_launches_in_parts():
+    """Rows of one element, more than a launch has threads for."""
+    rows = (1 << 28) + 45
+    x = torch.randn(rows, 1, device="cuda", dtype=torch.bfloat16)
+    q, s = torch.empty(rows, 1, device="cuda", dtype=F8), torch.empty(1, rows, device="cuda").t()
+    top = torch.tensor(448.0, device="cuda")                   # a number would be multiplied by its inverse
+
+    def check():
+        for i in range(0, rows, 1 << 26):
+            part = x[i:i + (1 << 26)]
+            assert torch.equal(q[i:i + (1 << 26)].view(torch.uint8), torch.where(part < 0, 0xFE, torch.where(part > 0, 0x7E, 0)).to(torch.uint8) | torch.signbit(part) * 128)
+            assert torch.equal(s[i:i + (1 << 26)], part.float().abs().clamp(min=TINY) / top)
+
+    P.dev_quantize_f8(x, (q, s))
+    check()
+    y = torch.empty_like(x)
+    P.dev_dequantize_f8(q, s, out=y)
+    for i in range(0, rows, 1 << 26):                         # scale * 448: an eighth of a step of bf16 off, at most
+        assert torch.equal(x[i:i + (1 << 26)], y[i:i + (1 << 26)])
+    q.view(torch.uint8).zero_()
+    s.zero_()
+    back = torch.arange(rows - 1, -1, -1, device="cuda", dtype=torch.int32)[:, None]
+    P.dev_moe_gather_f8(x, back, out=(q, s))
+    x = x.flip(0)
+    check()
+    del q, s
+    P.dev_moe_gather(x, back, y)
+    assert torch.equal(y, x.flip(0))
+    # a block has a token: 2^23 of them a launch
+    T = (1 << 23) + 9
+    d, rows_ = x[:T].contiguous(), y[:T].contiguous()
+    w = torch.rand(T, 1, device="cuda")
+    dy, dw = P.dev_moe_combine_backward(d, rows_, back[-T:].contiguous(), w)
+    assert torch.equal(dy, (d.float() * w).bfloat16().flip(0)) and torch.equal(dw, d.float() * rows_.flip(0).float())
+    del x, y, d, rows_, dy, dw, w, back
+    # two threads a row: 2^30 rows a launch
+    T = (1 << 30) + 5
+    x, back = torch.randn(T, 9, device="cuda", dtype=torch.bfloat16), torch.arange(T - 1, -1, -1, device="cuda", dtype=torch.int32)[:, None]
+    y, out = torch.empty_like(x), torch.empty_like(x)
+    P.dev_moe_gather(x, back, y)
+    P.dev_moe_combine(y, back, None, out=out)
+    for part in (slice(0, 5000), slice((1 << 30) - 5000, None)):
+        assert torch.equal(y[part], x[T - (part.stop or T):T - part.start].flip(0)) and torch.equal(out[part], x[part])
+
+
 def test_experts_of_one_matrix_and_of_offsets_out_of_range():
     a, sa, b, sb = codes(40, 200, 1), side(40, 200, 2), codes(130, 200, 3), blocks(130, 200, 4)
     # experts side by side in one tensor whose rows are further apart, one matrix for all of them
