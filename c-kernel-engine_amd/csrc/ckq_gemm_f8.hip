@@ -791,7 +791,7 @@ static int launch_f8_stream(const F8Args &a, hipStream_t s)
 typedef F8Half<2, 2, 2, 2> H128x128;
 typedef F8Half<2, 2, 1, 2> H64x128;
 typedef F8Half<2, 2, 1, 1> H64x64;
-typedef F8Split<8, 2, 2, 2> S32x32w8;
+typedef F8Split<7, 2, 3, 2> S48x32w7;
 typedef F8Split<4, 2, 2, 2> S32x32;
 typedef F8Split<8, 2, 1, 2> S16x32w8;
 typedef F8Split<4, 2, 1, 2> S16x32;
@@ -806,17 +806,17 @@ typedef F8Core<2, 2, 2, 2, 4, 4, 2> C64x64;
 
 /* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all places have a block; in a last round of fewer blocks less, `share` of it by how
  * many share a CU, the rest by how many there are in all, but no less than a block alone takes, `alone`.  Fitted to 700 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three
- * sets in turn): the kernel so chosen is 1.0 % (fp32 results) and 1.2 % (16 bits) slower than the fastest on average, 1.3 times at worst, as much on one half of them when fitted to the other; over experts (500
- * random products, 2 to 128 of them, none of which it was fitted to) 1.9 % and 1.4 times. */
+ * sets in turn): the kernel so chosen is 0.8 % (fp32 results) and 0.7 % (16 bits) slower than the fastest on average, 1.3 times at worst, as much on one half of them when fitted to the other; over experts (500
+ * random products, 2 to 128 of them, none of which it was fitted to) 1.6 % and 1.4 times. */
 struct F8Cost { int bt, bn, places, split; float t0, t_tile, step, share, alone; };
 static const F8Cost f8_costs[CKQ_F8_TILINGS] = {
-    {128, 128, 512, 1, 0.93f, 5.28f, 1.920f, 0.90f, 0.40f}, {64, 128, 768, 1, 1.20f, 3.76f, 1.610f, 1.00f, 0.44f}, {64, 64, 1024, 1, 1.67f, 2.52f, 1.324f, 1.00f, 0.40f},
-    {32, 32, 256, 8, 2.14f, 2.18f, 0.817f, 0.84f, 0.0f},    {32, 32, 512, 4, 2.15f, 2.16f, 0.738f, 1.00f, 0.72f},  {16, 32, 256, 8, 2.19f, 1.81f, 0.660f, 0.76f, 0.0f},
-    {16, 32, 768, 4, 2.37f, 1.65f, 0.779f, 1.00f, 0.56f},   {16, 32, 1536, 2, 2.17f, 1.75f, 0.812f, 1.00f, 0.54f}, {16, 16, 512, 8, 2.39f, 1.54f, 0.646f, 1.00f, 0.60f},
-    {256, 256, 256, 1, 0.00f, 7.80f, 1.959f, 0.62f, 0.0f},  {256, 128, 256, 1, 0.00f, 6.92f, 0.913f, 0.65f, 0.0f}, {128, 128, 256, 1, 1.45f, 4.69f, 0.587f, 0.67f, 0.0f},
-    {64, 128, 256, 1, 1.71f, 3.21f, 0.391f, 0.70f, 0.0f},   {64, 64, 512, 1, 1.94f, 2.34f, 0.416f, 1.00f, 0.55f},
+    {128, 128, 512, 1, 0.44f, 5.74f, 1.950f, 0.95f, 0.39f}, {64, 128, 768, 1, 1.41f, 3.54f, 1.673f, 1.00f, 0.44f}, {64, 64, 1024, 1, 1.68f, 2.54f, 1.373f, 1.00f, 0.39f},
+    {48, 32, 256, 7, 2.22f, 2.31f, 1.029f, 0.79f, 0.0f},    {32, 32, 512, 4, 2.15f, 1.96f, 0.818f, 1.00f, 0.68f},  {16, 32, 256, 8, 1.86f, 1.88f, 0.702f, 0.76f, 0.0f},
+    {16, 32, 768, 4, 2.36f, 1.42f, 0.877f, 1.00f, 0.52f},   {16, 32, 1536, 2, 2.07f, 1.62f, 0.871f, 1.00f, 0.53f}, {16, 16, 512, 8, 2.17f, 1.45f, 0.732f, 1.00f, 0.39f},
+    {256, 256, 256, 1, 0.00f, 8.08f, 1.888f, 0.66f, 0.0f},  {256, 128, 256, 1, 0.00f, 6.92f, 0.928f, 0.66f, 0.0f}, {128, 128, 256, 1, 1.48f, 4.77f, 0.585f, 0.68f, 0.0f},
+    {64, 128, 256, 1, 1.89f, 3.09f, 0.403f, 0.69f, 0.0f},   {64, 64, 512, 1, 2.01f, 2.29f, 0.428f, 1.00f, 0.56f},
 };
-static const F8Cost f8_cost_rest = {128, 192, 256, 1, 0.00f, 12.10f, 0.514f, 0.47f, 0.0f};
+static const F8Cost f8_cost_rest = {128, 192, 256, 1, 0.00f, 10.79f, 0.505f, 0.84f, 0.0f};
 
 static float f8_rounds(const F8Cost &c, float tiles, int K)
 {
@@ -887,7 +887,7 @@ static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
     case CKQ_F8_H128x128:    return launch_f8_half<E, H128x128>(a, s);
     case CKQ_F8_H64x128:     return launch_f8_half<E, H64x128>(a, s);
     case CKQ_F8_H64x64:      return launch_f8_half<E, H64x64>(a, s);
-    case CKQ_F8_S32x32w8:    return launch_f8_split<E, S32x32w8>(a, s);
+    case CKQ_F8_S48x32w7:    return launch_f8_split<E, S48x32w7>(a, s);
     case CKQ_F8_S32x32:      return launch_f8_split<E, S32x32>(a, s);
     case CKQ_F8_S16x32w8:    return launch_f8_split<E, S16x32w8>(a, s);
     case CKQ_F8_S16x32:      return launch_f8_split<E, S16x32>(a, s);

@@ -186,9 +186,9 @@ int ckq_launch_gemm_f8(const uint8_t *A, long lda, const float *sa, long ldsa, c
 int ckq_launch_gemm_f8_experts(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, long eb, const float *sb, long ldsb, long esb,
                                const float *bias, const int32_t *offsets, int experts, int type, void *C, long ldc, int M, int N, int K, void *stream);
 /* Which kernel takes a product of M rows against matrices of N x K (experts: their number, 0: one matrix without offsets), results of `type`: tiles of so many tokens x rows on the fp16 instructions (S:
- * with K split among a block's waves, w8, w2: eight or two of them) or on the e4m3 ones (C), two sizes of the latter in a launch, or the rows streamed; -1: in parts, since no launch has so many blocks.  Host arithmetic; exported for the test of the
+ * with K split among a block's waves, w8, w7, w2: eight, seven or two of them) or on the e4m3 ones (C), two sizes of the latter in a launch, or the rows streamed; -1: in parts, since no launch has so many blocks.  Host arithmetic; exported for the test of the
  * rules. */
-enum { CKQ_F8_H128x128, CKQ_F8_H64x128, CKQ_F8_H64x64, CKQ_F8_S32x32w8, CKQ_F8_S32x32, CKQ_F8_S16x32w8, CKQ_F8_S16x32, CKQ_F8_S16x32w2, CKQ_F8_S16x16, CKQ_F8_C256x256, CKQ_F8_C256x128,
+enum { CKQ_F8_H128x128, CKQ_F8_H64x128, CKQ_F8_H64x64, CKQ_F8_S48x32w7, CKQ_F8_S32x32, CKQ_F8_S16x32w8, CKQ_F8_S16x32, CKQ_F8_S16x32w2, CKQ_F8_S16x16, CKQ_F8_C256x256, CKQ_F8_C256x128,
        CKQ_F8_C128x128, CKQ_F8_C64x128, CKQ_F8_C64x64, CKQ_F8_TILINGS, CKQ_F8_TWO = CKQ_F8_TILINGS, CKQ_F8_STREAM };
 int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts);
 /* -1 = by shape (default), else that kernel wherever it can take the product, in all calls of the process. */
