@@ -9,6 +9,11 @@
  * Sums.  The matrix cores' e4m3 instructions add eight products at a time after aligning them to the largest of the eight and dropping what is
  * under 2^-13 of it (measured, in all their shapes; between eights they add as fp32 does): a sum of 128 random products is 1.5e-5 of its size off.
  * e4m3 values are exact in fp16, and the fp16 instructions add their products as fp32 does (1e-8), at half the rate.
+ *
+ * Forms.  One token: rows streamed, bound by reading them (11008 x 4096 from memory 8.4 us, 5.3 TB/s).  A few tokens: K split among the waves of a block, bound by a launch's and a block's start and a wave's
+ * steps one after the other (16 tokens 10.8 us, 64 11.8; one token through 8 of 64 experts of 2816 x 2048 10.6, 4.4 TB/s).  More: tiles, on the fp16 instructions bound by those and the
+ * conversions beside them (matrix cores busy 64 %, vector units 63 % of a CU's cycles: 8192^3 930 us, 1180 TFLOP/s, the library's fp16 product without scales 1371), on the e4m3 ones by the power limit and by what keeps
+ * scales in fp32 (64 and 49 %: 8192^3 468 us, 2350 TFLOP/s, the library's 2607; 2048 x 11008 x 4096 87 us).
  */
 #include "ckq_gemm_common.hpp"
 #include "ckq_int8.hpp"
@@ -153,7 +158,8 @@ __device__ __forceinline__ void f8_clear_tail(uint8_t *p, int rows, int tail, in
 /* ---- tiles on the fp16 instructions ----------------------------------------------------------------------------------- */
 
 /* WT x WN waves, each 32 TT tokens x 32 TN rows.  A step is a group of 128; its codes come to LDS as they are, eight rows of 128 bytes a copy, the chunk of 16 that a
- * lane fetches is the one that belongs in its place, c ^ (row / 2 % 8), so that a read of 16 bytes a lane meets all banks once. */
+ * lane fetches is the one that belongs in its place, c ^ (row / 2 % 8), so that a read of 16 bytes a lane meets all banks once.  Two to four blocks a CU (two, three and four of H128x128, H64x128, H64x64),
+ * each other's copies and barriers hidden: 16384 rows of 64 experts x 2816 x 2048 236 | 243 us, 4096 rows 106 | 95 (the first two). */
 template <int WT_, int WN_, int TT_, int TN_> struct F8Half {
     static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NW = WT * WN, BT = 32 * TT * WT, BN = 32 * TN * WN, S = 2;
     static constexpr int CODES = (BT + BN) * 128, STAGE = CODES + 4 * BT + 256, NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
@@ -332,7 +338,8 @@ static int launch_f8_half(const F8Args &a, hipStream_t s)
 /* ---- tiles on the e4m3 instructions ------------------------------------------------------------------------------------ */
 
 /* WT x WN waves that multiply, each 16 TT tokens x 16 TN rows; a group's product is one multiplication, 16 x 16 x 128, whose four sums a lane scales and adds while the next ones are
- * multiplied.  NP others that copy, or none (the former do it then); S stages in LDS; PERCU blocks a CU. */
+ * multiplied.  NP others that copy, or none (the former do it then); S stages in LDS; PERCU blocks a CU.  With others that copy, whose waits for the address unit hold up no multiplication, us: 512 x 11008 x
+ * 4096 36.0 -> 28.4, 1024 x 4096 x 4096 33.0 -> 22.8; eight waves of 256 x 256 leave no registers for them. */
 template <int WT_, int WN_, int TT_, int TN_, int NP_, int S_, int PERCU_> struct F8Core {
     static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NP = NP_, S = S_, PERCU = PERCU_, NW = WT * WN, WAVES = NW + NP, BT = 16 * TT * WT, BN = 16 * TN * WN, NB = (BN + 127) / 128;
     static constexpr int CODES = (BT + BN) * 128, SB = CODES + 4 * BT, STAGE = SB + 256 * NB;
@@ -551,7 +558,8 @@ static int launch_f8_core(const F8Args &a, hipStream_t s)
 /* ---- K split among the waves of a block -------------------------------------------------------------------------------- */
 
 /* 16 TG tokens x 16 RN rows a block of NW waves; every wave has all of the tile and each NW-th group of K, through S stages of its own, so that nothing is waited for
- * but its own copies until the waves' sums meet at the end, in the order of the waves. */
+ * but its own copies until the waves' sums meet at the end, in the order of the waves.  333 x 1001 x 4847, us: 16 x 32 on four waves 14.7, 32 x 32 on four 13.9, 48 x 32 on seven 11.3 (one round of the CUs),
+ * 64 x 32 on six 13.2; operands straight to registers, 16 rows x 64 bytes a load, take twice as long to come: 16.9. */
 template <int NW_, int RN_, int TG_, int S_> struct F8Split {
     static constexpr int NW = NW_, RN = RN_, TG = TG_, S = S_, BT = 16 * TG, BN = 16 * RN, CODES = (BT + BN) * 128, STAGE = CODES + 512, PITCH = BN * 4 + 16, NC = 2 * (RN + TG);
     static constexpr int LDS = NW * (S * STAGE > BT * PITCH ? S * STAGE : BT * PITCH);
