@@ -96,8 +96,8 @@ __device__ __forceinline__ bool f8_tile(const F8Args &a, int id, int BT, int nnt
     return false;
 }
 
-/* Blocks that have all tiles there can be: an expert's last tile may be one row. */
 enum { F8_LAUNCH_MOST = 1 << 23 };                              /* blocks of a launch stay below this: fewer than 2^32 threads */
+/* Tiles of rows that there can be: an expert's last one may be one row. */
 static long f8_most_tiles(int M, int experts, int BT) { return experts ? (long)M / BT + min(M, experts) : ((long)M + BT - 1) / BT; }
 static long f8_most_tiles(const F8Args &a, int BT) { return f8_most_tiles(a.M, a.offsets ? a.experts : 0, BT); }
 

@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
     store8((E *)a.out + (size_t)t * a.ldo + 8 * (size_t)v, f, left);
 }
 
-/* A block has a token, its slots four at a time: bound by the rows read and written (4096 tokens of 8 slots x 2048 in bf16, 285 MB in 59 us, 4.8 TB/s).  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
+/* A block has a token, its slots eight at a time: bound by the rows read and written (4096 tokens of 8 slots x 2048 in bf16, 285 MB in 59 us, 4.8 TB/s).  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
 template <class E, bool ONCE>
 __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
 {
@@ -185,25 +185,21 @@ __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
         for (long v = 8l * threadIdx.x; v < a.k; v += 2048) {
             const int left = (int)(a.k - v);
             const raw8<E> g = fetch8<false>(d + v, left);
+            raw8<E> y[8];
 #pragma unroll
-            for (int h = 0; h < 8; h += 4) {
-                if (j0 + h >= a.choices) break;
-                raw8<E> y[4];
+            for (int j = 0; j < 8; ++j)
+                if (j0 + j < a.choices) y[j] = fetch8<ONCE>((const E *)a.y + (size_t)((u32)p[j] < (u32)a.rows ? p[j] : 0) * a.ldy + v, left);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j0 + h + j < a.choices) y[j] = fetch8<ONCE>((const E *)a.y + (size_t)((u32)p[h + j] < (u32)a.rows ? p[h + j] : 0) * a.ldy + v, left);
+            for (int j = 0; j < 8; ++j)
+                if ((u32)p[j] < (u32)a.rows) {
+                    float f[8];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if ((u32)p[h + j] < (u32)a.rows) {
-                        float f[8];
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            sum[h + j] = __builtin_fmaf(raw_value<E>(g, c), raw_value<E>(y[j], c), sum[h + j]);
-                            f[c] = w[h + j] * raw_value<E>(g, c);
-                        }
-                        store8<E, ONCE>((E *)a.out + (size_t)p[h + j] * a.ldo + v, f, left);
+                    for (int c = 0; c < 8; ++c) {
+                        sum[j] = __builtin_fmaf(raw_value<E>(g, c), raw_value<E>(y[j], c), sum[j]);
+                        f[c] = w[j] * raw_value<E>(g, c);
                     }
-            }
+                    store8<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + v, f, left);
+                }
         }
         if (j0) __syncthreads();
 #pragma unroll
