@@ -119,21 +119,25 @@ __device__ __forceinline__ void moe_places(const MoeArgs &a, size_t t, F &&use)
     }
 }
 
+/* Where a thread's eight elements begin: a row's last thread has its last eight, some of which the one before has too (the same values), so that none has loads of its own. */
+__device__ __forceinline__ long moe_at(const MoeArgs &a, u32 v) { return max(0l, min(8 * (long)v, (long)a.k - 8)); }
+
 /* Eight elements a thread.  Bound by the rows it writes (8192 tokens of 8 slots x 2048 in bf16: 302 MB in 52 us, 5.8 TB/s).  ONCE here and in the backward pass: what is written leaves non-temporally (moe_past_cache). */
 template <class E, bool ONCE>
 __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
 {
     const u32 i = blockIdx.x * 256 + threadIdx.x, t = i / nvec, v = i - t * nvec;
     if (t >= (u32)a.tokens) return;
-    const int left = a.k - 8 * (int)v;
-    const raw8<E> r = fetch8<false>((const E *)a.x + (size_t)t * a.ldx + 8 * (size_t)v, left);
+    const long at = moe_at(a, v);
+    const int left = (int)(a.k - at);
+    const raw8<E> r = fetch8<false>((const E *)a.x + (size_t)t * a.ldx + at, left);
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = raw_value<E>(r, j);
     moe_places(a, t, [&](int, const int (&p)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if ((u32)p[j] < (u32)a.rows) store8<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + 8 * (size_t)v, f, left);
+            if ((u32)p[j] < (u32)a.rows) store8<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + at, f, left);
     });
 }
 
@@ -144,8 +148,9 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
 {
     const u32 i = blockIdx.x * 256 + threadIdx.x, t = i / nvec, v = i - t * nvec;
     if (t >= (u32)a.tokens) return;
-    const int left = a.k - 8 * (int)v;
-    const E *y = (const E *)a.x + 8 * (size_t)v;
+    const long at = moe_at(a, v);
+    const int left = (int)(a.k - at);
+    const E *y = (const E *)a.x + at;
     float f[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) f[j] = 0.0f;
@@ -164,7 +169,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
                 for (int c = 0; c < 8; ++c) f[c] = __builtin_fmaf(w[j], raw_value<E>(r[j], c), f[c]);
             }
     });
-    store8((E *)a.out + (size_t)t * a.ldo + 8 * (size_t)v, f, left);
+    store8((E *)a.out + (size_t)t * a.ldo + at, f, left);
 }
 
 /* A block has a token, its slots eight at a time: bound by the rows read and written (4096 tokens of 8 slots x 2048 in bf16, 285 MB in 59 us, 4.8 TB/s).  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
