@@ -807,24 +807,24 @@ typedef F8Split<2, 2, 1, 2> S16x32w2;
 typedef F8Split<8, 1, 1, 2> S16x16;
 typedef F8Core<2, 4, 8, 4, 0, 2, 1> C256x256;
 typedef F8Core<4, 2, 4, 4, 4, 3, 1> C256x128;
-typedef F8Core<2, 2, 4, 6, 4, 3, 1> C128x192;            /* in two sizes of tiles */
+typedef F8Core<2, 2, 4, 6, 4, 3, 1> C128x192;
 typedef F8Core<2, 2, 4, 4, 4, 4, 1> C128x128;
 typedef F8Core<2, 2, 2, 4, 4, 4, 1> C64x128;
 typedef F8Core<2, 2, 2, 2, 4, 4, 2> C64x64;
 
 /* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all places have a block; in a last round of fewer blocks less, `share` of it by how
- * many share a CU, the rest by how many there are in all, but no less than a block alone takes, `alone`.  Fitted to 700 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three
- * sets in turn): the kernel so chosen is 0.8 % (fp32 results) and 0.7 % (16 bits) slower than the fastest on average, 1.3 times at worst, as much on one half of them when fitted to the other; over experts (500
- * random products, 2 to 128 of them, none of which it was fitted to) 1.6 % and 1.4 times. */
+ * many share a CU, the rest by how many there are in all, but no less than a block alone takes, `alone`.  Fitted to 800 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three
+ * sets in turn): the kernel so chosen is 0.8 % (fp32 results) and 0.7 % (16 bits) slower than the fastest on average, 1.2 times at worst, as much on one half of them when fitted to the other; over experts (500
+ * random products, 2 to 128 of them, none of which it was fitted to) 1.8 % and 1.4 times. */
 struct F8Cost { int bt, bn, places, split; float t0, t_tile, step, share, alone; };
 static const F8Cost f8_costs[CKQ_F8_TILINGS] = {
-    {128, 128, 512, 1, 0.44f, 5.74f, 1.950f, 0.95f, 0.39f}, {64, 128, 768, 1, 1.41f, 3.54f, 1.673f, 1.00f, 0.44f}, {64, 64, 1024, 1, 1.68f, 2.54f, 1.373f, 1.00f, 0.39f},
-    {48, 32, 256, 7, 2.22f, 2.31f, 1.029f, 0.79f, 0.0f},    {32, 32, 512, 4, 2.15f, 1.96f, 0.818f, 1.00f, 0.68f},  {16, 32, 256, 8, 1.86f, 1.88f, 0.702f, 0.76f, 0.0f},
-    {16, 32, 768, 4, 2.36f, 1.42f, 0.877f, 1.00f, 0.52f},   {16, 32, 1536, 2, 2.07f, 1.62f, 0.871f, 1.00f, 0.53f}, {16, 16, 512, 8, 2.17f, 1.45f, 0.732f, 1.00f, 0.39f},
-    {256, 256, 256, 1, 0.00f, 8.08f, 1.888f, 0.66f, 0.0f},  {256, 128, 256, 1, 0.00f, 6.92f, 0.928f, 0.66f, 0.0f}, {128, 128, 256, 1, 1.48f, 4.77f, 0.585f, 0.68f, 0.0f},
-    {64, 128, 256, 1, 1.89f, 3.09f, 0.403f, 0.69f, 0.0f},   {64, 64, 512, 1, 2.01f, 2.29f, 0.428f, 1.00f, 0.56f},
+    {128, 128, 512, 1, 1.48f, 5.25f, 1.886f, 0.90f, 0.28f}, {64, 128, 768, 1, 1.41f, 3.69f, 1.596f, 1.00f, 0.45f}, {64, 64, 1024, 1, 1.78f, 2.53f, 1.301f, 1.00f, 0.40f},
+    {48, 32, 256, 7, 1.99f, 2.53f, 0.976f, 0.86f, 0.0f},    {32, 32, 512, 4, 2.00f, 2.14f, 0.743f, 1.00f, 0.72f},  {16, 32, 256, 8, 1.95f, 1.86f, 0.662f, 0.78f, 0.0f},
+    {16, 32, 768, 4, 2.27f, 1.53f, 0.809f, 1.00f, 0.56f},   {16, 32, 1536, 2, 2.02f, 1.69f, 0.828f, 1.00f, 0.54f}, {16, 16, 512, 8, 2.07f, 1.57f, 0.654f, 1.00f, 0.57f},
+    {256, 256, 256, 1, 0.00f, 8.83f, 1.854f, 0.64f, 0.0f},  {256, 128, 256, 1, 0.00f, 7.22f, 0.895f, 0.65f, 0.0f}, {128, 128, 256, 1, 1.51f, 4.98f, 0.562f, 0.68f, 0.0f},
+    {64, 128, 256, 1, 1.73f, 3.30f, 0.374f, 0.73f, 0.0f},   {64, 64, 512, 1, 1.92f, 2.40f, 0.404f, 1.00f, 0.58f},  {128, 192, 256, 1, 1.28f, 6.69f, 0.720f, 0.70f, 0.0f},
 };
-static const F8Cost f8_cost_rest = {128, 192, 256, 1, 0.00f, 10.79f, 0.505f, 0.84f, 0.0f};
+static const F8Cost f8_cost_rest = {128, 192, 256, 1, 0.00f, 11.29f, 0.486f, 0.95f, 0.0f};         /* beside tiles of 256 x 256 */
 
 static float f8_rounds(const F8Cost &c, float tiles, int K)
 {
@@ -906,6 +906,7 @@ static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
     case CKQ_F8_C128x128:    return launch_f8_core<E, C128x128>(a, s);
     case CKQ_F8_C64x128:     return launch_f8_core<E, C64x128>(a, s);
     case CKQ_F8_C64x64:      return launch_f8_core<E, C64x64>(a, s);
+    case CKQ_F8_C128x192:    return launch_f8_core<E, C128x192>(a, s);
     case CKQ_F8_TWO:         return launch_f8_two<E, C256x256, C128x192>(a, f8_whole_columns(a.M, a.N), s);
     case CKQ_F8_STREAM:      return launch_f8_stream<E>(a, s);
     default:                 break;

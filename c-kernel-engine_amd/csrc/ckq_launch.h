@@ -189,7 +189,7 @@ int ckq_launch_gemm_f8_experts(const uint8_t *A, long lda, const float *sa, long
  * with K split among a block's waves, w8, w7, w2: eight, seven or two of them) or on the e4m3 ones (C), two sizes of the latter in a launch, or the rows streamed; -1: in parts, since no launch has so many blocks.  Host arithmetic; exported for the test of the
  * rules. */
 enum { CKQ_F8_H128x128, CKQ_F8_H64x128, CKQ_F8_H64x64, CKQ_F8_S48x32w7, CKQ_F8_S32x32, CKQ_F8_S16x32w8, CKQ_F8_S16x32, CKQ_F8_S16x32w2, CKQ_F8_S16x16, CKQ_F8_C256x256, CKQ_F8_C256x128,
-       CKQ_F8_C128x128, CKQ_F8_C64x128, CKQ_F8_C64x64, CKQ_F8_TILINGS, CKQ_F8_TWO = CKQ_F8_TILINGS, CKQ_F8_STREAM };
+       CKQ_F8_C128x128, CKQ_F8_C64x128, CKQ_F8_C64x64, CKQ_F8_C128x192, CKQ_F8_TILINGS, CKQ_F8_TWO = CKQ_F8_TILINGS, CKQ_F8_STREAM };
 int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts);
 /* -1 = by shape (default), else that kernel wherever it can take the product, in all calls of the process. */
 void ckq_launch_set_f8_kernel(int kernel);

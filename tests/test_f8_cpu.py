@@ -183,18 +183,18 @@ def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
 def test_kernel_of_a_matmul(L):
     """One token streams; fp32 results and experts stay on the fp16 instructions; every kernel has its sizes."""
     k = L.ckq_launch_f8_kernel
-    assert all(k(t, 1, N, K, 0) == 15 for t in (F32, BF16, F16) for N in (1, 5000, 151936) for K in (1, 896, 131072))
+    assert all(k(t, 1, N, K, 0) == 16 for t in (F32, BF16, F16) for N in (1, 5000, 151936) for K in (1, 896, 131072))
     Ms, Ns, Ks = (2, 5, 12, 16, 17, 40, 64, 100, 128, 200, 333, 512, 800, 1024, 1500, 2048, 5000, 1 << 19), (1, 64, 200, 512, 896, 1001, 1504, 2048, 3500, 4096, 4864, 8000, 11008, 17000, 28000, 151936), \
         (1, 64, 200, 512, 896, 1500, 2048, 4096, 4847, 11008, 131071)
     seen = {t: {k(t, M, N, K, 0) for M in Ms for N in Ns for K in Ks} for t in (F32, BF16)}
     experts = {k(t, M, N, K, E) for t in (F32, F16) for M in Ms + (1,) for N in Ns for K in Ks for E in (1, 2, 8, 60, 256)}
-    assert seen[F32] == set(range(9)) and experts <= set(range(9)) and seen[F32] | seen[BF16] | experts == set(range(15))
+    assert seen[F32] == set(range(9)) and experts <= set(range(9)) and seen[F32] | seen[BF16] | experts == set(range(16))
     assert k(F32, 1 << 22, 151936, 64, 0) == k(BF16, 1, 1 << 30, 64, 0) == k(BF16, 1 << 29, 4096, 64, 8) == -1          # in parts
     assert 0 <= k(F32, 1 << 29, 16, 64, 1 << 15) < 9
-    assert k(BF16, 2048, 11008, 4096, 0) == 14                # 344 tiles of 256 x 256: 256 of them, the rest smaller
+    assert k(BF16, 2048, 11008, 4096, 0) == 15                # 344 tiles of 256 x 256: 256 of them, the rest smaller
     assert k(BF16, 2048, 8192, 4096, 0) == 9                  # one round of them
-    for forced in range(16):
+    for forced in range(17):
         L.ckq_launch_set_f8_kernel(forced)
-        assert k(BF16, 2048, 11008, 4096, 0) == (forced if forced != 15 else 14)
-        assert k(BF16, 2048, 11008, 4096, 8) in ((forced,) if forced < 14 else range(9))
+        assert k(BF16, 2048, 11008, 4096, 0) == (forced if forced != 16 else 15)
+        assert k(BF16, 2048, 11008, 4096, 8) in ((forced,) if forced < 15 else range(9))
     L.ckq_launch_set_f8_kernel(-1)

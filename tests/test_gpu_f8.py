@@ -425,8 +425,8 @@ def test_experts(t, M, N, K, counts):
         check_experts(out, a, sa, b, sb, offsets, bias)
 
 
-KERNELS = range(16)             # CKQ_F8_* of ckq_launch.h
-CORES = range(9, 15)              # those on the e4m3 instructions
+KERNELS = range(17)             # CKQ_F8_* of ckq_launch.h
+CORES = range(9, 16)              # those on the e4m3 instructions
 
 
 @pytest.fixture
