@@ -33,6 +33,8 @@ struct F8RowsArgs {
 };
 
 struct __attribute__((packed, aligned(1))) row16f8 { u32 v[4]; };
+typedef u32 __attribute__((aligned(1))) u32_at_1;
+typedef uint16_t __attribute__((aligned(1))) u16_at_1;
 
 /* Sixteen values of a group, a' and 448 * 2^-e of it: their codes. */
 __device__ __forceinline__ row16f8 f8_codes(const float (&v)[16], float a1, float c, bool finite)
@@ -57,7 +59,7 @@ __device__ __forceinline__ row16f8 f8_codes(const float (&v)[16], float a1, floa
 
 /* Eight lanes have a group, sixteen elements each; a block has 2^rs rows beside each other and 32 >> rs groups of each: a row's codes leave in whole lines, a group's scales side by side.  Bound by memory:
  * 2048 x 11008 in bf16 68 MB in 15.4 us (4.4 TB/s), few rows by a launch (2). */
-template <int OP, class E>
+template <int OP, class E, bool EIGHT>
 __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 group_tiles)
 {
     const u32 rt = blockIdx.x / group_tiles, gt = blockIdx.x - rt * group_tiles;
@@ -73,17 +75,27 @@ __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 
         for (int j = 0; j < 8; ++j) to[j] = a.position[(size_t)row * a.choices + min(j, a.choices - 1)];
     }
     constexpr bool ONCE = OP != F8_GATHER;
-    raw8<E> r0 = fetch8<ONCE>(x, left), r1 = fetch8<ONCE>(x + 8, left - 8);
+    raw8<E> r0 = fetch8_of<ONCE, EIGHT>(x, left), r1 = fetch8_of<ONCE, EIGHT>(x + 8, left - 8);
     float v[16];
     if (OP == F8_SWIGLU) {
         const E *y = (const E *)a.y + (size_t)row * a.ldx + at;
-        const raw8<E> u0 = fetch8<ONCE>(y, left), u1 = fetch8<ONCE>(y + 8, left - 8);
+        raw8<E> u0 = fetch8_of<ONCE, EIGHT>(y, left), u1 = fetch8_of<ONCE, EIGHT>(y + 8, left - 8);
+        if (left < 16) {
+            drop_rest<EIGHT>(r0, left);
+            drop_rest<EIGHT>(r1, left - 8);
+            drop_rest<EIGHT>(u0, left);
+            drop_rest<EIGHT>(u1, left - 8);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             v[i] = row_swiglu(raw_value<E>(r0, i), raw_value<E>(u0, i));
             v[i + 8] = row_swiglu(raw_value<E>(r1, i), raw_value<E>(u1, i));
         }
     } else {
+        if (left < 16) {
+            drop_rest<EIGHT>(r0, left);
+            drop_rest<EIGHT>(r1, left - 8);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             v[i] = raw_value<E>(r0, i);
@@ -104,10 +116,25 @@ __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 
     auto put = [&](int to) {
         uint8_t *q = a.q + (size_t)to * a.ldq + at;
         if (left >= 16) *reinterpret_cast<row16f8 *>(q) = o;
-        else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (i < left) q[i] = (uint8_t)(o.v[i >> 2] >> (8 * (i & 3)));
+        else if (left > 0) {                                   /* eight, four, two and one */
+            u32 v0 = o.v[0], v1 = o.v[1];
+            if (left & 8) {
+                *reinterpret_cast<row8q *>(q) = row8q{{v0, v1}};
+                v0 = o.v[2];
+                v1 = o.v[3];
+                q += 8;
+            }
+            if (left & 4) {
+                *reinterpret_cast<u32_at_1 *>(q) = v0;
+                v0 = v1;
+                q += 4;
+            }
+            if (left & 2) {
+                *reinterpret_cast<u16_at_1 *>(q) = (uint16_t)v0;
+                v0 >>= 16;
+                q += 2;
+            }
+            if (left & 1) *q = (uint8_t)v0;
         }
         if (l == 0) a.scale[(size_t)g * a.lds + to] = scale;
     };
@@ -142,7 +169,7 @@ static int launch_rows_f8(F8RowsArgs a, hipStream_t s)
     for (int rows = a.rows;;) {
         const int now = min(rows, most);
         a.rows = now;
-        const int rc = i8_launch(rows_f8_kernel<OP, E>, dim3((u32)((now + (1 << rs) - 1) >> rs) * group_tiles), dim3(256), s, a, rs, group_tiles);
+        const int rc = i8_launch(a.k >= 8 ? rows_f8_kernel<OP, E, true> : rows_f8_kernel<OP, E, false>, dim3((u32)((now + (1 << rs) - 1) >> rs) * group_tiles), dim3(256), s, a, rs, group_tiles);
         if (rc || rows == now) return rc;
         rows -= now;
         a.x = (const E *)a.x + (size_t)now * a.ldx;

@@ -10,6 +10,8 @@ template <> struct RowType<CKQ_T_F16>  { typedef _Float16 type; };
 
 /* Eight consecutive elements; rows start anywhere an element can (the loads and stores take that as they are). */
 template <class E> struct __attribute__((packed, aligned(sizeof(E)))) row8 { E v[8]; };
+template <class E> struct __attribute__((packed, aligned(sizeof(E)))) row4 { E v[4]; };
+template <class E> struct __attribute__((packed, aligned(sizeof(E)))) row2 { E v[2]; };
 struct __attribute__((packed, aligned(1))) row8q { u32 v[2]; };
 
 /* The same as loaded, in whole registers. */
@@ -57,6 +59,23 @@ __device__ __forceinline__ void drop_first(raw8<E> &r, int drop)
             for (int i = 0; i < N; ++i) r.w[i] = i + by < N ? r.w[i + by] : 0u;
         }
 }
+/* The same as fetch8; EIGHT: of a row of at least eight elements, without a branch and loads of their own for its last: the row's last eight, those before them dropped (drop_rest). */
+template <bool ONCE, bool EIGHT, class E>
+__device__ __forceinline__ raw8<E> fetch8_of(const E *p, int left)
+{
+    return EIGHT ? fetch8<ONCE>(p + min(0, left - 8), 8) : fetch8<ONCE>(p, left);
+}
+template <bool EIGHT, class E>
+__device__ __forceinline__ void drop_rest(raw8<E> &r, int left)
+{
+    if (EIGHT && left < 8) {
+        drop_first(r, min(8 - left, 7));
+        if (left <= 0) {
+#pragma unroll
+            for (int i = 0; i < 2 * (int)sizeof(E); ++i) r.w[i] = 0;
+        }
+    }
+}
 template <class E>
 __device__ __forceinline__ float raw_value(const raw8<E> &r, int i)
 {
@@ -77,10 +96,22 @@ __device__ __forceinline__ void store8(E *p, const float (&f)[8], int left)
         } else
             *reinterpret_cast<row8<E> *>(p) = r;
         asm volatile("");                                    /* or what both branches store is moved behind them, in pieces */
-    } else {
+    } else if (left > 0) {                                   /* four, two and one */
+        E e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = (E)f[i];
+        for (int i = 0; i < 8; ++i) e[i] = (E)f[i];
+        if (left & 4) {
+            *reinterpret_cast<row4<E> *>(p) = row4<E>{{e[0], e[1], e[2], e[3]}};
+            p += 4;
+#pragma unroll
+            for (int i = 0; i < 3; ++i) e[i] = e[i + 4];
+        }
+        if (left & 2) {
+            *reinterpret_cast<row2<E> *>(p) = row2<E>{{e[0], e[1]}};
+            p += 2;
+            e[0] = e[2];
+        }
+        if (left & 1) *p = e[0];
     }
 }
 
