@@ -74,12 +74,11 @@ __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 
 #pragma unroll
         for (int j = 0; j < 8; ++j) to[j] = a.position[(size_t)row * a.choices + min(j, a.choices - 1)];
     }
-    constexpr bool ONCE = OP != F8_GATHER;
-    raw8<E> r0 = fetch8_of<ONCE, EIGHT>(x, left), r1 = fetch8_of<ONCE, EIGHT>(x + 8, left - 8);
+    raw8<E> r0 = fetch8_of<EIGHT>(x, left), r1 = fetch8_of<EIGHT>(x + 8, left - 8);
     float v[16];
     if (OP == F8_SWIGLU) {
         const E *y = (const E *)a.y + (size_t)row * a.ldx + at;
-        raw8<E> u0 = fetch8_of<ONCE, EIGHT>(y, left), u1 = fetch8_of<ONCE, EIGHT>(y + 8, left - 8);
+        raw8<E> u0 = fetch8_of<EIGHT>(y, left), u1 = fetch8_of<EIGHT>(y + 8, left - 8);
         if (left < 16) {
             drop_rest<EIGHT>(r0, left);
             drop_rest<EIGHT>(r1, left - 8);

@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
 }
 
 /* Eight elements a thread, the rows of eight slots on their way together (one token of 8 slots x 2048 6.8 us one after the other, 3.7 together), non-temporally, being read for the last
- * time, which leaves the caches to what is beside them (with a gather before it, 8192 tokens of 8 slots x 2048 in bf16 132 -> 115 us; alone 52, 5.8 TB/s). */
+ * time, which leaves the caches to what is beside them (with a gather before it, 8192 tokens of 8 slots x 2048 in bf16 132 -> 115 us; alone 52, 5.8 TB/s); fp32 not, whose loads take half a line each (119 -> 116). */
 template <class E>
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
 {
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
         for (int j = 0; j < 8; ++j) w[j] = a.w && j0 + j < a.choices ? a.w[(size_t)t * a.choices + j0 + j] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if (j0 + j < a.choices) r[j] = fetch8<true>(y + (size_t)((u32)p[j] < (u32)a.rows ? p[j] : 0) * a.ldx, left);
+            if (j0 + j < a.choices) r[j] = fetch8<sizeof(E) == 2>(y + (size_t)((u32)p[j] < (u32)a.rows ? p[j] : 0) * a.ldx, left);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
             if ((u32)p[j] < (u32)a.rows) {
@@ -239,19 +239,24 @@ static int moe_each(MoeArgs a, bool out_by_token, size_t threads, L &&launch)
 }
 
 /* Whether what is written, a row for each slot, is more than the 256 MB cache holds beside the rest: then it leaves non-temporally, and its reader finds it in memory either way.  us, kept | not: gather and
- * the combine of its rows, bf16 x 2048, 67 MB 25.6 | 28.5, 134 MB 47.0 | 51.7, 252 MB 115 | 100; the backward pass and the combine of its rows, 134 MB 73.0 | 80.6. */
-static bool moe_past_cache(const MoeArgs &a, size_t size) { return (size_t)a.tokens * a.choices * a.k * size > (size_t)192 << 20; }
+ * the combine of its rows, bf16 x 2048, 67 MB 25.6 | 28.5, 134 MB 47.0 | 51.7, 252 MB 115 | 100; the backward pass and the combine of its rows, 134 MB 73.0 | 80.6.  Not where a line leaves in pieces, that memory
+ * would get one by one: fp32, whose threads store two pieces of 32 bytes one after the other (gather and combine of 537 MB 257 | 360, backward and combine of rows x 2047 364 | 383), and gather's rows that do not begin at 16
+ * bytes (bf16 x 2047 126 | 137). */
+static bool moe_past_cache(const MoeArgs &a, size_t size, bool gather)
+{
+    return size == 2 && (size_t)a.tokens * a.choices * a.k * size > (size_t)192 << 20 && !(gather && ((uintptr_t)a.out % 16 || a.ldo % 8));
+}
 
 enum { MOE_GATHER, MOE_COMBINE, MOE_BACKWARD };
 template <int OP, class E>
 static int launch_moe(const MoeArgs &a, hipStream_t s)
 {
     const u32 nvec = (u32)(a.k / 8 + (a.k % 8 != 0));
-    const bool once = moe_past_cache(a, sizeof(E));
+    const bool once = moe_past_cache(a, sizeof(E), OP == MOE_GATHER);
     return moe_each<E>(a, OP == MOE_COMBINE, OP == MOE_BACKWARD ? 256 : nvec, [&](const MoeArgs &b) {
-        if (OP == MOE_BACKWARD) return i8_launch(once ? moe_combine_backward_kernel<E, true> : moe_combine_backward_kernel<E, false>, dim3((u32)b.tokens), dim3(256), s, b);
+        if (OP == MOE_BACKWARD) return i8_launch(once ? moe_combine_backward_kernel<E, sizeof(E) == 2> : moe_combine_backward_kernel<E, false>, dim3((u32)b.tokens), dim3(256), s, b);
         const dim3 grid((u32)(((size_t)b.tokens * nvec + 255) / 256));
-        return i8_launch(OP == MOE_COMBINE ? moe_combine_kernel<E> : once ? moe_gather_kernel<E, true> : moe_gather_kernel<E, false>, grid, dim3(256), s, b, nvec);
+        return i8_launch(OP == MOE_COMBINE ? moe_combine_kernel<E> : once ? moe_gather_kernel<E, sizeof(E) == 2> : moe_gather_kernel<E, false>, grid, dim3(256), s, b, nvec);
     });
 }
 template <int OP>

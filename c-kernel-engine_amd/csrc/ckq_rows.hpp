@@ -60,10 +60,10 @@ __device__ __forceinline__ void drop_first(raw8<E> &r, int drop)
         }
 }
 /* The same as fetch8; EIGHT: of a row of at least eight elements, without a branch and loads of their own for its last: the row's last eight, those before them dropped (drop_rest). */
-template <bool ONCE, bool EIGHT, class E>
+template <bool EIGHT, class E>
 __device__ __forceinline__ raw8<E> fetch8_of(const E *p, int left)
 {
-    return EIGHT ? fetch8<ONCE>(p + min(0, left - 8), 8) : fetch8<ONCE>(p, left);
+    return EIGHT ? fetch8<false>(p + min(0, left - 8), 8) : fetch8<false>(p, left);
 }
 template <bool EIGHT, class E>
 __device__ __forceinline__ void drop_rest(raw8<E> &r, int left)
