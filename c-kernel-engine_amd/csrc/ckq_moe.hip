@@ -21,7 +21,7 @@
 /* A block has an expert, the last one what has none.  Each goes through all slots: it counts those that belong before its own, and its own in each wave's run of slots, whose
  * places follow from that; then it writes its own.  No scratch memory, one launch, and the slots' order is kept without a sort.  A wave takes 64 NV slots at a time into
  * registers, one a lane and load; what it has compared it counts in scalar registers, two vector instructions a slot.  Runs of up to 64 NV slots are read once.  65536 slots of
- * 128 experts, us: one slot a lane and load, a load at a time, 41.6; four a lane, counted in vector registers, 19.8; this 11 (16384 of 64 5.5, 8 slots 3.0: a launch). */
+ * 128 experts, us: one slot a lane and load, a load at a time, 41.6; four a lane, counted in vector registers, 19.8; this 11 to 13 (16384 of 64 5.5, 8 slots 3.0: a launch), of which most are the instructions of both passes. */
 template <int NV>
 __global__ void __launch_bounds__(1024) moe_sort_kernel(const int32_t *__restrict__ ids, int slots, int run, int experts, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
                                                         int32_t *__restrict__ position)
@@ -90,7 +90,9 @@ extern "C" int ckq_launch_moe_sort(const int32_t *ids, int tokens, int choices, 
     const dim3 grid((u32)experts + 1);
     const hipStream_t s = (hipStream_t)stream;
     if (slots <= 4096) return i8_launch(moe_sort_kernel<4>, grid, dim3(64u * (u32)((slots - 1) / 256 + 1)), s, ids, slots, 256, experts, offsets, order, position);
-    return i8_launch(slots <= 16384 ? moe_sort_kernel<16> : moe_sort_kernel<64>, grid, dim3(1024), s, ids, slots, run, experts, offsets, order, position);
+    /* Read once where sixteen waves hold all slots and a CU has one block; else twice, by blocks of which a CU has two.  us, once | twice: 65536 slots of 128 experts 10.9 | 11.9, of 256 14.6 | 11.5, 262144 of 128
+     * (either way twice) 36.7 | 35.4. */
+    return i8_launch(slots > 16384 && slots <= 65536 && experts < 256 ? moe_sort_kernel<64> : moe_sort_kernel<16>, grid, dim3(1024), s, ids, slots, run, experts, offsets, order, position);
 }
 
 /* ---- rows there and back ------------------------------------------------------------------------------------------- */

@@ -326,12 +326,13 @@ int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t 
  * ckq_dequantize_f8_dev: y = scale * q, rounded to the type.
  * ckq_swiglu_f8_dev: gate / (1 + exp(-gate)) * up in 8 bits as above (the function as exact as ckq_swiglu_i8_dev's); gate and up have one pitch, ld.
  * ckq_gemm_nt_f8_dev: C[m*ldc + n] = sum over groups g of (sa[g*ldsa + m] * sb[(n/128)*ldsb + g]) * (sum over k in g of A[m][k] * B[n][k]) (+ bias[n]), in
- * fp32, rounded once to the type of C.  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are, multiples of 16 bytes, pitches at
+ * fp32, rounded once to the type of C (of 16 bits: the matrix instructions may drop what is under 2^-13 of the largest of eight products, 1.5e-5 of a sum of 128 random ones).  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are, multiples of 16 bytes, pitches at
  * most 4 MiB (else CKQ_EROWS).  K may be any number: of the 16 bytes that hold a row's last, those behind it may be read and are not used.  The gradient of the
  * activations is the same product with the transposed codes and scales of the weights.
  * ckq_gemm_nt_f8_experts_dev: the same of rows sorted by expert, each expert with a matrix, scales and bias of its own: rows offsets[e] .. offsets[e + 1] - 1 of A and C
  * with B + e * eb, sb + e * esb and bias + e * N (eb a multiple of 16).  offsets are on the device, experts + 1 of them, from 0 on and none less than the one before
- * (what lies outside 0 .. M counts as the nearest of these, and M is at most 2^29); an expert may have no rows, and rows of C that no expert has stay as they are. */
+ * (what lies outside 0 .. M counts as the nearest of these, and M is at most 2^29); an expert may have no rows, and rows of C that no expert has stay as they are.  Sums
+ * are fp32's whatever the type of C. */
 int ckq_quantize_f8_dev(ckq_ck_dtype type, const void *x, long ldx, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
 int ckq_dequantize_f8_dev(const uint8_t *q, long ldq, const float *scale, long lds, ckq_ck_dtype type, void *y, long ldy, int rows, int k, void *stream);
 int ckq_swiglu_f8_dev(ckq_ck_dtype type, const void *gate, const void *up, long ld, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);

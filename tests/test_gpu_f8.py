@@ -569,7 +569,7 @@ def sorted_slots(ids, E):
     return np.concatenate([[0], np.cumsum(np.bincount(key, minlength=E + 1)[:E])]), order, position.reshape(ids.shape)
 
 
-@pytest.mark.parametrize("T,c,E", [(1, 1, 1), (1, 8, 64), (3, 2, 2), (7, 6, 64), (63, 1, 5), (64, 4, 3), (65, 4, 256), (129, 2, 7), (300, 7, 16), (1000, 3, 100), (2049, 8, 128), (5000, 8, 4), (20000, 6, 60)])
+@pytest.mark.parametrize("T,c,E", [(1, 1, 1), (1, 8, 64), (3, 2, 2), (7, 6, 64), (63, 1, 5), (64, 4, 3), (65, 4, 256), (129, 2, 7), (300, 7, 16), (1000, 3, 100), (2049, 8, 128), (5000, 8, 4), (9000, 2, 300), (20000, 6, 60)])
 def test_sort(T, c, E):
     for none in (0.0, 0.1, 1.0):
         ids = random_ids(T, c, E, T + E, none)
