@@ -252,8 +252,8 @@ __global__ void __launch_bounds__(256) dequantize_f8_kernel(const uint8_t *__res
         f[i >> 1][4 * (i & 1) + 2] = s * hi[0];
         f[i >> 1][4 * (i & 1) + 3] = s * hi[1];
     }
-    store8(o, f[0], left);
-    if (left > 8) store8(o + 8, f[1], left - 8);
+    store8_pieces(o, f[0], left);
+    if (left > 8) store8_pieces(o + 8, f[1], left - 8);
 }
 
 extern "C" int ckq_launch_dequantize_f8(const uint8_t *q, long ldq, const float *scale, long lds, int type, void *y, long ldy, int rows, int k, void *stream)

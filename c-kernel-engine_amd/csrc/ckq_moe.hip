@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
     moe_places(a, t, [&](int, const int (&p)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-            if ((u32)p[j] < (u32)a.rows) store8<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + at, f, left);
+            if ((u32)p[j] < (u32)a.rows) store8_pieces<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + at, f, left);
     });
 }
 
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
                 for (int c = 0; c < 8; ++c) f[c] = __builtin_fmaf(w[j], raw_value<E>(r[j], c), f[c]);
             }
     });
-    store8((E *)a.out + (size_t)t * a.ldo + at, f, left);
+    store8_pieces((E *)a.out + (size_t)t * a.ldo + at, f, left);
 }
 
 /* A block has a token, its slots eight at a time: bound by the rows read and written (4096 tokens of 8 slots x 2048 in bf16, 285 MB in 58 us, 4.9 TB/s).  What vectors of eight leave of a row is read and written an element a lane, beside them: 93 tokens of 8 slots x 1001 in fp32 8.6 -> 6.0 us, 2048 of 8 x 2047 in bf16 50 -> 37.  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
                         sum[j] = __builtin_fmaf(raw_value<E>(g, c), raw_value<E>(y[j], c), sum[j]);
                         f[c] = w[j] * raw_value<E>(g, c);
                     }
-                    store8<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + v, f, 8);
+                    store_eight<E, ONCE>((E *)a.out + (size_t)p[j] * a.ldo + v, f);
                 }
         }
         if (j0) __syncthreads();
