@@ -484,6 +484,49 @@ def test_matmul_launches_in_parts(kernel):
         del out, aw, bw
 
 
+def test_experts_without_rows_and_as_many_experts_as_there_can_be():
+    a, sa, b, sb = codes(7, 300, 1), side(7, 300, 2), codes(50, 300, 3), blocks(50, 300, 4, 4)
+    out = torch.full((7, 50), 3.0, device="cuda")
+    P.dev_gemm_nt_f8_experts(a, sa, b[None].expand(4, -1, -1), sb, torch.zeros(5, dtype=torch.int32, device="cuda"), out=out)
+    assert (out == 3).all()
+    E, T = 65535, 3000
+    g = torch.Generator(device="cuda").manual_seed(1)
+    ids = torch.randint(0, E, (T, 2), device="cuda", dtype=torch.int32, generator=g)
+    ids[5], ids[6, 0] = E - 1, E
+    offsets, order, position = P.dev_moe_sort(ids, E)
+    key = ids.flatten().long()
+    key, slots = torch.sort(key, stable=True)
+    n = int((key < E).sum())
+    assert n == 2 * T - 1 and torch.equal(order[:n].long(), slots[:n]) and (order[n:] == -1).all()
+    assert torch.equal(offsets.long(), torch.searchsorted(key, torch.arange(E + 1, device="cuda")))
+    # whole numbers, scales that are powers of two: exact
+    b = torch.randint(-4, 5, (E, 16, 32), device="cuda", generator=g).float()
+    x = torch.randint(-4, 5, (T, 32), device="cuda", generator=g).to(F8)
+    rows = torch.zeros(2 * T, 32, device="cuda", dtype=torch.uint8)
+    rows[:n] = x.view(torch.uint8)[slots[:n] // 2]
+    y = P.dev_gemm_nt_f8_experts(rows.view(F8), torch.full((1, 2 * T), 2.0, device="cuda").t(), b.to(F8), torch.full((E, 1, 1), 0.5, device="cuda"), offsets)
+    assert torch.equal(y[:n], (b[key[:n]] * rows[:n].view(F8).float()[:, None]).sum(2))
+
+
+def test_a_hundred_choices_with_the_gradient_in_place():
+    T, c, k = 50, 100, 77
+    g = torch.Generator(device="cuda").manual_seed(2)
+    position = torch.randperm(T * c, device="cuda", generator=g).int().view(T, c)
+    position[3, 50:] = -1
+    there, slots = position.flatten() >= 0, position.flatten().long()
+    w, y, d = (torch.randn(*n, device="cuda", generator=g) for n in ((T, c), (T * c, k), (T, k)))
+    terms = torch.where(position[:, :, None] < 0, 0.0, y.double()[position.clamp(min=0).long()])
+    # c products and sums, each a half step of what they add up to
+    bound = (terms * w.double()[:, :, None]).abs().sum(1) * 2 * c * U
+    assert ((P.dev_moe_combine(y, position, w).double() - (terms * w.double()[:, :, None]).sum(1)).abs() <= bound).all()
+    dy, dw = y.clone(), torch.empty_like(w)
+    P.dev_moe_combine_backward(d, dy, position, w, out=(dy, dw))
+    products = terms * d.double()[:, None]
+    assert ((dw.double() - products.sum(2)).abs() <= products.abs().sum(2) * 2 * k * U).all()
+    assert torch.equal(dy[slots[there]], (w[:, :, None] * d[:, None]).reshape(-1, k)[there])
+    assert torch.equal(P.dev_moe_gather(d, position, dy)[slots[there]], d.repeat_interleave(c, 0)[there])
+
+
 def test_rows_launches_in_parts():
     """Rows of one element, more than a launch has threads for."""
     rows = (1 << 28) + 45
