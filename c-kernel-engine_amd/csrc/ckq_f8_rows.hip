@@ -220,40 +220,56 @@ extern "C" int ckq_launch_moe_gather_f8(int type, const void *x, long ldx, const
     return launch_rows_f8<F8_GATHER>(type, a, stream);
 }
 
-/* y = T(scale * q), sixteen elements a thread (2048 x 11008 to bf16 13 us, 5.2 TB/s). */
+/* y = T(scale * q), sixteen elements a thread, in pieces that are sixteen bytes of y: eight lanes store a line. */
 template <class E>
 __global__ void __launch_bounds__(256) dequantize_f8_kernel(const uint8_t *__restrict__ q, long ldq, const float *__restrict__ scale, long lds,
                                                             E *__restrict__ y, long ldy, int rows, int k, int rs, u32 group_tiles)
 {
+    constexpr int V = 16 / sizeof(E), NP = 16 / V;
     const u32 rt = blockIdx.x / group_tiles, gt = blockIdx.x - rt * group_tiles;
     const int team = threadIdx.x >> 3, l = threadIdx.x & 7;
     const int row = (int)(rt << rs) + (team & ((1 << rs) - 1)), g = (int)gt * (32 >> rs) + (team >> rs);
-    const long at = 128l * g + 16 * l;
+    const long at = 128l * g;
     if (row >= rows || at >= k) return;
-    const int left = k - (int)at;
-    const uint8_t *p = q + (size_t)row * ldq + at;
-    E *o = y + (size_t)row * ldy + at;
+    const int left = (int)min(128l, k - at) - V * l;           /* of piece i: 8 V i less */
+    const uint8_t *p = q + (size_t)row * ldq + at + V * l;
+    E *o = y + (size_t)row * ldy + at + V * l;
     const float s = scale[(size_t)g * lds + row];
-    row16f8 r;
-    if (left >= 16) r = *reinterpret_cast<const row16f8 *>(p);
-    else {
+    struct __attribute__((packed, aligned(1))) codes { u32 v[V / 4]; } r[NP];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r.v[i] = 0;
+    for (int i = 0; i < NP; ++i) {
+        const int n = left - 8 * V * i;
+        if (n >= V) r[i] = *reinterpret_cast<const codes *>(p + 8 * V * i);
+        else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < left) r.v[i >> 2] |= (u32)p[i] << (8 * (i & 3));
+            for (int j = 0; j < V / 4; ++j) r[i].v[j] = 0;
+#pragma unroll
+            for (int j = 0; j < V - 1; ++j)
+                if (j < n) r[i].v[j >> 2] |= (u32)p[8 * V * i + j] << (8 * (j & 3));
+        }
     }
-    float f[2][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)r.v[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)r.v[i], true);
-        f[i >> 1][4 * (i & 1)] = s * lo[0];
-        f[i >> 1][4 * (i & 1) + 1] = s * lo[1];
-        f[i >> 1][4 * (i & 1) + 2] = s * hi[0];
-        f[i >> 1][4 * (i & 1) + 3] = s * hi[1];
+    for (int i = 0; i < NP; ++i) {
+        const int n = left - 8 * V * i;
+        struct __attribute__((packed, aligned(sizeof(E)))) piece { E v[V]; } f;
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)r[i].v[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)r[i].v[j], true);
+            f.v[4 * j] = (E)(s * lo[0]);
+            f.v[4 * j + 1] = (E)(s * lo[1]);
+            f.v[4 * j + 2] = (E)(s * hi[0]);
+            f.v[4 * j + 3] = (E)(s * hi[1]);
+        }
+        E *to = o + 8 * V * i;
+        if (n >= V) {
+            *reinterpret_cast<piece *>(to) = f;
+            asm volatile("");                                /* or what both branches store is moved behind them, in pieces */
+        } else {
+#pragma unroll
+            for (int j = 0; j < V - 1; ++j)
+                if (j < n) to[j] = f.v[j];
+        }
     }
-    store8_pieces(o, f[0], left);
-    if (left > 8) store8_pieces(o + 8, f[1], left - 8);
 }
 
 extern "C" int ckq_launch_dequantize_f8(const uint8_t *q, long ldq, const float *scale, long lds, int type, void *y, long ldy, int rows, int k, void *stream)
