@@ -220,7 +220,7 @@ extern "C" int ckq_launch_moe_gather_f8(int type, const void *x, long ldx, const
     return launch_rows_f8<F8_GATHER>(type, a, stream);
 }
 
-/* y = T(scale * q), sixteen elements a thread, in pieces that are sixteen bytes of y: eight lanes store a line. */
+/* y = T(scale * q), sixteen elements a thread, in pieces that are sixteen bytes of y: eight lanes store a line (2048 x 11008 to bf16 12.2 us, 5.5 TB/s, to fp32 20.1; sixteen beside each other 14.0 and 32.5). */
 template <class E>
 __global__ void __launch_bounds__(256) dequantize_f8_kernel(const uint8_t *__restrict__ q, long ldq, const float *__restrict__ scale, long lds,
                                                             E *__restrict__ y, long ldy, int rows, int k, int rs, u32 group_tiles)

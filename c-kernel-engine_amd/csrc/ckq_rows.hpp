@@ -107,7 +107,7 @@ __device__ __forceinline__ void store8(E *p, const float (&f)[8], int left)
             if (i < left) p[i] = (E)f[i];
     }
 }
-/* The same, a row's last elements four, two and one at a time (rows of e4m3 read back in fp32, 2048 x 11008: 38.9 -> 32.1 us; RMSNorm with a residual in fp32 is 3 % slower with it). */
+/* The same, a row's last elements four, two and one at a time (RMSNorm with a residual in fp32, 2048 x 11008, is 3 % slower with it). */
 template <class E, bool ONCE = false>
 __device__ __forceinline__ void store8_pieces(E *p, const float (&f)[8], int left)
 {
