@@ -485,9 +485,14 @@ def empty_f8(rows, k, device="cuda"):
 
 
 def _f8_new(x, rows=None):
+    """`rows` given: some of them may be written by nothing, and are zeros."""
     if x.dim() != 2:
         raise CkqError("a tensor of the shape %s, not rows x k" % (tuple(x.shape),))
-    return empty_f8(x.shape[0] if rows is None else rows, x.shape[1], x.device)
+    if rows is None:
+        return empty_f8(*x.shape, x.device)
+    q, scale = empty_f8(rows, x.shape[1], x.device)
+    q.view(_torch.uint8).zero_()
+    return q, scale.zero_()
 
 
 def _f8_side(scale, rows, groups):
@@ -618,7 +623,7 @@ def dev_gemm_nt_f8(a, sa, b, sb, bias=None, dtype=None, out=None):
 
 def dev_gemm_nt_f8_experts(a, sa, b, sb, offsets, bias=None, dtype=None, out=None):
     """Rows offsets[e] .. offsets[e + 1] - 1 of C [M, N] as dev_gemm_nt_f8 has them with b[e], sb[e], bias[e]: b float8_e4m3fn [E, N, K], sb float32 [E, ceil(N / 128),
-    ceil(K / 128)], bias float32 [E, N], offsets int32 [E + 1].  Rows that no expert has stay as they are in `out`."""
+    ceil(K / 128)], bias float32 [E, N], offsets int32 [E + 1].  Rows that no expert has stay as they are in `out`, and are zeros without it."""
     if out is not None and dtype is None and _fast.experts(a, sa, b, sb, offsets, bias, out) == 0:
         return out
     dev, stream = _i8_where()
@@ -630,7 +635,7 @@ def dev_gemm_nt_f8_experts(a, sa, b, sb, offsets, bias=None, dtype=None, out=Non
     if (M | N | K | E) >> 31:
         _i8_too_many(M, N, K, E)
     G, blocks = -(-K // 128), -(-N // 128)
-    c = out if out is not None else _torch.empty(M, N, dtype=dtype or _F32, device=b.device)
+    c = out if out is not None else _torch.zeros(M, N, dtype=dtype or _F32, device=b.device)
     t = c.dtype
     kind = _I8_TYPES.get(t)
     ldsa = _f8_side(sa, M, G)
@@ -700,13 +705,14 @@ def _moe_refuse(dev, x, tokens, position, others, weights=()):
 
 
 def dev_moe_gather(x, position, out=None):
-    """y[position[t][j]] = x[t]: x [tokens, k], position as dev_moe_sort has it; y [tokens * choices, k], or into the rows of `out`.  Rows that have no slot stay as they are."""
+    """y[position[t][j]] = x[t]: x [tokens, k], position as dev_moe_sort has it; y [tokens * choices, k], or into the rows of `out`.  Rows that have no slot stay as they are in `out`, and
+    are zeros without it."""
     if out is not None and _fast.gather(x, position, out) == 0:
         return out
     dev, stream = _i8_where()
     shape, places, t = x.shape, position.shape, x.dtype
     if out is None and len(shape) == 2:
-        out = _torch.empty(position.numel(), shape[1], dtype=t, device=x.device)
+        out = _torch.zeros(position.numel(), shape[1], dtype=t, device=x.device)
     into, kind = out.shape if out is not None else (), _I8_TYPES.get(t)
     if (len(shape) != 2 or len(places) != 2 or len(into) != 2 or shape[0] != places[0] or into[1] != shape[1] or kind is None or out.dtype is not t or position.dtype is not _I32
             or not position.is_contiguous() or not x.get_device() == position.get_device() == out.get_device() == dev):
@@ -722,7 +728,7 @@ def dev_moe_gather(x, position, out=None):
 
 
 def dev_moe_gather_f8(x, position, out=None):
-    """The same in e4m3: (q [tokens * choices, k], scale)."""
+    """The same in e4m3: (q [tokens * choices, k], scale); codes and scales of rows that have no slot as there."""
     if out is not None and _fast.gather_f8(x, position, *out) == 0:
         return out
     dev, stream = _i8_where()
@@ -772,11 +778,12 @@ def dev_moe_combine(y, position, weights=None, out=None):
 
 def dev_moe_combine_backward(dout, y, position, weights, out=None):
     """Of dout [tokens, k], the gradient of dev_moe_combine's result: (dy, of y's shape, dweights float32 [tokens, choices]).  Rows of dy that have no slot stay as they
-    are; dy may be y."""
+    are in `out`, where dy may be y, and are zeros, their gradient, without it."""
     if out is not None and _fast.backward(dout, y, position, weights, *out) == 0:
         return out
     dev, stream = _i8_where()
-    if out is None:
+    made = out is None
+    if made:
         out = _torch.empty_strided(y.shape, y.stride(), dtype=y.dtype, device=y.device), _torch.empty(position.shape, dtype=_F32, device=y.device)
     dy, dw = out
     shape, places, of_y, t = dout.shape, position.shape, y.shape, dout.dtype
@@ -792,6 +799,8 @@ def dev_moe_combine_backward(dout, y, position, weights, out=None):
         _moe_refuse(dev, dout, T, position, [(y, "y", None), (dy, "dy", rows)])
     if rows == 1:
         ldy = ldg = k
+    if made:
+        dy.zero_()
     rc = lib().ckq_call_dev(_PACK_15(9, kind, dout.data_ptr(), ldd if T > 1 else k, y.data_ptr(), ldy, position.data_ptr(), weights.data_ptr(), dy.data_ptr(), ldg,
                                             dw.data_ptr(), T, c, rows, k, stream))
     if rc:

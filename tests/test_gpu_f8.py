@@ -733,6 +733,37 @@ def test_combine_backward(t, T, c, k):
     assert torch.equal(sy[:have], dy[:have]) and torch.equal(dw2, dw) and torch.equal(sy[have:].cpu(), y[have:])
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_rows_without_a_slot_are_zeros_where_the_call_makes_the_tensor(t):
+    """The gradient of a row that no token has is zero, and no caller may get what the memory held before."""
+    T, c, E, k, N = 40, 3, 5, 300, 70
+    S = T * c
+    offsets, order, position = P.dev_moe_sort(random_ids(T, c, E, 3, 0.4).cuda(), E)
+    have = int(offsets[-1])
+    assert 0 < have < S
+    x, y, w = normal(T, k, 1).to(TYPES[t]).cuda(), pitched(normal(S, k, 2).to(TYPES[t]), 8), torch.rand(T, c, device="cuda")
+    a, sa, b, sb = codes(S, k, 3), side(S, k, 4), codes(E * N, k, 5).view(torch.uint8), blocks(N, k, 6, E)
+    b = torch.nn.functional.pad(b, (0, -k % 16)).view(F8).view(E, N, -1)[:, :, :k]
+
+    def made(call):
+        nan = [torch.full((n,), 0xFF, dtype=torch.uint8, device="cuda") for n in 4 * [2 ** i for i in range(9, 22)]]        # what the next tensors get
+        del nan
+        return call()
+
+    for i in range(3):
+        dy, dw = made(lambda: P.dev_moe_combine_backward(x, y, position, w))
+        want = torch.zeros_like(dy)
+        P.dev_moe_combine_backward(x, y, position, w, out=(want, torch.empty_like(dw)))
+        assert dy.shape == y.shape and torch.equal(dy, want) and (dy[have:] == 0).all()
+        g = made(lambda: P.dev_moe_gather(x, position))
+        assert torch.equal(g, P.dev_moe_gather(x, position, out=torch.zeros_like(g))) and (g[have:] == 0).all()
+        q, s = made(lambda: P.dev_moe_gather_f8(x, position))
+        assert (q[have:].view(torch.uint8) == 0).all() and (s[have:] == 0).all() and q[:have].float().abs().max() == 448
+        o = made(lambda: P.dev_gemm_nt_f8_experts(a, sa, b, sb, offsets, dtype=TYPES[t]))
+        assert (o[have:] == 0).all()
+        check_experts(torch.cat([o[:have], torch.full_like(o[have:], 7)]), a, sa, b, sb, offsets, None)
+
+
 def test_gradients_against_differences():
     """Both functions are linear in each argument, so a difference of any width is the derivative; on fp32 whole numbers of few bits nothing is rounded, and the
     two agree to the last bit."""
