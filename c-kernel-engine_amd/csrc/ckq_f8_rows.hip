@@ -8,9 +8,11 @@
  *   q_i     = e4m3(448 v_i / a),  scale = a / 448
  *
  * The quotient is rounded correctly: 448 v / a of values with eight or eleven bits is often halfway between two codes, and a
- * product with 448 / a, which is rounded, would put half of those ties on the wrong side.  With a = a' 2^e, a' in [1, 2): 448 * 2^-e v
+ * product with 448 / a, which is rounded, would put half of those ties on the wrong side.  With a = a' 2^e, a' in [1, 2): n = 448 * 2^-e v
  * is exact for bf16 and fp16 (448 = 7 * 64), and a quotient from the correctly rounded inverse of a' and one
- * residual step is the correctly rounded one (Markstein, 1990).  Three operations an element more than the product.
+ * residual step is the correctly rounded one (Markstein, 1990).  Three operations an element more than the product.  Of an fp32 v, n
+ * has up to 27 bits: what its rounding takes, which a multiply-add gives exactly, goes into the residual (without it, of fp32 rows one code in
+ * some millions, and one in twenty next to a tie, is the wrong neighbour).  SwiGLU's v is off by more than that to begin with.
  *
  * A group with an infinity or a NaN in v has that as its scale and zeros as its codes; the maximum is taken over bit patterns, where
  * NaN > inf > everything else.
@@ -36,7 +38,8 @@ struct __attribute__((packed, aligned(1))) row16f8 { u32 v[4]; };
 typedef u32 __attribute__((aligned(1))) u32_at_1;
 typedef uint16_t __attribute__((aligned(1))) u16_at_1;
 
-/* Sixteen values of a group, a' and 448 * 2^-e of it: their codes. */
+/* Sixteen values of a group, a' and 448 * 2^-e of it: their codes.  LONG: values of more bits than the product with c keeps. */
+template <bool LONG>
 __device__ __forceinline__ row16f8 f8_codes(const float (&v)[16], float a1, float c, bool finite)
 {
 #pragma clang fp contract(off)
@@ -47,8 +50,8 @@ __device__ __forceinline__ row16f8 f8_codes(const float (&v)[16], float a1, floa
         float t[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float n = v[4 * i + j] * c, q = n * inv;
-            t[j] = __builtin_fmaf(__builtin_fmaf(-a1, q, n), inv, q);
+            const float n = v[4 * i + j] * c, q = n * inv, rest = __builtin_fmaf(-a1, q, n);
+            t[j] = __builtin_fmaf(LONG ? rest + __builtin_fmaf(v[4 * i + j], c, -n) : rest, inv, q);
         }
         int w = __builtin_amdgcn_cvt_pk_fp8_f32(t[0], t[1], 0, false);
         w = __builtin_amdgcn_cvt_pk_fp8_f32(t[2], t[3], w, true);
@@ -110,7 +113,7 @@ __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 
     const bool finite = top < 0x7f800000u;
     const u32 bits = finite ? max(top, 0x0d800000u) : 0x3f800000u;                       /* 2^-100 at least */
     const float scale = finite ? __builtin_bit_cast(float, bits) / 448.0f : __builtin_bit_cast(float, top);
-    const row16f8 o = f8_codes(v, __builtin_bit_cast(float, (bits & 0x7fffffu) | 0x3f800000u),
+    const row16f8 o = f8_codes<sizeof(E) == 4 && OP != F8_SWIGLU>(v, __builtin_bit_cast(float, (bits & 0x7fffffu) | 0x3f800000u),
                                __builtin_bit_cast(float, ((262u - (bits >> 23)) << 23) | 0x600000u), finite);
     auto put = [&](int to) {
         uint8_t *q = a.q + (size_t)to * a.ldq + at;

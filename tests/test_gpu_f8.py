@@ -190,6 +190,24 @@ def test_quantize_ties_go_to_even_codes():
         assert np.array_equal(P.dev_quantize_f8(y.cuda())[0].cpu().float().numpy(), wq)
 
 
+@pytest.mark.parametrize("rows,k", [(40, 128), (33, 500), (300, 1001)])
+def test_quantize_fp32_next_to_ties(rows, k):
+    """Quotients within two steps of fp32 of a tie between two codes: 448 x is no fp32 number there, the quotient is rounded once all the same."""
+    g = torch.Generator().manual_seed(k)
+    top = torch.rand(rows, -(-k // 128), generator=g, dtype=torch.float32) + 1
+    tie = (17 + 2 * torch.randint(0, 8, (rows, k), generator=g)).double() * 2.0 ** torch.randint(-5, 4, (rows, k), generator=g).double()
+    x = (tie * top.double().repeat_interleave(128, 1)[:, :k] / 448).float()
+    x = (x.view(torch.int32) + torch.randint(-2, 3, (rows, k), generator=g, dtype=torch.int32)).view(torch.float32)
+    x[:, ::128] = top
+    x *= torch.where(torch.rand(rows, k, generator=g) < 0.5, -1.0, 1.0)
+    v = grouped(x.double().numpy())
+    t = (v * 448 / np.abs(v).max(2)[:, :, None]).astype(np.float32)        # 448 v is exact in 64 bits
+    want = e4m3(t.astype(np.float64))[0].reshape(rows, -1)[:, :k]
+    assert np.array_equal(P.dev_quantize_f8(x.cuda())[0].cpu().float().numpy(), want)
+    back = torch.arange(rows - 1, -1, -1, device="cuda", dtype=torch.int32)[:, None]
+    assert np.array_equal(P.dev_moe_gather_f8(x.cuda(), back)[0].cpu().float().numpy()[::-1], want)
+
+
 def test_every_code_is_read_back():
     q = torch.arange(256, dtype=torch.uint8).view(2, 128).cuda()
     s = torch.tensor([[0.375], [3.0]]).cuda()
