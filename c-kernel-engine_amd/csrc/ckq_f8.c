@@ -59,6 +59,14 @@ int ckq_moe_combine_backward_dev(ckq_ck_dtype type, const void *dout, long ldd, 
     return ckq_launch_moe_combine_backward((int)type, dout, ldd, y, ldy, position, weights, dy, lddy, dweights, tokens, choices, rows, k, stream);
 }
 
+/* Which of a call's arguments are int: bit i, the i-th. */
+#define AT(i) (1u << (i))
+static const unsigned ints[] = {
+    AT(0) | AT(7) | AT(8), AT(4) | AT(7) | AT(8), AT(0) | AT(8) | AT(9), AT(9) | AT(12) | AT(13) | AT(14), AT(12) | AT(13) | AT(16) | AT(17) | AT(18),
+    AT(1) | AT(2) | AT(3), AT(0) | AT(6) | AT(7) | AT(8) | AT(9), AT(0) | AT(8) | AT(9) | AT(10) | AT(11), AT(0) | AT(7) | AT(8) | AT(9) | AT(10),
+    AT(0) | AT(10) | AT(11) | AT(12) | AT(13),
+};
+
 #define PTR(T, i) ((T *)(uintptr_t)a[i])
 #define INT(i)    ((int)a[i])
 #define LONG(i)   ((long)a[i])
@@ -71,6 +79,8 @@ int ckq_call_dev(const void *call)
     memcpy(&which, call, 8);
     if (which < 0 || which >= (int64_t)sizeof arguments) return CKQ_EINVAL;
     memcpy(a, (const char *)call + 8, 8u * arguments[which]);
+    for (int i = 0; i < arguments[which]; ++i)                 /* 2^32 + 16 rows are not 16 */
+        if ((ints[which] & AT(i)) && a[i] != (int)a[i]) return CKQ_EINVAL;
     switch (which) {
     case CKQ_CALL_QUANTIZE_F8:
         return ckq_launch_quantize_f8(INT(0), PTR(const void, 1), LONG(2), PTR(uint8_t, 3), LONG(4), PTR(float, 5), LONG(6), INT(7), INT(8), PTR(void, 9));

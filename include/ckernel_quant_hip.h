@@ -364,7 +364,7 @@ int ckq_moe_combine_backward_dev(ckq_ck_dtype type, const void *dout, long ldd, 
                                  void *dy, long lddy, float *dweights, int tokens, int choices, int rows, int k, void *stream);
 
 /* Any entry point from ckq_quantize_f8_dev to here, for callers whose arguments cost them one by one (ctypes: 0.09 us each): call[0] says which, its arguments
- * follow in order, 64 bits each, pointers as integers.  CKQ_EINVAL for a number that is none of these. */
+ * follow in order, 64 bits each, pointers as integers.  CKQ_EINVAL for a number that is none of these, and for an argument beyond its int. */
 enum { CKQ_CALL_QUANTIZE_F8, CKQ_CALL_DEQUANTIZE_F8, CKQ_CALL_SWIGLU_F8, CKQ_CALL_GEMM_NT_F8, CKQ_CALL_GEMM_NT_F8_EXPERTS, CKQ_CALL_MOE_SORT, CKQ_CALL_MOE_GATHER, CKQ_CALL_MOE_GATHER_F8,
        CKQ_CALL_MOE_COMBINE, CKQ_CALL_MOE_COMBINE_BACKWARD };
 int ckq_call_dev(const void *call);

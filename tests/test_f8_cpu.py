@@ -119,6 +119,29 @@ def test_any_call_by_its_number(L):
     assert call(-1, *good[4]) == EINVAL and call(10, *good[4]) == EINVAL and L.ckq_call_dev(None) == EINVAL
 
 
+def test_a_call_by_its_number_refuses_what_no_int_holds(L):
+    """64 bits come in and 32 go on: 2^32 + 2 rows would be 2.  Each size and type alone, in calls that are refused for their type if they get that far."""
+    import struct
+    call = lambda *a: L.ckq_call_dev(struct.pack("%dq" % len(a), *a))
+    p, n, far = 4096, 0, 1 << 40                               # pitches and pointers are 64 bits wide
+    bad = 5                                                    # no type of a row
+    calls = [(bad, p, far, p, far, p, far, 2, 64, n), (p, far, p, far, bad, p, far, 2, 64, n), (bad, p, p, far, p, far, p, far, 2, 64, n),
+             (p, far, p, far, p, far, p, far, p, bad, p, far, 2, 32, 64, n), (p, far, p, far, p, far, 2048, p, far, 1, p, p, 3, bad, p, far, 2, 32, 64, n), None,
+             (bad, p, far, p, p, far, 2, 2, 4, 64, n), (bad, p, far, p, p, far, p, far, 2, 2, 4, 64, n), (bad, p, far, p, p, p, far, 2, 2, 4, 64, n), (bad, p, far, p, far, p, p, p, far, p, 2, 2, 4, 64, n)]
+    sizes = [(7, 8), (7, 8), (8, 9), (12, 13, 14), (12, 16, 17, 18), (), (6, 7, 8, 9), (8, 9, 10, 11), (7, 8, 9, 10), (10, 11, 12, 13)]
+    for which, (a, at) in enumerate(zip(calls, sizes)):
+        if a is None:
+            continue
+        assert call(which, *a) == EFORMAT
+        for i in (*at, a.index(bad)):
+            for add in (1 << 32, 1 << 31, -(1 << 32), 1 << 62):
+                assert call(which, *a[:i], a[i] + add, *a[i + 1:]) == EINVAL, (which, i, add)
+    sort = (p + 2, 2, 2, 3, p, p, p, n)                        # refused for its pointer
+    assert call(5, *sort) == EROWS
+    for i in (1, 2, 3):
+        assert call(5, *sort[:i], sort[i] + (1 << 32), *sort[i + 1:]) == EINVAL
+
+
 def test_front_ends_refuse_what_a_pointer_cannot_tell():
     import torch
     par, err = ckq.parity, ckq.CkqError
