@@ -178,6 +178,37 @@ def test_the_module_that_reads_tensors_takes_none_of_the_host(L):
     assert without_module(par).gemm(x) == -1000
 
 
+def test_make_leaves_the_module_out_where_there_is_no_torch_and_builds_it_anew_for_another(tmp_path):
+    """A compiler that only says that it was called; a Python without site packages, and one with another torch."""
+    import shutil
+    import subprocess
+    import sys
+    for f in ("Makefile", "ckq_tensors.cpp"):
+        shutil.copy(os.path.join(ckq.api.CSRC, f), tmp_path)
+    (tmp_path / "g++").write_text('#!/bin/sh\nwhile [ "$1" != -o ]; do shift; done\necho made > "$2"\n')
+    (tmp_path / "g++").chmod(0o755)
+    other = tmp_path / "other"
+    (other / "torch" / "include" / "c10" / "hip").mkdir(parents=True)
+    (other / "torch" / "include" / "c10" / "hip" / "HIPStream.h").write_text("")
+    (other / "torch" / "__init__.py").write_text('__version__ = "0.1.2"\n')
+    so, env = tmp_path / "ckq_tensors.so", dict(os.environ, PATH="%s:%s" % (tmp_path, os.environ["PATH"]))
+
+    def make(python=sys.executable, **more):
+        r = subprocess.run(["make", "-f", str(tmp_path / "Makefile"), "tensors", "PYTHON=" + python], env=dict(env, **more), capture_output=True, text=True)
+        assert r.returncode == 0, r.stderr
+        return r.stdout
+
+    assert "left out" in make(sys.executable + " -S") and not so.exists()
+    make()
+    assert so.read_text() == "made\n"
+    so.write_text("kept\n")
+    make()
+    assert so.read_text() == "kept\n"                          # nothing has changed
+    make(PYTHONPATH=str(other))
+    assert so.read_text() == "made\n"
+    assert "left out" in make(sys.executable + " -S") and not so.exists()          # none that is of neither
+
+
 def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
     """ctypes passes the lowest 32 bits of an int: 2^32 + 16 rows would be 16.  Memory that nothing touches, and a library that nothing reaches."""
     import torch
