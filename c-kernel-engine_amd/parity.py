@@ -9,6 +9,8 @@ import ctypes
 import importlib.util
 import os
 import struct
+import sys
+import warnings
 
 import numpy as np
 
@@ -444,10 +446,10 @@ def _f8_refuse(dev, rows, scales=(), wholes=()):
 
 
 # With `out` given, a call is first offered to csrc/ckq_tensors.so, which reads the same of the tensors in C++ (a call of dev_gemm_nt_f8_experts 6.1 -> 3.5 us, of dev_moe_gather 4.7 -> 3.0); what that does not take, or the library
-# refuses, comes back and is looked at here.  Without that module all of it happens here.
+# refuses, comes back and is looked at here.  Without that module all of it happens here, and with one that was built for another torch or Python, or cannot be loaded.
 
 class _Fast:
-    """Stands for the module until the first call, and for good where it has not been built."""
+    """Stands for the module until the first call, and for good where there is none that can be used."""
     absent = False
 
     def __getattr__(self, name):
@@ -459,16 +461,27 @@ _fast = _Fast()
 
 def _load_fast():
     global _fast
-    _i8_torch()
+    torch = _i8_torch()
     path = os.path.join(CSRC, "ckq_tensors.so")
+    why, here = None, "torch-%s-python-%d.%d" % (torch.__version__, *sys.version_info[:2])
     if os.path.exists(path):
-        spec = importlib.util.spec_from_file_location("ckq_tensors", path)
-        module = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(module)
-        module.bind(ctypes.cast(lib().ckq_call_dev, _vp).value)
-        _fast = module
-    else:
-        _fast.absent = True
+        try:
+            spec = importlib.util.spec_from_file_location("ckq_tensors", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as e:
+            why = str(e)
+        else:
+            built = getattr(module, "built_for", None)
+            if built == here:
+                module.bind(ctypes.cast(lib().ckq_call_dev, _vp).value)
+                _fast = module
+                return _fast
+            why = "it was built for %s, this is %s" % (built, here)
+    if why:
+        warnings.warn("%s is not used, calls go through ctypes (`make tensors` builds it anew): %s" % (path, why))
+    _fast = _Fast()
+    _fast.absent = True
     return _fast
 
 

@@ -209,6 +209,31 @@ def test_make_leaves_the_module_out_where_there_is_no_torch_and_builds_it_anew_f
     assert "left out" in make(sys.executable + " -S") and not so.exists()          # none that is of neither
 
 
+@pytest.mark.parametrize("what", ["cut short", "no library", "of another torch"])
+def test_a_module_that_cannot_be_used_leaves_the_python_checks(L, monkeypatch, tmp_path, what):
+    """Each call with `out` then goes the way that it has without the module."""
+    import shutil
+    import torch
+    par = ckq.parity
+    so, made = tmp_path / "ckq_tensors.so", os.path.join(ckq.api.CSRC, "ckq_tensors.so")
+    if what == "cut short":
+        so.write_bytes(open(made, "rb").read()[:50])
+    elif what == "no library":
+        so.write_text("not a library")
+    else:
+        shutil.copy(made, so)
+        monkeypatch.setattr(torch, "__version__", "0.1.2")
+    monkeypatch.setattr(par, "CSRC", str(tmp_path))
+    monkeypatch.setattr(par, "_fast", par._Fast())
+    x = torch.zeros(3, 32)
+    with pytest.warns(UserWarning, match="built for" if what == "of another torch" else "is not used"):
+        with pytest.raises(ckq.CkqError, match="not on the current device"):
+            par.dev_quantize_f8(x, out=par.empty_f8(3, 32, device="cpu"))
+    assert par._fast.absent
+    with pytest.raises(ckq.CkqError, match="not on the current device"):        # and again, without another word
+        par.dev_moe_gather(x, torch.zeros(3, 1, dtype=torch.int32), out=x)
+
+
 def test_front_ends_refuse_sizes_beyond_31_bits(monkeypatch):
     """ctypes passes the lowest 32 bits of an int: 2^32 + 16 rows would be 16.  Memory that nothing touches, and a library that nothing reaches."""
     import torch
