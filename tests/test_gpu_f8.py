@@ -502,6 +502,57 @@ def test_matmul_launches_in_parts(kernel):
         del out, aw, bw
 
 
+def whole_product(M, N, K, seed, t, E=0):
+    """Operands of small whole numbers, scales that are powers of two, and their product: every sum is a multiple of 1/8 below 2^18, exact in fp32 in any order, and no
+    product is below 2^-13 of another.  Bytes behind K are NaNs."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    whole = lambda *s: torch.randint(-4, 5, s, device="cuda", generator=g).float()
+    power = lambda *s: 2.0 ** torch.randint(-1, 2, s, device="cuda", generator=g).float()
+    held = lambda v: torch.nn.functional.pad(v.to(F8).view(torch.uint8), (0, -K % 16), value=0x7F).view(F8)[..., :K]
+    lead = (E,) if E else ()
+    a, b, sa, sb, bias = whole(M, K), whole(*lead, N, K), power(-(-K // 128), M).t(), 0.5 * power(*lead, -(-N // 128), -(-K // 128)), whole(*lead, N)
+    x = a * sa.repeat_interleave(128, 1)[:, :K]
+    w = b * sb.repeat_interleave(128, -1)[..., :K].repeat_interleave(128, -2)[..., :N, :]
+    return held(a), sa, held(b), sb, bias, lambda rows=slice(None), e=None: ((x[rows] @ (w if e is None else w[e]).t().contiguous()) + (bias if e is None else bias[e])).to(t)
+
+
+EXACT = [(2, 129, 127), (65, 130, 65), (129, 255, 1000), (257, 513, 896), (333, 1001, 1111), (520, 390, 1284)]
+# at least 256 tiles of 256 x 256; N that ends within a tile of 192 and a block of 128, and a whole column of tiles less
+TWO_EXACT = [(4000, 4300, 300), (4100, 3900, 1000), (2048, 8300, 640), (2000, 8500, 129), (9000, 2100, 77)]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("kernel", KERNELS, indirect=True)
+def test_matmul_is_exact_on_whole_numbers_on_every_kernel(kernel, t):
+    sizes = [(1, N, K) for _, N, K in EXACT] if kernel == 16 else TWO_EXACT if kernel == 15 else EXACT
+    for M, N, K in sizes:
+        assert ckq.lib().ckq_launch_f8_kernel(list(TYPES).index(t), M, N, K, 0) == kernel            # and no other one
+        a, sa, b, sb, bias, want = whole_product(M, N, K, M + N, TYPES[t])
+        assert torch.equal(P.dev_gemm_nt_f8(a, sa, b, sb, bias, dtype=TYPES[t]), want()), (M, N, K)
+
+
+@pytest.mark.parametrize("kernel", range(15), indirect=True)
+def test_experts_are_exact_on_whole_numbers_on_every_kernel(kernel):
+    for M, N, K, counts in ((700, 256, 640, [130, 1, 0, 256, 65, 127, 64]), (300, 390, 1001, [0, 290, 0, 1]), (90, 70, 200, [0, 64, 1, 0, 15])):
+        assert ckq.lib().ckq_launch_f8_kernel(1, M, N, K, len(counts)) == kernel
+        a, sa, b, sb, bias, want = whole_product(M, N, K, M + N, torch.bfloat16, len(counts))
+        o = [0] + np.cumsum(counts).tolist()
+        out = torch.full((M, N), 7.0, device="cuda", dtype=torch.bfloat16)
+        P.dev_gemm_nt_f8_experts(a, sa, b, sb, torch.tensor(o, dtype=torch.int32, device="cuda"), bias, out=out)
+        for e in range(len(counts)):
+            assert torch.equal(out[o[e]:o[e + 1]], want(slice(o[e], o[e + 1]), e)), e
+        assert (out[o[-1]:] == 7).all()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+def test_a_long_prompt_is_exact_on_whole_numbers(t):
+    """The size for which two sizes of tiles are chosen without being forced."""
+    M, N, K = 2048, 11008, 4096
+    assert ckq.lib().ckq_launch_f8_kernel(list(TYPES).index(t), M, N, K, 0) == 15
+    a, sa, b, sb, bias, want = whole_product(M, N, K, 1, TYPES[t])
+    assert torch.equal(P.dev_gemm_nt_f8(a, sa, b, sb, bias, dtype=TYPES[t]), want())
+
+
 def test_experts_without_rows_and_as_many_experts_as_there_can_be():
     a, sa, b, sb = codes(7, 300, 1), side(7, 300, 2), codes(50, 300, 3), blocks(50, 300, 4, 4)
     out = torch.full((7, 50), 3.0, device="cuda")
