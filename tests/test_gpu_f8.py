@@ -553,6 +553,27 @@ def test_a_long_prompt_is_exact_on_whole_numbers(t):
     assert torch.equal(P.dev_gemm_nt_f8(a, sa, b, sb, bias, dtype=TYPES[t]), want())
 
 
+@pytest.mark.parametrize("kernel", range(9, 15), indirect=True)
+def test_sums_of_the_e4m3_instructions_lose_no_more_than_they_may(kernel):
+    """Codes of every size, signs that cancel: each eight products may lose eight times 2^-13 of their largest, and nothing else."""
+    M, N, K = 70, 90, 500
+    g = torch.Generator().manual_seed(kernel)
+
+    def any_codes(n):
+        q = torch.randint(0, 256, (n, 512), generator=g, dtype=torch.uint8)
+        return torch.where((q & 0x7F) == 0x7F, 0x7E, q).to(torch.uint8).cuda().view(F8)[:, :K]
+
+    a, b, sa, sb = any_codes(M), any_codes(N), side(M, K, 1), blocks(N, K, 2)
+    assert ckq.lib().ckq_launch_f8_kernel(0, M, N, K, 0) == kernel
+    c = P.dev_gemm_nt_f8(a, sa, b, sb).cpu().double()
+    want, off = product(a, sa, b, sb, None)
+    x, w = values(a, sa), block_values(b, sb)
+    largest = torch.nn.functional.pad((x[:, None] * w).abs(), (0, -K % 8)).view(M, N, -1, 8).amax(3)
+    off = off + 8 * 2.0 ** -13 * largest.sum(2)
+    assert ((c - want).abs() <= off).all(), ((c - want).abs() / off).max().item()
+    assert (((c - want).abs() - product(a, sa, b, sb, None)[1]) > 0).any()         # and it is them that are meant
+
+
 def test_experts_without_rows_and_as_many_experts_as_there_can_be():
     a, sa, b, sb = codes(7, 300, 1), side(7, 300, 2), codes(50, 300, 3), blocks(50, 300, 4, 4)
     out = torch.full((7, 50), 3.0, device="cuda")
