@@ -854,6 +854,39 @@ def test_rows_without_a_slot_are_zeros_where_the_call_makes_the_tensor(t):
         check_experts(torch.cat([o[:have], torch.full_like(o[have:], 7)]), a, sa, b, sb, offsets, None)
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("k", [2048, 2047, 2044])
+def test_rows_there_and_back_beyond_the_cache(t, k):
+    """Rows of 16 bits, more than 192 MB of them, which leave past the caches; the same in place."""
+    D, T, c, E = TYPES[t], 7000, 8, 40
+    g = torch.Generator(device="cuda").manual_seed(k)
+    assert T * c * k * 2 > 192 << 20
+    rows = lambda n, fill=None: (torch.randn(n, 2048, device="cuda", generator=g) if fill is None else torch.full((n, 2048), fill, device="cuda")).to(D)[:, :k]
+    ids = torch.randint(-1, E, (T, c), device="cuda", generator=g, dtype=torch.int32)
+    offsets, order, position = P.dev_moe_sort(ids, E)
+    have = int(offsets[-1])
+    assert have < T * c
+    x, w, y = rows(T), torch.rand(T, c, device="cuda", generator=g), rows(T * c)
+    out = P.dev_moe_gather(x, position, out=rows(T * c, 7.0))
+    slots = order[:have].long()
+    assert torch.equal(out[:have], x[slots // c]) and (out[have:] == 7).all()
+    del out
+    dy, dw = P.dev_moe_combine_backward(x, y, position, w, out=(rows(T * c, 7.0), torch.empty(T, c, device="cuda")))
+    assert (dy[have:] == 7).all()
+    h, depth = half_step(D), 8 * -(-k // 2048) + 6 + 4        # every thread's chain, the tree of a wave, four waves
+    for part in slots.split(1 << 13):
+        # w * dout has 24 + 11 bits: rounded to fp32 first (U of it) and then to the type, or at once
+        want = w.view(-1)[part, None].double() * x[part // c].double()
+        d = dy[position.view(-1)[part].long()].double()
+        assert ((d - want).abs() <= U * (1 + h) * want.abs() + rounding(D, want * (1 + U))).all()
+        terms = x[part // c].double() * y[position.view(-1)[part].long()].double()
+        assert ((dw.view(-1)[part].double() - terms.sum(1)).abs() <= depth * U * terms.abs().sum(1)).all()
+    assert (dw[position < 0] == 0).all()
+    again, behind = torch.empty_like(dw), y[have:].clone()
+    P.dev_moe_combine_backward(x, y, position, w, out=(y, again))
+    assert torch.equal(y[:have], dy[:have]) and torch.equal(y[have:], behind) and torch.equal(again, dw)
+
+
 def test_gradients_against_differences():
     """Both functions are linear in each argument, so a difference of any width is the derivative; on fp32 whole numbers of few bits nothing is rounded, and the
     two agree to the last bit."""
