@@ -443,6 +443,36 @@ def test_experts(t, M, N, K, counts):
         check_experts(out, a, sa, b, sb, offsets, bias)
 
 
+def test_transposed_weights_of_experts_give_the_gradient():
+    """dX = dY W of each expert's rows, against the product of the values and against differences of the product."""
+    M, N, K, counts = 150, 300, 200, [40, 0, 3, 100, 1]
+    E, o = len(counts), [0] + np.cumsum(counts).tolist()
+    offsets = torch.tensor(o, dtype=torch.int32, device="cuda")
+    w = torch.stack([torch.nn.functional.pad(codes(N, K, e).view(torch.uint8), (0, -K % 16)) for e in range(E)]).view(F8)[:, :, :K]
+    sw = blocks(N, K, 2, E)
+    dy, sy = P.dev_quantize_f8(normal(M, N, 3).cuda())
+    wt = torch.nn.functional.pad(w.view(torch.uint8).transpose(1, 2), (0, -N % 16)).contiguous().view(F8)[:, :, :N]
+    dx = P.dev_gemm_nt_f8_experts(dy, sy, wt, sw.transpose(1, 2).contiguous(), offsets)
+    x, one = normal(M, K, 5).mul_(30).clamp_(-448, 448).to(F8).float(), torch.ones(-(-K // 128), M, device="cuda").t()
+    product_of = lambda v: P.dev_gemm_nt_f8_experts(torch.nn.functional.pad(v, (0, -K % 16)).to(F8).cuda()[:, :K], one, w, sw, offsets).cpu().double()
+    for e in range(E):
+        rows = slice(o[e], o[e + 1])
+        v, m = values(dy, sy)[rows], block_values(w[e], sw[e])
+        # one sum of 128 at a time, scales and groups, as `product` counts them
+        off = (2 * 128 + 2 * -(-N // 128) + 4) * U * (v.abs() @ m.abs())
+        assert ((dx.cpu().double()[rows] - v @ m).abs() <= off).all()
+    for k in (0, 130, K - 1):
+        up, down = x.clone(), x.clone()
+        up[:, k], down[:, k] = 8, -8
+        slope = ((product_of(up) - product_of(down)) * values(dy, sy)).sum(1) / 16
+        for e in range(E):
+            rows = slice(o[e], o[e + 1])
+            m, v = block_values(w[e], sw[e]), values(dy, sy)[rows].abs()
+            size = up[rows].double().abs() @ m.abs().T                             # |up| and |down| are alike
+            slack = ((2 * (2 * 128 + 2 * 2 + 4) * U * size) * v).sum(1) / 16 + (2 * 128 + 2 * -(-N // 128) + 4) * U * (v @ m.abs()[:, k])
+            assert ((slope[rows] - dx.cpu().double()[rows, k]).abs() <= slack).all()
+
+
 KERNELS = range(17)             # CKQ_F8_* of ckq_launch.h
 CORES = range(9, 16)              # those on the e4m3 instructions
 
