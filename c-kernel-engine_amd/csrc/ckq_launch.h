@@ -176,6 +176,7 @@ void ckq_launch_set_i8_kernel(int kernel);
 
 /* Rows in e4m3 with one scale for each 128 elements, and tokens sorted by expert (ckq_f8_rows.hip, ckq_gemm_f8.hip, ckq_moe.hip).  See ckernel_quant_hip.h for what
  * they compute and take. */
+#define CKQ_SUMS_FP32 256                        /* CKQ_F8_SUMS_FP32 of ckernel_quant_hip.h: in a matmul's type, no kernel on the e4m3 instructions */
 #define CKQ_MOE_EXPERTS_MAX 65535
 #define CKQ_MOE_SLOTS_MAX (1l << 29)
 int ckq_launch_quantize_f8(int type, const void *x, long ldx, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);

@@ -594,10 +594,11 @@ def dev_swiglu_f8(gate, up, out=None):
     return q, scale
 
 
-def dev_gemm_nt_f8(a, sa, b, sb, bias=None, dtype=None, out=None):
+def dev_gemm_nt_f8(a, sa, b, sb, bias=None, dtype=None, out=None, fp32_sums=False):
     """C [M, N] = a b^T (+ bias[n]) of the values that the codes stand for: float8_e4m3fn rows a [M, K] (tokens) with scales sa [M, ceil(K / 128)], b [N, K]
-    (channels) with float32 scales sb [ceil(N / 128), ceil(K / 128)]; C of dtype (float32), or into `out`."""
-    if out is not None and dtype is None and _fast.gemm(a, sa, b, sb, bias, out) == 0:
+    (channels) with float32 scales sb [ceil(N / 128), ceil(K / 128)]; C of dtype (float32), or into `out`.  A C of 16 bits may come from instructions that drop, of each eight products, what is under 2^-13
+    of their largest; with fp32_sums it does not (2048 x 11008 x 4096 twice the time)."""
+    if out is not None and dtype is None and not fp32_sums and _fast.gemm(a, sa, b, sb, bias, out) == 0:
         return out
     dev, stream = _i8_where()
     of_a, of_b = a.shape, b.shape
@@ -628,7 +629,7 @@ def dev_gemm_nt_f8(a, sa, b, sb, bias=None, dtype=None, out=None):
         lda, ldc = -(-K // 16) * 16, N
     if N == 1:
         ldb = -(-K // 16) * 16
-    rc = lib().ckq_call_dev(_PACK_16(3, a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, sb.data_ptr(), G, bp, kind, c.data_ptr(), ldc, M, N, K, stream))
+    rc = lib().ckq_call_dev(_PACK_16(3, a.data_ptr(), lda, sa.data_ptr(), ldsa, b.data_ptr(), ldb, sb.data_ptr(), G, bp, kind | 256 if fp32_sums else kind, c.data_ptr(), ldc, M, N, K, stream))
     if rc:
         check(rc, "ckq_gemm_nt_f8_dev")
     return c

@@ -326,7 +326,8 @@ int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t 
  * ckq_dequantize_f8_dev: y = scale * q, rounded to the type.
  * ckq_swiglu_f8_dev: gate / (1 + exp(-gate)) * up in 8 bits as above (the function as exact as ckq_swiglu_i8_dev's); gate and up have one pitch, ld.
  * ckq_gemm_nt_f8_dev: C[m*ldc + n] = sum over groups g of (sa[g*ldsa + m] * sb[(n/128)*ldsb + g]) * (sum over k in g of A[m][k] * B[n][k]) (+ bias[n]), in
- * fp32, rounded once to the type of C (of 16 bits: the matrix instructions may drop what is under 2^-13 of the largest of eight products, 1.5e-5 of a sum of 128 random ones).  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are, multiples of 16 bytes, pitches at
+ * fp32, rounded once to the type of C.  Of 16 bits, where that takes less time: by the e4m3 matrix instructions, in which a product may lose up to 2^-13 of the largest of the eight that it
+ * is added with (1.5e-5 of a sum of 128 random ones; all of a small one between two large ones that cancel).  Not so with type | CKQ_F8_SUMS_FP32.  A (M rows, lda apart) and B (N rows, ldb apart) start on, and lda and ldb are, multiples of 16 bytes, pitches at
  * most 4 MiB (else CKQ_EROWS).  K may be any number: of the 16 bytes that hold a row's last, those behind it may be read and are not used.  The gradient of the
  * activations is the same product with the transposed codes and scales of the weights.
  * ckq_gemm_nt_f8_experts_dev: the same of rows sorted by expert, each expert with a matrix, scales and bias of its own: rows offsets[e] .. offsets[e + 1] - 1 of A and C
@@ -336,6 +337,7 @@ int ckq_gemm_nt_i8_dev(const int8_t *A, long lda, const float *sa, const int8_t 
 int ckq_quantize_f8_dev(ckq_ck_dtype type, const void *x, long ldx, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
 int ckq_dequantize_f8_dev(const uint8_t *q, long ldq, const float *scale, long lds, ckq_ck_dtype type, void *y, long ldy, int rows, int k, void *stream);
 int ckq_swiglu_f8_dev(ckq_ck_dtype type, const void *gate, const void *up, long ld, uint8_t *q, long ldq, float *scale, long lds, int rows, int k, void *stream);
+enum { CKQ_F8_SUMS_FP32 = 256 };
 int ckq_gemm_nt_f8_dev(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, const float *sb, long ldsb, const float *bias,
                        ckq_ck_dtype type, void *C, long ldc, int M, int N, int K, void *stream);
 int ckq_gemm_nt_f8_experts_dev(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, long eb, const float *sb, long ldsb, long esb,

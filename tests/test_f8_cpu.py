@@ -277,3 +277,22 @@ def test_kernel_of_a_matmul(L):
         assert k(BF16, 2048, 11008, 4096, 0) == (forced if forced != 16 else 15)
         assert k(BF16, 2048, 11008, 4096, 8) in ((forced,) if forced < 15 else range(9))
     L.ckq_launch_set_f8_kernel(-1)
+
+
+def test_kernel_of_a_matmul_with_fp32_sums(L):
+    """The fp32 result's choice, whatever the type and whichever kernel is forced on those that may have it."""
+    k, wide = L.ckq_launch_f8_kernel, 256
+    for M in (1, 2, 40, 300, 2048, 1 << 19):
+        for N in (64, 1001, 11008):
+            for K in (64, 4096):
+                for E in (0, 8):
+                    L.ckq_launch_set_f8_kernel(-1)
+                    want = k(F32, M, N, K, E)
+                    assert want < 9 or want == 16 and M == 1
+                    for forced in (-1, *range(9, 16)):
+                        L.ckq_launch_set_f8_kernel(forced)
+                        assert k(BF16 | wide, M, N, K, E) == k(F16 | wide, M, N, K, E) == k(F32 | wide, M, N, K, E) == want
+    L.ckq_launch_set_f8_kernel(3)
+    assert k(BF16 | wide, 300, 1001, 4096, 0) == 3
+    gemm = lambda t, b=P: L.ckq_gemm_nt_f8_dev(P, 64, P, 2, b, 64, P, 1, P, t, P, 32, 2, 32, 50, None)
+    assert all(gemm(t | wide) == EFORMAT for t in (-1, 3, 7, 9)) and gemm(BF16 | wide, odd(4)) == EROWS and gemm(BF16 | 512) == EFORMAT

@@ -405,6 +405,29 @@ def test_offsets_beyond_32_bits():
         check_matmul(out[:rows], b[:rows], sa1[:rows], a, sb1, None)
 
 
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(1, 300, 640), (40, 130, 300), (300, 520, 1000), (2048, 8300, 640)])
+def test_16_bit_results_of_fp32_sums(t, M, N, K):
+    """Where the caller says so no product is dropped: the fp32 result's bits, rounded; kernels on the e4m3 instructions do not take such a call even if forced."""
+    a, sa, b, sb = codes(M, K, 1).clone(), side(M, K, 2), codes(N, K, 3).clone(), blocks(N, K, 4)
+    a, b = (torch.nn.functional.pad(v.view(torch.uint8), (0, -K % 16)).view(F8)[:, :K] for v in (a, b))
+    a.view(torch.uint8)[:, 8], a.view(torch.uint8)[:, 9], b.view(torch.uint8)[:, 8:10] = 0x7E, 0xFE, 0x7E            # 448^2 - 448^2 among each eight's products
+    bias = normal(1, N, 5)[0].cuda()
+    whole = P.dev_gemm_nt_f8(a, sa, b, sb, bias)
+    check_matmul(whole, a, sa, b, sb, bias)
+    want = whole.to(TYPES[t])
+    assert torch.equal(P.dev_gemm_nt_f8(a, sa, b, sb, bias, dtype=TYPES[t], fp32_sums=True), want)
+    out = torch.empty_like(want)
+    assert P.dev_gemm_nt_f8(a, sa, b, sb, bias, out=out, fp32_sums=True) is out and torch.equal(out, want)
+    assert torch.equal(P.dev_gemm_nt_f8(a, sa, b, sb, bias, fp32_sums=True), whole)
+    for kernel in CORES:
+        ckq.lib().ckq_launch_set_f8_kernel(kernel)
+        try:
+            assert torch.equal(P.dev_gemm_nt_f8(a, sa, b, sb, bias, dtype=TYPES[t], fp32_sums=True), want)
+        finally:
+            ckq.lib().ckq_launch_set_f8_kernel(-1)
+
+
 # ---- matmul over experts ----------------------------------------------------------------
 
 def experts(M, N, K, counts, t, bias, seed=0):
