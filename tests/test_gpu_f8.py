@@ -1083,6 +1083,36 @@ def test_experts_captured_replayed_and_on_two_streams(T):
     assert all(torch.equal(a, b) for a, b in zip(m.run(), got))
 
 
+def test_captured_calls_that_make_their_tensors():
+    """Rows without a slot are zeros in every replay, also where the replay before had written them."""
+    T, c, E, k, N = 40, 3, 5, 300, 70
+    x, w, y, b, sb = normal(T, k, 1).cuda(), torch.rand(T, c, device="cuda"), normal(T * c, k, 2).cuda(), codes(E * N, k, 5).view(torch.uint8), blocks(N, k, 6, E)
+    b = torch.nn.functional.pad(b, (0, -k % 16)).view(F8).view(E, N, -1)[:, :, :k]
+    ids = torch.zeros(T, c, dtype=torch.int32, device="cuda")
+
+    def all_of_them():
+        offsets, order, position = P.dev_moe_sort(ids, E)
+        q, s = P.dev_moe_gather_f8(x, position)
+        return [offsets, order, position, q.view(torch.uint8), s, P.dev_moe_gather(x, position), P.dev_gemm_nt_f8_experts(q, s, b, sb, offsets), *P.dev_moe_combine_backward(x, y, position, w)]
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        all_of_them()
+        stream.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            made = all_of_them()
+    for none in (0.0, 0.5, 1.0, 0.2):
+        ids.copy_(random_ids(T, c, E, 7, none))
+        want = all_of_them()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(made, want))
+        have = int(want[0][-1])
+        assert all((v[have:] == 0).all() for v in made[3:8])
+
+
 def test_the_same_with_and_without_the_module_that_reads_tensors(monkeypatch):
     """Every call that it takes is made by the Python checks with the same result; what those refuse it does not take."""
     assert P._fast.gemm() == -1000 and P._fast.__name__ == "ckq_tensors"
