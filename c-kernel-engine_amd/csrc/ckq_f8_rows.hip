@@ -60,8 +60,9 @@ __device__ __forceinline__ row16f8 f8_codes(const float (&v)[16], float a1, floa
     return o;
 }
 
-/* Eight lanes have a group, sixteen elements each; a block has 2^rs rows beside each other and 32 >> rs groups of each: a row's codes leave in whole lines, a group's scales side by side.  Bound by memory:
- * 2048 x 11008 in bf16 68 MB in 13.4 to 15 us (4.5 to 5.1 TB/s; loads past the caches, half a line each, 16.2), few rows by a launch (2). */
+/* Eight lanes have a group, sixteen elements each; a block has 2^rs rows beside each other and 32 >> rs groups of each: a row's codes leave in
+ * whole lines, a group's scales side by side.  Bound by memory: 2048 x 11008 in bf16 68 MB in 13.4 to 15 us (4.5 to 5.1 TB/s; loads past the
+ * caches, half a line each, 16.2), few rows by a launch (2). */
 template <int OP, class E, bool EIGHT>
 __global__ void __launch_bounds__(256) rows_f8_kernel(F8RowsArgs a, int rs, u32 group_tiles)
 {
@@ -223,7 +224,8 @@ extern "C" int ckq_launch_moe_gather_f8(int type, const void *x, long ldx, const
     return launch_rows_f8<F8_GATHER>(type, a, stream);
 }
 
-/* y = T(scale * q), sixteen elements a thread, in pieces that are sixteen bytes of y: eight lanes store a line (2048 x 11008 to bf16 12.2 us, 5.5 TB/s, to fp32 20.1; sixteen beside each other 14.0 and 32.5). */
+/* y = T(scale * q), sixteen elements a thread, in pieces that are sixteen bytes of y: eight lanes store a line (2048 x 11008 to bf16 12.2 us, 5.5
+ * TB/s, to fp32 20.1; sixteen beside each other 14.0 and 32.5). */
 template <class E>
 __global__ void __launch_bounds__(256) dequantize_f8_kernel(const uint8_t *__restrict__ q, long ldq, const float *__restrict__ scale, long lds,
                                                             E *__restrict__ y, long ldy, int rows, int k, int rs, u32 group_tiles)

@@ -3,17 +3,18 @@
  *
  *   C[m][n] = T(sum_g (sa[g][m] * sb[n / 128][g]) * (sum over k in group g of A[m][k] B[n][k])  (+ bias[n]))
  *
- * and the same of rows sorted by expert, each expert with a matrix of its own.  A group's sum starts from zero; the groups' sums are scaled and
- * added in fp32.
+ * and the same of rows sorted by expert, each expert with a matrix of its own.  A group's sum starts from zero; the groups' sums are scaled and added
+ * in fp32.
  *
- * Sums.  The matrix cores' e4m3 instructions add eight products at a time after aligning them to the largest of the eight and dropping what is
- * under 2^-13 of it (measured, in all their shapes; between eights they add as fp32 does): a sum of 128 random products is 1.5e-5 of its size off.
- * e4m3 values are exact in fp16, and the fp16 instructions add their products as fp32 does (1e-8), at half the rate.
+ * Sums.  The matrix cores' e4m3 instructions add eight products at a time after aligning them to the largest of the eight and dropping what is under
+ * 2^-13 of it (measured, in all their shapes; between eights they add as fp32 does): a sum of 128 random products is 1.5e-5 of its size off. e4m3
+ * values are exact in fp16, and the fp16 instructions add their products as fp32 does (1e-8), at half the rate.
  *
- * Forms.  One token: rows streamed, bound by reading them (11008 x 4096 from memory 8.4 us, 5.3 TB/s).  A few tokens: K split among the waves of a block, bound by a launch's and a block's start and a wave's
- * steps one after the other (16 tokens 10.8 us, 64 11.8; one token through 8 of 64 experts of 2816 x 2048 10.6, 4.4 TB/s).  More: tiles, on the fp16 instructions bound by those and the
- * conversions beside them (matrix cores busy 64 %, vector units 63 % of a CU's cycles: 8192^3 930 us, 1180 TFLOP/s, the library's fp16 product without scales 1371), on the e4m3 ones by the power limit and by what keeps
- * scales in fp32 (64 and 49 %: 8192^3 468 us, 2350 TFLOP/s, the library's 2607; 2048 x 11008 x 4096 87 us).
+ * Forms.  One token: rows streamed, bound by reading them (11008 x 4096 from memory 8.4 us, 5.3 TB/s).  A few tokens: K split among the waves of a
+ * block, bound by a launch's and a block's start and a wave's steps one after the other (16 tokens 10.8 us, 64 11.8; one token through 8 of 64
+ * experts of 2816 x 2048 10.6, 4.4 TB/s).  More: tiles, on the fp16 instructions bound by those and the conversions beside them (matrix cores busy 64
+ * %, vector units 63 % of a CU's cycles: 8192^3 930 us, 1180 TFLOP/s, the library's fp16 product without scales 1371), on the e4m3 ones by the power
+ * limit and by what keeps scales in fp32 (64 and 49 %: 8192^3 468 us, 2350 TFLOP/s, the library's 2607; 2048 x 11008 x 4096 87 us).
  */
 #include "ckq_gemm_common.hpp"
 #include "ckq_int8.hpp"
@@ -52,9 +53,9 @@ __device__ __forceinline__ int wave_scan(int v)
 
 struct F8Tile { int e, m0, mend, nt; };                        /* expert, rows m0 .. mend - 1 of A, tile of weight rows */
 
-/* Which tile of BT rows x a tile of weight rows the `id`-th block has.  Tiles are dealt to the XCDs in equal runs (gemm_deal), and in the order of a run eight
- * tiles of rows lie beside each other for every tile of weight rows, so that the tiles an XCD works on at a time share both operands in its L2.  Of experts, the
- * tiles that there are are counted first, from the offsets: 64 experts at a time, one a lane. */
+/* Which tile of BT rows x a tile of weight rows the `id`-th block has.  Tiles are dealt to the XCDs in equal runs (gemm_deal), and in the order of
+ * a run eight tiles of rows lie beside each other for every tile of weight rows, so that the tiles an XCD works on at a time share both operands
+ * in its L2.  Of experts, the tiles that there are are counted first, from the offsets: 64 experts at a time, one a lane. */
 __device__ __forceinline__ bool f8_tile(const F8Args &a, int id, int BT, int nnt, F8Tile &w)
 {
     const int lane = threadIdx.x & 63;
@@ -113,8 +114,9 @@ __device__ __forceinline__ f8_v8h f8_half(int lo, int hi)
 
 template <class E> struct __attribute__((packed, aligned(sizeof(E)))) f8_out8 { E v[8]; };
 
-/* Eight rows' results of a token to C[t][n ..].  ONCE: non-temporally, as the large tiles' leave, since what stays in the L2s is written back when the launch ends, with nothing beside it (2048 x 11008 x 4096
- * in bf16 88.3 -> 81.9 us); a few rows' are read from the caches by what follows (one token through eight experts 28.5 -> 28.0). */
+/* Eight rows' results of a token to C[t][n ..].  ONCE: non-temporally, as the large tiles' leave, since what stays in the L2s is written back when
+ * the launch ends, with nothing beside it (2048 x 11008 x 4096 in bf16 88.3 -> 81.9 us); a few rows' are read from the caches by what follows (one
+ * token through eight experts 28.5 -> 28.0). */
 template <class E, bool ONCE>
 __device__ __forceinline__ void f8_store8(const F8Args &a, const float *bias, const float (&f)[8], int t, int n)
 {
@@ -157,9 +159,11 @@ __device__ __forceinline__ void f8_clear_tail(uint8_t *p, int rows, int tail, in
 
 /* ---- tiles on the fp16 instructions ----------------------------------------------------------------------------------- */
 
-/* WT x WN waves, each 32 TT tokens x 32 TN rows.  A step is a group of 128; its codes come to LDS as they are, eight rows of 128 bytes a copy, the chunk of 16 that a
- * lane fetches is the one that belongs in its place, c ^ (row / 2 % 8), so that a read of 16 bytes a lane meets all banks once.  Two to four blocks a CU (two, three and four of H128x128, H64x128, H64x64),
- * each other's copies and barriers hidden: 16384 rows of 64 experts x 2816 x 2048 236 | 243 us, 4096 rows 106 | 95 (the first two). */
+/* WT x WN waves, each 32 TT tokens x 32 TN rows.  A step is a group of 128; its codes come to LDS as they are, eight rows of 128 bytes a copy, the
+ * chunk of 16 that a lane fetches is the one that belongs in its place, c ^ (row / 2 % 8), so that a read of 16 bytes a lane meets all banks once.
+ * Two to four blocks a CU (two, three and four of H128x128, H64x128, H64x64), each other's copies and barriers hidden: 16384 rows of 64 experts x
+ * 2816 x 2048 236 | 243 us, 4096 rows 106 | 95 (the first two).  The former's busy CUs have their matrix cores at work 45 % of the time, vector
+ * instructions 51, LDS 5 (of 8192^3 64 and 63 %): 5 of a tile's 35 us are its start and end, and about 160 tiles of 128 have the 16384 rows. */
 template <int WT_, int WN_, int TT_, int TN_> struct F8Half {
     static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NW = WT * WN, BT = 32 * TT * WT, BN = 32 * TN * WN, S = 2;
     static constexpr int CODES = (BT + BN) * 128, STAGE = CODES + 4 * BT + 256, NC = (BT + BN) / 8 / NW, NCA = BT / 8 / NW;
@@ -230,9 +234,9 @@ __global__ void __launch_bounds__(64 * T::NW, 2) gemm_f8_half_kernel(F8Args a, i
         __builtin_amdgcn_s_barrier();
         if (it + 1 == last && tail < 128) clear_tail((it + 1) & 1);
     };
-    /* The steps of a wave with LIVE groups of 32 tokens.  Quarters of a step, 32 of its 128: the products of one while the codes of the next become fp16, one operand's
-     * half between two multiplications, and those of the one after it leave LDS.  A tile's sums are scaled while the next one's are made, the last tile's in the step
-     * after. */
+    /* The steps of a wave with LIVE groups of 32 tokens.  Quarters of a step, 32 of its 128: the products of one while the codes of the next
+     * become fp16, one operand's half between two multiplications, and those of the one after it leave LDS.  A tile's sums are scaled while the
+     * next one's are made, the last tile's in the step after. */
     auto steps = [&](auto live) {
         constexpr int LIVE = decltype(live)::value, NF = LIVE + TN, NM = LIVE * TN;
         f8_v8h h[2][NF][2];                                    /* operands: tokens first, then rows; quarter, halves of 16 */
@@ -337,9 +341,10 @@ static int launch_f8_half(const F8Args &a, hipStream_t s)
 
 /* ---- tiles on the e4m3 instructions ------------------------------------------------------------------------------------ */
 
-/* WT x WN waves that multiply, each 16 TT tokens x 16 TN rows; a group's product is one multiplication, 16 x 16 x 128, whose four sums a lane scales and adds while the next ones are
- * multiplied.  NP others that copy, or none (the former do it then); S stages in LDS; PERCU blocks a CU.  With others that copy, whose waits for the address unit hold up no multiplication, us: 512 x 11008 x
- * 4096 36.0 -> 28.4, 1024 x 4096 x 4096 33.0 -> 22.8; eight waves of 256 x 256 leave no registers for them. */
+/* WT x WN waves that multiply, each 16 TT tokens x 16 TN rows; a group's product is one multiplication, 16 x 16 x 128, whose four sums a lane
+ * scales and adds while the next ones are multiplied.  NP others that copy, or none (the former do it then); S stages in LDS; PERCU blocks a CU.
+ * With others that copy, whose waits for the address unit hold up no multiplication, us: 512 x 11008 x 4096 36.0 -> 28.4, 1024 x 4096 x 4096 33.0
+ * -> 22.8; eight waves of 256 x 256 leave no registers for them. */
 template <int WT_, int WN_, int TT_, int TN_, int NP_, int S_, int PERCU_> struct F8Core {
     static constexpr int WT = WT_, WN = WN_, TT = TT_, TN = TN_, NP = NP_, S = S_, PERCU = PERCU_, NW = WT * WN, WAVES = NW + NP, BT = 16 * TT * WT, BN = 16 * TN * WN, NB = (BN + 127) / 128;
     static constexpr int CODES = (BT + BN) * 128, SB = CODES + 4 * BT, STAGE = SB + 256 * NB;
@@ -387,8 +392,8 @@ __device__ __forceinline__ void f8_core_tile(const F8Args &a, const F8Tile &w, i
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
     };
-    /* Step `it` has stage it % S.  A step's last operands are read before its last tokens are multiplied; the barrier is there: all have step it's operands in registers, and step it + 1 has
-     * arrived; from there on the stage takes the copies of step it + S. */
+    /* Step `it` has stage it % S.  A step's last operands are read before its last tokens are multiplied; the barrier is there: all have step it's
+     * operands in registers, and step it + 1 has arrived; from there on the stage takes the copies of step it + S. */
     if (NP > 0 && wave >= NW) {
         constexpr int EACH_STEP = NC + T::NS;
 #pragma unroll
@@ -557,9 +562,10 @@ static int launch_f8_core(const F8Args &a, hipStream_t s)
 
 /* ---- K split among the waves of a block -------------------------------------------------------------------------------- */
 
-/* 16 TG tokens x 16 RN rows a block of NW waves; every wave has all of the tile and each NW-th group of K, through S stages of its own, so that nothing is waited for
- * but its own copies until the waves' sums meet at the end, in the order of the waves.  333 x 1001 x 4847, us: 16 x 32 on four waves 14.7, 32 x 32 on four 13.9, 48 x 32 on seven 11.3 (one round of the CUs),
- * 64 x 32 on six 13.2; operands straight to registers, 16 rows x 64 bytes a load, take twice as long to come: 16.9. */
+/* 16 TG tokens x 16 RN rows a block of NW waves; every wave has all of the tile and each NW-th group of K, through S stages of its own, so that
+ * nothing is waited for but its own copies until the waves' sums meet at the end, in the order of the waves.  333 x 1001 x 4847, us: 16 x 32 on
+ * four waves 14.7, 32 x 32 on four 13.9, 48 x 32 on seven 11.3 (one round of the CUs), 64 x 32 on six 13.2; operands straight to registers, 16
+ * rows x 64 bytes a load, take twice as long to come: 16.9. */
 template <int NW_, int RN_, int TG_, int S_> struct F8Split {
     static constexpr int NW = NW_, RN = RN_, TG = TG_, S = S_, BT = 16 * TG, BN = 16 * RN, CODES = (BT + BN) * 128, STAGE = CODES + 512, PITCH = BN * 4 + 16, NC = 2 * (RN + TG);
     static constexpr int LDS = NW * (S * STAGE > BT * PITCH ? S * STAGE : BT * PITCH);
@@ -691,8 +697,9 @@ static int launch_f8_split(const F8Args &a, hipStream_t s)
 
 /* ---- one token: rows streamed ------------------------------------------------------------------------------------------ */
 
-/* A wave has R rows and every KS-th piece of KU KB of K; 4 waves a block.  A lane has sixteen elements of a group at a time: their products in pairs (v_dot2_f32_f16), times the group's scales, onto
- * its sum.  Rows are loaded non-temporally: a decode step goes through more weights than any cache holds. */
+/* A wave has R rows and every KS-th piece of KU KB of K; 4 waves a block.  A lane has sixteen elements of a group at a time: their products in
+ * pairs (v_dot2_f32_f16), times the group's scales, onto its sum.  Rows are loaded non-temporally: a decode step goes through more weights than
+ * any cache holds. */
 template <class E, int R, int KU, int KS>
 __global__ void __launch_bounds__(256) gemm_f8_stream_kernel(F8Args a)
 {
@@ -785,8 +792,8 @@ static int launch_f8_stream(const F8Args &a, hipStream_t s)
     constexpr int per = 4 / KS * R;
     return i8_launch(gemm_f8_stream_kernel<E, R, KU, KS>, dim3((u32)((a.N + per - 1) / per)), dim3(256), s, a);
 }
-/* us, rows x K, (rows a wave, KB a trip, waves of a row): 11008 x 4096, 4, 1, 2 9.66 | 4, 1, 4 9.23 | 2, 2, 2 9.18 | 2, 1, 4 9.82 | 1, 2, 4 13.2; 4096 x 11008, 4, 1, 4 9.97 | 2, 1, 4 9.32 | 2, 4, 4 10.0; 11008 x 2048, 4, 1, 2 5.76 |
- * 2, 2, 2 5.88; 4000 x 1000, 4, 1, 1 2.94 | 4, 1, 4 3.23. */
+/* us, rows x K, (rows a wave, KB a trip, waves of a row): 11008 x 4096, 4, 1, 2 9.66 | 4, 1, 4 9.23 | 2, 2, 2 9.18 | 2, 1, 4 9.82 | 1, 2, 4 13.2;
+ * 4096 x 11008, 4, 1, 4 9.97 | 2, 1, 4 9.32 | 2, 4, 4 10.0; 11008 x 2048, 4, 1, 2 5.76 | 2, 2, 2 5.88; 4000 x 1000, 4, 1, 1 2.94 | 4, 1, 4 3.23. */
 template <class E>
 static int launch_f8_stream(const F8Args &a, hipStream_t s)
 {
@@ -812,10 +819,11 @@ typedef F8Core<2, 2, 4, 4, 4, 4, 1> C128x128;
 typedef F8Core<2, 2, 2, 4, 4, 4, 1> C64x128;
 typedef F8Core<2, 2, 2, 2, 4, 4, 2> C64x64;
 
-/* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all places have a block; in a last round of fewer blocks less, `share` of it by how
- * many share a CU, the rest by how many there are in all, but no less than a block alone takes, `alone`.  Fitted to 800 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three
- * sets in turn): the kernel so chosen is 0.8 % (fp32 results) and 0.7 % (16 bits) slower than the fastest on average, 1.2 times at worst, as much on one half of them when fitted to the other; over experts (500
- * random products, 2 to 128 of them, none of which it was fitted to) 1.8 % and 1.4 times. */
+/* What a launch takes, in us: t0, and for every round of blocks t_tile and as many steps of K as a wave has, each of `step` where all places have
+ * a block; in a last round of fewer blocks less, `share` of it by how many share a CU, the rest by how many there are in all, but no less than a
+ * block alone takes, `alone`.  Fitted to 800 random products of one matrix (2 to 4096 tokens, 32 to 32000 rows, K 32 to 11008; three sets in
+ * turn): the kernel so chosen is 0.8 % (fp32 results) and 0.7 % (16 bits) slower than the fastest on average, 1.2 times at worst, as much on one
+ * half of them when fitted to the other; over experts (500 random products, 2 to 128 of them, none of which it was fitted to) 1.8 % and 1.4 times. */
 struct F8Cost { int bt, bn, places, split; float t0, t_tile, step, share, alone; };
 static const F8Cost f8_costs[CKQ_F8_TILINGS] = {
     {128, 128, 512, 1, 1.48f, 5.25f, 1.886f, 0.90f, 0.28f}, {64, 128, 768, 1, 1.41f, 3.69f, 1.596f, 1.00f, 0.45f}, {64, 64, 1024, 1, 1.78f, 2.53f, 1.301f, 1.00f, 0.40f},
@@ -843,8 +851,8 @@ static float f8_row_tiles(int bt, int M, int experts)
 }
 static float f8_tiles(const F8Cost &c, int M, int N, int experts) { return f8_row_tiles(c.bt, M, experts) * (float)((N + (long)c.bn - 1) / c.bn); }
 
-/* Columns of 256 x 256 tiles that make whole rounds of the 256 CUs: what they leave goes in tiles of 128 x 192, a shorter last round (2048 x 11008 x 4096: 344 tiles of 256 x 256 in two rounds 105 us; 256 of
- * them and 240 small ones 87). */
+/* Columns of 256 x 256 tiles that make whole rounds of the 256 CUs: what they leave goes in tiles of 128 x 192, a shorter last round (2048 x 11008
+ * x 4096: 344 tiles of 256 x 256 in two rounds 105 us; 256 of them and 240 small ones 87). */
 static int f8_whole_columns(int M, int N)
 {
     const long ntt = (M + 255l) / 256, nnt = (N + 255l) / 256;
@@ -863,10 +871,11 @@ static bool f8_fits(int kernel, int M, int N, int experts)
 static std::atomic<int> g_f8_kernel{-1};
 extern "C" void ckq_launch_set_f8_kernel(int kernel) { g_f8_kernel.store(kernel < 0 || kernel > CKQ_F8_STREAM ? -1 : kernel); }
 
-/* The e4m3 instructions' sums, 1.5e-5 off on random products and by 2^-13 of the largest of each eight at most for every other one of them, are taken where the result is rounded to 16 bits (bf16 2^-9, fp16
- * 2^-12 off) and nothing but that: not for fp32 results, not where the caller says so (CKQ_SUMS_FP32), and not over experts, whose first product's results go through another quantizer, where each change of a
- * value moves some of them by a sixteenth (an MLP with 32 experts in fp16: 0.0017 off the definition, with fp32 sums 0.0003).  Random products of one matrix gain 5.8 % by them on average, 2048 x 11008 x 4096
- * 174 -> 87 us. */
+/* The e4m3 instructions' sums, 1.5e-5 off on random products and by 2^-13 of the largest of each eight at most for every other one of them, are
+ * taken where the result is rounded to 16 bits (bf16 2^-9, fp16 2^-12 off) and nothing but that: not for fp32 results, not where the caller says
+ * so (CKQ_SUMS_FP32), and not over experts, whose first product's results go through another quantizer, where each change of a value moves some of
+ * them by a sixteenth (an MLP with 32 experts in fp16: 0.0017 off the definition, with fp32 sums 0.0003).  Random products of one matrix gain 5.8
+ * % by them on average, 2048 x 11008 x 4096 174 -> 87 us. */
 /* -1: none takes it in one launch. */
 extern "C" int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts)
 {
@@ -879,7 +888,8 @@ extern "C" int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts)
     int best = -1;
     float t = 1e30f;
     for (int i = 0; i < (cores ? CKQ_F8_TILINGS : CKQ_F8_C256x256); ++i) {
-        /* of an expert's last tile of 128, groups of 32 tokens that are not there cost nothing (160 products of 256 to 65536 rows over 8 to 128 experts: 1.3 % from the fastest on average without the factor, 1.0 with it) */
+        /* of an expert's last tile of 128, groups of 32 tokens that are not there cost nothing (160 products of 256 to 65536 rows over 8 to 128
+         * experts: 1.3 % from the fastest on average without the factor, 1.0 with it) */
         const float ti = (f8_costs[i].t0 + f8_rounds(f8_costs[i], f8_tiles(f8_costs[i], M, N, experts), K)) * (experts && i == CKQ_F8_H128x128 ? 0.95f : 1.0f);
         if (ti < t && f8_fits(i, M, N, experts)) { t = ti; best = i; }
     }
@@ -890,7 +900,8 @@ extern "C" int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts)
     return best;
 }
 
-/* What one launch does not take goes in halves, of the tokens or of the weights' rows, which are whole tiles and blocks of scales; over experts of the latter only. */
+/* What one launch does not take goes in halves, of the tokens or of the weights' rows, which are whole tiles and blocks of scales; over experts of
+ * the latter only. */
 template <class E>
 static int launch_gemm_f8(const F8Args &a, int type, hipStream_t s)
 {

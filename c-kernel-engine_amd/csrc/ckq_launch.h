@@ -88,8 +88,9 @@ void ckq_launch_set_gemm_policy(int policy);
  * either.  Host arithmetic; exported for the test of the rules. */
 enum { CKQ_ROUTE_STREAM = 0, CKQ_ROUTE_TILES = 1, CKQ_ROUTE_ROWS16_STREAM = 2, CKQ_ROUTE_ROWS16_TILES = 3 };
 int ckq_launch_route(int fmt, int nrows, int K, int ntok, int aligned);
-/* Where n (2..4) K-quant matrices of rows[i] rows against the same tokens go together: up to eight tokens CKQ_ROUTE_STREAM or CKQ_ROUTE_ROWS16_STREAM, beyond any of the routes (one launch for
- * all) or CKQ_ENOGROUP, one by one.  Host arithmetic; exported for the test of the rules. */
+/* Where n (2..4) K-quant matrices of rows[i] rows against the same tokens go together: up to eight tokens CKQ_ROUTE_STREAM or
+ * CKQ_ROUTE_ROWS16_STREAM, beyond any of the routes (one launch for all) or CKQ_ENOGROUP, one by one.  Host arithmetic; exported for the test of
+ * the rules. */
 int ckq_launch_group_route(int fmt, int n, const int *rows, int K, int ntok);
 /* Token tile of the Q4_K x Q8_K matrix-core GEMM: 0 = by shape (default), 64 or 96 = that kernel wherever the GEMM is taken. */
 void ckq_launch_set_q4k_tile(int tokens);
@@ -174,8 +175,8 @@ int ckq_launch_i8_kernel(int M, int N, int K);
 /* -1 = by shape (default), else that kernel wherever it can take the product, in all calls of the process. */
 void ckq_launch_set_i8_kernel(int kernel);
 
-/* Rows in e4m3 with one scale for each 128 elements, and tokens sorted by expert (ckq_f8_rows.hip, ckq_gemm_f8.hip, ckq_moe.hip).  See ckernel_quant_hip.h for what
- * they compute and take. */
+/* Rows in e4m3 with one scale for each 128 elements, and tokens sorted by expert (ckq_f8_rows.hip, ckq_gemm_f8.hip, ckq_moe.hip).  See
+ * ckernel_quant_hip.h for what they compute and take. */
 #define CKQ_SUMS_FP32 256                        /* CKQ_F8_SUMS_FP32 of ckernel_quant_hip.h: in a matmul's type, no kernel on the e4m3 instructions */
 #define CKQ_MOE_EXPERTS_MAX 65535
 #define CKQ_MOE_SLOTS_MAX (1l << 29)
@@ -186,9 +187,10 @@ int ckq_launch_gemm_f8(const uint8_t *A, long lda, const float *sa, long ldsa, c
                        int type, void *C, long ldc, int M, int N, int K, void *stream);
 int ckq_launch_gemm_f8_experts(const uint8_t *A, long lda, const float *sa, long ldsa, const uint8_t *B, long ldb, long eb, const float *sb, long ldsb, long esb,
                                const float *bias, const int32_t *offsets, int experts, int type, void *C, long ldc, int M, int N, int K, void *stream);
-/* Which kernel takes a product of M rows against matrices of N x K (experts: their number, 0: one matrix without offsets), results of `type`: tiles of so many tokens x rows on the fp16 instructions (S:
- * with K split among a block's waves, w8, w7, w2: eight, seven or two of them) or on the e4m3 ones (C), two sizes of the latter in a launch, or the rows streamed; -1: in parts, since no launch has so many blocks.  Host arithmetic; exported for the test of the
- * rules. */
+/* Which kernel takes a product of M rows against matrices of N x K (experts: their number, 0: one matrix without offsets), results of `type`:
+ * tiles of so many tokens x rows on the fp16 instructions (S: with K split among a block's waves, w8, w7, w2: eight, seven or two of them) or on
+ * the e4m3 ones (C), two sizes of the latter in a launch, or the rows streamed; -1: in parts, since no launch has so many blocks.  Host
+ * arithmetic; exported for the test of the rules. */
 enum { CKQ_F8_H128x128, CKQ_F8_H64x128, CKQ_F8_H64x64, CKQ_F8_S48x32w7, CKQ_F8_S32x32, CKQ_F8_S16x32w8, CKQ_F8_S16x32, CKQ_F8_S16x32w2, CKQ_F8_S16x16, CKQ_F8_C256x256, CKQ_F8_C256x128,
        CKQ_F8_C128x128, CKQ_F8_C64x128, CKQ_F8_C64x64, CKQ_F8_C128x192, CKQ_F8_TILINGS, CKQ_F8_TWO = CKQ_F8_TILINGS, CKQ_F8_STREAM };
 int ckq_launch_f8_kernel(int type, int M, int N, int K, int experts);

@@ -18,10 +18,12 @@
 
 /* ---- sort ---------------------------------------------------------------------------------------------------------- */
 
-/* A block has an expert, the last one what has none.  Each goes through all slots: it counts those that belong before its own, and its own in each wave's run of slots, whose
- * places follow from that; then it writes its own.  No scratch memory, one launch, and the slots' order is kept without a sort.  A wave takes 64 NV slots at a time into
- * registers, one a lane and load; what it has compared it counts in scalar registers, two vector instructions a slot.  Runs of up to 64 NV slots are read once.  65536 slots of
- * 128 experts, us: one slot a lane and load, a load at a time, 41.6; four a lane, counted in vector registers, 19.8; this 11 to 13 (16384 of 64 5.5, 8 slots 3.0: a launch), of which most are the instructions of both passes. */
+/* A block has an expert, the last one what has none.  Each goes through all slots: it counts those that belong before its own, and its own in each
+ * wave's run of slots, whose places follow from that; then it writes its own.  No scratch memory, one launch, and the slots' order is kept without
+ * a sort.  A wave takes 64 NV slots at a time into registers, one a lane and load; what it has compared it counts in scalar registers, two vector
+ * instructions a slot.  Runs of up to 64 NV slots are read once.  65536 slots of 128 experts, us: one slot a lane and load, a load at a time,
+ * 41.6; four a lane, counted in vector registers, 19.8; this 11 to 13 (16384 of 64 5.5, 8 slots 3.0: a launch), of which most are the instructions
+ * of both passes. */
 template <int NV>
 __global__ void __launch_bounds__(1024) moe_sort_kernel(const int32_t *__restrict__ ids, int slots, int run, int experts, int32_t *__restrict__ offsets, int32_t *__restrict__ order,
                                                         int32_t *__restrict__ position)
@@ -90,8 +92,8 @@ extern "C" int ckq_launch_moe_sort(const int32_t *ids, int tokens, int choices, 
     const dim3 grid((u32)experts + 1);
     const hipStream_t s = (hipStream_t)stream;
     if (slots <= 4096) return i8_launch(moe_sort_kernel<4>, grid, dim3(64u * (u32)((slots - 1) / 256 + 1)), s, ids, slots, 256, experts, offsets, order, position);
-    /* Read once where sixteen waves hold all slots and a CU has one block; else twice, by blocks of which a CU has two.  us, once | twice: 65536 slots of 128 experts 10.9 | 11.9, of 256 14.6 | 11.5, 262144 of 128
-     * (either way twice) 36.7 | 35.4. */
+    /* Read once where sixteen waves hold all slots and a CU has one block; else twice, by blocks of which a CU has two.  us, once | twice: 65536
+     * slots of 128 experts 10.9 | 11.9, of 256 14.6 | 11.5, 262144 of 128 (either way twice) 36.7 | 35.4. */
     return i8_launch(slots > 16384 && slots <= 65536 && experts < 256 ? moe_sort_kernel<64> : moe_sort_kernel<16>, grid, dim3(1024), s, ids, slots, run, experts, offsets, order, position);
 }
 
@@ -121,10 +123,12 @@ __device__ __forceinline__ void moe_places(const MoeArgs &a, size_t t, F &&use)
     }
 }
 
-/* Where a thread's eight elements begin: a row's last thread has its last eight, some of which the one before has too (the same values), so that none has loads of its own. */
+/* Where a thread's eight elements begin: a row's last thread has its last eight, some of which the one before has too (the same values), so that
+ * none has loads of its own. */
 __device__ __forceinline__ long moe_at(const MoeArgs &a, u32 v) { return max(0l, min(8 * (long)v, (long)a.k - 8)); }
 
-/* Eight elements a thread.  Bound by the rows it writes (8192 tokens of 8 slots x 2048 in bf16: 302 MB in 52 us, 5.8 TB/s).  ONCE here and in the backward pass: what is written leaves non-temporally (moe_past_cache). */
+/* Eight elements a thread.  Bound by the rows it writes (8192 tokens of 8 slots x 2048 in bf16: 302 MB in 52 us, 5.8 TB/s).  ONCE here and in the
+ * backward pass: what is written leaves non-temporally (moe_past_cache). */
 template <class E, bool ONCE>
 __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
 {
@@ -143,8 +147,9 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(MoeArgs a, u32 nvec)
     });
 }
 
-/* Eight elements a thread, the rows of eight slots on their way together (one token of 8 slots x 2048 6.8 us one after the other, 3.7 together), non-temporally, being read for the last
- * time, which leaves the caches to what is beside them (with a gather before it, 8192 tokens of 8 slots x 2048 in bf16 132 -> 115 us; alone 52, 5.8 TB/s); fp32 not, whose loads take half a line each (119 -> 116). */
+/* Eight elements a thread, the rows of eight slots on their way together (one token of 8 slots x 2048 6.8 us one after the other, 3.7 together),
+ * non-temporally, being read for the last time, which leaves the caches to what is beside them (with a gather before it, 8192 tokens of 8 slots x
+ * 2048 in bf16 132 -> 115 us; alone 52, 5.8 TB/s); fp32 not, whose loads take half a line each (119 -> 116). */
 template <class E>
 __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
 {
@@ -174,7 +179,9 @@ __global__ void __launch_bounds__(256) moe_combine_kernel(MoeArgs a, u32 nvec)
     store8_pieces((E *)a.out + (size_t)t * a.ldo + at, f, left);
 }
 
-/* A block has a token, its slots eight at a time: bound by the rows read and written (4096 tokens of 8 slots x 2048 in bf16, 285 MB in 58 us, 4.9 TB/s).  What vectors of eight leave of a row is read and written an element a lane, beside them: 93 tokens of 8 slots x 1001 in fp32 8.6 -> 6.0 us, 2048 of 8 x 2047 in bf16 50 -> 37.  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
+/* A block has a token, its slots eight at a time: bound by the rows read and written (4096 tokens of 8 slots x 2048 in bf16, 285 MB in 58 us, 4.9
+ * TB/s).  What vectors of eight leave of a row is read and written an element a lane, beside them: 93 tokens of 8 slots x 1001 in fp32 8.6 -> 6.0
+ * us, 2048 of 8 x 2047 in bf16 50 -> 37.  Sums of dw: each thread's elements in turn, the tree of a wave's lanes, the waves in turn. */
 template <class E, bool ONCE>
 __global__ void __launch_bounds__(256) moe_combine_backward_kernel(MoeArgs a)
 {
@@ -254,10 +261,11 @@ static int moe_each(MoeArgs a, bool out_by_token, size_t threads, L &&launch)
     }
 }
 
-/* Whether what is written, a row for each slot, is more than the 256 MB cache holds beside the rest: then it leaves non-temporally, and its reader finds it in memory either way.  us, kept | not: gather and
- * the combine of its rows, bf16 x 2048, 67 MB 25.6 | 28.5, 134 MB 47.0 | 51.7, 252 MB 115 | 100; the backward pass and the combine of its rows, 134 MB 73.0 | 80.6.  Not where a line leaves in pieces, that memory
- * would get one by one: fp32, whose threads store two pieces of 32 bytes one after the other (gather and combine of 537 MB 257 | 360, backward and combine of rows x 2047 364 | 383), and gather's rows that do not begin at 16
- * bytes (bf16 x 2047 126 | 137). */
+/* Whether what is written, a row for each slot, is more than the 256 MB cache holds beside the rest: then it leaves non-temporally, and its reader
+ * finds it in memory either way.  us, kept | not: gather and the combine of its rows, bf16 x 2048, 67 MB 25.6 | 28.5, 134 MB 47.0 | 51.7, 252 MB
+ * 115 | 100; the backward pass and the combine of its rows, 134 MB 73.0 | 80.6.  Not where a line leaves in pieces, that memory would get one by
+ * one: fp32, whose threads store two pieces of 32 bytes one after the other (gather and combine of 537 MB 257 | 360, backward and combine of rows
+ * x 2047 364 | 383), and gather's rows that do not begin at 16 bytes (bf16 x 2047 126 | 137). */
 static bool moe_past_cache(const MoeArgs &a, size_t size, bool gather)
 {
     return size == 2 && (size_t)a.tokens * a.choices * a.k * size > (size_t)192 << 20 && !(gather && ((uintptr_t)a.out % 16 || a.ldo % 8));

@@ -59,7 +59,8 @@ __device__ __forceinline__ void drop_first(raw8<E> &r, int drop)
             for (int i = 0; i < N; ++i) r.w[i] = i + by < N ? r.w[i + by] : 0u;
         }
 }
-/* The same as fetch8; EIGHT: of a row of at least eight elements, without a branch and loads of their own for its last: the row's last eight, those before them dropped (drop_rest). */
+/* The same as fetch8; EIGHT: of a row of at least eight elements, without a branch and loads of their own for its last: the row's last eight,
+ * those before them dropped (drop_rest). */
 template <bool EIGHT, class E>
 __device__ __forceinline__ raw8<E> fetch8_of(const E *p, int left)
 {
@@ -133,10 +134,10 @@ __device__ __forceinline__ void store8_pieces(E *p, const float (&f)[8], int lef
     }
 }
 
-/* gate / (1 + exp(-gate)) * up.  v_exp_f32 and v_rcp_f32, an ulp each: what they and the exponent's rounding are off is (2 + |gate|) 2^-23 of a value that is about to
- * be rounded to one part in 254 of the row's largest or to four bits (integer and fraction of the exponent apart, it would be an ulp or two at any gate: int8 rows, 512 x 4864 5.35 -> 5.82 us,
- * 2048 x 11008 23.5 -> 24.2).  A quarter of both sides of the fraction, so that the reciprocal of no finite sum is below the normal numbers, where the
- * instruction has zeros: those values count where up is large enough. */
+/* gate / (1 + exp(-gate)) * up.  v_exp_f32 and v_rcp_f32, an ulp each: what they and the exponent's rounding are off is (2 + |gate|) 2^-23 of a
+ * value that is about to be rounded to one part in 254 of the row's largest or to four bits (integer and fraction of the exponent apart, it would
+ * be an ulp or two at any gate: int8 rows, 512 x 4864 5.35 -> 5.82 us, 2048 x 11008 23.5 -> 24.2).  A quarter of both sides of the fraction, so
+ * that the reciprocal of no finite sum is below the normal numbers, where the instruction has zeros: those values count where up is large enough. */
 __device__ __forceinline__ float row_swiglu(float gate, float up)
 {
     const float e = __builtin_amdgcn_exp2f(gate * -1.44269504f);

@@ -1,8 +1,9 @@
 /*
- * ckq_tensors.cpp - the calls that parity.py's fp8 and experts' front-ends make when nothing is wrong with their tensors, as a CPython module: it reads types,
- * shapes, strides and devices from the tensors themselves, where Python pays 0.06 us for each, and calls ckq_call_dev on the current stream.  A call it does not take (NOT_TAKEN) has changed
- * nothing; parity.py then looks at the same tensors and says why.  Every check here is made there too, and in the library behind both.
- * `built_for` names the torch and the Python it was compiled for (CKQ_BUILT_FOR, from the Makefile): parity.py uses it with no others.
+ * ckq_tensors.cpp - the calls that parity.py's fp8 and experts' front-ends make when nothing is wrong with their tensors, as a CPython module: it
+ * reads types, shapes, strides and devices from the tensors themselves, where Python pays 0.06 us for each, and calls ckq_call_dev on the current
+ * stream.  A call it does not take (NOT_TAKEN) has changed nothing; parity.py then looks at the same tensors and says why.  Every check here is made
+ * there too, and in the library behind both. `built_for` names the torch and the Python it was compiled for (CKQ_BUILT_FOR, from the Makefile):
+ * parity.py uses it with no others.
  */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
